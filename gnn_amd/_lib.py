@@ -28,9 +28,19 @@ class MgnWeightSlice(C.Structure):
     _fields_ = [("w", C.c_void_p), ("ld", C.c_int32), ("col0", C.c_int32), ("k", C.c_int32), ("reserved", C.c_int32)]
 
 
+class MgnAttn(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_st", C.c_int64), ("q_sh", C.c_int64), ("k_st", C.c_int64), ("k_sh", C.c_int64), ("v_st", C.c_int64), ("v_sh", C.c_int64),
+                ("q_ptr", C.c_void_p), ("k_ptr", C.c_void_p), ("key_mask", C.c_void_p), ("bias_table", C.c_void_p),
+                ("bucket_lut", C.c_void_p), ("q_pos", C.c_void_p), ("k_pos", C.c_void_p), ("n_q", C.c_int64), ("n_k", C.c_int64),
+                ("n_seg", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32),
+                ("n_bucket", C.c_int32), ("reach", C.c_int32), ("axes", C.c_int32), ("scale", C.c_float), ("out_f32", C.c_int32)]
+
+
 MAX_PACK_SLICES = 112                   # MGN_MAX_PACK_SLICES
 _P, _I32, _I64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 _MLP = C.POINTER(MgnMlp)
+_ATT = C.POINTER(MgnAttn)
 
 # name -> (restype, argtypes); must list every symbol include/mgn_hip.h declares
 SIGNATURES = {
@@ -102,6 +112,10 @@ SIGNATURES = {
     "mgn_fps": (C.c_int, [_P, _I32, _P, _P, _P, _I32, _I64, _P, _P, _P]),
     "mgn_fps_workspace_floats": (_I64, [_I64]),
     "mgn_fps_single": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "mgn_attn_fwd_workspace_bytes": (_I64, [_ATT]),
+    "mgn_attn_fwd": (C.c_int, [_ATT, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
+    "mgn_attn_bwd_workspace_bytes": (_I64, [_ATT, _I32]),
+    "mgn_attn_bwd": (C.c_int, [_ATT, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P]),
     "mgn_knn_graph": (C.c_int, [_P, _I32, _P, _P, _P, _I32, _I64, _I32, _P, _P, _P]),
 }
 

@@ -1,0 +1,113 @@
+"""Attention of one set of states over another, with gradients: the fine nodes of a mesh reading the states of its coarse
+graph, a probe point reading the states of a mesh, ragged batches of both.
+
+    buckets = RelativeBuckets(32, reach=128, axes=2)
+    out = cross_attention(q, k, v, bias_table=table, bucket_lut=buckets.lut(q.device), q_pos=cells_q, k_pos=cells_k)
+
+``out_i = sum_j softmax_j(scale * <q_i, k_j> + bias_table[head, bucket]) v_j`` over the keys of query i's own segment.  The
+arithmetic runs in ``libmgn_hip.so`` (``ops.cross_attention``, ``ops.cross_attention_bwd``); torch.autograd carries the
+gradients of q, k, v and the bias table.
+
+The reference's coarse branch hands its states to the sampled nodes only (core/meshgraphnet.py:192-194: all other rows of
+the mapped-back tensor are zero); :class:`CrossScaleReadout` lets every fine node read all of them."""
+from __future__ import annotations
+
+import weakref
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from . import ops
+from ._lib import H
+
+
+class RelativeBuckets:
+    """Buckets of relative places for the learned bias of :func:`cross_attention`.
+
+    The first half of the buckets holds one distance each, the others are spaced evenly in the logarithm up to ``reach``;
+    everything further shares the last one.  ``axes`` 1: signed distances k - q on a line, half of the buckets for either
+    side; 2 or 3: the whole part of the Euclidean distance between lattice points.  Borders come from whole-number
+    comparisons, so no bucket depends on a rounding."""
+
+    def __init__(self, num_buckets: int, reach: int, axes: int = 1):
+        if axes not in (1, 2, 3) or not 1 <= reach <= 1024 or not 2 <= num_buckets <= 64 or (axes == 1 and (num_buckets % 2 or num_buckets < 4)):
+            raise ValueError("RelativeBuckets: axes 1 .. 3, reach 1 .. 1024, 2 .. 64 buckets (an even number of at least 4 on a line)")
+        self.num_buckets, self.reach, self.axes = num_buckets, reach, axes
+        n = num_buckets // 2 if axes == 1 else num_buckets
+        exact = max(1, n // 2)
+        line, b = [], exact
+        for d in range(reach + 1):
+            if d >= exact:
+                # (d / exact)^(n - exact) >= (reach / exact)^(b + 1 - exact), in whole numbers
+                while b + 1 < n and reach > exact and d ** (n - exact) * exact ** (b + 1 - exact) >= reach ** (b + 1 - exact) * exact ** (n - exact):
+                    b += 1
+            line.append(d if d < exact else b)
+        if axes == 1:
+            line = [line[-r] for r in range(-reach, 0)] + [line[0]] + [n + v for v in line[1:]]
+        self.table = torch.tensor(line, dtype=torch.int32)
+        self._by_dev = {}
+
+    def lut(self, device) -> torch.Tensor:
+        """Bucket of every place, int32 [2 * reach + 1] on a line, else [reach + 1]."""
+        key = str(device)
+        if key not in self._by_dev:
+            self._by_dev[key] = self.table.to(device)
+        return self._by_dev[key]
+
+
+class _Live:
+    """Stands for an eager autograd graph of this module that is still alive, with the leaves it accumulates into."""
+    alive: "weakref.WeakSet" = weakref.WeakSet()
+
+    def __init__(self, leaves):
+        self.leaves = leaves
+        _Live.alive.add(self)
+
+
+def _guard_capture(tensors):
+    """Leaves of a graph that is recorded into a HIP graph must not be held by an eager graph: their gradients would be
+    accumulated on the eager graph's stream, which is not being captured, and the process would end."""
+    leaves = tuple(id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf)
+    if not torch.cuda.is_current_stream_capturing():
+        return _Live(leaves)
+    for other in list(_Live.alive):
+        if set(other.leaves) & set(leaves):
+            raise RuntimeError("cross_attention: an eager result of the same leaves is still alive while a HIP graph is being captured; "
+                               "delete it first (its gradients would be accumulated outside the capture)")
+    return None
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias_table, q_ptr, k_ptr, key_mask, bucket_lut, q_pos, k_pos, scale):
+        stats = torch.empty(2, q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
+        out32 = None
+        if ctx.needs_input_grad[3] and q.dtype is not torch.float32:          # the table's gradient needs unrounded outputs
+            out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        out = ops.cross_attention(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale, stats=stats, out32=out32)
+        ctx.save_for_backward(q, k, v, bias_table, q_ptr, k_ptr, key_mask, bucket_lut, q_pos, k_pos, out if out32 is None else out32, stats)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, bias_table, q_ptr, k_ptr, key_mask, bucket_lut, q_pos, k_pos, out, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv, dt = ops.cross_attention_bwd(g, q, k, v, out, stats, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos,
+                                                 ctx.scale, table_grad=need[3])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dt) + (None,) * 7
+
+
+def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=None, bucket_lut=None, q_pos=None, k_pos=None,
+                    scale: Optional[float] = None):
+    """:func:`gnn_amd.ops.cross_attention` with gradients of ``q``, ``k``, ``v`` and ``bias_table`` where they are wanted."""
+    grads = (q, k, v, bias_table)
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in grads):
+        return ops.cross_attention(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
+    live = _guard_capture(grads)
+    out = _CrossAttention.apply(q, k, v, bias_table, q_ptr, k_ptr, key_mask, bucket_lut, q_pos, k_pos, scale)
+    if live is not None:
+        out.grad_fn.live = live
+    return out

@@ -1,0 +1,207 @@
+// Shared by the attention kernels (mgn_attn_fwd.hip, mgn_attn_bwd.hip, mgn_attn_few.hip).
+//
+//   o_i = sum_j p_ij v_j,   p_ij = exp(s_ij) / sum_j exp(s_ij),   s_ij = scale <q_i, k_j> + table[head][lut[place(i, j)]]
+//
+// over the keys j of query i's own segment that are not masked.  Scores are kept in base 2 (scale and bias times log2 e).
+//
+// Operand images.  The matrix instruction v_mfma_f32_32x32x16 takes, from lane (i = lane & 31, h = lane >> 5), eight
+// consecutive k values of row i.  Keys, values, queries and gradients are laid out once per call as the very 16 bytes each
+// lane will feed, in subtiles of 32 tokens of one head, so that the main kernels copy linear memory into LDS and read it
+// back linearly (no bank conflicts, no address arithmetic, no padding or masking left to do):
+//   image R (contraction over the head's width):  [plane][width / 16][lane][8],  element = x[token i][16 c + 8 h + e]
+//   image T (contraction over the 32 tokens):     [plane][2][width / 32][lane][8], element = x[token t(kc, h, e)][32 b + i]
+// with t = 16 kc + 4 h + e (e < 4), 16 kc + 8 + 4 h + e - 4 (e >= 4): the order in which a lane already holds the scores of
+// one column after a product (rows 8 g + 4 h + t), so probabilities go from one product into the next without a shuffle.
+// A segment's first subtile in an image is floor(first token / 32) + segment: no two segments share a subtile, and no table
+// of tile offsets is needed.  Rows past a segment's end and masked keys are zeros.
+//
+// Number formats.  bf16: operands as they are.  fp16: one plane, scaled per subtile by a power of two.  fp32: two fp16 planes
+// x = 2^e (h1 + h2) with the subtile's own e (residual 2^-22 of the value, 2^-39 of the subtile's largest magnitude), three
+// partial products per product.  The exponents go into constants that each product is multiplied with anyway.
+#pragma once
+#include "mgn_device.h"
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+enum { AT_BF16 = 0, AT_F16 = 1, AT_F32 = 2 };
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float F32_MOST = 3.402823466e38f;
+constexpr int TOP = 14;                 // operands are scaled to magnitudes below 2^TOP
+constexpr int FAR_EXP = -60;            // a subtile so much smaller than the largest adds nothing in fp16; its shift stops here
+constexpr int ATT_TQ = 128;             // queries (or keys, in the key-gradient kernel) of a workgroup: 32 per wave
+constexpr int ATT_MAX_REACH = 1024;
+constexpr int ATT_MAX_BUCKETS = 64;
+
+template <int KIND> constexpr int planes() { return KIND == AT_F32 ? 2 : 1; }
+
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+
+template <int KIND>
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (KIND == AT_BF16) return mfma32_bf16(a, b, c);
+    else return mfma32_f16(a, b, c);
+}
+
+template <int KIND>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+    const f32x2 v = {a, b};
+    if constexpr (KIND == AT_BF16) return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+    else return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+}
+
+// eight consecutive values as one operand (hi), and for two planes what is left of them (lo)
+template <int KIND, bool TWO = KIND == AT_F32>
+__device__ __forceinline__ void pack8(const float* v, u32x4& hi, u32x4& lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (KIND == AT_F32 || (KIND == AT_F16 && TWO)) {
+            unsigned a, b;
+            split2_pair(v[2 * i], v[2 * i + 1], a, b);
+            hi[i] = a; lo[i] = b;
+        } else if constexpr (TWO) {
+            const unsigned a = pack2<KIND>(v[2 * i], v[2 * i + 1]);
+            hi[i] = a;
+            lo[i] = pack2<KIND>(v[2 * i] - __uint_as_float(a << 16), v[2 * i + 1] - __uint_as_float(a & 0xffff0000u));
+        } else {
+            hi[i] = pack2<KIND>(v[2 * i], v[2 * i + 1]);
+        }
+    }
+}
+
+// eight consecutive elements of a row as floats; 16 bytes (32 for fp32), 16-byte aligned
+template <int KIND>
+__device__ __forceinline__ void load8(const void* base, long long off, float* v) {
+    if constexpr (KIND == AT_F32) {
+        const f32x4* p = (const f32x4*)((const float*)base + off);
+        const f32x4 a = p[0], b = p[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    } else {
+        const u32x4 a = *(const u32x4*)((const unsigned short*)base + off);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (KIND == AT_BF16) {
+                v[2 * i] = __uint_as_float(a[i] << 16);
+                v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+            } else {
+                const unsigned word = a[i];                   // a copy: a bit cast of the vector's element takes element 0
+                const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
+                v[2 * i] = f[0]; v[2 * i + 1] = f[1];
+            }
+        }
+    }
+}
+
+template <int KIND>
+__device__ __forceinline__ void store4(void* base, long long off, f32x4 v) {
+    if constexpr (KIND == AT_F32) *(f32x4*)((float*)base + off) = v;
+    else *(u32x2*)((unsigned short*)base + off) = u32x2{pack2<KIND>(v[0], v[1]), pack2<KIND>(v[2], v[3])};
+}
+
+// exponent that brings magnitudes up to `top` below 2^TOP (fp16 formats); infinities get the largest
+template <int KIND>
+__device__ __forceinline__ int scale_exp(float top) {
+    if constexpr (KIND == AT_BF16) return 0;
+    const int e = (int)((__float_as_uint(top) >> 23) & 0xff) - 127;
+    return top == 0.f ? -126 : min(max(e + 1 - TOP, -126), 114);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
+    return v;
+}
+
+__device__ __forceinline__ int attn_dp_device(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
+// ------------------------------------------------------------------------------------------------ segments
+// Offsets are clamped to [0, T] wherever they are read, so wrong ones give wrong results but no access out of bounds.
+__device__ __forceinline__ long long seg_at(const int* ptr, int s, int n_seg, long long T) {
+    if (!ptr) return s == 0 ? 0 : T;
+    const long long v = ptr[s];
+    return v < 0 ? 0 : v > T ? T : v;
+}
+
+struct Seg { int seg; int local; long long first; int len; };
+
+// segment and tile within it of tile `tile` when every segment s starts at tile floor(first / 2^shift) + s
+__device__ __forceinline__ Seg find_tile(const int* ptr, int n_seg, long long T, int shift, int tile) {
+    int lo = 0, hi = n_seg;                                   // the last s whose first tile is <= tile
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((seg_at(ptr, mid, n_seg, T) >> shift) + mid <= tile) lo = mid; else hi = mid;
+    }
+    Seg g;
+    g.seg = lo;
+    g.first = seg_at(ptr, lo, n_seg, T);
+    const long long end = seg_at(ptr, lo + 1, n_seg, T);
+    g.len = (int)(end > g.first ? end - g.first : 0);
+    g.local = tile - (int)((g.first >> shift) + lo);
+    return g;
+}
+
+// ------------------------------------------------------------------------------------------------ places and buckets
+// Index into the bucket table of the key at `k` seen from the query at `q`.
+//   line (one axis): k - q held to [-reach, reach], plus reach
+//   lattice (two or three axes): the whole part of the Euclidean distance, held to reach.  d2 = dx^2 + dy^2 + dz^2 is exact
+//   below 2^24 and only grows beyond, and sqrt(d2 + 1/2) lies at least 1/(4 reach) off every whole number for d2 <= reach^2:
+//   with reach <= 1024 that is 4 units in the last place, so the hardware root (1 ulp) gives the exact whole part.
+template <int BIAS>
+__device__ __forceinline__ int place(int qx, int qy, int qz, int kx, int ky, int kz, int axes, int reach, float most) {
+    if constexpr (BIAS == 1) {
+        return min(max(kx - qx, -reach), reach) + reach;
+    } else {
+        const float dx = (float)(kx - qx), dy = (float)(ky - qy);
+        float d2 = __builtin_fmaf(dx, dx, 0.5f);
+        d2 = __builtin_fmaf(dy, dy, d2);
+        if (axes == 3) { const float dz = (float)(kz - qz); d2 = __builtin_fmaf(dz, dz, d2); }
+        return (int)__builtin_amdgcn_sqrtf(fminf(d2, most));
+    }
+}
+
+__device__ __forceinline__ float bias_log2(float b) {          // finite biases stay finite in base 2
+    const float v = b * LOG2E;
+    return __builtin_isinf(b) ? v : fminf(fmaxf(v, -F32_MOST), F32_MOST);
+}
+
+// ------------------------------------------------------------------------------------------------ copies into LDS
+// 16 bytes per lane straight from memory into LDS (lane l's land at dst + 16 l); complete after the next workgroup barrier.
+__device__ __forceinline__ void copy16(const void* src, void* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+__device__ __forceinline__ void copy4(const void* src, void* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
+}
+__device__ __forceinline__ void barrier_all() {               // transfers into LDS have landed, then every wave meets
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------------------ operand images
+struct ImageJob {
+    const void* x; long long st, sh;             // rows: element strides of tokens and heads
+    const int* ptr; const uint8_t* mask;
+    long long T; int heads, n_sub, first_unit;   // n_sub: subtiles of a head; units of this job start at first_unit
+    unsigned short* R; unsigned short* Tt;       // images (either may be null)
+    int* ex; int* valid;                         // exponent of (head, subtile), 4 ints apart; valid bits of the tokens
+    const int* pos; int* pos_out; int axes;      // places [T][axes] -> [subtile][axes][32]
+    const void* o; long long o_st, o_sh;         // gradient job: the outputs (fp32 or the type of the rows), ...
+    int o_f32;
+    int alternate;                               // negate odd subtiles (see mgn_attn_bwd.hip)
+    const float* stats; float* rows;             // rows: [head][subtile][3][32] = maximum, 1/sum (fp32: 1), <do, o> (fp32: / sum)
+};
+struct ImageArgs { ImageJob job[4]; int n_job, units, n_seg, dim; };
+
+}  // namespace
+
+int mgn_attn_launch_images(int kind, int dp, const void* args, void* stream);     // mgn_attn_fwd.hip

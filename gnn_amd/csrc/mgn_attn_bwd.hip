@@ -1,0 +1,540 @@
+// Attention of one set of states over another, backwards.  With P the probabilities and dO the output's gradient:
+//   dV = P^T dO,  dP = dO V^T,  dS = P o (dP - <dO_i, o_i>),  dQ = scale dS K,  dK = scale dS^T Q,
+//   dtable[head][b] = sum of dS over the pairs in bucket b.
+// P is recomputed from the scores and the row statistics of the forward pass.  Two kernels, one that owns queries (dQ and the
+// table) and one that owns keys (dK, dV): seven products instead of the five that are needed, but no atomics, so every sum has
+// a fixed order and two runs agree bit for bit.
+//
+// The table's gradient sums dS over very many pairs, and every row of dS sums to zero: an error that all entries share grows
+// with their number where the sum itself cancels.  Two such errors are kept out.  The fp16 matrix instruction rounds its sums
+// downwards, so dP comes out low everywhere (a 1e-5 error of the table at 20 000 queries): the values' images of odd subtiles
+// are negated, dP of those comes out high, and what is left has either sign (3e-7).  And <dO_i, o_i> has to be made of outputs
+// that were not rounded to 16 bits: the forward pass keeps them in fp32 where a table is trained (out32).
+#include "mgn_attn_host.h"
+
+namespace {
+
+struct AttnBwd {
+    const int *q_ptr, *k_ptr; long long n_q, n_k; int n_seg, heads, kv_heads, dim; float c0, scale;
+    const unsigned short *q_r, *q_t, *g_r, *g_t;       // images of queries and output gradients, [heads][ns_q]
+    const unsigned short *k_r, *k_t, *v_r;             // images of keys and values, [kv_heads][ns_k]
+    const i32x4 *rec_q, *rec_k;                        // exponents {q, g} and {k, v, valid keys}
+    const float* rows;                                 // [heads][ns_q][3][32]
+    int ns_q, ns_k;
+    const int *qpos, *kpos;                            // places [subtile][axes][32]
+    const float* table; const int* lut; int n_bucket, reach, axes;
+    void *dq, *dk, *dv;                                // dense [tokens][heads][dim]
+    double* tpart; float* dtable; int q_tiles;         // [q_tiles][heads][n_bucket]
+    int splits; float* part;                           // [split][2][kv_heads][ns_k][32][DP]
+};
+
+constexpr int PSHIFT = 13;
+
+// ------------------------------------------------------------------------------------------------ query side
+template <int KIND, int DP, int BIAS>
+__global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void attn_dq_kernel(AttnBwd a) {
+    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
+    // fp32 at width 128 with a table: the sums by bucket take up to 64 KB, so the values are read past LDS
+    constexpr int IMAGES = KIND == AT_F32 && DP == 128 && BIAS > 0 ? 2 : 3;
+    __shared__ __attribute__((aligned(1024))) unsigned short buf[2][IMAGES * SUB];     // K as R, K as T, V as R
+    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 2 : 1][BIAS ? 128 : 1];
+    __shared__ unsigned char lutb[BIAS ? 2 * ATT_MAX_REACH + 1 : 1];
+    __shared__ float tab[BIAS ? ATT_MAX_BUCKETS : 1];
+    extern __shared__ float hist[];                                                    // [4 waves][n_bucket][64], with a table gradient
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), tile = blockIdx.x / a.heads;
+    const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 7, tile);
+    const bool live = g.local >= 0 && g.local * ATT_TQ < g.len;
+    if (!live) {
+        if (BIAS > 0 && a.tpart && t < a.n_bucket) a.tpart[((long long)tile * a.heads + head) * a.n_bucket + t] = 0.0;
+        return;
+    }
+    const long long k0 = seg_at(a.k_ptr, g.seg, a.n_seg, a.n_k), k1 = seg_at(a.k_ptr, g.seg + 1, a.n_seg, a.n_k);
+    const int n_sub = k1 > k0 ? (int)((k1 - k0 + 31) >> 5) : 0;
+    const long long ksub = (long long)kvh * a.ns_k + (k0 >> 5) + g.seg;
+    const i32x4* rec = a.rec_k + ksub;
+    const int qi = g.local * ATT_TQ + 32 * w + j, nsq = (g.len + 31) >> 5;
+    const bool mine = qi < g.len;
+    const long long row = g.first + min(qi, g.len - 1);
+    const long long qsub = (long long)head * a.ns_q + (g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1);
+
+    auto stage = [&](int b, int s) {
+        constexpr int BYTES = SUB * 2;
+        const char* src[3] = {(const char*)(a.k_r + (ksub + s) * SUB), (const char*)(a.k_t + (ksub + s) * SUB), (const char*)(a.v_r + (ksub + s) * SUB)};
+#pragma unroll
+        for (int n = 0; n < IMAGES * BYTES; n += 4096) {
+            const int off = n + w * 1024;
+            if (off < IMAGES * BYTES) copy16(src[off / BYTES] + off % BYTES + lane * 16, (char*)buf[b] + off);
+        }
+        if constexpr (BIAS > 0)
+            if (w == 3)
+                for (int ax = 0; ax < a.axes; ax += 2)
+                    if (ax * 32 + lane < a.axes * 32)
+                        copy4(a.kpos + (((k0 >> 5) + g.seg + s) * a.axes + ax) * 32 + lane, pbuf[b] + 32 * ax);
+    };
+    if (n_sub > 0) stage(0, 0);
+
+    u32x4 qf[PL][NC], gf[PL][NC];
+    {
+        const u32x4 *qp = (const u32x4*)(a.q_r + qsub * SUB) + lane, *gp = (const u32x4*)(a.g_r + qsub * SUB) + lane;
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) { qf[p][c] = qp[(p * NC + c) * 64]; gf[p][c] = gp[(p * NC + c) * 64]; }
+    }
+    const i32x4 rq = a.rec_q[qsub];
+    const float* rp = a.rows + qsub * 96;
+    const float m = mine ? rp[j] : __builtin_inff(), norm = rp[32 + j], delta = mine ? rp[64 + j] : 0.f;
+    int qx = 0, qy = 0, qz = 0;
+    float most = 0.f;
+    if constexpr (BIAS > 0) {
+        const int* p = a.qpos + ((g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1)) * (long long)a.axes * 32 + j;
+        qx = p[0];
+        if (a.axes > 1) qy = p[32];
+        if (a.axes > 2) qz = p[64];
+        most = (float)(a.reach * a.reach) + 0.5f;
+        const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
+        for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
+        if (t < a.n_bucket) tab[t] = bias_log2(a.table[head * a.n_bucket + t]);
+        if (a.tpart)
+            for (int r = t; r < a.n_bucket * 256; r += 256) hist[r] = 0.f;
+    }
+    int ek = 0, ev = 0;                                       // common exponents of this segment's keys and values
+    if constexpr (KIND != AT_BF16) {
+        ek = ev = -126;
+        for (int s = lane; s < n_sub; s += 64) { const i32x4 r = rec[s]; ek = max(ek, r[0]); ev = max(ev, r[1]); }
+        ek = wave_max_i(ek); ev = wave_max_i(ev);
+    }
+    // unit of dS in the second product: |dP - delta| < 2^(2 TOP + log2 width + 1) in units of the operands, held below 2^15
+    const int unit = KIND == AT_BF16 ? 0 : min(max(rq[1] + ev + 2 * TOP + LOG_DP - 14, -126), 126);
+    const float down = KIND == AT_BF16 ? norm : norm * pow2i(-unit);
+    float* sums = hist + w * a.n_bucket * 64 + lane;           // this lane's sums of dS by bucket
+
+    f32x16 dq[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) dq[b] = zero16();
+    barrier_all();
+    for (int sub = 0; sub < n_sub; ++sub) {
+        const int b = sub & 1;
+        if (sub + 1 < n_sub) stage(b ^ 1, sub + 1);
+        const i32x4 r = rec[sub];
+        const u32x4 *kr = (const u32x4*)buf[b] + lane, *kt = (const u32x4*)(buf[b] + SUB) + lane, *vr = IMAGES == 3 ? (const u32x4*)(buf[b] + 2 * SUB) + lane : (const u32x4*)(a.v_r + (ksub + sub) * SUB) + lane;
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if constexpr (PL == 2) {
+                s = mma<KIND>(kr[(NC + c) * 64], qf[0][c], s);
+                dp = mma<KIND>(vr[(NC + c) * 64], gf[0][c], dp);
+                s = mma<KIND>(kr[c * 64], qf[PL - 1][c], s);
+                dp = mma<KIND>(vr[c * 64], gf[PL - 1][c], dp);
+            }
+            s = mma<KIND>(kr[c * 64], qf[0][c], s);
+            dp = mma<KIND>(vr[c * 64], gf[0][c], dp);
+        }
+        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r[0]) * pow2i(rq[0]);
+        const int sh = KIND == AT_BF16 ? 0 : max(r[0] - ek, FAR_EXP);
+        const float up = KIND == AT_BF16 ? 1.f : sub & 1 ? -pow2i(r[1] + rq[1]) : pow2i(r[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
+        const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
+        const unsigned valid = (unsigned)r[2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            int bk[4] = {0, 0, 0, 0};
+            if constexpr (BIAS > 0) {
+                const int* p = pbuf[b] + 8 * q + 4 * h;
+                const i32x4 x = *(const i32x4*)p, y = a.axes > 1 ? *(const i32x4*)(p + 32) : x, z = a.axes > 2 ? *(const i32x4*)(p + 64) : x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.axes, a.reach, most)];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = 4 * q + e;
+                float x = s[n] * c;
+                if constexpr (BIAS > 0) x = __builtin_fmaf(s[n], c, tab[bk[e]]);
+                float pe = __builtin_amdgcn_exp2f(x - m);
+                if (valid != 0xffffffffu) pe = (valid >> (8 * q + 4 * h + e) & 1) ? pe : 0.f;
+                const float d = KIND == AT_BF16 ? dp[n] - delta : __builtin_fmaf(dp[n], up, -delta);
+                s[n] = pe * dn * d;
+                if constexpr (BIAS > 0)
+                    if (a.tpart) sums[bk[e] * 64] += s[n] * whole;
+            }
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = s[8 * kc + e];
+            u32x4 hi, lo;
+            pack8<KIND>(v, hi, lo);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if constexpr (PL == 2) {
+                    dq[n] = mma<KIND>(kt[((2 + kc) * NB + n) * 64], hi, dq[n]);
+                    dq[n] = mma<KIND>(kt[(kc * NB + n) * 64], lo, dq[n]);
+                }
+                dq[n] = mma<KIND>(kt[(kc * NB + n) * 64], hi, dq[n]);
+            }
+        }
+        barrier_all();
+    }
+    if (mine) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = 32 * n + 8 * q + 4 * h;
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? dq[n][4 * q + e] * a.scale : ldexpf(dq[n][4 * q + e] * a.scale, unit + ek);
+                if (d < a.dim) store4<KIND>(a.dq, (row * a.heads + head) * a.dim + d, v);
+            }
+    }
+    if constexpr (BIAS > 0) {
+        if (a.tpart) {
+            __syncthreads();
+            for (int b = w; b < a.n_bucket; b += 4) {          // one wave sums a bucket's 256 columns, in a fixed order
+                double v = 0.0;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v += (double)hist[(x * a.n_bucket + b) * 64 + lane];
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) v += __shfl_down(v, o);
+                if (lane == 0) a.tpart[((long long)tile * a.heads + head) * a.n_bucket + b] = v;
+            }
+        }
+    }
+}
+
+// dtable[head][b] = sum over the query tiles, one wave per entry, fixed order
+__global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict__ part, float* __restrict__ out, int tiles, int entries) {
+    const int e = blockIdx.x, lane = threadIdx.x;
+    double v = 0.0;
+    for (int i = lane; i < tiles; i += 64) v += part[(long long)i * entries + e];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_down(v, o);
+    if (lane == 0) out[e] = (float)v;
+}
+
+// ------------------------------------------------------------------------------------------------ key side
+// A workgroup: 128 keys of one key head, 32 per wave, against its share of the (query head, query subtile) pairs that read
+// them.  Here the lane owns a key: rows of the products are queries, whose statistics come through LDS.
+template <int KIND, int DP, int BIAS>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
+    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
+    __shared__ __attribute__((aligned(1024))) unsigned short buf[2][4 * SUB];          // Q as R, Q as T, dO as R, dO as T
+    __shared__ __attribute__((aligned(16))) float rbuf[2][128];
+    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 2 : 1][BIAS ? 128 : 1];
+    __shared__ unsigned char lutb[BIAS ? 2 * ATT_MAX_REACH + 1 : 1];
+    extern __shared__ float tab[];                                                     // [heads per key head][n_bucket], with a bias
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x % a.kv_heads, rep = a.heads / a.kv_heads, split = blockIdx.y;
+    const Seg g = find_tile(a.k_ptr, a.n_seg, a.n_k, 7, blockIdx.x / a.kv_heads);
+    if (g.local < 0 || g.local * ATT_TQ >= g.len) return;
+    const long long q0 = seg_at(a.q_ptr, g.seg, a.n_seg, a.n_q), q1 = seg_at(a.q_ptr, g.seg + 1, a.n_seg, a.n_q);
+    const int n_sub = q1 > q0 ? (int)((q1 - q0 + 31) >> 5) : 0, items = n_sub * rep;
+    const int per = (items + a.splits - 1) / a.splits, i0 = min(split * per, items), i1 = min(i0 + per, items);
+    const long long qbase = (q0 >> 5) + g.seg, head0 = (long long)kvh * rep;
+    const int ki = g.local * ATT_TQ + 32 * w + j, nsk = (g.len + 31) >> 5, wsub = min(g.local * 4 + w, nsk - 1);
+    const long long kplace = (g.first >> 5) + g.seg + wsub, ksub = (long long)kvh * a.ns_k + kplace;
+
+    auto qsub_of = [&](int item) { return (head0 + item / n_sub) * a.ns_q + qbase + item % n_sub; };
+    auto stage = [&](int b, int item) {
+        constexpr int BYTES = SUB * 2;
+        const long long s = qsub_of(item);
+        const char* src[4] = {(const char*)(a.q_r + s * SUB), (const char*)(a.q_t + s * SUB), (const char*)(a.g_r + s * SUB), (const char*)(a.g_t + s * SUB)};
+#pragma unroll
+        for (int n = 0; n < 4 * BYTES; n += 4096) {
+            const int off = n + w * 1024;
+            copy16(src[off / BYTES] + off % BYTES + lane * 16, (char*)buf[b] + off);
+        }
+        if (w < 2 && w * 64 + lane < 96) copy4(a.rows + s * 96 + w * 64 + lane, rbuf[b] + w * 64);
+        if constexpr (BIAS > 0)
+            if (w == 3)
+                for (int ax = 0; ax < a.axes; ax += 2)
+                    if (ax * 32 + lane < a.axes * 32)
+                        copy4(a.qpos + ((qbase + item % n_sub) * a.axes + ax) * 32 + lane, pbuf[b] + 32 * ax);
+    };
+    if (i0 < i1) stage(0, i0);
+
+    u32x4 kf[PL][NC], vf[PL][NC];
+    {
+        const u32x4 *kp = (const u32x4*)(a.k_r + ksub * SUB) + lane, *vp = (const u32x4*)(a.v_r + ksub * SUB) + lane;
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) { kf[p][c] = kp[(p * NC + c) * 64]; vf[p][c] = vp[(p * NC + c) * 64]; }
+    }
+    const i32x4 rk = a.rec_k[ksub];
+    int kx = 0, ky = 0, kz = 0;
+    float most = 0.f;
+    if constexpr (BIAS > 0) {
+        const int* p = a.kpos + kplace * a.axes * 32 + j;
+        kx = p[0];
+        if (a.axes > 1) ky = p[32];
+        if (a.axes > 2) kz = p[64];
+        most = (float)(a.reach * a.reach) + 0.5f;
+        const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
+        for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
+        for (int r = t; r < rep * a.n_bucket; r += 256) tab[r] = bias_log2(a.table[head0 * a.n_bucket + r]);
+    }
+    int eq = 0, eg = 0;                                       // common exponents of the queries and gradients in this range
+    if constexpr (KIND != AT_BF16) {
+        eq = eg = -126;
+        for (int i = i0 + lane; i < i1; i += 64) { const i32x4 r = a.rec_q[qsub_of(i)]; eq = max(eq, r[0]); eg = max(eg, r[1]); }
+        eq = wave_max_i(eq); eg = wave_max_i(eg);
+    }
+    const int unit = KIND == AT_BF16 ? 0 : min(max(rk[1] + eg + 2 * TOP + LOG_DP - 14, -126), 126);
+
+    f32x16 dk[NB], dv[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) { dk[b] = zero16(); dv[b] = zero16(); }
+    barrier_all();
+    for (int item = i0; item < i1; ++item) {
+        const int b = (item - i0) & 1;
+        if (item + 1 < i1) stage(b ^ 1, item + 1);
+        const i32x4 r = a.rec_q[qsub_of(item)];
+        const u32x4 *qr = (const u32x4*)buf[b] + lane, *qt = (const u32x4*)(buf[b] + SUB) + lane;
+        const u32x4 *gr = (const u32x4*)(buf[b] + 2 * SUB) + lane, *gt = (const u32x4*)(buf[b] + 3 * SUB) + lane;
+        f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if constexpr (PL == 2) {
+                s = mma<KIND>(qr[(NC + c) * 64], kf[0][c], s);
+                dp = mma<KIND>(gr[(NC + c) * 64], vf[0][c], dp);
+                s = mma<KIND>(qr[c * 64], kf[PL - 1][c], s);
+                dp = mma<KIND>(gr[c * 64], vf[PL - 1][c], dp);
+            }
+            s = mma<KIND>(qr[c * 64], kf[0][c], s);
+            dp = mma<KIND>(gr[c * 64], vf[0][c], dp);
+        }
+        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r[0]) * pow2i(rk[0]);
+        const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r[1] + rk[1]) : pow2i(r[1] + rk[1]);
+        const float fp = KIND == AT_BF16 ? 1.f : pow2i(PSHIFT + max(r[1] - eg, FAR_EXP));              // of P in the product with dO
+        const float fs = KIND == AT_BF16 ? 1.f : pow2i(max(r[0] - eq, FAR_EXP) - unit);               // of dS in the product with Q
+        const float* tb = tab + (item / max(n_sub, 1)) * a.n_bucket;
+        f32x16 p;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float* rr = rbuf[b] + 8 * q + 4 * h;
+            const f32x4 m = *(const f32x4*)rr, norm = *(const f32x4*)(rr + 32), delta = *(const f32x4*)(rr + 64);
+            int bk[4] = {0, 0, 0, 0};
+            if constexpr (BIAS > 0) {
+                const int* pp = pbuf[b] + 8 * q + 4 * h;
+                const i32x4 x = *(const i32x4*)pp, y = a.axes > 1 ? *(const i32x4*)(pp + 32) : x, z = a.axes > 2 ? *(const i32x4*)(pp + 64) : x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(x[e], y[e], z[e], kx, ky, kz, a.axes, a.reach, most)];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = 4 * q + e;
+                float x = s[n] * c;
+                if constexpr (BIAS > 0) x = __builtin_fmaf(s[n], c, tb[bk[e]]);
+                float pe = __builtin_amdgcn_exp2f(x - m[e]);
+                if constexpr (KIND != AT_F32) pe *= norm[e];
+                const float d = KIND == AT_BF16 ? dp[n] - delta[e] : __builtin_fmaf(dp[n], up, -delta[e]);
+                s[n] = KIND == AT_BF16 ? pe * d : (pe * fs) * d;
+                p[n] = KIND == AT_BF16 ? pe : pe * fp;
+            }
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            float v[8];
+            u32x4 phi, plo, shi, slo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = p[8 * kc + e];
+            pack8<KIND>(v, phi, plo);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = s[8 * kc + e];
+            pack8<KIND>(v, shi, slo);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if constexpr (PL == 2) {
+                    dv[n] = mma<KIND>(gt[((2 + kc) * NB + n) * 64], phi, dv[n]);
+                    dk[n] = mma<KIND>(qt[((2 + kc) * NB + n) * 64], shi, dk[n]);
+                    dv[n] = mma<KIND>(gt[(kc * NB + n) * 64], plo, dv[n]);
+                    dk[n] = mma<KIND>(qt[(kc * NB + n) * 64], slo, dk[n]);
+                }
+                dv[n] = mma<KIND>(gt[(kc * NB + n) * 64], phi, dv[n]);
+                dk[n] = mma<KIND>(qt[(kc * NB + n) * 64], shi, dk[n]);
+            }
+        }
+        barrier_all();
+    }
+    if (ki >= g.len) return;
+    const bool keep = (unsigned)rk[2] >> j & 1;                // a masked key has no gradient
+    const long long row = g.first + ki;
+    float* part = a.part + ((long long)split * 2 * a.kv_heads * a.ns_k + ksub) * 32 * DP + j * DP;
+    const long long vpart = (long long)a.kv_heads * a.ns_k * 32 * DP;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * n + 8 * q + 4 * h;
+            if (d >= a.dim) continue;
+            f32x4 vk, vv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = dk[n][4 * q + e] * a.scale, y = dv[n][4 * q + e];
+                vk[e] = !keep ? 0.f : KIND == AT_BF16 ? x : ldexpf(x, unit + eq);
+                vv[e] = !keep ? 0.f : KIND == AT_BF16 ? y : ldexpf(y, eg - PSHIFT);
+            }
+            if (a.splits > 1) {
+                *(f32x4*)(part + d) = vk; *(f32x4*)(part + vpart + d) = vv;
+            } else {
+                store4<KIND>(a.dk, (row * a.kv_heads + kvh) * a.dim + d, vk);
+                store4<KIND>(a.dv, (row * a.kv_heads + kvh) * a.dim + d, vv);
+            }
+        }
+}
+
+// dK, dV of a key = sum over the splits, in order; one thread per four values
+template <int KIND>
+__global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a, int dp) {
+    const int quads = a.dim / 4;
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x, units = (long long)a.kv_heads * a.ns_k;
+    if (item >= units * 32 * quads) return;
+    const int quad = (int)(item % quads), i = (int)(item / quads % 32);
+    const long long unit = item / quads / 32;
+    const int kvh = (int)(unit / a.ns_k), sub = (int)(unit % a.ns_k);
+    const Seg g = find_tile(a.k_ptr, a.n_seg, a.n_k, 5, sub);
+    if (g.local < 0 || g.local * 32 + i >= g.len) return;
+    const float* p = a.part + (unit * 32 + i) * dp + 4 * quad;
+    f32x4 k = {0.f, 0.f, 0.f, 0.f}, v = k;
+    for (int s = 0; s < a.splits; ++s) {
+        k += *(const f32x4*)(p + (long long)(2 * s) * units * 32 * dp);
+        v += *(const f32x4*)(p + (long long)(2 * s + 1) * units * 32 * dp);
+    }
+    const long long at = ((g.first + g.local * 32 + i) * a.kv_heads + kvh) * a.dim + 4 * quad;
+    store4<KIND>(a.dk, at, k);
+    store4<KIND>(a.dv, at, v);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct BwdSpace { size_t q_r, q_t, g_r, g_t, k_r, k_t, v_r, rec_q, rec_k, rows, qpos, kpos, tpart, part, total; int ns_q, ns_k, q_tiles, k_tiles, splits; };
+
+BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
+    BwdSpace s{};
+    const int dp = attn_dp(a.dim), pl = a.dtype == MGN_F32 ? 2 : 1;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) & ~(size_t)255; return p; };
+    s.ns_q = attn_subtiles(a.n_q, a.n_seg); s.ns_k = attn_subtiles(a.n_k, a.n_seg);
+    s.q_tiles = (int)(a.n_q / ATT_TQ) + a.n_seg; s.k_tiles = (int)(a.n_k / ATT_TQ) + a.n_seg;
+    // workgroups of the key side: about four per compute unit, in shares of at least four query subtiles
+    const int64_t blocks = (int64_t)s.k_tiles * a.kv_heads, items = (a.n_q / 32 / a.n_seg + 1) * (a.heads / a.kv_heads);
+    int64_t sp = blocks > 0 ? 1024 / blocks : 1;
+    if (sp > items / 4) sp = items / 4;
+    s.splits = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
+    const size_t qi = (size_t)a.heads * s.ns_q * pl * 64 * dp, ki = (size_t)a.kv_heads * s.ns_k * pl * 64 * dp;
+    s.q_r = take(qi); s.q_t = take(qi); s.g_r = take(qi); s.g_t = take(qi);
+    s.k_r = take(ki); s.k_t = take(ki); s.v_r = take(ki);
+    s.rec_q = take((size_t)a.heads * s.ns_q * 16); s.rec_k = take((size_t)a.kv_heads * s.ns_k * 16);
+    s.rows = take((size_t)a.heads * s.ns_q * 96 * 4);
+    if (a.bias_table) { s.qpos = take((size_t)s.ns_q * a.axes * 128); s.kpos = take((size_t)s.ns_k * a.axes * 128); }
+    if (table_grad) s.tpart = take((size_t)s.q_tiles * a.heads * a.n_bucket * 8);
+    if (s.splits > 1) s.part = take((size_t)s.splits * 2 * a.kv_heads * s.ns_k * 32 * dp * 4);
+    s.total = at;
+    return s;
+}
+
+// Whether the kernel fits the 160 KB of LDS with this much dynamic memory, which beyond 64 KB has to be asked for.  A launch
+// that does not fit is never made: it would end the process's queue, not return an error.
+template <typename K>
+bool lds_fits(K kernel, int dynamic) {
+    if (dynamic == 0) return true;
+    hipFuncAttributes at;
+    if (hipFuncGetAttributes(&at, (const void*)kernel) != hipSuccess || at.sharedSizeBytes + (size_t)dynamic > 160 * 1024) return false;
+    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, dynamic) == hipSuccess;
+}
+
+template <int KIND, int DP, int BIAS>
+bool bwd_launch(const AttnBwd& b, const BwdSpace& s, hipStream_t st) {
+    const int hist = BIAS > 0 && b.tpart ? b.n_bucket * 1024 : 0, tab = BIAS > 0 ? b.heads / b.kv_heads * b.n_bucket * 4 : 0;
+    if (!lds_fits(attn_dq_kernel<KIND, DP, BIAS>, hist) || !lds_fits(attn_dkv_kernel<KIND, DP, BIAS>, tab)) return false;
+    hipLaunchKernelGGL((attn_dq_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.q_tiles * b.heads)), dim3(256), hist, st, b);
+    if (b.n_k > 0) hipLaunchKernelGGL((attn_dkv_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.k_tiles * b.kv_heads), (unsigned)s.splits), dim3(256), tab, st, b);
+    return true;
+}
+template <int KIND, int DP>
+bool bwd_bias(const AttnBwd& b, const BwdSpace& s, int bias, hipStream_t st) {
+    if (bias == 0) return bwd_launch<KIND, DP, 0>(b, s, st);
+    if (bias == 1) return bwd_launch<KIND, DP, 1>(b, s, st);
+    return bwd_launch<KIND, DP, 2>(b, s, st);
+}
+template <int KIND>
+bool bwd_kind(const AttnBwd& b, const BwdSpace& s, int dp, int bias, hipStream_t st) {
+    const bool fits = dp == 32 ? bwd_bias<KIND, 32>(b, s, bias, st) : dp == 64 ? bwd_bias<KIND, 64>(b, s, bias, st) : bwd_bias<KIND, 128>(b, s, bias, st);
+    if (!fits) return false;
+    if (s.splits > 1) {
+        const long long items = (long long)b.kv_heads * s.ns_k * 32 * (b.dim / 4);
+        hipLaunchKernelGGL((attn_dkv_sum_kernel<KIND>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, b, dp);
+    }
+    return true;
+}
+
+}  // namespace
+
+extern "C" int64_t mgn_attn_bwd_workspace_bytes(const MgnAttn* a, int32_t table_grad) {
+    if (attn_check(a, "mgn_attn_bwd_workspace_bytes") != 0) return -1;
+    return (int64_t)bwd_space(*a, table_grad && a->bias_table).total;
+}
+
+extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int64_t g_sh, const void* out, int64_t out_st,
+                            int64_t out_sh, const float* stats, void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    if (const int rc = attn_check(ap, "mgn_attn_bwd")) return rc;
+    const MgnAttn& a = *ap;
+    const char* bad = nullptr;
+    const BwdSpace s = bwd_space(a, dtable != nullptr);
+    if (a.n_q > 0 && (!g || !out || !stats || !dq)) bad = "null operand";
+    else if (a.n_k > 0 && (!dk || !dv)) bad = "null key or value gradient";
+    else if (dtable && !a.bias_table) bad = "a table gradient without a table";
+    else if (a.n_q > 0 && (attn_bad_rows(g, g_st, g_sh, a.dtype) || attn_bad_rows(out, out_st, out_sh, a.out_f32 ? MGN_F32 : a.dtype))) bad = "rows must start on 16-byte borders";
+    else if (((uintptr_t)dq & 15) || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15)) bad = "gradients must start on 16-byte borders";
+    else if (!workspace || workspace_bytes < (int64_t)s.total) bad = "the workspace is missing or too small";
+    else if (a.bias_table && a.heads / a.kv_heads * a.n_bucket > 4096) bad = "more than 4096 table entries per key head";
+    if (bad) { mgn_set_error("mgn_attn_bwd: %s", bad); return MGN_E_ARG; }
+    char* ws = (char*)workspace;
+    const int kind = attn_kind(a.dtype), dp = attn_dp(a.dim), bias = attn_bias(a);
+    const hipStream_t st = (hipStream_t)stream;
+    auto half = [&](size_t at) { return (unsigned short*)(ws + at); };
+    int *rec_q = (int*)(ws + s.rec_q), *rec_k = (int*)(ws + s.rec_k);
+    ImageArgs im{};
+    im.n_seg = a.n_seg; im.dim = a.dim;
+    int units = 0;
+    auto add = [&](const void* x, long long xst, long long xsh, bool query) -> ImageJob& {
+        ImageJob& jb = im.job[im.n_job++];
+        jb.x = x; jb.st = xst; jb.sh = xsh; jb.ptr = query ? a.q_ptr : a.k_ptr; jb.T = query ? a.n_q : a.n_k;
+        jb.heads = query ? a.heads : a.kv_heads; jb.n_sub = query ? s.ns_q : s.ns_k; jb.axes = a.axes;
+        jb.first_unit = units; units += jb.heads * jb.n_sub;
+        if (!query) jb.mask = a.key_mask;
+        return jb;
+    };
+    if (a.n_q > 0) {
+        ImageJob& q = add(a.q, a.q_st, a.q_sh, true);
+        q.R = half(s.q_r); q.Tt = half(s.q_t); q.ex = rec_q; q.pos = bias ? a.q_pos : nullptr; q.pos_out = (int*)(ws + s.qpos);
+        ImageJob& o = add(g, g_st, g_sh, true);
+        o.R = half(s.g_r); o.Tt = half(s.g_t); o.ex = rec_q + 1; o.o = out; o.o_f32 = a.out_f32 || a.dtype == MGN_F32; o.o_st = out_st; o.o_sh = out_sh; o.stats = stats; o.rows = (float*)(ws + s.rows);
+    }
+    if (a.n_k > 0) {
+        ImageJob& k = add(a.k, a.k_st, a.k_sh, false);
+        k.R = half(s.k_r); k.Tt = half(s.k_t); k.ex = rec_k; k.valid = rec_k + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = (int*)(ws + s.kpos);
+        ImageJob& v = add(a.v, a.v_st, a.v_sh, false);
+        v.R = half(s.v_r); v.ex = rec_k + 1; v.alternate = kind != AT_BF16;
+    }
+    im.units = units;
+    if (units > 0) mgn_attn_launch_images(kind, dp, &im, stream);
+    AttnBwd b{};
+    b.q_ptr = a.q_ptr; b.k_ptr = a.k_ptr; b.n_q = a.n_q; b.n_k = a.n_k; b.n_seg = a.n_seg; b.heads = a.heads; b.kv_heads = a.kv_heads; b.dim = a.dim;
+    b.c0 = a.scale * LOG2E; b.scale = a.scale;
+    b.q_r = half(s.q_r); b.q_t = half(s.q_t); b.g_r = half(s.g_r); b.g_t = half(s.g_t); b.k_r = half(s.k_r); b.k_t = half(s.k_t); b.v_r = half(s.v_r);
+    b.rec_q = (const i32x4*)rec_q; b.rec_k = (const i32x4*)rec_k; b.rows = (const float*)(ws + s.rows); b.ns_q = s.ns_q; b.ns_k = s.ns_k;
+    b.qpos = (const int*)(ws + s.qpos); b.kpos = (const int*)(ws + s.kpos);
+    b.table = a.bias_table; b.lut = a.bucket_lut; b.n_bucket = a.n_bucket; b.reach = a.reach; b.axes = a.axes;
+    b.dq = dq; b.dk = dk; b.dv = dv; b.dtable = dtable; b.tpart = dtable ? (double*)(ws + s.tpart) : nullptr; b.q_tiles = s.q_tiles;
+    b.splits = s.splits; b.part = (float*)(ws + s.part);
+    const bool fits = kind == AT_BF16 ? bwd_kind<AT_BF16>(b, s, dp, bias, st) : kind == AT_F16 ? bwd_kind<AT_F16>(b, s, dp, bias, st)
+                                                                                           : bwd_kind<AT_F32>(b, s, dp, bias, st);
+    if (!fits) { mgn_set_error("mgn_attn_bwd: %d buckets at width %d do not fit the compute unit's local memory", a.n_bucket, a.dim); return MGN_E_ARG; }
+    if (dtable) hipLaunchKernelGGL(attn_table_kernel, dim3((unsigned)(a.heads * a.n_bucket)), dim3(64), 0, st, b.tpart, dtable, s.q_tiles, a.heads * a.n_bucket);
+    return check_launch("mgn_attn_bwd");
+}

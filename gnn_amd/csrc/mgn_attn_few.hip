@@ -1,0 +1,194 @@
+// Attention with few queries per segment (a probe point, one step of a stream): keys and values are read once, where they
+// lie, in whole rows, and all arithmetic is fp32.
+//
+// Memory bound: bytes = keys x (key + value row).  A workgroup takes one query token, up to eight query heads that share a
+// key head, and one piece of the keys; LPR lanes share a row (8 elements each), so a wave has 64 / LPR rows in flight per
+// load and four loads of keys and four of values outstanding.  Every row group keeps its own running maximum and sum, joined
+// over the wave by exchanges and over the waves through LDS; pieces are joined by attn_join_kernel in a fixed order.
+#include "mgn_attn_host.h"
+
+namespace {
+
+template <int KIND, int LPR, int REP>
+__global__ __launch_bounds__(256) void attn_few_kernel(AttnFwd a) {
+    constexpr int RPW = 64 / LPR, U = 4;
+    __shared__ float joined[4][REP][LPR * 8 + 2];
+    __shared__ unsigned char lutb[2 * ATT_MAX_REACH + 1];
+    __shared__ float tab[REP][ATT_MAX_BUCKETS];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, part = lane % LPR, rg = lane / LPR;
+    const int rep = a.heads / a.kv_heads, chunks = (rep + REP - 1) / REP;
+    const int chunk = blockIdx.x % chunks, kvh = blockIdx.x / chunks % a.kv_heads, split = blockIdx.y;
+    const long long row = blockIdx.x / chunks / a.kv_heads;
+    int lo = 0, hi = a.n_seg;                                   // the last segment that starts at or before this token
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (seg_at(a.q_ptr, mid, a.n_seg, a.n_q) <= row) lo = mid; else hi = mid;
+    }
+    if (row < seg_at(a.q_ptr, lo, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, lo + 1, a.n_seg, a.n_q)) return;
+    const long long f = seg_at(a.k_ptr, lo, a.n_seg, a.n_k), e = seg_at(a.k_ptr, lo + 1, a.n_seg, a.n_k);
+    const long long len = e > f ? e - f : 0, per = (len + a.splits - 1) / a.splits;
+    const long long k0 = f + (split * per < len ? split * per : len), k1 = k0 + per < f + len ? k0 + per : f + len;
+
+    const int head0 = kvh * rep + chunk * REP, d = 8 * part;
+    float q[REP][8], o[REP][8], m[REP], l[REP];
+#pragma unroll
+    for (int r = 0; r < REP; ++r) {
+        const bool on = chunk * REP + r < rep && d < a.dim;
+        if (on) load8<KIND>(a.q, row * a.q_st + (head0 + r) * a.q_sh + d, q[r]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) { q[r][c] = on ? q[r][c] * a.c0 : 0.f; o[r][c] = 0.f; }
+        m[r] = -__builtin_inff(); l[r] = 0.f;
+    }
+    const bool bias = a.table != nullptr;
+    int qx = 0, qy = 0, qz = 0;
+    const float most = (float)(a.reach * a.reach) + 0.5f;
+    if (bias) {
+        const int* p = a.q_pos + row * a.axes;
+        qx = p[0];
+        if (a.axes > 1) qy = p[1];
+        if (a.axes > 2) qz = p[2];
+        const int entries = a.axes == 1 ? 2 * a.reach + 1 : a.reach + 1;
+        for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
+        for (int r = t; r < REP * a.n_bucket; r += 256) {
+            const int hd = r / a.n_bucket, b = r % a.n_bucket;
+            tab[hd][b] = chunk * REP + hd < rep ? bias_log2(a.table[(head0 + hd) * a.n_bucket + b]) : 0.f;
+        }
+        __syncthreads();
+    }
+
+    for (long long base = k0; base < k1; base += 4 * RPW * U) {
+        float kv[U][8], vv[U][8];
+        bool use[U];
+        int bucket[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long key = base + (u * 4 + w) * RPW + rg;
+            use[u] = key < k1 && (!a.mask || a.mask[key]);
+            if (use[u] && d < a.dim) {
+                load8<KIND>(a.k, key * a.k_st + kvh * a.k_sh + d, kv[u]);
+                load8<KIND>(a.v, key * a.v_st + kvh * a.v_sh + d, vv[u]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) kv[u][c] = vv[u][c] = 0.f;
+            }
+            bucket[u] = 0;
+            if (bias && use[u]) {
+                const int* p = a.k_pos + key * a.axes;
+                const int kx = p[0], ky = a.axes > 1 ? p[1] : 0, kz = a.axes > 2 ? p[2] : 0;
+                bucket[u] = lutb[a.axes == 1 ? place<1>(qx, qy, qz, kx, ky, kz, 1, a.reach, most) : place<2>(qx, qy, qz, kx, ky, kz, a.axes, a.reach, most)];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < REP; ++r) {
+            float s[U], top = m[r];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s[u] = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s[u] = __builtin_fmaf(q[r][c], kv[u][c], s[u]);
+#pragma unroll
+                for (int x = 1; x < LPR; x <<= 1) s[u] += __shfl_xor(s[u], x);
+                if (bias) s[u] += tab[r][bucket[u]];
+                s[u] = use[u] ? s[u] : -__builtin_inff();
+                top = fmaxf(top, s[u]);
+            }
+            const float to = top == -__builtin_inff() ? 0.f : top, al = __builtin_amdgcn_exp2f(m[r] - to);
+            m[r] = top;
+            l[r] *= al;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[r][c] *= al;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float p = __builtin_amdgcn_exp2f(s[u] - to);
+                l[r] += p;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[r][c] = __builtin_fmaf(p, vv[u][c], o[r][c]);
+            }
+        }
+    }
+    // join the row groups of the wave, then the four waves
+#pragma unroll
+    for (int r = 0; r < REP; ++r) {
+#pragma unroll
+        for (int x = LPR; x < 64; x <<= 1) {
+            const float m2 = __shfl_xor(m[r], x), l2 = __shfl_xor(l[r], x), top = fmaxf(m[r], m2), to = top == -__builtin_inff() ? 0.f : top;
+            const float f1 = __builtin_amdgcn_exp2f(m[r] - to), f2 = __builtin_amdgcn_exp2f(m2 - to);
+            // the lower lane's share is added first on both sides: both hold the same sums
+            const bool low = (lane & x) == 0;
+            const float a1 = l[r] * f1, a2 = l2 * f2;
+            l[r] = low ? a1 + a2 : a2 + a1;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float o2 = __shfl_xor(o[r][c], x) * f2, o1 = o[r][c] * f1;
+                o[r][c] = low ? o1 + o2 : o2 + o1;
+            }
+            m[r] = top;
+        }
+        if (rg == 0) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) joined[w][r][part * 8 + c] = o[r][c];
+            if (part == 0) { joined[w][r][LPR * 8] = m[r]; joined[w][r][LPR * 8 + 1] = l[r]; }
+        }
+    }
+    __syncthreads();
+    const int dp = attn_dp_device(a.dim);
+    for (int x = t; x < REP * LPR * 2; x += 256) {              // four output values each
+        const int r = x / (LPR * 2), c = 4 * (x % (LPR * 2));
+        if (chunk * REP + r >= rep || c >= a.dim) continue;
+        float top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) top = fmaxf(top, joined[g][r][LPR * 8]);
+        const float to = top == -__builtin_inff() ? 0.f : top;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float s = __builtin_amdgcn_exp2f(joined[g][r][LPR * 8] - to);
+            sum += s * joined[g][r][LPR * 8 + 1];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) v[n] += s * joined[g][r][c + n];
+        }
+        const int head = head0 + r;
+        if (a.splits > 1) {
+            const long long at = ((long long)split * a.heads + head) * a.n_q + row;
+            *(f32x4*)(a.part + at * dp + c) = v;
+            if (c == 0) { a.part_ml[2 * at] = top; a.part_ml[2 * at + 1] = sum; }
+        } else {
+            v *= sum > 0.f ? 1.0f / sum : 0.f;
+            store4<KIND>(a.out, row * a.o_st + head * a.o_sh + c, v);
+            if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + c) = v;
+            if (c == 0 && a.stats) {
+                a.stats[(long long)head * a.n_q + row] = top;
+                a.stats[(long long)(a.heads + head) * a.n_q + row] = sum;
+            }
+        }
+    }
+}
+
+template <int KIND, int LPR>
+void few_rep(const AttnFwd& f, int rep, dim3 grid, hipStream_t st) {
+    if (rep == 1) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 1>), grid, dim3(256), 0, st, f);
+    else if (rep == 2) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 2>), grid, dim3(256), 0, st, f);
+    else if (rep == 4) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 4>), grid, dim3(256), 0, st, f);
+    else hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 8>), grid, dim3(256), 0, st, f);
+}
+template <int KIND>
+void few_kind(const AttnFwd& f, int rep, dim3 grid, hipStream_t st) {
+    if (f.dim <= 32) few_rep<KIND, 4>(f, rep, grid, st);
+    else if (f.dim <= 64) few_rep<KIND, 8>(f, rep, grid, st);
+    else few_rep<KIND, 16>(f, rep, grid, st);
+}
+
+}  // namespace
+
+int mgn_attn_launch_few(int kind, const AttnFwd* fp, void* stream) {
+    const AttnFwd& f = *fp;
+    MgnAttn a{};
+    a.heads = f.heads; a.kv_heads = f.kv_heads; a.n_q = f.n_q;
+    const int rep = attn_few_chunk(a);
+    const dim3 grid((unsigned)attn_few_blocks(a), (unsigned)f.splits);
+    const hipStream_t st = (hipStream_t)stream;
+    if (kind == AT_BF16) few_kind<AT_BF16>(f, rep, grid, st);
+    else if (kind == AT_F16) few_kind<AT_F16>(f, rep, grid, st);
+    else few_kind<AT_F32>(f, rep, grid, st);
+    return 0;
+}

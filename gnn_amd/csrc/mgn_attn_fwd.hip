@@ -1,0 +1,519 @@
+// Attention of one set of states over another, forwards: operand images, the tiled kernel, the join of split key ranges.
+#include "mgn_attn.h"
+#include "mgn_attn_host.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------- operand images
+// One wave per (head, subtile): lane (i, h) reads the elements 16 c + 8 h .. + 7 of token i, which are its share of image R;
+// image T is read back from a row-major copy in LDS.  Memory bound: 4 bytes read and 4 (R) or 8 (R and T) written per element.
+template <int KIND, int DP>
+__global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
+    constexpr int PL = planes<KIND>(), NC = DP / 16, LD = DP + 2;
+    __shared__ unsigned short tr[4][32 * LD];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
+    const int unit = min((int)blockIdx.x * 4 + w, a.units - 1);          // the last units are done twice, with equal results
+    int jb = 0;
+    while (jb + 1 < a.n_job && unit >= a.job[jb + 1].first_unit) ++jb;
+    const ImageJob& job = a.job[jb];
+    const int u = unit - job.first_unit, head = u % job.heads, sub = u / job.heads;
+    const Seg g = find_tile(job.ptr, a.n_seg, job.T, 5, sub);
+    const int tok = 32 * g.local + i;
+    const bool inside = g.local >= 0 && tok < g.len;
+    const long long row = inside ? g.first + tok : 0;
+    const bool use = inside && (!job.mask || job.mask[row]);
+
+    float v[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = 16 * c + 8 * h;
+        if (use && d < a.dim) load8<KIND>(job.x, row * job.st + head * job.sh + d, v[c]);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+    }
+    const long long at = (long long)head * job.n_sub + sub;
+    if (job.rows) {
+        float m = 0.f, l = 0.f, dot = 0.f;
+        if (use) {
+            m = job.stats[(long long)head * job.T + row];
+            l = job.stats[(long long)(job.heads + head) * job.T + row];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 16 * c + 8 * h;
+                if (d < a.dim) {
+                    float o[8];
+                    const long long at = row * job.o_st + head * job.o_sh + d;
+                    if (job.o_f32) load8<AT_F32>(job.o, at, o); else load8<KIND>(job.o, at, o);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(v[c][e], o[e], dot);
+                }
+            }
+        }
+        dot += __shfl_xor(dot, 32);
+        const float il = l > 0.f ? 1.0f / l : 0.f;
+        if constexpr (KIND == AT_F32) {
+            dot *= il;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] *= il;
+        }
+        if (h == 0) {
+            float* r = job.rows + at * 96;
+            r[i] = l > 0.f ? m : __builtin_inff();            // an empty row, or none: every exp2(score - m) is zero
+            r[32 + i] = KIND == AT_F32 ? 1.f : il;
+            r[64 + i] = l > 0.f ? dot : 0.f;
+        }
+    }
+    if (job.pos && head == 0 && h == 0)
+        for (int ax = 0; ax < job.axes; ++ax) job.pos_out[((long long)sub * job.axes + ax) * 32 + i] = inside ? job.pos[row * job.axes + ax] : 0;
+
+    float top = 0.f;
+    if constexpr (KIND != AT_BF16) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
+        top = wave_max(top);
+    }
+    const int ex = scale_exp<KIND>(top);
+    if (KIND != AT_BF16) {
+        const float by = job.alternate && (g.local & 1) ? -pow2i(-ex) : pow2i(-ex);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[c][e] *= by;
+    }
+    const unsigned long long bits = __ballot(use);
+    if (lane == 0) {
+        job.ex[at * 4] = ex;
+        if (job.valid) job.valid[at * 4] = (int)(unsigned)bits;
+    }
+    u32x4 hi[NC], lo[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) pack8<KIND>(v[c], hi[c], lo[c]);
+    if (job.R) {
+        u32x4* dst = (u32x4*)(job.R + at * (PL * 32 * DP)) + lane;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            dst[c * 64] = hi[c];
+            if constexpr (PL == 2) dst[(NC + c) * 64] = lo[c];
+        }
+    }
+    // every wave of the workgroup takes both rounds, whatever its job asks for: the barriers are met by all
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+        __syncthreads();
+        unsigned* line = (unsigned*)(tr[w] + i * LD);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) line[8 * c + 4 * h + e] = p ? lo[c][e] : hi[c][e];
+        __syncthreads();
+        if (job.Tt) {
+            u32x4* dst = (u32x4*)(job.Tt + at * (PL * 32 * DP)) + lane;
+#pragma unroll
+            for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+                for (int b = 0; b < DP / 32; ++b) {
+                    const unsigned short* src = tr[w] + (16 * kc + 4 * h) * LD + 32 * b + i;
+                    u32x4 r;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int t0 = e < 2 ? 2 * e : 8 + 2 * (e - 2);
+                        r[e] = (unsigned)src[t0 * LD] | ((unsigned)src[(t0 + 1) * LD] << 16);
+                    }
+                    dst[((p * 2 + kc) * (DP / 32) + b) * 64] = r;
+                }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- tiled kernel
+// A workgroup: 128 queries of one head, 32 per wave, against the key range of its split, 64 keys at a time.  Both products
+// are transposed (S^T = K Q^T, O^T = V^T P^T), so a lane holds scores of ONE query: the running maximum and sum of its softmax
+// are a register each, and its probabilities are the second product's operand as they stand.
+// P2: 16-bit types with probabilities in two planes, for the fp32 outputs that the gradient of a bias table needs.
+template <int KIND, int DP, int BIAS, bool P2>
+__global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void attn_fwd_kernel(AttnFwd a) {
+    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, KT = 2;
+    constexpr int SHIFT = KIND == AT_BF16 ? 0 : 13;            // probabilities are scaled by 2^13: small ones keep their bits in fp16
+    constexpr int NCOPY = KT * SUB * 2 / 4096;                 // 16-byte copies per thread and image
+    __shared__ __attribute__((aligned(1024))) unsigned short kbuf[2][KT * SUB];
+    __shared__ __attribute__((aligned(1024))) unsigned short vbuf[2][KT * SUB];
+    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 2 : 1][BIAS ? KT * 3 * 32 : 1];
+    __shared__ float lutb[BIAS ? 2 * ATT_MAX_REACH + 1 : 1];
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), split = blockIdx.y;
+    const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 7, blockIdx.x / a.heads);
+    if (g.local < 0 || g.local * ATT_TQ >= g.len) return;
+    const long long k0 = seg_at(a.k_ptr, g.seg, a.n_seg, a.n_k), k1 = seg_at(a.k_ptr, g.seg + 1, a.n_seg, a.n_k);
+    const int n_sub = k1 > k0 ? (int)((k1 - k0 + 31) >> 5) : 0;
+    const int per = (((n_sub + a.splits - 1) / a.splits) + KT - 1) / KT * KT;
+    const int s0 = min(split * per, n_sub), s1 = min(s0 + per, n_sub), n_it = (s1 - s0 + KT - 1) / KT;
+    const long long sub0 = (k0 >> 5) + g.seg + s0;             // first subtile of the range in the images
+    const unsigned short* kimg = a.kimg + ((long long)kvh * a.ns_k + sub0) * SUB;
+    const unsigned short* vimg = a.vimg + ((long long)kvh * a.ns_k + sub0) * SUB;
+    const i32x4* rec = a.rec + (long long)kvh * a.ns_k + sub0;
+
+    const int qi = g.local * ATT_TQ + 32 * w + j;
+    const bool mine = qi < g.len;
+    const long long row = g.first + min(qi, g.len - 1);
+
+    auto stage = [&](int b, int it) {
+        const int have = min(KT, s1 - s0 - it * KT) * SUB * 2;             // bytes; what is missing of the last pair is zeros
+#pragma unroll
+        for (int n = 0; n < NCOPY; ++n) {
+            const int off = n * 4096 + w * 1024;
+            const long long src = (long long)it * KT * SUB * 2 + off + lane * 16;
+            if (off < have) {
+                copy16((const char*)kimg + src, (char*)kbuf[b] + off);
+                copy16((const char*)vimg + src, (char*)vbuf[b] + off);
+            } else {
+                *(u32x4*)((char*)kbuf[b] + off + lane * 16) = u32x4{0, 0, 0, 0};
+                *(u32x4*)((char*)vbuf[b] + off + lane * 16) = u32x4{0, 0, 0, 0};
+            }
+        }
+        if constexpr (BIAS > 0) {
+            if (w == 0)
+                for (int ax = 0; ax < a.axes; ++ax)
+                    copy4(a.kpos + ((sub0 + (long long)it * KT) * a.axes + 2 * ax) * 32 + lane, pbuf[b] + 64 * ax);
+        }
+    };
+    if (n_it > 0) stage(0, 0);
+
+    // the queries' operand, scaled per row
+    u32x4 qh[NC], ql[NC];
+    float cq = a.c0;
+    {
+        float v[NC][8], top = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = 16 * c + 8 * h;
+            if (d < a.dim) load8<KIND>(a.q, row * a.q_st + head * a.q_sh + d, v[c]);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+            if constexpr (KIND != AT_BF16)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
+        }
+        if constexpr (KIND != AT_BF16) {
+            const int ex = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
+            cq *= pow2i(ex);
+            const float by = pow2i(-ex);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] *= by;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) pack8<KIND>(v[c], qh[c], ql[c]);
+    }
+    int qx = 0, qy = 0, qz = 0;
+    float most = 0.f;
+    if constexpr (BIAS > 0) {
+        const int* p = a.q_pos + row * a.axes;
+        qx = p[0];
+        if (a.axes > 1) qy = p[1];
+        if (a.axes > 2) qz = p[2];
+        most = (float)(a.reach * a.reach) + 0.5f;
+        const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
+        for (int r = t; r < entries; r += 256)
+            lutb[r] = bias_log2(a.table[head * a.n_bucket + min(max(a.lut[r], 0), a.n_bucket - 1)]);
+    }
+    int ev = 0;                                                 // common exponent of the values in this range
+    if constexpr (KIND != AT_BF16) {
+        ev = -126;
+        for (int s = lane; s < s1 - s0; s += 64) ev = max(ev, rec[s][1]);
+        ev = wave_max_i(ev);
+    }
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = zero16();
+    float m = -__builtin_inff(), l = 0.f;
+    if (n_it > 0) barrier_all();
+
+    for (int it = 0; it < n_it; ++it) {
+        const int b = it & 1;
+        if (it + 1 < n_it) stage(b ^ 1, it + 1);
+        i32x4 r[KT];
+#pragma unroll
+        for (int u = 0; u < KT; ++u) r[u] = it * KT + u < s1 - s0 ? rec[it * KT + u] : i32x4{-126, -126, 0, 0};
+        f32x16 s[KT];
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+            const u32x4* kp = (const u32x4*)(kbuf[b] + u * SUB) + lane;
+            s[u] = zero16();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if constexpr (PL == 2) {
+                    s[u] = mma<KIND>(kp[(NC + c) * 64], qh[c], s[u]);
+                    s[u] = mma<KIND>(kp[c * 64], ql[c], s[u]);
+                }
+                s[u] = mma<KIND>(kp[c * 64], qh[c], s[u]);
+            }
+        }
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+            const float c = KIND == AT_BF16 ? cq : cq * pow2i(r[u][0]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (BIAS > 0) {
+                    const int* p = pbuf[b] + u * a.axes * 32 + 8 * q + 4 * h;
+                    const i32x4 x = *(const i32x4*)p, y = a.axes > 1 ? *(const i32x4*)(p + 32) : x, z = a.axes > 2 ? *(const i32x4*)(p + 64) : x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[u][4 * q + e] = __builtin_fmaf(s[u][4 * q + e], c, lutb[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.axes, a.reach, most)]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u][4 * q + e] *= c;
+                }
+            }
+            if (r[u][2] != -1) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!((unsigned)r[u][2] >> (8 * (e >> 2) + 4 * h + (e & 3)) & 1)) s[u][e] = -__builtin_inff();
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float al = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.f : mn));
+            l *= al;
+#pragma unroll
+            for (int b2 = 0; b2 < NB; ++b2)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[b2][e] *= al;
+            m = mn;
+        }
+        float base = m == -__builtin_inff() ? 0.f : m;
+        if (BIAS > 0 && __any(fabsf(base) > 0x1p20f)) {        // biases near the ends of their type: a shift added to the
+#pragma unroll                                                 // maximum would be rounded away
+            for (int u = 0; u < KT; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] -= base;
+            base = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+            const float sh = KIND == AT_BF16 ? 0.f : (float)(SHIFT + max(r[u][1] - ev, FAR_EXP)), back = sh - base;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[u][e] = __builtin_amdgcn_exp2f(s[u][e] + back);
+                sum += s[u][e];
+            }
+            l += KIND == AT_BF16 ? sum : sum * __builtin_amdgcn_exp2f(-sh);
+            const u32x4* vp = (const u32x4*)(vbuf[b] + u * SUB) + lane;
+#pragma unroll
+            for (int kc = 0; kc < 2; ++kc) {
+                float pv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pv[e] = s[u][8 * kc + e];
+                u32x4 ph, plo;
+                pack8<KIND, P2>(pv, ph, plo);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    if constexpr (PL == 1 && P2) o[n] = mma<KIND>(vp[(kc * NB + n) * 64], plo, o[n]);
+                    if constexpr (PL == 2) {
+                        o[n] = mma<KIND>(vp[((2 + kc) * NB + n) * 64], ph, o[n]);
+                        o[n] = mma<KIND>(vp[(kc * NB + n) * 64], plo, o[n]);
+                    }
+                    o[n] = mma<KIND>(vp[(kc * NB + n) * 64], ph, o[n]);
+                }
+            }
+        }
+        barrier_all();
+    }
+
+    l += __shfl_xor(l, 32);
+    if (!mine) return;
+    const float inv = a.splits > 1 ? 1.f : l > 0.f ? 1.0f / l : 0.f;
+    const int back = KIND == AT_BF16 ? 0 : ev - SHIFT;
+    const long long prow = ((long long)split * a.heads + head) * a.n_q + row;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * n + 8 * q + 4 * h;
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[n][4 * q + e] * inv : ldexpf(o[n][4 * q + e] * inv, back);
+            if (a.splits > 1) *(f32x4*)(a.part + prow * DP + d) = v;
+            else if (d < a.dim) {
+                store4<KIND>(a.out, row * a.o_st + head * a.o_sh + d, v);
+                if (P2) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + d) = v;
+            }
+        }
+    if (h == 0) {
+        if (a.splits > 1) {
+            a.part_ml[2 * prow] = m; a.part_ml[2 * prow + 1] = l;
+        } else if (a.stats) {
+            a.stats[(long long)head * a.n_q + row] = m;
+            a.stats[(long long)(a.heads + head) * a.n_q + row] = l;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- join of split key ranges
+// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s; one thread per four output values.  Rows that belong to no segment are
+// left as they are.
+template <int KIND>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a, int dp) {
+    const int quads = a.dim / 4;
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x, n = a.n_q * a.heads * quads;
+    if (item >= n) return;
+    const int quad = (int)(item % quads), head = (int)(item / quads % a.heads);
+    const long long row = item / quads / a.heads;
+    if (row < seg_at(a.q_ptr, 0, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, a.n_seg, a.n_seg, a.n_q)) return;
+    float m = -__builtin_inff();
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (((long long)s * a.heads + head) * a.n_q + row)]);
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const long long at = ((long long)s * a.heads + head) * a.n_q + row;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base);
+        l += f * a.part_ml[2 * at + 1];
+        o += f * *(const f32x4*)(a.part + at * dp + 4 * quad);
+    }
+    o *= l > 0.f ? 1.0f / l : 0.f;
+    store4<KIND>(a.out, row * a.o_st + head * a.o_sh + 4 * quad, o);
+    if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + 4 * quad) = o;
+    if (quad == 0 && a.stats) {
+        a.stats[(long long)head * a.n_q + row] = m;
+        a.stats[(long long)(a.heads + head) * a.n_q + row] = l;
+    }
+}
+
+template <int KIND, int DP>
+void fwd_bias(const AttnFwd& f, int bias, dim3 grid, hipStream_t st) {
+    constexpr bool TWO = KIND != AT_F32;
+    if (f.out32) {
+        if (bias == 0) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 0, TWO>), grid, dim3(256), 0, st, f);
+        else if (bias == 1) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 1, TWO>), grid, dim3(256), 0, st, f);
+        else hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 2, TWO>), grid, dim3(256), 0, st, f);
+    } else {
+        if (bias == 0) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 0, false>), grid, dim3(256), 0, st, f);
+        else if (bias == 1) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 1, false>), grid, dim3(256), 0, st, f);
+        else hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 2, false>), grid, dim3(256), 0, st, f);
+    }
+}
+template <int KIND>
+void fwd_kind(const AttnFwd& f, int dp, int bias, dim3 grid, hipStream_t st) {
+    if (dp == 32) fwd_bias<KIND, 32>(f, bias, grid, st);
+    else if (dp == 64) fwd_bias<KIND, 64>(f, bias, grid, st);
+    else fwd_bias<KIND, 128>(f, bias, grid, st);
+}
+template <int KIND>
+void image_kind(const ImageArgs& a, int dp, hipStream_t st) {
+    const dim3 grid((a.units + 3) / 4);
+    if (dp == 32) hipLaunchKernelGGL((attn_image_kernel<KIND, 32>), grid, dim3(256), 0, st, a);
+    else if (dp == 64) hipLaunchKernelGGL((attn_image_kernel<KIND, 64>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_image_kernel<KIND, 128>), grid, dim3(256), 0, st, a);
+}
+
+// workspace of the forward pass, in this order (256-byte aligned pieces)
+struct FwdSpace { size_t kimg, vimg, rec, kpos, part, ml, total; int ns_k, splits; };
+
+FwdSpace fwd_space(const MgnAttn& a, bool few) {
+    FwdSpace s{};
+    const int dp = attn_dp(a.dim), pl = a.dtype == MGN_F32 ? 2 : 1;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) & ~(size_t)255; return p; };
+    s.ns_k = attn_subtiles(a.n_k, a.n_seg);
+    s.splits = few ? attn_few_splits(a) : attn_fwd_splits(a);
+    if (!few) {
+        // one spare subtile: a pair of subtiles is copied (and its second half ignored) past the end
+        s.kimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
+        s.vimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
+        s.rec = take((size_t)a.kv_heads * s.ns_k * 16);
+        s.kpos = take(a.bias_table ? (size_t)(s.ns_k + 1) * a.axes * 128 : 0);
+    }
+    if (s.splits > 1) {
+        s.part = take((size_t)s.splits * a.heads * a.n_q * dp * 4);
+        s.ml = take((size_t)s.splits * a.heads * a.n_q * 8);
+    }
+    s.total = at;
+    return s;
+}
+
+}  // namespace
+
+int mgn_attn_launch_images(int kind, int dp, const void* args, void* stream) {
+    const ImageArgs& a = *(const ImageArgs*)args;
+    const hipStream_t st = (hipStream_t)stream;
+    if (kind == AT_BF16) image_kind<AT_BF16>(a, dp, st);
+    else if (kind == AT_F16) image_kind<AT_F16>(a, dp, st);
+    else image_kind<AT_F32>(a, dp, st);
+    return 0;
+}
+
+extern "C" int64_t mgn_attn_fwd_workspace_bytes(const MgnAttn* a) {
+    if (attn_check(a, "mgn_attn_fwd_workspace_bytes") != 0) return -1;
+    return (int64_t)fwd_space(*a, attn_is_few(*a)).total;
+}
+
+extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_t out_sh, float* stats, float* out32, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    if (const int rc = attn_check(ap, "mgn_attn_fwd")) return rc;
+    const MgnAttn& a = *ap;
+    if (a.n_q == 0) return 0;
+    const bool few = attn_is_few(a);
+    const FwdSpace sp = fwd_space(a, few);
+    if (!out || (sp.total > 0 && (!workspace || workspace_bytes < (int64_t)sp.total))) {
+        mgn_set_error("mgn_attn_fwd: null output, or a workspace of %lld bytes where %lld are needed", (long long)workspace_bytes, (long long)sp.total);
+        return MGN_E_ARG;
+    }
+    if (attn_bad_rows(out, out_st, out_sh, a.dtype)) { mgn_set_error("mgn_attn_fwd: output rows must be 16-byte aligned"); return MGN_E_ARG; }
+    if ((uintptr_t)out32 & 15) { mgn_set_error("mgn_attn_fwd: out32 must start on a 16-byte border"); return MGN_E_ARG; }
+    char* ws = (char*)workspace;
+    const int kind = attn_kind(a.dtype), dp = attn_dp(a.dim), bias = attn_bias(a);
+    const hipStream_t st = (hipStream_t)stream;
+    AttnFwd f{};
+    f.q = a.q; f.q_st = a.q_st; f.q_sh = a.q_sh;
+    f.k = a.k; f.k_st = a.k_st; f.k_sh = a.k_sh; f.v = a.v; f.v_st = a.v_st; f.v_sh = a.v_sh; f.mask = a.key_mask; f.k_pos = a.k_pos;
+    f.q_ptr = a.q_ptr; f.k_ptr = a.k_ptr; f.n_seg = a.n_seg; f.n_q = a.n_q; f.n_k = a.n_k;
+    f.heads = a.heads; f.kv_heads = a.kv_heads; f.dim = a.dim; f.c0 = a.scale * LOG2E;
+    f.q_pos = a.q_pos; f.table = a.bias_table; f.lut = a.bucket_lut; f.n_bucket = a.n_bucket; f.reach = a.reach; f.axes = a.axes;
+    f.out = out; f.o_st = out_st; f.o_sh = out_sh; f.stats = stats; f.out32 = a.dtype == MGN_F32 ? nullptr : out32; f.splits = sp.splits;
+    if (sp.splits > 1) { f.part = (float*)(ws + sp.part); f.part_ml = (float*)(ws + sp.ml); }
+    if (few) {
+        mgn_attn_launch_few(kind, &f, stream);
+    } else {
+        unsigned short *kimg = (unsigned short*)(ws + sp.kimg), *vimg = (unsigned short*)(ws + sp.vimg);
+        int* rec = (int*)(ws + sp.rec);
+        int* kpos = (int*)(ws + sp.kpos);
+        if (a.n_k > 0) {
+            ImageArgs im{};
+            const int units = sp.ns_k * a.kv_heads;
+            im.n_job = 2; im.units = 2 * units; im.n_seg = a.n_seg; im.dim = a.dim;
+            ImageJob& k = im.job[0];
+            k.x = a.k; k.st = a.k_st; k.sh = a.k_sh; k.ptr = a.k_ptr; k.mask = a.key_mask; k.T = a.n_k; k.heads = a.kv_heads; k.n_sub = sp.ns_k;
+            k.R = kimg; k.ex = rec; k.valid = rec + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = kpos; k.axes = a.axes;
+            ImageJob& v = im.job[1];
+            v = k; v.x = a.v; v.st = a.v_st; v.sh = a.v_sh; v.first_unit = units; v.R = nullptr; v.Tt = vimg; v.ex = rec + 1; v.valid = nullptr; v.pos = nullptr;
+            mgn_attn_launch_images(kind, dp, &im, stream);
+        }
+        f.kimg = kimg; f.vimg = vimg; f.rec = (const i32x4*)rec; f.ns_k = sp.ns_k; f.kpos = kpos;
+        const dim3 grid((unsigned)((a.n_q / ATT_TQ + a.n_seg) * a.heads), (unsigned)sp.splits);
+        if (kind == AT_BF16) fwd_kind<AT_BF16>(f, dp, bias, grid, st);
+        else if (kind == AT_F16) fwd_kind<AT_F16>(f, dp, bias, grid, st);
+        else fwd_kind<AT_F32>(f, dp, bias, grid, st);
+    }
+    if (sp.splits > 1) {
+        const long long items = a.n_q * a.heads * (a.dim / 4);
+        const dim3 grid((unsigned)((items + 255) / 256));
+        if (kind == AT_BF16) hipLaunchKernelGGL((attn_join_kernel<AT_BF16>), grid, dim3(256), 0, st, f, dp);
+        else if (kind == AT_F16) hipLaunchKernelGGL((attn_join_kernel<AT_F16>), grid, dim3(256), 0, st, f, dp);
+        else hipLaunchKernelGGL((attn_join_kernel<AT_F32>), grid, dim3(256), 0, st, f, dp);
+    }
+    return check_launch("mgn_attn_fwd");
+}

@@ -1,0 +1,84 @@
+// Host side of the attention entry points: argument checks, launch shapes, kernel arguments.
+#pragma once
+#include "mgn_attn.h"
+
+#include <cmath>
+
+// Arguments of the forward kernels (tiled, few queries, join).
+struct AttnFwd {
+    const void *q, *k, *v; long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
+    const uint8_t* mask; const int* k_pos;
+    const int *q_ptr, *k_ptr; long long n_q, n_k; int n_seg, heads, kv_heads, dim; float c0;
+    const unsigned short *kimg, *vimg; const i32x4* rec; int ns_k; const int* kpos;
+    const int* q_pos; const float* table; const int* lut; int n_bucket, reach, axes;
+    void* out; long long o_st, o_sh; float *stats, *out32;
+    int splits; float *part, *part_ml;
+};
+
+int mgn_attn_launch_few(int kind, const AttnFwd* f, void* stream);      // mgn_attn_few.hip
+
+namespace {
+
+inline int attn_kind(int dtype) { return dtype == MGN_BF16 ? AT_BF16 : dtype == MGN_F16 ? AT_F16 : AT_F32; }
+inline int attn_dp(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+inline int attn_bias(const MgnAttn& a) { return !a.bias_table ? 0 : a.axes == 1 ? 1 : 2; }
+inline int attn_subtiles(int64_t n, int n_seg) { return (int)(n / 32) + n_seg; }
+
+inline bool attn_bad_rows(const void* p, int64_t st, int64_t sh, int dtype) {
+    const int per = dtype == MGN_F32 ? 4 : 8;                           // elements of 16 bytes
+    return ((uintptr_t)p & 15) || st % per || sh % per || st < 0 || sh < 0;
+}
+
+inline int attn_check(const MgnAttn* a, const char* name) {
+    const char* bad = nullptr;
+    if (!a) bad = "null arguments";
+    else if (a->dtype != MGN_F32 && a->dtype != MGN_BF16 && a->dtype != MGN_F16) bad = "unknown type";
+    else if (a->dim < 8 || a->dim > 128 || a->dim % 8) bad = "the head width must be a multiple of 8 up to 128";
+    else if (a->heads < 1 || a->kv_heads < 1 || a->heads > 1024 || a->heads % a->kv_heads) bad = "heads must be a multiple of kv_heads, 1024 at most";
+    else if (a->n_q < 0 || a->n_k < 0 || a->n_q > 0x7fffffffLL - 4096 || a->n_k > 0x7fffffffLL - 4096) bad = "token counts must fit 32 bits";
+    else if (a->n_seg < 1 || a->n_seg > (1 << 20) || (a->n_seg > 1 && (!a->q_ptr || !a->k_ptr))) bad = "more than one segment needs both offset arrays";
+    else if ((a->q_ptr == nullptr) != (a->k_ptr == nullptr)) bad = "segment offsets come for queries and keys, or for neither";
+    else if (!(a->scale > 0.f) || !std::isfinite(a->scale)) bad = "the scale must be positive and finite";
+    else if ((a->n_q > 0 && !a->q) || (a->n_k > 0 && (!a->k || !a->v))) bad = "null operand";
+    else if ((a->n_q > 0 && attn_bad_rows(a->q, a->q_st, a->q_sh, a->dtype)) ||
+             (a->n_k > 0 && (attn_bad_rows(a->k, a->k_st, a->k_sh, a->dtype) || attn_bad_rows(a->v, a->v_st, a->v_sh, a->dtype))))
+        bad = "rows must start on 16-byte borders";
+    else if ((a->n_q / 32 + a->n_seg) * (int64_t)a->heads > 0x3fffffffLL || (a->n_k / 32 + a->n_seg) * (int64_t)a->kv_heads > 0x3fffffffLL)
+        bad = "too many tokens x heads";
+    else if (a->bias_table) {
+        if (!a->bucket_lut || (a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos)) bad = "the bias needs a bucket table and places";
+        else if (a->axes < 1 || a->axes > 3) bad = "places have one to three axes";
+        else if (a->reach < 1 || a->reach > ATT_MAX_REACH) bad = "reach must be 1 .. 1024";
+        else if (a->n_bucket < 1 || a->n_bucket > ATT_MAX_BUCKETS) bad = "1 .. 64 buckets";
+    }
+    if (bad) { mgn_set_error("%s: %s", name, bad); return MGN_E_ARG; }
+    return 0;
+}
+
+// Few queries per segment: keys and values are read once where they lie, without images.
+inline bool attn_is_few(const MgnAttn& a) { return a.n_q <= 4 * (int64_t)a.n_seg; }
+
+inline int attn_few_chunk(const MgnAttn& a) {                           // query heads that share a pass over a key head
+    const int rep = a.heads / a.kv_heads;
+    return rep >= 8 ? 8 : rep > 2 ? 4 : rep;
+}
+inline int attn_few_blocks(const MgnAttn& a) {
+    const int rep = a.heads / a.kv_heads, c = attn_few_chunk(a);
+    return (int)(a.n_q * a.kv_heads * ((rep + c - 1) / c));
+}
+// Split key ranges until there are about four workgroups per compute unit, in pieces of at least 256 keys.
+inline int attn_few_splits(const MgnAttn& a) {
+    const int64_t blocks = attn_few_blocks(a), keys = a.n_k / a.n_seg;
+    int64_t s = blocks > 0 ? 1024 / blocks : 1;
+    if (s > keys / 256) s = keys / 256;
+    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+}
+// The tiled kernel: the same, in pieces of at least 256 keys, when its query tiles leave compute units idle.
+inline int attn_fwd_splits(const MgnAttn& a) {
+    const int64_t blocks = (a.n_q / ATT_TQ + a.n_seg) * a.heads, keys = a.n_k / a.n_seg;
+    int64_t s = blocks > 0 ? 512 / blocks : 1;
+    if (s > keys / 256) s = keys / 256;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+}  // namespace

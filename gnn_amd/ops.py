@@ -71,6 +71,24 @@ def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+class _on_device:
+    """Makes ``device`` the current one for a call, when it is not already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        same = device.index is None or device.index == torch.cuda.current_device()
+        self.guard = None if same else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
 def _bad_tensor(t, dtype, shape, name: str):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"{name}: expected a CUDA/HIP tensor (the HIP path has no CPU fallback)")
@@ -203,6 +221,132 @@ def receiver_csr_dev(edge_index: torch.Tensor, num_nodes: int):
                                              cr.data_ptr(), perm.data_ptr(), _stream())
         _lib.check(rc, "mgn_receiver_csr_dev")
     return rowptr, cs, cr, perm
+
+
+# --------------------------------------------------------------------------- device: attention over another set of states
+_ATT_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _att_rows(t, dtype, device, tail, name: str):
+    """[tokens, heads, dim] rows the attention kernels can read: same type and device as the queries, the last axis dense,
+    every row on a 16-byte border (other axes may be strided, so slices of a packed projection work)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: expected a CUDA/HIP tensor (the HIP path has no CPU fallback)")
+    if t.dtype is not dtype or t.device != device:
+        raise RuntimeError(f"{name}: expected dtype {dtype} on {device}, got {t.dtype} on {t.device}")
+    if t.dim() != 3 or t.shape[1:] != tail:
+        raise RuntimeError(f"{name}: expected shape [tokens, {tail[0]}, {tail[1]}], got {tuple(t.shape)}")
+    per = 16 // t.element_size()
+    st, sh, sd = t.stride()
+    if t.numel() and (sd != 1 or st % per or sh % per or t.data_ptr() % 16):
+        raise RuntimeError(f"{name}: the last axis must be dense and every row start on a 16-byte border "
+                           f"(strides {t.stride()}): call .contiguous()")
+    return t.data_ptr(), (st if t.shape[0] > 1 else sh * t.shape[1]), sh
+
+
+def _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise RuntimeError("cross_attention: q [queries, heads, dim] and k, v [keys, kv_heads, dim]")
+    if q.dtype not in _ATT_DTYPES:
+        raise RuntimeError(f"cross_attention: float32, bfloat16 or float16, got {q.dtype}")
+    dev, (nq, heads, dim), (nk, kv_heads) = q.device, q.shape, k.shape[:2]
+    if dim % 8 or not 8 <= dim <= 128:
+        raise RuntimeError(f"cross_attention: the head width must be a multiple of 8 up to 128, got {dim}")
+    if kv_heads < 1 or heads % kv_heads:
+        raise RuntimeError(f"cross_attention: {heads} query heads are not a multiple of {kv_heads} key heads")
+    if (q_ptr is None) != (k_ptr is None):
+        raise RuntimeError("cross_attention: segment offsets come for queries and keys, or for neither")
+    n_seg = 1 if q_ptr is None else q_ptr.shape[0] - 1
+    if n_seg < 1:
+        raise RuntimeError("cross_attention: segment offsets hold one entry more than there are segments")
+    if v.shape[0] != nk:
+        raise RuntimeError(f"cross_attention: {nk} keys but {v.shape[0]} values")
+    if key_mask is not None and key_mask.dtype is torch.bool:
+        key_mask = key_mask.view(torch.uint8)
+    reach = axes = n_bucket = 0
+    if bias_table is not None:
+        if bucket_lut is None or q_pos is None or k_pos is None:
+            raise RuntimeError("cross_attention: the bias needs bucket_lut, q_pos and k_pos")
+        n_bucket, axes = bias_table.shape[-1], q_pos.shape[-1]
+        reach = bucket_lut.shape[0] // 2 if axes == 1 else bucket_lut.shape[0] - 1
+        if not 1 <= axes <= 3 or not 1 <= reach <= 1024 or not 1 <= n_bucket <= 64 or (axes == 1 and bucket_lut.shape[0] % 2 == 0):
+            raise RuntimeError("cross_attention: places have one to three axes, bucket_lut 2 * reach + 1 (one axis) or reach + 1 entries "
+                               "with reach <= 1024, the table at most 64 buckets")
+    elif bucket_lut is not None or q_pos is not None or k_pos is not None:
+        raise RuntimeError("cross_attention: bucket_lut, q_pos and k_pos belong to a bias_table")
+    small = [("q_ptr", q_ptr), ("k_ptr", k_ptr), ("key_mask", key_mask), ("bias_table", bias_table), ("bucket_lut", bucket_lut),
+             ("q_pos", q_pos), ("k_pos", k_pos)]
+    for name, t in small:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"cross_attention: {name} is on {t.device}, the queries on {dev}")
+    tail = (kv_heads, dim)
+    (qp, qt, qh), (kp, kt, kh), (vp, vt, vh) = (_att_rows(q, q.dtype, dev, (heads, dim), "q"), _att_rows(k, q.dtype, dev, tail, "k"),
+                                                _att_rows(v, q.dtype, dev, tail, "v"))
+    return _lib.MgnAttn(qp, kp, vp, qt, qh, kt, kh, vt, vh,
+                        _opt(q_ptr, torch.int32, (n_seg + 1,), "q_ptr"), _opt(k_ptr, torch.int32, (n_seg + 1,), "k_ptr"),
+                        _opt(key_mask, torch.uint8, (nk,), "key_mask"), _opt(bias_table, torch.float32, (heads, n_bucket), "bias_table"),
+                        _opt(bucket_lut, torch.int32, None, "bucket_lut"), _opt(q_pos, torch.int32, (nq, axes), "q_pos"),
+                        _opt(k_pos, torch.int32, (nk, axes), "k_pos"), nq, nk, n_seg, heads, kv_heads, dim, _ATT_DTYPES[q.dtype],
+                        n_bucket, reach, axes, float(dim ** -0.5 if scale is None else scale), 0)
+
+
+def _att_workspace(need: int, device) -> torch.Tensor:
+    if need < 0:
+        raise RuntimeError("cross_attention: " + _lib.lib().mgn_last_error().decode("utf-8", "replace"))
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+
+
+def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=None, bucket_lut=None, q_pos=None, k_pos=None,
+                    scale: Optional[float] = None, out=None, stats=None, out32=None):
+    """Every query reads the values of another set of states, weighted by a softmax over their keys (``mgn_attn_fwd``).
+
+    ``q`` [queries, heads, dim]; ``k``, ``v`` [keys, kv_heads, dim], one type (float32, bfloat16, float16); ``scale`` defaults
+    to dim^-1/2.  ``q_ptr`` / ``k_ptr`` int32 [segments + 1]: a query reads the keys of its own segment; rows outside all
+    segments are left as they are in ``out`` (zeros in an output made here).  ``key_mask`` [keys] bool: False leaves a key
+    out.  A query without keys gives zeros.  ``bias_table`` float32 [heads, buckets] with ``bucket_lut`` int32 and the places
+    ``q_pos`` / ``k_pos`` int32 [tokens, axes] adds a learned bias by distance (:class:`gnn_amd.attention.RelativeBuckets`).
+    ``stats`` float32 [2, heads, queries] receives what :func:`cross_attention_bwd` needs; ``out32`` (bfloat16 and float16,
+    float32 [queries, heads, dim]) the outputs before they are rounded, for the gradient of a bias table."""
+    a = _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_ptr is None else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    o = _att_rows(out, q.dtype, q.device, q.shape[1:], "out")
+    if out.shape[0] != q.shape[0]:
+        raise RuntimeError(f"cross_attention: {q.shape[0]} queries but {out.shape[0]} output rows")
+    st = _opt(stats, torch.float32, (2, q.shape[1], q.shape[0]), "stats")
+    o32 = _opt(out32, torch.float32, tuple(q.shape), "out32")
+    with _on_device(q.device):
+        ws = _att_workspace(_lib.lib().mgn_attn_fwd_workspace_bytes(C.byref(a)), q.device)
+        with timed("cross_attention"):
+            rc = _lib.lib().mgn_attn_fwd(C.byref(a), *o, st, o32, ws.data_ptr(), ws.numel(), _stream())
+    _lib.check(rc, "mgn_attn_fwd")
+    return out
+
+
+def cross_attention_bwd(g, q, k, v, out, stats, q_ptr=None, k_ptr=None, key_mask=None, bias_table=None, bucket_lut=None,
+                        q_pos=None, k_pos=None, scale: Optional[float] = None, table_grad: bool = True):
+    """Gradients (dq, dk, dv, dtable) of :func:`cross_attention` for the output gradient ``g`` (``mgn_attn_bwd``); ``out`` and
+    ``stats`` as the forward call left them (``out32`` in place of ``out`` keeps ``dtable`` at float32 accuracy), the other arguments as given to it.  ``dtable`` is None without a table or with
+    ``table_grad`` False.  Rows outside all segments get zeros.  Every sum has a fixed order."""
+    a = _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
+    if isinstance(g, torch.Tensor) and g.dim() == 3 and (g.stride(2) != 1 or g.stride(0) % 8 or g.stride(1) % 8 or g.data_ptr() % 16):
+        g = g.contiguous()                     # an expanded or transposed gradient as autograd hands it over
+    new = torch.empty_like if q_ptr is None else torch.zeros_like
+    dq, dk, dv = (new(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    table_grad = table_grad and bias_table is not None
+    dt = torch.empty_like(bias_table) if table_grad else None
+    gr, o = _att_rows(g, q.dtype, q.device, q.shape[1:], "g"), _att_rows(out, out.dtype if out.dtype is torch.float32 else q.dtype, q.device, q.shape[1:], "out")
+    a.out_f32 = int(out.dtype is torch.float32)
+    if g.shape[0] != q.shape[0] or out.shape[0] != q.shape[0]:
+        raise RuntimeError("cross_attention_bwd: g and out have one row per query")
+    st = _dev(stats, torch.float32, (2, q.shape[1], q.shape[0]), "stats")
+    with _on_device(q.device):
+        ws = _att_workspace(_lib.lib().mgn_attn_bwd_workspace_bytes(C.byref(a), int(table_grad)), q.device)
+        with timed("cross_attention_bwd"):
+            rc = _lib.lib().mgn_attn_bwd(C.byref(a), *gr, *o, st, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                         0 if dt is None else dt.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
+    _lib.check(rc, "mgn_attn_bwd")
+    return dq, dk, dv, dt
 
 
 # --------------------------------------------------------------------------- device: processor

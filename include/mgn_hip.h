@@ -517,6 +517,53 @@ int mgn_knn_graph(const float* points /*[N][dim]*/, int32_t dim, const int64_t* 
                   const int32_t* coarse_ptr /*[n_blocks+1]*/, const int64_t* edge_ptr /*[n_blocks+1]*/, int32_t n_blocks,
                   int64_t max_block_points, int32_t k, int64_t* out_sender, int64_t* out_recv, void* stream);
 
+/* ---- attention of one set of states over another (queries of one length, keys and values of another) ------------
+ * o_i = sum_j p_ij v_j,  p_ij = softmax over j of  scale * <q_i, k_j> + bias_table[head][bucket_lut[place(i, j)]]
+ * over the keys j of query i's segment whose mask is not zero.  Beside the message weights of the attention option
+ * (core/meshgraphnet.py:100-108), which run along mesh edges, this reads all states of a segment: the fine nodes of a
+ * mesh the states of its coarse graph (core/meshgraphnet.py:179-194), a probe point the states of a mesh.
+ *
+ * Rows: q [n_q][heads][dim], k and v [n_k][kv_heads][dim], heads a multiple of kv_heads (query head h reads key head
+ * h / (heads / kv_heads)); strides in elements, the last axis dense, every row on a 16-byte border; dim a multiple of
+ * 8 up to 128; fp32, bf16 or fp16.  Sums, softmax statistics and products are fp32 (fp32 operands as two fp16 terms).
+ * Segments: q_ptr / k_ptr [n_seg + 1] (device, ascending); null: one segment.  Rows outside all segments are neither
+ * read nor written.  key_mask [n_k]: 0 leaves a key out; nothing is read from its rows.  A query with no key left (or
+ * only keys at a bias of minus infinity) gives a row of zeros and gradients of zero.
+ * Bias: places [n][axes] of queries and keys as whole numbers within +-2^30; one axis: place = k - q held to
+ * [-reach, reach], plus reach (table of 2 reach + 1 entries); two or three: the whole part of the distance, held to reach
+ * (reach + 1 entries).  bucket_lut values are held to [0, n_bucket).  reach <= 1024, n_bucket <= 64.
+ * stats [2][heads][n_q] (base-2 maximum and sum of each softmax): kept for mgn_attn_bwd; may be null.  out32
+ * [n_q][heads][dim] (bf16 / fp16, or null): the outputs before they are rounded, which mgn_attn_bwd takes in place of out
+ * (out_f32 set) where a bias table is trained: <g, o> enters every entry of dS and the table's gradient cancels.        */
+#define MGN_F32  0
+#define MGN_BF16 1
+#define MGN_F16  2
+
+typedef struct {
+    const void* q; const void* k; const void* v;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;      /* strides of tokens and heads, in elements                */
+    const int32_t* q_ptr; const int32_t* k_ptr;
+    const uint8_t* key_mask;
+    const float* bias_table;                         /* [heads][n_bucket] or null                               */
+    const int32_t* bucket_lut; const int32_t* q_pos; const int32_t* k_pos;
+    int64_t n_q, n_k;
+    int32_t n_seg, heads, kv_heads, dim, dtype, n_bucket, reach, axes;
+    float scale;
+    int32_t out_f32;                                 /* mgn_attn_bwd: out is fp32 whatever the operands' type       */
+} MgnAttn;
+
+int64_t mgn_attn_fwd_workspace_bytes(const MgnAttn* a);
+int mgn_attn_fwd(const MgnAttn* a, void* out, int64_t out_st, int64_t out_sh, float* stats, float* out32,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients for the output gradient g: dq [n_q][heads][dim], dk and dv [n_k][kv_heads][dim] (dense, type of the operands,
+ * summed over the query heads that share a key head), dtable [heads][n_bucket] fp32 or null.  out and stats as mgn_attn_fwd
+ * left them.  All sums have a fixed order.  Rows outside all segments are not written; masked keys get zeros.           */
+int64_t mgn_attn_bwd_workspace_bytes(const MgnAttn* a, int32_t table_grad);
+int mgn_attn_bwd(const MgnAttn* a, const void* g, int64_t g_st, int64_t g_sh, const void* out, int64_t out_st,
+                 int64_t out_sh, const float* stats, void* dq, void* dk, void* dv, float* dtable, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

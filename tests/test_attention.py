@@ -1,0 +1,84 @@
+"""Host side of the attention over another set of states: the buckets, and what is refused before anything is launched."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_buckets_are_whole_number_exact():
+    from gnn_amd.attention import RelativeBuckets
+    b = RelativeBuckets(32, 128, 2).table.tolist()
+    assert len(b) == 129 and b[:16] == list(range(16)) and b[128] == 31 and b == sorted(b)
+    # bucket n of the second half starts at the first d with (d / 16)^16 >= (128 / 16)^(n - 16), i.e. d >= 16 * 2^(3 (n - 16) / 16)
+    for n in range(17, 32):
+        first = b.index(n) if n in b else None
+        d = next(d for d in range(16, 129) if d ** 16 >= 16 ** 16 * 8 ** (n - 16))
+        assert first == d or first is None
+    line = RelativeBuckets(32, 128, 1).table.tolist()
+    assert len(line) == 257 and line[128] == 0 and line[127] == 1 and line[129] == 17 and line[0] == 15 and line[256] == 31
+    assert max(RelativeBuckets(64, 1024, 3).table.tolist()) == 63
+    assert RelativeBuckets(2, 1, 2).table.tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("args", [(1, 10, 2), (65, 10, 2), (32, 0, 2), (32, 1025, 2), (32, 10, 4), (31, 10, 1), (2, 10, 1)])
+def test_bucket_refusals(args):
+    from gnn_amd.attention import RelativeBuckets
+    with pytest.raises(ValueError):
+        RelativeBuckets(*args)
+
+
+def test_cpu_tensors_are_refused():
+    from gnn_amd import attention
+    x = torch.zeros(4, 2, 32)
+    with pytest.raises(RuntimeError, match="CUDA/HIP"):
+        attention.cross_attention(x, x, x)
+
+
+def args(**kw):
+    from gnn_amd import _lib
+    a = _lib.MgnAttn()
+    base = dict(q=4096, k=4096, v=4096, q_st=128, q_sh=32, k_st=128, k_sh=32, v_st=128, v_sh=32, n_q=10, n_k=20, n_seg=1, heads=4,
+                kv_heads=4, dim=32, dtype=0, scale=0.1)
+    for k, v in dict(base, **kw).items():
+        setattr(a, k, v)
+    return a
+
+
+BAD = [dict(dtype=3), dict(dtype=-1), dict(dim=0), dict(dim=12), dict(dim=136), dict(heads=0), dict(kv_heads=3), dict(kv_heads=0),
+       dict(heads=2048, kv_heads=1), dict(n_q=-1), dict(n_k=-1), dict(n_q=2 ** 31), dict(n_seg=0), dict(n_seg=2), dict(n_seg=2, q_ptr=64),
+       dict(q_ptr=64), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=0), dict(k=0), dict(v=0),
+       dict(q=4100), dict(q_st=129), dict(k_sh=33), dict(dtype=1, v_st=132), dict(bias_table=64), dict(bias_table=64, bucket_lut=64, q_pos=64),
+       dict(bias_table=64, bucket_lut=64, q_pos=64, k_pos=64, axes=0, reach=5, n_bucket=4),
+       dict(bias_table=64, bucket_lut=64, q_pos=64, k_pos=64, axes=2, reach=1025, n_bucket=4),
+       dict(bias_table=64, bucket_lut=64, q_pos=64, k_pos=64, axes=2, reach=0, n_bucket=4),
+       dict(bias_table=64, bucket_lut=64, q_pos=64, k_pos=64, axes=2, reach=5, n_bucket=65)]
+
+
+@pytest.mark.parametrize("bad", BAD, ids=lambda d: ",".join(f"{k}={v}" for k, v in d.items()))
+def test_the_library_refuses(bad):
+    """Every check runs on the host before a pointer is used."""
+    from gnn_amd import _lib
+    lib, a = _lib.lib(), args(**bad)
+    assert lib.mgn_attn_fwd_workspace_bytes(ctypes.byref(a)) == -1
+    assert lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(a), 1) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(a), 4096, 128, 32, None, None, 4096, 1 << 40, None) == -1
+    assert lib.mgn_attn_bwd(ctypes.byref(a), 4096, 128, 32, 4096, 128, 32, 4096, 4096, 4096, 4096, None, 4096, 1 << 40, None) == -1
+    assert lib.mgn_last_error()
+
+
+def test_null_arguments_and_small_workspaces_are_refused():
+    from gnn_amd import _lib
+    lib, a = _lib.lib(), args()
+    need = lib.mgn_attn_fwd_workspace_bytes(ctypes.byref(args(n_q=1000)))
+    assert need > 0
+    assert lib.mgn_attn_fwd(None, 4096, 128, 32, None, None, 4096, 1 << 40, None) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(args(n_q=1000)), 4096, 128, 32, None, None, 4096, need - 1, None) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(args(n_q=1000)), 4096, 128, 32, None, None, None, need, None) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(a), None, 128, 32, None, None, 4096, 1 << 40, None) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(a), 4100, 128, 32, None, None, 4096, 1 << 40, None) == -1
+    need = lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(a), 0)
+    ok = [4096, 128, 32, 4096, 128, 32, 4096, 4096, 4096, 4096, None, 4096, need, None]
+    for i, v in ((0, None), (3, None), (6, None), (7, None), (8, None), (9, None), (10, 4096), (11, None), (12, need - 1), (7, 4100)):
+        bad = list(ok)
+        bad[i] = v
+        assert lib.mgn_attn_bwd(ctypes.byref(a), *bad) == -1, i
