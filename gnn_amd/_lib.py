@@ -112,6 +112,10 @@ SIGNATURES = {
     "mgn_fps": (C.c_int, [_P, _I32, _P, _P, _P, _I32, _I64, _P, _P, _P]),
     "mgn_fps_workspace_floats": (_I64, [_I64]),
     "mgn_fps_single": (C.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "mgn_q8_rows": (C.c_int, [_P, _I32, _I64, _I32, _I32, _P, _P, _P]),
+    "mgn_q8_restore": (C.c_int, [_P, _P, _I64, _I32, _I32, _P, _P]),
+    "mgn_train_linear_bwd_q8": (C.c_int, [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _P, _P, _I64, _P]),
+    "mgn_train_edge_bwd_q8": (C.c_int, [_P] * 20 + [_I64, _I64, _P]),
     "mgn_attn_fwd_workspace_bytes": (_I64, [_ATT]),
     "mgn_attn_fwd": (C.c_int, [_ATT, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
     "mgn_attn_bwd_workspace_bytes": (_I64, [_ATT, _I32]),

@@ -8,7 +8,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 SOURCES = ["mgn_kernels.hip", "mgn_train.hip", "mgn_graph.hip", "mgn_halo.hip", "mgn_coarse.hip", "mgn_attn_fwd.hip",
-           "mgn_attn_bwd.hip", "mgn_attn_few.hip", "mgn_host.cpp"]
+           "mgn_attn_bwd.hip", "mgn_attn_few.hip", "mgn_q8.hip", "mgn_host.cpp"]
 OUT = os.path.join(PKG, "libmgn_hip.so")
 # No packed fp32 instructions (v_pk_add/mul/fma_f32): some of their forms have given wrong results on this hardware.  The
 # host pass of the compiler does not know the feature and says so; that warning is harmless.

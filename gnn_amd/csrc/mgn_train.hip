@@ -208,6 +208,25 @@ __global__ __launch_bounds__(NT) void train_ln_bwd_kernel(const float* __restric
 struct LinBwdArgs {
     const float* G; const float* A; const float* W; int ldw; int koff;
     const float* mask; const float* res; float* GA; float* partial; long long rows;
+    const signed char* codes; const float* scale; int mask_codes;      // A in 8 bits (mgn_train_linear_bwd_q8)
+};
+
+// Four consecutive features of a row as they were requested: fp32, or 8-bit codes and the row's scale.
+template <bool Q8> struct RowPiece {
+    f32x4 v;
+    __device__ __forceinline__ void request(const float* a, const signed char*, const float*, size_t, size_t at) { v = *(const f32x4*)(a + at); }
+    __device__ __forceinline__ f32x4 get() const { return v; }
+    __device__ __forceinline__ void arrived() { asm volatile("" : "+v"(v)); }
+};
+template <> struct RowPiece<true> {
+    int c; float s;
+    __device__ __forceinline__ void request(const float*, const signed char* codes, const float* scale, size_t row, size_t at) {
+        c = *(const int*)(codes + at); s = scale[row];
+    }
+    __device__ __forceinline__ f32x4 get() const {
+        return f32x4{(float)(int)(signed char)c * s, (float)(int)(signed char)(c >> 8) * s, (float)(int)(signed char)(c >> 16) * s, (float)(c >> 24) * s};
+    }
+    __device__ __forceinline__ void arrived() { asm volatile("" : "+v"(c), "+v"(s)); }
 };
 
 template <bool DO_GA, bool DO_DW>
@@ -422,9 +441,9 @@ __device__ __forceinline__ void load_wplanes32_t(WPlanes32& w, const float* __re
     }
 }
 
-struct TileRows { f32x4 g[4], a[4], m[4], r[4]; };     // one thread's share of a tile: rows srow + 8*it, columns 4*sq ..
+template <bool A8> struct TileRows { f32x4 g[4]; RowPiece<A8> a[4]; f32x4 m[4], r[4]; };     // one thread's share of a tile: rows srow + 8*it, columns 4*sq ..
 
-template <bool DO_GA, bool DO_DW>
+template <bool DO_GA, bool DO_DW, bool A8>
 __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned short Gs[3 * SPL];                    // G tile, three planes
     __shared__ __attribute__((aligned(16))) unsigned short As[DO_DW ? 3 * SPL : 8];        // A tile, three planes
@@ -445,23 +464,23 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
     // An absent mask / residual is read all the same, every lane at offset 0 of G (a line that stays in the cache), and
     // dropped by a select: the tile loop has no branch around a load.
     // A mask that is the layer input itself (the usual case: the ReLU output that fed this Linear) is not read twice.
-    const bool has_mask = DO_GA && a.mask, has_res = DO_GA && a.res, mask_is_a = DO_GA && DO_DW && a.mask == a.A;
+    const bool has_mask = DO_GA && (a.mask || (A8 && a.mask_codes)), has_res = DO_GA && a.res, mask_is_a = DO_GA && DO_DW && (A8 ? a.mask_codes != 0 : a.mask == a.A);
     const float* mask_p = (has_mask && !mask_is_a) ? a.mask : a.G;
     const float* res_p = has_res ? a.res : a.G;
     const size_t mmul = (has_mask && !mask_is_a) ? 1 : 0, rmul = has_res ? 1 : 0;
-    auto request = [&](TileRows& p, int tile) {
+    auto request = [&](TileRows<A8>& p, int tile) {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-            const size_t o = (size_t)min((long long)tile * TM + srow + 8 * it, a.rows - 1) * H + 4 * sq;
+            const size_t row = (size_t)min((long long)tile * TM + srow + 8 * it, a.rows - 1), o = row * H + 4 * sq;
             p.g[it] = *(const f32x4*)(a.G + o);
-            if constexpr (DO_DW) p.a[it] = *(const f32x4*)(a.A + o);
+            if constexpr (DO_DW) p.a[it].request(a.A, a.codes, a.scale, row, o);
             if constexpr (DO_GA) { p.m[it] = *(const f32x4*)(mask_p + o * mmul); p.r[it] = *(const f32x4*)(res_p + o * rmul); }
         }
     };
     // One tile: `cur` holds its rows; the next tile's are requested into `nxt` before anything else, so they have the
     // whole pass to arrive.  The two register sets swap roles from pass to pass (the loop below is unrolled by two):
     // nothing is copied from one to the other, and no pass ends waiting for its own requests or stores.
-    auto pass = [&](TileRows& cur, TileRows& nxt, int tile) {
+    auto pass = [&](TileRows<A8>& cur, TileRows<A8>& nxt, int tile) {
         const long long base = (long long)tile * TM;
         const int nvalid = (int)min((long long)TM, a.rows - base);
         request(nxt, min(tile + 1, t1 - 1));         // the last pass requests its own rows again (never used)
@@ -471,7 +490,7 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
             const f32x4 g = srow + 8 * it < nvalid ? cur.g[it] : zero4;     // rows past the end add nothing to the sums
             dbacc += g;
             splanes_store4(Gs, srow + 8 * it, 4 * sq, g);
-            if constexpr (DO_DW) splanes_store4(As, srow + 8 * it, 4 * sq, cur.a[it]);
+            if constexpr (DO_DW) splanes_store4(As, srow + 8 * it, 4 * sq, cur.a[it].get());
         }
         __syncthreads();
         if constexpr (DO_GA) {
@@ -488,16 +507,17 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 asm volatile("" : "+v"(nxt.g[it]), "+v"(nxt.m[it]), "+v"(nxt.r[it]));
-                if constexpr (DO_DW) asm volatile("" : "+v"(nxt.a[it]));
+                if constexpr (DO_DW) nxt.a[it].arrived();
             }
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 const int row = srow + 8 * it;
                 if (row < nvalid) {
                     f32x4 val = *(const f32x4*)(Ot + toff(row, sq, H / 4));
+                    const f32x4 am = DO_DW && mask_is_a ? cur.a[it].get() : cur.m[it];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float mk = (DO_DW && mask_is_a) ? cur.a[it][k] : cur.m[it][k];
+                        const float mk = am[k];
                         val[k] = (!has_mask || mk > 0.f) ? val[k] : 0.f;
                         val[k] += has_res ? cur.r[it][k] : 0.f;
                     }
@@ -506,7 +526,7 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
             }
         }
     };
-    TileRows ra, rb;
+    TileRows<A8> ra, rb;
     if (t0 < t1) request(ra, t0);
     for (int tile = t0; tile < t1; tile += 2) {
         pass(ra, rb, tile);
@@ -550,12 +570,14 @@ struct EdgeBwdArgs {
     const int* sender; const int* recv; const int* rowptr;
     const float* w0; const float* w1; const float* b1; const float* ln_w;
     float* g1; float* dpr; float* partial; int n_nodes; int n_edges;
+    const signed char* codes; const float* scale;              // e in 8 bits (mgn_train_edge_bwd_q8)
 };
 
 constexpr int PARTIAL_E = H * H + 3 * H;     // dW2 | db2 | dgamma | dbeta
 constexpr int PKH = H + 8;                   // halves per row of an fp16 plane
 constexpr int PLH = TM * PKH;                // halves per fp16 plane
 
+template <bool E8>
 __global__ __launch_bounds__(NT, 1) void train_edge_bwd_kernel(EdgeBwdArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned short elP[2 * PLH];        // e tile, fp16 planes
     __shared__ __attribute__((aligned(16))) unsigned short h1P[2 * PLH];        // h1 tile, fp16 planes; then Ot
@@ -585,7 +607,9 @@ __global__ __launch_bounds__(NT, 1) void train_edge_bwd_kernel(EdgeBwdArgs a) {
     const int e0 = __builtin_amdgcn_readfirstlane(srange[0]), e1 = __builtin_amdgcn_readfirstlane(srange[1]);
     const int last = e1 - e0 - 1;                    // row offsets are relative to e0 and clamped to [0, last]
     if (e0 < e1) {
-    const float* el_g = a.el + (size_t)e0 * H;
+    const float* el_g = E8 ? nullptr : a.el + (size_t)e0 * H;
+    const signed char* code_g = E8 ? a.codes + (size_t)e0 * H : nullptr;
+    const float* scale_g = E8 ? a.scale + e0 : nullptr;
     const float* ge_g = a.ge ? a.ge + (size_t)e0 * H : nullptr;
     float* g1_g = a.g1 + (size_t)e0 * H;
     const int* snd_g = a.sender + e0;
@@ -594,12 +618,16 @@ __global__ __launch_bounds__(NT, 1) void train_edge_bwd_kernel(EdgeBwdArgs a) {
     const int sc = t & (H - 1);                      // scan map: column sc, rows 16*sg .. 16*sg+15
     const int sg = __builtin_amdgcn_readfirstlane(t >> 7);
 
-    f32x4 pre[4];
+    RowPiece<E8> pre[4];
 #pragma unroll
-    for (int it = 0; it < 4; ++it) pre[it] = *(const f32x4*)(el_g + (unsigned)(min(srow + 8 * it, last) * H + 4 * sq));
+    for (int it = 0; it < 4; ++it) {
+        const int row = min(srow + 8 * it, last);
+        pre[it].request(el_g, code_g, scale_g, row, (unsigned)(row * H + 4 * sq));
+    }
     int s_cur = snd_g[min(j, last)], r_cur = rcv_g[min(j, last)];
-    // an absent edge-latent gradient is read all the same (row 0 of e, a line that stays in the cache) and dropped by a select
-    const float* ge_p = ge_g ? ge_g : el_g;
+    // an absent edge-latent gradient is read all the same (row 0 of e, or of the aggregate's gradient where e is in 8 bits: a
+    // line that stays in the cache) and dropped by a select
+    const float* ge_p = ge_g ? ge_g : E8 ? a.gaggr : el_g;
     const unsigned ge_mul = ge_g ? 1u : 0u;
     f32x4 gs[4], gr[4];
     {
@@ -608,7 +636,7 @@ __global__ __launch_bounds__(NT, 1) void train_edge_bwd_kernel(EdgeBwdArgs a) {
         for (int g = 0; g < 4; ++g) { gs[g] = *(const f32x4*)(a.ps + so + 8 * g); gr[g] = *(const f32x4*)(a.pr + ro + 8 * g); }
     }
 #pragma unroll
-    for (int it = 0; it < 4; ++it) hplanes_store4(elP, PLH, PKH, srow + 8 * it, 4 * sq, pre[it]);
+    for (int it = 0; it < 4; ++it) hplanes_store4(elP, PLH, PKH, srow + 8 * it, 4 * sq, pre[it].get());
     __syncthreads();
     STAMP_DECL
     for (int rel = 0; rel <= last; rel += TM) {
@@ -619,8 +647,10 @@ __global__ __launch_bounds__(NT, 1) void train_edge_bwd_kernel(EdgeBwdArgs a) {
         // the previous one)
         f32x4 ye[4], ya[4];
 #pragma unroll
-        for (int it = 0; it < 4; ++it)
-            pre[it] = *(const f32x4*)(el_g + (unsigned)(min(rel + TM + srow + 8 * it, last) * H + 4 * sq));
+        for (int it = 0; it < 4; ++it) {
+            const int row = min(rel + TM + srow + 8 * it, last);
+            pre[it].request(el_g, code_g, scale_g, row, (unsigned)(row * H + 4 * sq));
+        }
         const int s_nxt = snd_g[min(rel + TM + j, last)], r_nxt = rcv_g[min(rel + TM + j, last)];
         const int ra = r_cur;
         const int rb = (rel + j + 1 <= last) ? rcv_g[rel + j + 1] : -1;
@@ -661,7 +691,7 @@ __global__ __launch_bounds__(NT, 1) void train_edge_bwd_kernel(EdgeBwdArgs a) {
         acc = relu16(acc);                                                   // W_SCALE * v
         ln_local_stats_rows(acc, red, w, j, h);
 #pragma unroll
-        for (int it = 0; it < 4; ++it) hplanes_store4(elP, PLH, PKH, srow + 8 * it, 4 * sq, pre[it]);   // next tile
+        for (int it = 0; it < 4; ++it) hplanes_store4(elP, PLH, PKH, srow + 8 * it, 4 * sq, pre[it].get());   // next tile
         STAMP(5);
         __syncthreads();                                                     // (C) statistics exchanged; h1P dead
         STAMP(6);
@@ -1217,15 +1247,15 @@ extern "C" int mgn_train_linear_bwd(const float* G, const float* A, const float*
     MGN_REQUIRE(!dW || (A && scratch && lddw >= H), "mgn_train_linear_bwd");
     MGN_REQUIRE(!db || dW, "mgn_train_linear_bwd");
     MGN_REQUIRE(ldw % 4 == 0 || !GA, "mgn_train_linear_bwd");
-    LinBwdArgs a{G, A, W, ldw, koff, mask, res, GA, (float*)scratch, rows};
+    LinBwdArgs a{G, A, W, ldw, koff, mask, res, GA, (float*)scratch, rows, nullptr, nullptr, 0};
     const bool split = mgn_matmul_mode() >= 1;           // bf16 split products; "f32" keeps the fp32 matrix pipe
     int g = train_grid(rows, split ? 1 : 2);
     if (g > TRAIN_BLOCKS_MAX) g = TRAIN_BLOCKS_MAX - TRAIN_BLOCKS_MAX % 8;
     hipStream_t s = (hipStream_t)stream;
     if (split) {
-        if (GA && dW) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, true>), dim3(g), dim3(NT), 0, s, a);
-        else if (GA) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, false>), dim3(g), dim3(NT), 0, s, a);
-        else hipLaunchKernelGGL((train_linear_bwd3_kernel<false, true>), dim3(g), dim3(NT), 0, s, a);
+        if (GA && dW) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, true, false>), dim3(g), dim3(NT), 0, s, a);
+        else if (GA) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, false, false>), dim3(g), dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((train_linear_bwd3_kernel<false, true, false>), dim3(g), dim3(NT), 0, s, a);
     } else if (GA && dW) hipLaunchKernelGGL((train_linear_bwd_kernel<true, true>), dim3(g), dim3(NT), 0, s, a);
     else if (GA) hipLaunchKernelGGL((train_linear_bwd_kernel<true, false>), dim3(g), dim3(NT), 0, s, a);
     else hipLaunchKernelGGL((train_linear_bwd_kernel<false, true>), dim3(g), dim3(NT), 0, s, a);
@@ -1234,24 +1264,58 @@ extern "C" int mgn_train_linear_bwd(const float* G, const float* A, const float*
     return check_launch("mgn_train_linear_bwd");
 }
 
+static int edge_bwd(const char* name, EdgeBwdArgs a, float* dW1, float* db1, float* dgamma, float* dbeta, int64_t n_nodes, int64_t n_edges, hipStream_t s) {
+    MGN_REQUIRE(n_nodes > 0 && n_edges > 0 && n_nodes < (1ll << 24) && n_edges < (1ll << 24), name);
+    MGN_REQUIRE((a.el || (a.codes && a.scale)) && a.gaggr && a.ps && a.pr && a.sender && a.recv && a.rowptr && a.w0 && a.w1 && a.b1 && a.ln_w, name);
+    MGN_REQUIRE(a.g1 && a.dpr && dW1 && db1 && dgamma && dbeta && a.partial, name);
+    // receivers without in-edges are never visited by the scan
+    if (hipMemsetAsync(a.dpr, 0, (size_t)n_nodes * H * sizeof(float), s) != hipSuccess) return check_launch(name);
+    a.n_nodes = (int)n_nodes; a.n_edges = (int)n_edges;
+    const int g = train_grid(n_edges, 1);
+    if (a.codes) hipLaunchKernelGGL(train_edge_bwd_kernel<true>, dim3(g), dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL(train_edge_bwd_kernel<false>, dim3(g), dim3(NT), 0, s, a);
+    if (launch_reduce(a.partial, g, PARTIAL_E, PARTIAL_W, H, dW1, 3, db1, dgamma, dbeta, s))
+        { mgn_set_error("%s: the deferred-reduction list is full", name); return MGN_E_CAP; }
+    return check_launch(name);
+}
+
 extern "C" int mgn_train_edge_bwd(const float* e_in, const float* g_e, const float* g_aggr, const float* ps,
                                   const float* pr, const int32_t* sender, const int32_t* recv, const int32_t* rowptr,
                                   const float* w0, const float* w1, const float* b1, const float* ln_w, float* g1,
                                   float* dpr, float* dW1, float* db1, float* dgamma, float* dbeta, void* scratch,
                                   int64_t n_nodes, int64_t n_edges, void* stream) {
-    MGN_REQUIRE(n_nodes > 0 && n_edges > 0 && n_nodes < (1ll << 24) && n_edges < (1ll << 24), "mgn_train_edge_bwd");
-    MGN_REQUIRE(e_in && g_aggr && ps && pr && sender && recv && rowptr && w0 && w1 && b1 && ln_w, "mgn_train_edge_bwd");
-    MGN_REQUIRE(g1 && dpr && dW1 && db1 && dgamma && dbeta && scratch, "mgn_train_edge_bwd");
-    hipStream_t s = (hipStream_t)stream;
-    // receivers without in-edges are never visited by the scan
-    if (hipMemsetAsync(dpr, 0, (size_t)n_nodes * H * sizeof(float), s) != hipSuccess) return check_launch("mgn_train_edge_bwd");
-    EdgeBwdArgs a{e_in, g_e, g_aggr, ps, pr, sender, recv, rowptr, w0, w1, b1, ln_w, g1, dpr, (float*)scratch,
-                  (int)n_nodes, (int)n_edges};
-    const int g = train_grid(n_edges, 1);
-    hipLaunchKernelGGL(train_edge_bwd_kernel, dim3(g), dim3(NT), 0, s, a);
-    if (launch_reduce((const float*)scratch, g, PARTIAL_E, PARTIAL_W, H, dW1, 3, db1, dgamma, dbeta, s))
-        { mgn_set_error("mgn_train_edge_bwd: the deferred-reduction list is full"); return MGN_E_CAP; }
-    return check_launch("mgn_train_edge_bwd");
+    return edge_bwd("mgn_train_edge_bwd", EdgeBwdArgs{e_in, g_e, g_aggr, ps, pr, sender, recv, rowptr, w0, w1, b1, ln_w, g1, dpr, (float*)scratch, 0, 0, nullptr, nullptr},
+                    dW1, db1, dgamma, dbeta, n_nodes, n_edges, (hipStream_t)stream);
+}
+
+extern "C" int mgn_train_edge_bwd_q8(const int8_t* codes, const float* scale, const float* g_e, const float* g_aggr, const float* ps,
+                                     const float* pr, const int32_t* sender, const int32_t* recv, const int32_t* rowptr,
+                                     const float* w0, const float* w1, const float* b1, const float* ln_w, float* g1,
+                                     float* dpr, float* dW1, float* db1, float* dgamma, float* dbeta, void* scratch,
+                                     int64_t n_nodes, int64_t n_edges, void* stream) {
+    MGN_REQUIRE(codes && scale && ((uintptr_t)codes & 3) == 0, "mgn_train_edge_bwd_q8");
+    return edge_bwd("mgn_train_edge_bwd_q8", EdgeBwdArgs{nullptr, g_e, g_aggr, ps, pr, sender, recv, rowptr, w0, w1, b1, ln_w, g1, dpr, (float*)scratch, 0, 0,
+                                                         (const signed char*)codes, scale},
+                    dW1, db1, dgamma, dbeta, n_nodes, n_edges, (hipStream_t)stream);
+}
+
+extern "C" int mgn_train_linear_bwd_q8(const float* G, const int8_t* codes, const float* scale, const float* W, int32_t ldw, int32_t koff,
+                                       int32_t mask_codes, const float* mask, const float* res, float* GA, float* dW, int32_t lddw,
+                                       float* db, void* scratch, int64_t rows, void* stream) {
+    const char* name = "mgn_train_linear_bwd_q8";
+    MGN_REQUIRE(rows > 0 && rows < (1ll << 31) && G && codes && scale && ((uintptr_t)codes & 3) == 0, name);
+    MGN_REQUIRE(dW && scratch && lddw >= H, name);                        // codes are read for the weight gradient
+    MGN_REQUIRE(!GA || (W && ldw >= H && koff >= 0 && koff + H <= ldw && ldw % 4 == 0), name);
+    MGN_REQUIRE(!(mask_codes && mask) && (GA || !(mask_codes || mask || res)), name);
+    LinBwdArgs a{G, nullptr, W, ldw, koff, mask, res, GA, (float*)scratch, rows, (const signed char*)codes, scale, mask_codes};
+    int g = train_grid(rows, 1);
+    if (g > TRAIN_BLOCKS_MAX) g = TRAIN_BLOCKS_MAX - TRAIN_BLOCKS_MAX % 8;
+    const hipStream_t s = (hipStream_t)stream;
+    if (GA) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, true, true>), dim3(g), dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((train_linear_bwd3_kernel<false, true, true>), dim3(g), dim3(NT), 0, s, a);
+    if (launch_reduce((const float*)scratch, g, PARTIAL, PARTIAL_W, lddw, dW, db ? 1 : 0, db, nullptr, nullptr, s))
+        { mgn_set_error("%s: the deferred-reduction list is full", name); return MGN_E_CAP; }
+    return check_launch(name);
 }
 
 extern "C" int mgn_segment_sum(const float* src, const int32_t* rowptr, const int32_t* order, float* out,

@@ -7,7 +7,7 @@ RuntimeError on any non-zero return code.  torch is used for memory and streams 
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
@@ -221,6 +221,50 @@ def receiver_csr_dev(edge_index: torch.Tensor, num_nodes: int):
                                              cr.data_ptr(), perm.data_ptr(), _stream())
         _lib.check(rc, "mgn_receiver_csr_dev")
     return rowptr, cs, cr, perm
+
+
+# --------------------------------------------------------------------------- device: activations in 8 bits
+class Q8Rows(NamedTuple):
+    """Rows of activations in 8 bits: ``codes`` int8 [rows, width], ``scale`` float32 [rows]; x = codes * scale."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+def q8_rows(x, keep_nonzero: bool = False, out: Optional[Q8Rows] = None) -> Q8Rows:
+    """Keeps the rows of ``x`` [rows, width] (float32, bfloat16, float16) in 8 bits with a scale per row (``mgn_q8_rows``):
+    within half a scale of x.  ``keep_nonzero``: no other value than zero becomes zero (a ReLU's pattern is kept)."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _ATT_DTYPES:
+        raise RuntimeError("q8_rows: expected [rows, width] of float32, bfloat16 or float16")
+    rows, width = x.shape
+    if out is None:
+        out = Q8Rows(torch.empty(rows, width, dtype=torch.int8, device=x.device), torch.empty(rows, dtype=torch.float32, device=x.device))
+    with _on_device(x.device):
+        rc = _lib.lib().mgn_q8_rows(_dev(x, x.dtype, None, "x"), _ATT_DTYPES[x.dtype], rows, width, int(bool(keep_nonzero)),
+                                    _dev(out.codes, torch.int8, (rows, width), "codes"), _dev(out.scale, torch.float32, (rows,), "scale"), _stream())
+    _lib.check(rc, "mgn_q8_rows")
+    return out
+
+
+def q8_restore(kept: Q8Rows, dtype=torch.float32, out=None) -> torch.Tensor:
+    """The rows as values again (``mgn_q8_restore``)."""
+    rows, width = kept.codes.shape
+    if dtype not in _ATT_DTYPES:
+        raise RuntimeError(f"q8_restore: float32, bfloat16 or float16, got {dtype}")
+    if out is None:
+        out = torch.empty(rows, width, dtype=dtype, device=kept.codes.device)
+    with _on_device(kept.codes.device):
+        rc = _lib.lib().mgn_q8_restore(_dev(kept.codes, torch.int8, (rows, width), "codes"), _dev(kept.scale, torch.float32, (rows,), "scale"),
+                                       rows, width, _ATT_DTYPES[dtype], _dev(out, dtype, (rows, width), "out"), _stream())
+    _lib.check(rc, "mgn_q8_restore")
+    return out
+
+
+def _q8_128(kept: Q8Rows, name, rows=None):
+    return (_dev(kept.codes, torch.int8, (rows, H), name + " codes"), _dev(kept.scale, torch.float32, (kept.codes.shape[0],), name + " scale"))
 
 
 # --------------------------------------------------------------------------- device: attention over another set of states
@@ -998,7 +1042,8 @@ def train_ln_bwd(v, gamma, gpre, dgamma, dbeta, scratch, g=None, gg=None, idx=No
 
 @_timed_op
 def train_linear_bwd(g, scratch, a=None, w=None, koff=0, mask=None, res=None, ga=None, dw=None, dw_koff=0, db=None):
-    """``dw`` is the full [128, ld] gradient tensor; its columns dw_koff .. dw_koff+127 are written."""
+    """``dw`` is the full [128, ld] gradient tensor; its columns dw_koff .. dw_koff+127 are written.  ``a`` may be kept in
+    8 bits (:class:`Q8Rows`), and ``mask`` may then be the same object."""
     rows = g.shape[0]
     if ga is None and dw is None:
         raise RuntimeError("train_linear_bwd: nothing to compute")
@@ -1012,6 +1057,17 @@ def train_linear_bwd(g, scratch, a=None, w=None, koff=0, mask=None, res=None, ga
         if dw_koff < 0 or dw_koff + H > dw.shape[1]:
             raise RuntimeError("train_linear_bwd: dW column block out of range")
         dw_ptr, lddw = C.c_void_p(dw.data_ptr() + 4 * dw_koff), dw.shape[1]
+    if isinstance(a, Q8Rows):
+        if dw is None:
+            raise RuntimeError("train_linear_bwd: an 8-bit layer input is read for the weight gradient; without one leave it out")
+        if isinstance(mask, Q8Rows) and mask is not a:
+            raise RuntimeError("train_linear_bwd: an 8-bit mask is the layer input itself")
+        rc = _lib.lib().mgn_train_linear_bwd_q8(
+            _rows128(g, "G"), *_q8_128(a, "A", rows), C.c_void_p(0) if w is None else _wblock(w, koff, "W"), 0 if w is None else w.shape[1], koff,
+            int(mask is a), 0 if mask is a else _opt(mask, torch.float32, (rows, H), "mask"), _opt(res, torch.float32, (rows, H), "res"),
+            _opt(ga, torch.float32, (rows, H), "GA"), dw_ptr, lddw, _opt(db, torch.float32, (H,), "db"), _scratch(scratch, 0, rows), rows, _stream())
+        _lib.check(rc, "mgn_train_linear_bwd_q8")
+        return
     rc = _lib.lib().mgn_train_linear_bwd(
         _rows128(g, "G"), _opt(a, torch.float32, (rows, H), "A"),
         C.c_void_p(0) if w is None else _wblock(w, koff, "W"), 0 if w is None else w.shape[1], koff,
@@ -1024,10 +1080,12 @@ def train_linear_bwd(g, scratch, a=None, w=None, koff=0, mask=None, res=None, ga
 @_timed_op
 def train_edge_bwd(e_in, g_e, g_aggr, ps, pr, sender, recv, rowptr, w0, w1, b1, ln_w, g1, dpr, dw1, db1, dgamma, dbeta,
                    scratch):
-    """Fused backward of one block's edge MLP with recomputed hidden activations (default matrix path)."""
+    """Fused backward of one block's edge MLP with recomputed hidden activations (default matrix path).  ``e_in`` may be kept
+    in 8 bits (:class:`Q8Rows`): the activations are then recomputed from the restored rows."""
     e, n = e_in.shape[0], dpr.shape[0]
-    rc = _lib.lib().mgn_train_edge_bwd(
-        _rows128(e_in, "e_in"), _opt(g_e, torch.float32, (e, H), "g_e"), _dev(g_aggr, torch.float32, (None, H), "g_aggr"),
+    q8 = isinstance(e_in, Q8Rows)
+    rc = (_lib.lib().mgn_train_edge_bwd_q8 if q8 else _lib.lib().mgn_train_edge_bwd)(
+        *(_q8_128(e_in, "e_in") if q8 else (_rows128(e_in, "e_in"),)), _opt(g_e, torch.float32, (e, H), "g_e"), _dev(g_aggr, torch.float32, (None, H), "g_aggr"),
         _dev(ps, torch.float32, (None, H), "ps"), _dev(pr, torch.float32, (None, H), "pr"),
         _dev(sender, torch.int32, (e,), "sender"), _dev(recv, torch.int32, (e,), "recv"),
         _dev(rowptr, torch.int32, (n + 1,), "rowptr"), _dev(w0, torch.float32, (H, 3 * H), "w0"),

@@ -36,6 +36,10 @@ extern "C" {
 #define MGN_MAX_DEC_OUT 32   /* widest decoder output (node_out_dim * time_dim)      */
 #define MGN_MAX_PACK_SLICES 112   /* weight sets per mgn_pack_weights call           */
 
+#define MGN_F32  0           /* element types of the entry points that take one      */
+#define MGN_BF16 1
+#define MGN_F16  2
+
 #define MGN_E_ARG   (-1)     /* bad argument (null pointer, size out of range, ...)  */
 #define MGN_E_RANGE (-2)     /* index outside [0, N)                                 */
 #define MGN_E_CAP   (-3)     /* output capacity too small                            */
@@ -517,6 +521,29 @@ int mgn_knn_graph(const float* points /*[N][dim]*/, int32_t dim, const int64_t* 
                   const int32_t* coarse_ptr /*[n_blocks+1]*/, const int64_t* edge_ptr /*[n_blocks+1]*/, int32_t n_blocks,
                   int64_t max_block_points, int32_t k, int64_t* out_sender, int64_t* out_recv, void* stream);
 
+/* ---- activations in 8 bits for the backward pass -------------------------------------------------------------------
+ * What the training step keeps of its forward pass (the reference's autograd graph keeps fp32 tensors,
+ * run_train_multiscale.py:139-141) takes a quarter of the memory as codes -127 .. 127 with one fp32 scale per row:
+ *   scale = fl(m / 127), code = nearest whole number (ties to even) of x * fl(127 / m), m = largest magnitude of the row.
+ * x is off by at most half a scale.  keep_nonzero: a value other than zero keeps a code other than zero, so a ReLU's
+ * pattern survives (such a value is off by at most one scale).  A row that holds an infinity or a NaN comes back as NaN;
+ * rows below 2^-119 come back as zeros.  x [rows][width] dense, width 1 .. 1024, dtype MGN_F32 / MGN_BF16 / MGN_F16.      */
+int mgn_q8_rows(const void* x, int32_t dtype, int64_t rows, int32_t width, int32_t keep_nonzero, int8_t* codes, float* scale, void* stream);
+int mgn_q8_restore(const int8_t* codes, const float* scale, int64_t rows, int32_t width, int32_t dtype, void* x, void* stream);
+
+/* mgn_train_linear_bwd with the layer input in 8 bits, in every matrix mode on the split-bf16 products: dW = G^T A with
+ * A[r] = scale[r] * codes[r]; mask_codes: GA is zero where A is not positive (the ReLU that produced the layer input).       */
+int mgn_train_linear_bwd_q8(const float* G, const int8_t* codes, const float* scale, const float* W, int32_t ldw, int32_t koff,
+                            int32_t mask_codes, const float* mask, const float* res, float* GA, float* dW, int32_t lddw,
+                            float* db, void* scratch, int64_t rows, void* stream);
+
+/* mgn_train_edge_bwd with the edge latents that entered the block in 8 bits.                                                 */
+int mgn_train_edge_bwd_q8(const int8_t* codes, const float* scale, const float* g_e, const float* g_aggr, const float* ps,
+                          const float* pr, const int32_t* sender, const int32_t* recv, const int32_t* rowptr,
+                          const float* w0, const float* w1, const float* b1, const float* ln_w, float* g1,
+                          float* dpr, float* dW1, float* db1, float* dgamma, float* dbeta, void* scratch,
+                          int64_t n_nodes, int64_t n_edges, void* stream);
+
 /* ---- attention of one set of states over another (queries of one length, keys and values of another) ------------
  * o_i = sum_j p_ij v_j,  p_ij = softmax over j of  scale * <q_i, k_j> + bias_table[head][bucket_lut[place(i, j)]]
  * over the keys j of query i's segment whose mask is not zero.  Beside the message weights of the attention option
@@ -535,10 +562,6 @@ int mgn_knn_graph(const float* points /*[N][dim]*/, int32_t dim, const int64_t* 
  * stats [2][heads][n_q] (base-2 maximum and sum of each softmax): kept for mgn_attn_bwd; may be null.  out32
  * [n_q][heads][dim] (bf16 / fp16, or null): the outputs before they are rounded, which mgn_attn_bwd takes in place of out
  * (out_f32 set) where a bias table is trained: <g, o> enters every entry of dS and the table's gradient cancels.        */
-#define MGN_F32  0
-#define MGN_BF16 1
-#define MGN_F16  2
-
 typedef struct {
     const void* q; const void* k; const void* v;
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;      /* strides of tokens and heads, in elements                */
