@@ -111,3 +111,80 @@ def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=N
     if live is not None:
         out.grad_fn.live = live
     return out
+
+
+class CrossScaleReadout(nn.Module):
+    """What the coarse branch's final states tell every fine node: ``to_out(attention(to_q(x), to_k(xc), to_v(xc)))`` with a
+    learned bias by the distance between the two nodes, in lattice cells of the mesh (``reach`` cells along its longest side;
+    its table starts at zero).  Takes the place of the copy onto the sampled nodes (core/meshgraphnet.py:192-193) in
+    ``EncodeProcessDecodeMultiScale(coarse_readout="attention")``; every mesh of a batch reads its own coarse graph."""
+
+    def __init__(self, hidden_dim: int = H, heads: int = 4, num_buckets: int = 32, reach: int = 128):
+        super().__init__()
+        if hidden_dim != H:
+            raise NotImplementedError(f"CrossScaleReadout: hidden_dim must be {H} for the HIP kernels")
+        if heads < 1 or H % heads or (H // heads) % 8:
+            raise ValueError(f"CrossScaleReadout: {heads} heads do not divide {H} into widths that are multiples of 8")
+        self.heads, self.reach, self.num_buckets = heads, reach, num_buckets
+        self.to_q, self.to_k, self.to_v, self.to_out = (nn.Linear(H, H) for _ in range(4))
+        self.bias_table = nn.Parameter(torch.zeros(heads, num_buckets))
+        RelativeBuckets(num_buckets, reach, 2)                       # refuses sizes the kernels do not take
+        self.__dict__["_buckets"] = {}
+
+    def plan(self, mesh_pos: torch.Tensor, first: torch.Tensor, sizes=None, counts=None) -> dict:
+        """Places and segments of one mesh, or of the blocks of a batch (``sizes`` fine and ``counts`` coarse nodes each);
+        ``first``: the sampled nodes.  Depends on the mesh alone: kept with its coarse graph."""
+        pos = mesh_pos.detach().to(torch.float32)
+        axes = pos.shape[1]
+        if axes not in (2, 3):
+            raise RuntimeError(f"CrossScaleReadout: mesh coordinates have two or three axes, got {axes}")
+        cells, at = [], 0
+        for n in (sizes or (pos.shape[0],)):
+            p = pos[at: at + n]
+            low = p.amin(dim=0, keepdim=True)
+            side = (p - low).amax().clamp_min(1e-30)
+            cells.append(((p - low) * (self.reach / side)).to(torch.int32))
+            at += n
+        q_pos = torch.cat(cells).contiguous()
+        by_axes = self.__dict__["_buckets"]
+        if axes not in by_axes:
+            by_axes[axes] = RelativeBuckets(self.num_buckets, self.reach, axes)
+        many = sizes is not None and len(sizes) > 1
+        return dict(q_pos=q_pos, k_pos=q_pos[first].contiguous(), bucket_lut=by_axes[axes].lut(pos.device),
+                    q_ptr=ops._block_ptr(sizes, pos.device) if many else None, k_ptr=ops._block_ptr(counts, pos.device) if many else None)
+
+    def run(self, x: torch.Tensor, xc: torch.Tensor, plan: dict, out: torch.Tensor, keep: bool = False):
+        """``x`` [n, 128] fine and ``xc`` [m, 128] coarse states -> ``out`` [n, 128]; with ``keep`` returns what
+        :meth:`backward` needs."""
+        def linear(lin, rows, to=None):
+            to = torch.empty_like(rows) if to is None else to
+            ops.train_linear_fwd(rows, lin.weight.detach(), 0, to, bias=lin.bias.detach())
+            return to
+        q, k, v = linear(self.to_q, x), linear(self.to_k, xc), linear(self.to_v, xc)
+        split = lambda t: t.view(t.shape[0], self.heads, H // self.heads)  # noqa: E731
+        stats = torch.empty(2, self.heads, x.shape[0], dtype=torch.float32, device=x.device) if keep else None
+        o = torch.empty_like(q)
+        ops.cross_attention(split(q), split(k), split(v), bias_table=self.bias_table.detach(), out=split(o), stats=stats, **plan)
+        linear(self.to_out, o, out)
+        return (x, xc, q, k, v, o, stats, plan) if keep else None
+
+    def backward(self, kept, g: torch.Tensor, gx: torch.Tensor, gxc: torch.Tensor, scratch) -> dict:
+        """For the gradient ``g`` of the output: adds the fine states' gradient to ``gx``, writes the coarse states' to
+        ``gxc`` and returns the parameters' (deterministic sums throughout)."""
+        x, xc, q, k, v, o, stats, plan = kept
+        grads = {}
+
+        def linear_bwd(name, g_out, a, ga, res=None):
+            lin = getattr(self, name)
+            dw, db = torch.empty_like(lin.weight), torch.empty_like(lin.bias)
+            ops.train_linear_bwd(g_out, scratch, a=a, w=lin.weight.detach(), res=res, ga=ga, dw=dw, db=db)
+            grads[name + ".weight"], grads[name + ".bias"] = dw, db
+        split = lambda t: t.view(t.shape[0], self.heads, H // self.heads)  # noqa: E731
+        go = torch.empty_like(o)
+        linear_bwd("to_out", g, o, go)
+        dq, dk, dv, grads["bias_table"] = ops.cross_attention_bwd(split(go), split(q), split(k), split(v), split(o), stats,
+                                                                  bias_table=self.bias_table.detach(), **plan)
+        linear_bwd("to_q", dq.view_as(q), x, gx, res=gx)
+        linear_bwd("to_k", dk.view_as(k), xc, gxc)
+        linear_bwd("to_v", dv.view_as(v), xc, gxc, res=gxc)
+        return grads

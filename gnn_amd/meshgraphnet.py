@@ -233,8 +233,15 @@ class EncodeProcessDecodeMultiScale(nn.Module):
                  with_mat_params=True,
                  sample_ratio=0.5,
                  time_dim=1,
-                 device="cpu"):
+                 device="cpu",
+                 coarse_readout="copy",
+                 readout_heads=4):
+        """Arguments of the reference (core/meshgraphnet.py:123-134), and ``coarse_readout``: how the coarse branch's states
+        reach the fine nodes -- "copy" (the reference: rows of the sampled nodes, zeros elsewhere) or "attention" (every fine
+        node reads all coarse states of its mesh, ``attention.CrossScaleReadout`` with ``readout_heads`` heads)."""
         super().__init__()
+        if coarse_readout not in ("copy", "attention") or (coarse_readout == "attention" and not sample_ratio > 0):
+            raise ValueError('EncodeProcessDecodeMultiScale: coarse_readout is "copy" or, with sample_ratio > 0, "attention"')
         if hidden_size != H:
             raise NotImplementedError(f"EncodeProcessDecodeMultiScale: hidden_size must be {H}")
         if edge_in_dim != 7:
@@ -258,6 +265,13 @@ class EncodeProcessDecodeMultiScale(nn.Module):
                                               nn.Linear(hidden_size, node_out_dim * time_dim))
         else:
             self.node_decoder = MLP(hidden_size, node_out_dim * time_dim, hidden_dims=(hidden_size,), layer_norm=False)
+        self.coarse_readout = coarse_readout
+        if coarse_readout == "attention":
+            from .attention import CrossScaleReadout
+            self.readout = CrossScaleReadout(hidden_size, readout_heads)
+        # bits in which a training step keeps the activations of the processor blocks for its backward pass: 32, or 8
+        # (ops.Q8Rows: a quarter of the memory; the backward pass then sees activations within half a step of 1 / 127)
+        self.activation_bits = 32
         # first sample of the coarse graph's farthest-point sampling: None = drawn anew on every call, as the
         # reference does (core/meshgraphnet.py:248); an int pins it (and lets the coarse graph be cached)
         self.__dict__["coarse_start"] = None
@@ -352,6 +366,16 @@ class EncodeProcessDecodeMultiScale(nn.Module):
             hit = (key, CoarsePartition(halo, mesh_local, self.sample_ratio, int(start)), mesh_local, halo)
             self.__dict__["_coarse"] = hit
         return hit[1]
+
+    def _readout_plan(self, cg, mesh_pos, halo, graph):
+        """Places and segments of the attention readout; kept with the coarse graph they belong to."""
+        if halo is not None:
+            raise NotImplementedError('coarse_readout="attention": not on a partitioned mesh')
+        plan = cg.__dict__.get("readout_plan")
+        if plan is None:
+            sizes = tuple(int(b) for b in graph["batch_sizes"]) if "batch_sizes" in graph else None
+            plan = cg.__dict__["readout_plan"] = self.readout.plan(mesh_pos, cg.first, sizes, cg.block_sizes)
+        return plan
 
     def _coarse_workspace(self, device, cg, n_own):
         nc, ec = cg.num_nodes, cg.topology.num_edges
@@ -448,8 +472,11 @@ class EncodeProcessDecodeMultiScale(nn.Module):
                 proc.step_csr(cw.x, cw.e, cg.topology, cw.ps, cw.pr, cw.aggr, chalo, projected=i > 0,
                               next_block=None if last else cblocks[i + 1], store_edges=not last,
                               packed=(cpk.edge[i], cpk.node[i]) if cpk is not None else None)
-            cw.map_back.zero_()
-            ops.scatter_rows(cw.x[:nc_own], c_first, cw.map_back)
+            if self.coarse_readout == "attention":
+                self.readout.run(ws.x[:n_own], cw.x[:nc_own], self._readout_plan(cg, graph["mesh_pos"], halo, graph), cw.map_back)
+            else:
+                cw.map_back.zero_()
+                ops.scatter_rows(cw.x[:nc_own], c_first, cw.map_back)
         return ws, topo
 
     # ----------------------------------------------------------------- reference API

@@ -51,6 +51,11 @@ class _Deferred:
         return d
 
 
+def _keep8(t: torch.Tensor, relu: bool = False):
+    """One tensor of the forward pass in 8 bits (``relu``: its pattern of zeros is kept exactly)."""
+    return ops.q8_rows(t, keep_nonzero=relu)
+
+
 def _pad_cols(w: torch.Tensor) -> torch.Tensor:
     """[128, F] -> [128, 128] with zero columns (first Linear of an encoder)."""
     out = torch.zeros(H, H, dtype=torch.float32, device=w.device)
@@ -83,6 +88,12 @@ def forward_saving(model, graph, target_norm: torch.Tensor, fused=None, keep_hid
     dev = graph["mesh_pos"].device
     if dev.type != "cuda":
         raise RuntimeError("the training kernels run on the GPU only")
+    bits = model.__dict__.get("activation_bits", 32)
+    if bits not in (8, 32):
+        raise ValueError(f"activation_bits: 32 or 8, got {bits}")
+    if bits == 8 and (halo is not None or model.attention or not fused or keep_hidden):
+        raise NotImplementedError("activation_bits = 8: with the default matrix path (MGN_MATMUL=f16x2, fused edge update), without the attention "
+                                  "option and not on a partitioned mesh")
     if model.node_out_dim != 3:
         raise RuntimeError("loss: node_out_dim must be 3")
     f32 = model._f32
@@ -122,7 +133,7 @@ def forward_saving(model, graph, target_norm: torch.Tensor, fused=None, keep_hid
         ops.train_linear_fwd(inp, w0p, 0, h1, bias=seq[0].bias.detach(), relu=True)
         ops.train_linear_fwd(h1, seq[2].weight.detach(), 0, v, bias=seq[2].bias.detach())
         ops.train_ln_fwd(v, seq[3].weight.detach(), seq[3].bias.detach(), y=y)
-        return y, (inp, h1, v)
+        return y, ((inp, _keep8(h1, True), _keep8(v)) if bits == 8 else (inp, h1, v))
 
     x, enc_n = encoder(model.node_encoder, nf_pad)
     el, enc_e = encoder(model.edge_encoder, ef_pad)
@@ -187,8 +198,11 @@ def forward_saving(model, graph, target_norm: torch.Tensor, fused=None, keep_hid
             ops.train_linear_fwd(h1n, nm[2].weight.detach(), 0, vn, bias=nm[2].bias.detach(), relu=True)
             ops.train_ln_fwd(vn, nm[4].weight.detach(), nm[4].bias.detach(), res=x, yres=x_next)
             # with attention: the projected rows, alpha, the weights and the messages (fused path: as e_next - el)
-            layers.append((x, el, h1e, ve, aggr, h1n, vn, ps if fused else None, pr if fused else None,
-                           None if att is None else att + ((e_next, el) if fused else (eprime, None))))
+            if bits == 8:                           # the per-node projections are formed anew in the backward pass
+                layers.append((_keep8(x), _keep8(el), None, None, _keep8(aggr), _keep8(h1n, True), _keep8(vn, True), None, None, None))
+            else:
+                layers.append((x, el, h1e, ve, aggr, h1n, vn, ps if fused else None, pr if fused else None,
+                               None if att is None else att + ((e_next, el) if fused else (eprime, None))))
             x, el = x_next, e_next
 
         return x, layers
@@ -219,9 +233,14 @@ def forward_saving(model, graph, target_norm: torch.Tensor, fused=None, keep_hid
     map_back = None
     if model.sample_ratio > 0:
         xc, layers_c = run_blocks(list(model.coarse_processors), xc, elc, cg.topology, nc, nc_loc, ec, chalo)
-        map_back = torch.zeros(n, H, dtype=torch.float32, device=dev)
-        ops.scatter_rows(xc, c_first, map_back)                      # :192-193
-        coarse = dict(cg=cg, enc_c=enc_c, layers=layers_c, halo=chalo, first=c_first, nc=nc, nc_loc=nc_loc, ec=ec)
+        readout = None
+        if model.coarse_readout == "attention":
+            map_back = _empty(n, dev)
+            readout = model.readout.run(x, xc, model._readout_plan(cg, graph["mesh_pos"], halo, graph), map_back, keep=True)
+        else:
+            map_back = torch.zeros(n, H, dtype=torch.float32, device=dev)
+            ops.scatter_rows(xc, c_first, map_back)                  # :192-193
+        coarse = dict(cg=cg, enc_c=enc_c, layers=layers_c, halo=chalo, first=c_first, nc=nc, nc_loc=nc_loc, ec=ec, readout=readout)
 
     dec = model.node_decoder
     hd, decoded = _empty(n, dev), _empty(n, dev)
@@ -297,16 +316,26 @@ def _backward(model, saved, grad3, scratch, flush) -> Dict[str, torch.Tensor]:
         dps_loc = _empty(n_loc, dev)
         dps = dps_loc[:n]
         g2e, g1e = (None if saved["fused"] else _empty(e, dev)), _empty(e, dev)
+        restored = proj = None
+        if layers and isinstance(layers[0][1], ops.Q8Rows):
+            restored, proj = _empty(n, dev), (_empty(n_loc, dev), _empty(n_loc, dev))
         s_rowptr, s_order = topo.sender_view()
         rowptr = topo.rowptr[: n + 1]
         for i in range(len(blocks) - 1, -1, -1):
             blk, pre = blocks[i], f"{prefix}.{i}."
             em, nm = blk.edge_mlp, blk.node_mlp
             x, el, h1e, ve, aggr, h1n, vn, ps_b, pr_b, att = layers[i]
+            if isinstance(el, ops.Q8Rows):              # kept in 8 bits: the Linear and edge kernels read the codes themselves
+                vn = ops.q8_restore(vn, out=restored)
+                ps_b, pr_b = proj
             # node MLP: x_next = x + LN(ReLU(V2 ReLU(V1 [x, aggr] + c1) + c2))
             dg, dbt = vec(), vec()
             ops.train_ln_bwd(vn, nm[4].weight.detach(), g2n, dg, dbt, scratch, g=gx, relu_mask=True)
             grads[pre + "node_mlp.4.weight"], grads[pre + "node_mlp.4.bias"] = dg, dbt
+            if isinstance(x, ops.Q8Rows):
+                x_full = ops.q8_restore(x, out=restored)
+                ops.train_linear_fwd(x_full, em[0].weight.detach(), 0, ps_b)
+                ops.train_linear_fwd(x_full, em[0].weight.detach(), H, pr_b, bias=em[0].bias.detach())
             dw, db = g_like(nm[2].weight), vec()
             ops.train_linear_bwd(g2n, scratch, a=h1n, w=nm[2].weight.detach(), mask=h1n, ga=g1n, dw=dw, db=db)
             grads[pre + "node_mlp.2.weight"], grads[pre + "node_mlp.2.bias"] = dw, db
@@ -376,7 +405,11 @@ def _backward(model, saved, grad3, scratch, flush) -> Dict[str, torch.Tensor]:
     if coarse is not None:
         cg, nc, nc_loc, ec, c_first = coarse["cg"], coarse["nc"], coarse["nc_loc"], coarse["ec"], coarse["first"]
         gxc = _empty(nc, dev)
-        ops.gather_rows(gmap, c_first, gxc)           # rows of the mapped-back tensor that came from the coarse nodes
+        if coarse["readout"] is not None:             # every fine node read all coarse states of its mesh
+            for k, g in model.readout.backward(coarse["readout"], gmap, gx, gxc, scratch).items():
+                grads["readout." + k] = g
+        else:
+            ops.gather_rows(gmap, c_first, gxc)       # rows of the mapped-back tensor that came from the coarse nodes
         gec, g2ec, g1ec, _, _ = blocks_backward(list(model.coarse_processors), "coarse_processors", coarse["layers"], cg.topology,
                                                 coarse["halo"], gxc, nc, nc_loc, ec)
     ge, g2e, g1e, g2n, g1n = blocks_backward(list(model.processors), "processors", saved["layers"], topo, halo, gx, n, n_loc, e)
@@ -386,6 +419,8 @@ def _backward(model, saved, grad3, scratch, flush) -> Dict[str, torch.Tensor]:
     # ---- encoders: y = LN(W1 ReLU(W0 feat + b0) + b1), no gradient wanted for the features
     def encoder_bwd(seq, name, saved_enc, gy, g_a, g_b):
         inp, h1, v = saved_enc
+        if isinstance(v, ops.Q8Rows):
+            v = ops.q8_restore(v)
         dg, dbt = vec(), vec()
         ops.train_ln_bwd(v, seq[3].weight.detach(), g_a, dg, dbt, scratch, g=gy, relu_mask=False)
         grads[name + ".3.weight"], grads[name + ".3.bias"] = dg, dbt

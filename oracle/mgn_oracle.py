@@ -52,6 +52,7 @@ class OracleConfig:
     attention: bool = False            # core/meshgraphnet.py:60-61, :100-108
     sample_ratio: float = 0.0          # > 0: coarse branch, core/meshgraphnet.py:148-156, :179-194, :237-283
     coarse_process_steps: int = 0
+    coarse_readout: str = "copy"       # "attention": every fine node reads all coarse states (not in the reference)
 
 
 # --------------------------------------------------------------------------- edge build
@@ -397,8 +398,11 @@ def forward(sd, cfg: OracleConfig, norms: Dict[str, NormStats], g, *, return_lat
     if cfg.sample_ratio > 0:                                    # :187-194
         for i in range(cfg.coarse_process_steps):
             cx_h, ce_h = mp_layer(sd, f"coarse_processors.{i}", cx_h, cei, ce_h)
-        map_back = torch.zeros_like(x_h)
-        map_back[first] = cx_h
+        if cfg.coarse_readout == "attention":
+            map_back = attention_readout(sd, x_h, cx_h, g["mesh_pos"], first)
+        else:
+            map_back = torch.zeros_like(x_h)
+            map_back[first] = cx_h
         x_h = torch.cat([x_h, map_back], dim=-1)
     dec = mlp(sd, "node_decoder", x_h, final_relu=False, layer_norm=False)
     delta = dec.view(-1, cfg.time_dim, cfg.node_out_dim).permute(1, 0, 2)
@@ -407,6 +411,31 @@ def forward(sd, cfg: OracleConfig, norms: Dict[str, NormStats], g, *, return_lat
     if return_latents:
         return out, {"x_enc": x0, "e_enc": e0, "x_proc": x_h, "e_proc": e_h}
     return out
+
+
+def attention_readout(sd, x, cx, mesh_pos, first, reach: int = 128):
+    """Attention readout of the coarse branch in plain torch, differentiable, in the type of the weights: softmax over the
+    coarse nodes of scale <q, k> + table[head, bucket of the distance in lattice cells], heads side by side."""
+    def lin(name, t):
+        return t @ sd[f"readout.{name}.weight"].T + sd[f"readout.{name}.bias"]
+    table = sd["readout.bias_table"]
+    heads, n = table.shape
+    p = mesh_pos.float()
+    p = p - p.amin(dim=0, keepdim=True)
+    cells = (p * (reach / p.amax().clamp_min(1e-30))).to(torch.int32).long()
+    d2 = (cells[:, None] - cells[first][None]).square().sum(-1)
+    dist = d2.double().sqrt().long().clamp(max=reach)
+    exact, lut = n // 2, []
+    for d in range(reach + 1):
+        b = d
+        if d >= exact:                      # the last b with d >= exact (reach / exact)^((b - exact) / (n - exact))
+            b = max(c for c in range(exact, n) if c == exact or d ** (n - exact) * exact ** (c - exact) >= reach ** (c - exact) * exact ** (n - exact))
+        lut.append(b)
+    bias = table[:, torch.tensor(lut)[dist]]
+    split = lambda t: t.reshape(t.shape[0], heads, -1).transpose(0, 1)  # noqa: E731
+    q, k, v = split(lin("to_q", x)), split(lin("to_k", cx)), split(lin("to_v", cx))
+    w = torch.softmax(q @ k.transpose(1, 2) * q.shape[-1] ** -0.5 + bias, dim=-1)
+    return lin("to_out", (w @ v).transpose(0, 1).reshape(x.shape[0], -1))
 
 
 def predict(sd, cfg: OracleConfig, norms: Dict[str, NormStats], g, coarse_start: int = 0) -> torch.Tensor:
