@@ -32,6 +32,7 @@ constexpr float F32_MOST = 3.402823466e38f;
 constexpr int TOP = 14;                 // operands are scaled to magnitudes below 2^TOP
 constexpr int FAR_EXP = -60;            // a subtile so much smaller than the largest adds nothing in fp16; its shift stops here
 constexpr int ATT_TQ = 128;             // queries (or keys, in the key-gradient kernel) of a workgroup: 32 per wave
+constexpr int ATT_MAX_SPLITS = 256;
 constexpr int ATT_MAX_REACH = 1024;
 constexpr int ATT_MAX_BUCKETS = 64;
 
@@ -71,28 +72,41 @@ __device__ __forceinline__ void pack8(const float* v, u32x4& hi, u32x4& lo) {
     }
 }
 
-// eight consecutive elements of a row as floats; 16 bytes (32 for fp32), 16-byte aligned
-template <int KIND>
-__device__ __forceinline__ void load8(const void* base, long long off, float* v) {
-    if constexpr (KIND == AT_F32) {
-        const f32x4* p = (const f32x4*)((const float*)base + off);
-        const f32x4 a = p[0], b = p[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-    } else {
-        const u32x4 a = *(const u32x4*)((const unsigned short*)base + off);
+// eight consecutive elements of a row as they lie in memory; 16 bytes (32 for fp32), 16-byte aligned
+template <int KIND> struct Raw8 {
+    u32x4 w[KIND == AT_F32 ? 2 : 1];
+    __device__ __forceinline__ void zero() {
+        w[0] = u32x4{0, 0, 0, 0};
+        if constexpr (KIND == AT_F32) w[1] = w[0];
+    }
+    __device__ __forceinline__ void load(const void* base, long long off) {
+        const u32x4* p = (const u32x4*)((const char*)base + off * (KIND == AT_F32 ? 4 : 2));
+        w[0] = p[0];
+        if constexpr (KIND == AT_F32) w[1] = p[1];
+    }
+    __device__ __forceinline__ void get(float* v) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (KIND == AT_BF16) {
-                v[2 * i] = __uint_as_float(a[i] << 16);
-                v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+            const unsigned a = w[0][i];                       // a copy: a bit cast of the vector's element takes element 0
+            if constexpr (KIND == AT_F32) {
+                const unsigned b = w[1][i];
+                v[i] = __uint_as_float(a); v[4 + i] = __uint_as_float(b);
+            } else if constexpr (KIND == AT_BF16) {
+                v[2 * i] = __uint_as_float(a << 16);
+                v[2 * i + 1] = __uint_as_float(a & 0xffff0000u);
             } else {
-                const unsigned word = a[i];                   // a copy: a bit cast of the vector's element takes element 0
-                const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
+                const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, a), f32x2);
                 v[2 * i] = f[0]; v[2 * i + 1] = f[1];
             }
         }
     }
+};
+
+template <int KIND>
+__device__ __forceinline__ void load8(const void* base, long long off, float* v) {
+    Raw8<KIND> r;
+    r.load(base, off);
+    r.get(v);
 }
 
 template <int KIND>

@@ -2,19 +2,33 @@
 // lie, in whole rows, and all arithmetic is fp32.
 //
 // Memory bound: bytes = keys x (key + value row).  A workgroup takes one query token, up to eight query heads that share a
-// key head, and one piece of the keys; LPR lanes share a row (8 elements each), so a wave has 64 / LPR rows in flight per
-// load and four loads of keys and four of values outstanding.  Every row group keeps its own running maximum and sum, joined
+// key head, and one piece of the keys; LPR lanes share a row (8 elements each), so a load of a wave
+// covers 64 / LPR rows; four loads (two for fp32) of keys and of values are worked on while as many are on their way.  Every row group keeps its own running maximum and sum, joined
 // over the wave by exchanges and over the waves through LDS; pieces are joined by attn_join_kernel in a fixed order.
 #include "mgn_attn_host.h"
 
+#include <type_traits>
+
 namespace {
 
-template <int KIND, int LPR, int REP>
-__global__ __launch_bounds__(256) void attn_few_kernel(AttnFwd a) {
-    constexpr int RPW = 64 / LPR, U = 4;
+// Sum over the LPR lanes that share a row, by data-parallel exchanges within groups of 16 lanes (no LDS): neighbours, pairs,
+// then mirrored halves -- at each step both partners add the same two numbers, so all lanes hold the same sum.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+    auto add = [&](auto ctrl) { v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    add(std::integral_constant<int, 0xB1>());                        // lanes 1 0 3 2
+    add(std::integral_constant<int, 0x4E>());                        // lanes 2 3 0 1
+    if constexpr (LPR >= 8) add(std::integral_constant<int, 0x141>());    // mirrored in 8
+    if constexpr (LPR >= 16) add(std::integral_constant<int, 0x140>());   // mirrored in 16
+    return v;
+}
+
+template <int KIND, int LPR, int REP, bool bias>
+__global__ __launch_bounds__(256, REP == 8 && (bias || KIND == AT_F32) ? 1 : 2) void attn_few_kernel(AttnFwd a) {
+    constexpr int RPW = 64 / LPR, U = KIND == AT_F32 || REP == 8 || (bias && REP == 4) ? 2 : 4;
     __shared__ float joined[4][REP][LPR * 8 + 2];
-    __shared__ unsigned char lutb[2 * ATT_MAX_REACH + 1];
-    __shared__ float tab[REP][ATT_MAX_BUCKETS];
+    __shared__ unsigned char lutb[bias ? 2 * ATT_MAX_REACH + 1 : 1];
+    __shared__ float tab[REP][bias ? ATT_MAX_BUCKETS : 1];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6, part = lane % LPR, rg = lane / LPR;
     const int rep = a.heads / a.kv_heads, chunks = (rep + REP - 1) / REP;
     const int chunk = blockIdx.x % chunks, kvh = blockIdx.x / chunks % a.kv_heads, split = blockIdx.y;
@@ -39,7 +53,29 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnFwd a) {
         for (int c = 0; c < 8; ++c) { q[r][c] = on ? q[r][c] * a.c0 : 0.f; o[r][c] = 0.f; }
         m[r] = -__builtin_inff(); l[r] = 0.f;
     }
-    const bool bias = a.table != nullptr;
+    struct Piece { Raw8<KIND> k[U], v[U]; int use, x[bias ? U : 1], y[bias ? U : 1], z[bias ? U : 1]; } one, two;
+    auto request = [&](Piece& p, long long base) {
+        p.use = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long key = base + (u * 4 + w) * RPW + rg;
+            const bool use = key < k1 && (!a.mask || a.mask[key]);
+            p.use |= use ? 1 << u : 0;
+            p.k[u].zero(); p.v[u].zero();
+            if (use && d < a.dim) {
+                p.k[u].load(a.k, key * a.k_st + kvh * a.k_sh + d);
+                p.v[u].load(a.v, key * a.v_st + kvh * a.v_sh + d);
+            }
+            if constexpr (bias) {
+                p.x[u] = p.y[u] = p.z[u] = 0;
+                const int* at = a.k_pos + key * a.axes;
+                if (use) p.x[u] = at[0];
+                if (use && a.axes > 1) p.y[u] = at[1];
+                if (use && a.axes > 2) p.z[u] = at[2];
+            }
+        }
+    };
+    request(one, k0);                                           // on its way while the bias is set up
     int qx = 0, qy = 0, qz = 0;
     const float most = (float)(a.reach * a.reach) + 0.5f;
     if (bias) {
@@ -55,43 +91,31 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnFwd a) {
         }
         __syncthreads();
     }
-
-    for (long long base = k0; base < k1; base += 4 * RPW * U) {
-        float kv[U][8], vv[U][8];
-        bool use[U];
-        int bucket[U];
+    auto take = [&](const Piece& p) {
+        float s[U][REP];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long key = base + (u * 4 + w) * RPW + rg;
-            use[u] = key < k1 && (!a.mask || a.mask[key]);
-            if (use[u] && d < a.dim) {
-                load8<KIND>(a.k, key * a.k_st + kvh * a.k_sh + d, kv[u]);
-                load8<KIND>(a.v, key * a.v_st + kvh * a.v_sh + d, vv[u]);
-            } else {
+            float kv[8];
+            p.k[u].get(kv);
+            int bucket = 0;
+            if constexpr (bias)
+                bucket = lutb[a.axes == 1 ? place<1>(qx, qy, qz, p.x[u], p.y[u], p.z[u], 1, a.reach, most)
+                                          : place<2>(qx, qy, qz, p.x[u], p.y[u], p.z[u], a.axes, a.reach, most)];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) kv[u][c] = vv[u][c] = 0.f;
-            }
-            bucket[u] = 0;
-            if (bias && use[u]) {
-                const int* p = a.k_pos + key * a.axes;
-                const int kx = p[0], ky = a.axes > 1 ? p[1] : 0, kz = a.axes > 2 ? p[2] : 0;
-                bucket[u] = lutb[a.axes == 1 ? place<1>(qx, qy, qz, kx, ky, kz, 1, a.reach, most) : place<2>(qx, qy, qz, kx, ky, kz, a.axes, a.reach, most)];
+            for (int r = 0; r < REP; ++r) {
+                float x = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) x = __builtin_fmaf(q[r][c], kv[c], x);
+                x = row_sum<LPR>(x);
+                if constexpr (bias) x += tab[r][bucket];
+                s[u][r] = p.use >> u & 1 ? x : -__builtin_inff();
             }
         }
 #pragma unroll
         for (int r = 0; r < REP; ++r) {
-            float s[U], top = m[r];
+            float top = m[r];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                s[u] = 0.f;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) s[u] = __builtin_fmaf(q[r][c], kv[u][c], s[u]);
-#pragma unroll
-                for (int x = 1; x < LPR; x <<= 1) s[u] += __shfl_xor(s[u], x);
-                if (bias) s[u] += tab[r][bucket[u]];
-                s[u] = use[u] ? s[u] : -__builtin_inff();
-                top = fmaxf(top, s[u]);
-            }
+            for (int u = 0; u < U; ++u) top = fmaxf(top, s[u][r]);
             const float to = top == -__builtin_inff() ? 0.f : top, al = __builtin_amdgcn_exp2f(m[r] - to);
             m[r] = top;
             l[r] *= al;
@@ -99,12 +123,27 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnFwd a) {
             for (int c = 0; c < 8; ++c) o[r][c] *= al;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float p = __builtin_amdgcn_exp2f(s[u] - to);
-                l[r] += p;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) o[r][c] = __builtin_fmaf(p, vv[u][c], o[r][c]);
+                s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - to);
+                l[r] += s[u][r];
             }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float vv[8];
+            p.v[u].get(vv);
+#pragma unroll
+            for (int r = 0; r < REP; ++r)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[r][c] = __builtin_fmaf(s[u][r], vv[c], o[r][c]);
+        }
+    };
+    // two sets of rows that swap roles: the next one is on its way while this one is worked on
+    constexpr int STEP = 4 * RPW * U;
+    for (long long base = k0; base < k1; base += 2 * STEP) {
+        request(two, base + STEP);
+        take(one);
+        request(one, base + 2 * STEP);
+        if (base + STEP < k1) take(two);
     }
     // join the row groups of the wave, then the four waves
 #pragma unroll
@@ -164,12 +203,17 @@ __global__ __launch_bounds__(256) void attn_few_kernel(AttnFwd a) {
     }
 }
 
+template <int KIND, int LPR, int REP>
+void few_bias(const AttnFwd& f, dim3 grid, hipStream_t st) {
+    if (f.table) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, REP, true>), grid, dim3(256), 0, st, f);
+    else hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, REP, false>), grid, dim3(256), 0, st, f);
+}
 template <int KIND, int LPR>
 void few_rep(const AttnFwd& f, int rep, dim3 grid, hipStream_t st) {
-    if (rep == 1) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 1>), grid, dim3(256), 0, st, f);
-    else if (rep == 2) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 2>), grid, dim3(256), 0, st, f);
-    else if (rep == 4) hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 4>), grid, dim3(256), 0, st, f);
-    else hipLaunchKernelGGL((attn_few_kernel<KIND, LPR, 8>), grid, dim3(256), 0, st, f);
+    if (rep == 1) few_bias<KIND, LPR, 1>(f, grid, st);
+    else if (rep == 2) few_bias<KIND, LPR, 2>(f, grid, st);
+    else if (rep == 4) few_bias<KIND, LPR, 4>(f, grid, st);
+    else few_bias<KIND, LPR, 8>(f, grid, st);
 }
 template <int KIND>
 void few_kind(const AttnFwd& f, int rep, dim3 grid, hipStream_t st) {

@@ -363,34 +363,75 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
 }
 
 // ---------------------------------------------------------------------------------------------- join of split key ranges
-// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s; one thread per four output values.  Rows that belong to no segment are
-// left as they are.
-template <int KIND>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnFwd a, int dp) {
-    const int quads = a.dim / 4;
-    const long long item = (long long)blockIdx.x * 256 + threadIdx.x, n = a.n_q * a.heads * quads;
-    if (item >= n) return;
-    const int quad = (int)(item % quads), head = (int)(item / quads % a.heads);
-    const long long row = item / quads / a.heads;
-    if (row < seg_at(a.q_ptr, 0, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, a.n_seg, a.n_seg, a.n_q)) return;
+// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  A workgroup per (query, head) -- one wave where there are few pieces --:
+// the lanes first hold the factors of the pieces, then share the output's quads, groups of lanes taking every so-manieth piece
+// (latency bound: the loads of a group do not depend on each other); fixed order.  Rows that belong to no segment are left.
+template <int KIND, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_join_kernel(AttnFwd a) {
+    constexpr int QUADS = DP / 4, GROUPS = 64 * NW / QUADS;
+    __shared__ float fac[ATT_MAX_SPLITS], part_l[NW];
+    __shared__ f32x4 sums[NW][QUADS];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const int head = blockIdx.x % a.heads;
+    const long long row = blockIdx.x / a.heads, stride = a.heads * a.n_q, at = head * a.n_q + row;
     float m = -__builtin_inff();
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (((long long)s * a.heads + head) * a.n_q + row)]);
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * stride + at)]);
+    m = wave_max(m);                                             // every wave finds it for itself
     const float base = m == -__builtin_inff() ? 0.f : m;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const long long at = ((long long)s * a.heads + head) * a.n_q + row;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base);
-        l += f * a.part_ml[2 * at + 1];
-        o += f * *(const f32x4*)(a.part + at * dp + 4 * quad);
+    for (int s = t; s < a.splits; s += 64 * NW) {
+        const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * (s * stride + at));
+        const float f = __builtin_amdgcn_exp2f(ml[0] - base);
+        fac[s] = f;
+        l = __builtin_fmaf(f, ml[1], l);
     }
-    o *= l > 0.f ? 1.0f / l : 0.f;
-    store4<KIND>(a.out, row * a.o_st + head * a.o_sh + 4 * quad, o);
-    if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + 4 * quad) = o;
-    if (quad == 0 && a.stats) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    if (lane == 0) part_l[w] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) l += part_l[x];
+    const int quad = t % QUADS, group = t / QUADS;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = group; s < a.splits; s += GROUPS) o += fac[s] * *(const f32x4*)(a.part + (s * stride + at) * DP + 4 * quad);
+#pragma unroll
+    for (int x = QUADS; x < 64; x <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x);
+    if constexpr (NW > 1) {
+        if (lane < QUADS) sums[w][lane] = o;
+        __syncthreads();
+        if (t < QUADS) {
+            o = sums[0][t];
+#pragma unroll
+            for (int x = 1; x < NW; ++x) o += sums[x][t];
+        }
+    }
+    if (row < seg_at(a.q_ptr, 0, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, a.n_seg, a.n_seg, a.n_q)) return;
+    if (t < QUADS && 4 * quad < a.dim) {
+        o *= l > 0.f ? 1.0f / l : 0.f;
+        store4<KIND>(a.out, row * a.o_st + head * a.o_sh + 4 * quad, o);
+        if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + 4 * quad) = o;
+    }
+    if (t == 0 && a.stats) {
         a.stats[(long long)head * a.n_q + row] = m;
         a.stats[(long long)(a.heads + head) * a.n_q + row] = l;
     }
+}
+
+template <int KIND, int DP>
+void join_dp(const AttnFwd& f, hipStream_t st) {
+    const dim3 grid((unsigned)(f.n_q * f.heads));
+    if (f.splits > 32) hipLaunchKernelGGL((attn_join_kernel<KIND, DP, 4>), grid, dim3(256), 0, st, f);
+    else hipLaunchKernelGGL((attn_join_kernel<KIND, DP, 1>), grid, dim3(64), 0, st, f);
+}
+template <int KIND>
+void join_kind(const AttnFwd& f, int dp, hipStream_t st) {
+    if (dp == 32) join_dp<KIND, 32>(f, st);
+    else if (dp == 64) join_dp<KIND, 64>(f, st);
+    else join_dp<KIND, 128>(f, st);
 }
 
 template <int KIND, int DP>
@@ -509,11 +550,9 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
         else fwd_kind<AT_F32>(f, dp, bias, grid, st);
     }
     if (sp.splits > 1) {
-        const long long items = a.n_q * a.heads * (a.dim / 4);
-        const dim3 grid((unsigned)((items + 255) / 256));
-        if (kind == AT_BF16) hipLaunchKernelGGL((attn_join_kernel<AT_BF16>), grid, dim3(256), 0, st, f, dp);
-        else if (kind == AT_F16) hipLaunchKernelGGL((attn_join_kernel<AT_F16>), grid, dim3(256), 0, st, f, dp);
-        else hipLaunchKernelGGL((attn_join_kernel<AT_F32>), grid, dim3(256), 0, st, f, dp);
+        if (kind == AT_BF16) join_kind<AT_BF16>(f, dp, st);
+        else if (kind == AT_F16) join_kind<AT_F16>(f, dp, st);
+        else join_kind<AT_F32>(f, dp, st);
     }
     return check_launch("mgn_attn_fwd");
 }

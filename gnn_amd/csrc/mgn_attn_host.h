@@ -71,7 +71,7 @@ inline int attn_few_splits(const MgnAttn& a) {
     const int64_t blocks = attn_few_blocks(a), keys = a.n_k / a.n_seg;
     int64_t s = blocks > 0 ? 1024 / blocks : 1;
     if (s > keys / 256) s = keys / 256;
-    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    return (int)(s < 1 ? 1 : s > ATT_MAX_SPLITS ? ATT_MAX_SPLITS : s);
 }
 // The tiled kernel: the same, in pieces of at least 256 keys, when its query tiles leave compute units idle.
 inline int attn_fwd_splits(const MgnAttn& a) {
