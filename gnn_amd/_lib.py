@@ -34,7 +34,7 @@ class MgnAttn(C.Structure):
                 ("q_ptr", C.c_void_p), ("k_ptr", C.c_void_p), ("key_mask", C.c_void_p), ("bias_table", C.c_void_p),
                 ("bucket_lut", C.c_void_p), ("q_pos", C.c_void_p), ("k_pos", C.c_void_p), ("n_q", C.c_int64), ("n_k", C.c_int64),
                 ("n_seg", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32),
-                ("n_bucket", C.c_int32), ("reach", C.c_int32), ("axes", C.c_int32), ("scale", C.c_float), ("out_f32", C.c_int32)]
+                ("n_bucket", C.c_int32), ("reach", C.c_int32), ("axes", C.c_int32), ("scale", C.c_float), ("zero_outside", C.c_int32), ("out_f32", C.c_int32)]
 
 
 MAX_PACK_SLICES = 112                   # MGN_MAX_PACK_SLICES

@@ -104,7 +104,7 @@ def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=N
                     scale: Optional[float] = None):
     """:func:`gnn_amd.ops.cross_attention` with gradients of ``q``, ``k``, ``v`` and ``bias_table`` where they are wanted."""
     grads = (q, k, v, bias_table)
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in grads):
+    if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)):
         return ops.cross_attention(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
     live = _guard_capture(grads)
     out = _CrossAttention.apply(q, k, v, bias_table, q_ptr, k_ptr, key_mask, bucket_lut, q_pos, k_pos, scale)

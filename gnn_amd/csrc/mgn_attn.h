@@ -110,6 +110,13 @@ __device__ __forceinline__ void load8(const void* base, long long off, float* v)
 }
 
 template <int KIND>
+__device__ __forceinline__ float load1(const void* base, long long off) {
+    if constexpr (KIND == AT_F32) return ((const float*)base)[off];
+    else if constexpr (KIND == AT_BF16) return __uint_as_float((unsigned)((const unsigned short*)base)[off] << 16);
+    else return (float)((const _Float16*)base)[off];
+}
+
+template <int KIND>
 __device__ __forceinline__ void store4(void* base, long long off, f32x4 v) {
     if constexpr (KIND == AT_F32) *(f32x4*)((float*)base + off) = v;
     else *(u32x2*)((unsigned short*)base + off) = u32x2{pack2<KIND>(v[0], v[1]), pack2<KIND>(v[2], v[3])};
@@ -160,6 +167,19 @@ __device__ __forceinline__ Seg find_tile(const int* ptr, int n_seg, long long T,
     g.len = (int)(end > g.first ? end - g.first : 0);
     g.local = tile - (int)((g.first >> shift) + lo);
     return g;
+}
+
+// Rows of a dense or strided output that belong to no segment, set to zero by all workgroups of a launch together.
+template <int KIND>
+__device__ __forceinline__ void zero_outside(const int* ptr, int n_seg, long long T, void* out, long long st, long long sh, int heads, int dim) {
+    const long long lo = seg_at(ptr, 0, n_seg, T), hi = seg_at(ptr, n_seg, n_seg, T), n = lo + (T - hi);
+    if (!ptr || n <= 0 || hi < lo) return;
+    const int quads = dim / 4;
+    for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x; i < n * heads * quads;
+         i += (long long)gridDim.x * gridDim.y * blockDim.x) {
+        const long long r = i / quads / heads, row = r < lo ? r : hi + (r - lo);
+        store4<KIND>(out, row * st + i / quads % heads * sh + 4 * (i % quads), f32x4{0.f, 0.f, 0.f, 0.f});
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ places and buckets

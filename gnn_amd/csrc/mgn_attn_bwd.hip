@@ -26,6 +26,7 @@ struct AttnBwd {
     void *dq, *dk, *dv;                                // dense [tokens][heads][dim]
     double* tpart; float* dtable; int q_tiles;         // [q_tiles][heads][n_bucket]
     int splits; float* part;                           // [split][2][kv_heads][ns_k][32][DP]
+    int zero;                                          // rows outside all segments become zeros
 };
 
 constexpr int PSHIFT = 13;
@@ -44,6 +45,7 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), tile = blockIdx.x / a.heads;
+    if (a.zero) zero_outside<KIND>(a.q_ptr, a.n_seg, a.n_q, a.dq, (long long)a.heads * a.dim, a.dim, a.heads, a.dim);
     const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 7, tile);
     const bool live = g.local >= 0 && g.local * ATT_TQ < g.len;
     if (!live) {
@@ -228,6 +230,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x % a.kv_heads, rep = a.heads / a.kv_heads, split = blockIdx.y;
+    if (a.zero) {
+        zero_outside<KIND>(a.k_ptr, a.n_seg, a.n_k, a.dk, (long long)a.kv_heads * a.dim, a.dim, a.kv_heads, a.dim);
+        zero_outside<KIND>(a.k_ptr, a.n_seg, a.n_k, a.dv, (long long)a.kv_heads * a.dim, a.dim, a.kv_heads, a.dim);
+    }
     const Seg g = find_tile(a.k_ptr, a.n_seg, a.n_k, 7, blockIdx.x / a.kv_heads);
     if (g.local < 0 || g.local * ATT_TQ >= g.len) return;
     const long long q0 = seg_at(a.q_ptr, g.seg, a.n_seg, a.n_q), q1 = seg_at(a.q_ptr, g.seg + 1, a.n_seg, a.n_q);
@@ -531,7 +537,7 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     b.qpos = (const int*)(ws + s.qpos); b.kpos = (const int*)(ws + s.kpos);
     b.table = a.bias_table; b.lut = a.bucket_lut; b.n_bucket = a.n_bucket; b.reach = a.reach; b.axes = a.axes;
     b.dq = dq; b.dk = dk; b.dv = dv; b.dtable = dtable; b.tpart = dtable ? (double*)(ws + s.tpart) : nullptr; b.q_tiles = s.q_tiles;
-    b.splits = s.splits; b.part = (float*)(ws + s.part);
+    b.zero = a.zero_outside && a.q_ptr; b.splits = s.splits; b.part = (float*)(ws + s.part);
     const bool fits = kind == AT_BF16 ? bwd_kind<AT_BF16>(b, s, dp, bias, st) : kind == AT_F16 ? bwd_kind<AT_F16>(b, s, dp, bias, st)
                                                                                            : bwd_kind<AT_F32>(b, s, dp, bias, st);
     if (!fits) { mgn_set_error("mgn_attn_bwd: %d buckets at width %d do not fit the compute unit's local memory", a.n_bucket, a.dim); return MGN_E_ARG; }

@@ -38,7 +38,14 @@ __global__ __launch_bounds__(256, REP == 8 && (bias || KIND == AT_F32) ? 1 : 2) 
         const int mid = (lo + hi) >> 1;
         if (seg_at(a.q_ptr, mid, a.n_seg, a.n_q) <= row) lo = mid; else hi = mid;
     }
-    if (row < seg_at(a.q_ptr, lo, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, lo + 1, a.n_seg, a.n_q)) return;
+    if (row < seg_at(a.q_ptr, lo, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, lo + 1, a.n_seg, a.n_q)) {
+        const int quads = a.dim / 4;
+        if (a.zero && split == 0)
+            for (int x = t; x < REP * quads; x += 256)
+                if (chunk * REP + x / quads < rep)
+                    store4<KIND>(a.out, row * a.o_st + (kvh * rep + chunk * REP + x / quads) * a.o_sh + 4 * (x % quads), f32x4{0.f, 0.f, 0.f, 0.f});
+        return;
+    }
     const long long f = seg_at(a.k_ptr, lo, a.n_seg, a.n_k), e = seg_at(a.k_ptr, lo + 1, a.n_seg, a.n_k);
     const long long len = e > f ? e - f : 0, per = (len + a.splits - 1) / a.splits;
     const long long k0 = f + (split * per < len ? split * per : len), k1 = k0 + per < f + len ? k0 + per : f + len;

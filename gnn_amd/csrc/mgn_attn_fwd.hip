@@ -147,6 +147,7 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), split = blockIdx.y;
+    if (a.zero) zero_outside<KIND>(a.q_ptr, a.n_seg, a.n_q, a.out, a.o_st, a.o_sh, a.heads, a.dim);
     const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 7, blockIdx.x / a.heads);
     if (g.local < 0 || g.local * ATT_TQ >= g.len) return;
     const long long k0 = seg_at(a.k_ptr, g.seg, a.n_seg, a.n_k), k1 = seg_at(a.k_ptr, g.seg + 1, a.n_seg, a.n_k);
@@ -362,6 +363,224 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
     }
 }
 
+// ---------------------------------------------------------------------------------------------- small problems
+// One launch and no images: a workgroup takes 32 queries of a head, its four waves every fourth subtile of the keys, which they
+// read where they lie (keys row by row, values column by column, both straight into operand registers) and scale themselves;
+// the waves' sums meet in LDS.  Latency bound: what counts is the length of the chain, not the conversions done again in
+// every workgroup.
+template <int KIND, int DP, int BIAS, bool P2>
+__global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 : 2) void attn_small_kernel(AttnFwd a) {
+    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, LD = DP + 4;
+    constexpr int SHIFT = KIND == AT_BF16 ? 0 : 13;
+    __shared__ float lutb[BIAS ? 2 * ATT_MAX_REACH + 1 : 1];
+    __shared__ __attribute__((aligned(16))) float sums[4][32][LD];
+    __shared__ float mls[4][2][32];
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads);
+    if (a.zero) zero_outside<KIND>(a.q_ptr, a.n_seg, a.n_q, a.out, a.o_st, a.o_sh, a.heads, a.dim);
+    const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 5, blockIdx.x / a.heads);
+    if (g.local < 0 || g.local * 32 >= g.len) return;
+    const long long k0 = seg_at(a.k_ptr, g.seg, a.n_seg, a.n_k), k1 = seg_at(a.k_ptr, g.seg + 1, a.n_seg, a.n_k);
+    const int klen = (int)(k1 > k0 ? k1 - k0 : 0), n_sub = (klen + 31) >> 5;
+    const int qi = g.local * 32 + j;
+    const long long row = g.first + min(qi, g.len - 1);
+
+    u32x4 qh[NC], ql[NC];
+    float cq = a.c0;
+    {
+        float v[NC][8], top = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = 16 * c + 8 * h;
+            if (d < a.dim) load8<KIND>(a.q, row * a.q_st + head * a.q_sh + d, v[c]);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
+        }
+        if constexpr (KIND != AT_BF16) {
+            const int ex = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
+            cq *= pow2i(ex);
+            const float by = pow2i(-ex);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] *= by;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) pack8<KIND>(v[c], qh[c], ql[c]);
+    }
+    int qx = 0, qy = 0, qz = 0;
+    float most = 0.f;
+    if constexpr (BIAS > 0) {
+        const int* p = a.q_pos + row * a.axes;
+        qx = p[0];
+        if (a.axes > 1) qy = p[1];
+        if (a.axes > 2) qz = p[2];
+        most = (float)(a.reach * a.reach) + 0.5f;
+        const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
+        for (int r = t; r < entries; r += 256)
+            lutb[r] = bias_log2(a.table[head * a.n_bucket + min(max(a.lut[r], 0), a.n_bucket - 1)]);
+        __syncthreads();
+    }
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = zero16();
+    float m = -__builtin_inff(), l = 0.f;
+    int ev = -126;                                              // exponent of the values' sums so far
+    for (int sub = w; sub < n_sub; sub += 4) {
+        const int key = 32 * sub + j;
+        const bool use = key < klen && (!a.mask || a.mask[k0 + key]);
+        const unsigned valid = (unsigned)__ballot(use);         // both halves of the wave hold the same keys
+        u32x4 kh[NC], kl[NC], vh[2][NB], vl[2][NB];
+        int ek = 0, e1 = 0;
+        {
+            float v[NC][8], top = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 16 * c + 8 * h;
+                if (use && d < a.dim) load8<KIND>(a.k, (k0 + key) * a.k_st + kvh * a.k_sh + d, v[c]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+            }
+            float x[2][NB][8], topv = 0.f;                      // values: column 32 b + j of keys 16 kc + 4 h + (0 .. 3, 8 .. 11)
+#pragma unroll
+            for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int n = 16 * kc + 4 * h + (e & 3) + 8 * (e >> 2), d = 32 * b + j;
+                        x[kc][b][e] = (valid >> n & 1) && d < a.dim ? load1<KIND>(a.v, (k0 + 32 * sub + n) * a.v_st + kvh * a.v_sh + d) : 0.f;
+                    }
+            if constexpr (KIND != AT_BF16) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
+#pragma unroll
+                for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) topv = fmaxf(topv, fabsf(x[kc][b][e]));
+#pragma unroll
+                for (int o2 = 32; o2 > 0; o2 >>= 1) { top = fmaxf(top, __shfl_xor(top, o2)); topv = fmaxf(topv, __shfl_xor(topv, o2)); }
+                ek = scale_exp<KIND>(top); e1 = scale_exp<KIND>(topv);
+                const float bk = pow2i(-ek), bv = pow2i(-e1);
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[c][e] *= bk;
+#pragma unroll
+                for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[kc][b][e] *= bv;
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) pack8<KIND>(v[c], kh[c], kl[c]);
+#pragma unroll
+            for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) pack8<KIND>(x[kc][b], vh[kc][b], vl[kc][b]);
+        }
+        f32x16 s = zero16();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if constexpr (PL == 2) {
+                s = mma<KIND>(kl[c], qh[c], s);
+                s = mma<KIND>(kh[c], ql[c], s);
+            }
+            s = mma<KIND>(kh[c], qh[c], s);
+        }
+        const float c = KIND == AT_BF16 ? cq : cq * pow2i(ek);
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int n = 8 * (e >> 2) + 4 * h + (e & 3);
+            float x = s[e] * c;
+            if constexpr (BIAS > 0) {
+                const int* p = a.k_pos + (k0 + min(32 * sub + n, klen - 1)) * a.axes;
+                x = __builtin_fmaf(s[e], c, lutb[place<BIAS>(qx, qy, qz, p[0], a.axes > 1 ? p[1] : 0, a.axes > 2 ? p[2] : 0, a.axes, a.reach, most)]);
+            }
+            s[e] = valid >> n & 1 ? x : -__builtin_inff();
+            top = fmaxf(top, s[e]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
+        const int en = max(ev, e1);
+        const float al = __builtin_amdgcn_exp2f(m - base), ao = al * pow2i(ev - en), sh = pow2i(SHIFT + max(e1 - en, FAR_EXP));
+        l *= al;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[b][e] *= ao;
+        m = mn; ev = en;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = __builtin_amdgcn_exp2f(s[e] - base);
+            l += s[e];
+            if constexpr (KIND != AT_BF16) s[e] *= sh;
+        }
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+            float pv[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pv[e] = s[8 * kc + e];
+            u32x4 ph, plo;
+            pack8<KIND, P2 || PL == 2>(pv, ph, plo);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if constexpr (PL == 2) o[n] = mma<KIND>(vl[kc][n], ph, o[n]);
+                if constexpr (P2 || PL == 2) o[n] = mma<KIND>(vh[kc][n], plo, o[n]);
+                o[n] = mma<KIND>(vh[kc][n], ph, o[n]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+    const int back = KIND == AT_BF16 ? 0 : ev - SHIFT;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[n][4 * q + e] : ldexpf(o[n][4 * q + e], back);
+            *(f32x4*)&sums[w][j][32 * n + 8 * q + 4 * h] = v;
+        }
+    if (h == 0) { mls[w][0][j] = m; mls[w][1][j] = l; }
+    __syncthreads();
+    for (int x = t; x < 32 * (DP / 4); x += 256) {
+        const int r = x / (DP / 4), d = 4 * (x % (DP / 4));
+        if (g.local * 32 + r >= g.len || d >= a.dim) continue;
+        float top = -__builtin_inff(), total = 0.f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) top = fmaxf(top, mls[n][0][r]);
+        const float base = top == -__builtin_inff() ? 0.f : top;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float f = __builtin_amdgcn_exp2f(mls[n][0][r] - base);
+            total = __builtin_fmaf(f, mls[n][1][r], total);
+            v += f * *(const f32x4*)&sums[n][r][d];
+        }
+        v *= total > 0.f ? 1.0f / total : 0.f;
+        const long long out = g.first + g.local * 32 + r;
+        store4<KIND>(a.out, out * a.o_st + head * a.o_sh + d, v);
+        if (P2) *(f32x4*)(a.out32 + (out * a.heads + head) * a.dim + d) = v;
+        if (d == 0 && a.stats) {
+            a.stats[(long long)head * a.n_q + out] = top;
+            a.stats[(long long)(a.heads + head) * a.n_q + out] = total;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- join of split key ranges
 // o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  A workgroup per (query, head) -- one wave where there are few pieces --:
 // the lanes first hold the factors of the pieces, then share the output's quads, groups of lanes taking every so-manieth piece
@@ -434,24 +653,29 @@ void join_kind(const AttnFwd& f, int dp, hipStream_t st) {
     else join_dp<KIND, 128>(f, st);
 }
 
+template <int KIND, int DP, int BIAS, bool P2>
+void fwd_launch(const AttnFwd& f, bool small, dim3 grid, hipStream_t st) {
+    if (small) hipLaunchKernelGGL((attn_small_kernel<KIND, DP, BIAS, P2>), grid, dim3(256), 0, st, f);
+    else hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, BIAS, P2>), grid, dim3(256), 0, st, f);
+}
 template <int KIND, int DP>
-void fwd_bias(const AttnFwd& f, int bias, dim3 grid, hipStream_t st) {
+void fwd_bias(const AttnFwd& f, bool small, int bias, dim3 grid, hipStream_t st) {
     constexpr bool TWO = KIND != AT_F32;
     if (f.out32) {
-        if (bias == 0) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 0, TWO>), grid, dim3(256), 0, st, f);
-        else if (bias == 1) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 1, TWO>), grid, dim3(256), 0, st, f);
-        else hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 2, TWO>), grid, dim3(256), 0, st, f);
+        if (bias == 0) fwd_launch<KIND, DP, 0, TWO>(f, small, grid, st);
+        else if (bias == 1) fwd_launch<KIND, DP, 1, TWO>(f, small, grid, st);
+        else fwd_launch<KIND, DP, 2, TWO>(f, small, grid, st);
     } else {
-        if (bias == 0) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 0, false>), grid, dim3(256), 0, st, f);
-        else if (bias == 1) hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 1, false>), grid, dim3(256), 0, st, f);
-        else hipLaunchKernelGGL((attn_fwd_kernel<KIND, DP, 2, false>), grid, dim3(256), 0, st, f);
+        if (bias == 0) fwd_launch<KIND, DP, 0, false>(f, small, grid, st);
+        else if (bias == 1) fwd_launch<KIND, DP, 1, false>(f, small, grid, st);
+        else fwd_launch<KIND, DP, 2, false>(f, small, grid, st);
     }
 }
 template <int KIND>
-void fwd_kind(const AttnFwd& f, int dp, int bias, dim3 grid, hipStream_t st) {
-    if (dp == 32) fwd_bias<KIND, 32>(f, bias, grid, st);
-    else if (dp == 64) fwd_bias<KIND, 64>(f, bias, grid, st);
-    else fwd_bias<KIND, 128>(f, bias, grid, st);
+void fwd_kind(const AttnFwd& f, bool small, int dp, int bias, dim3 grid, hipStream_t st) {
+    if (dp == 32) fwd_bias<KIND, 32>(f, small, bias, grid, st);
+    else if (dp == 64) fwd_bias<KIND, 64>(f, small, bias, grid, st);
+    else fwd_bias<KIND, 128>(f, small, bias, grid, st);
 }
 template <int KIND>
 void image_kind(const ImageArgs& a, int dp, hipStream_t st) {
@@ -464,14 +688,14 @@ void image_kind(const ImageArgs& a, int dp, hipStream_t st) {
 // workspace of the forward pass, in this order (256-byte aligned pieces)
 struct FwdSpace { size_t kimg, vimg, rec, kpos, part, ml, total; int ns_k, splits; };
 
-FwdSpace fwd_space(const MgnAttn& a, bool few) {
+FwdSpace fwd_space(const MgnAttn& a, bool few, bool small) {
     FwdSpace s{};
     const int dp = attn_dp(a.dim), pl = a.dtype == MGN_F32 ? 2 : 1;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) & ~(size_t)255; return p; };
     s.ns_k = attn_subtiles(a.n_k, a.n_seg);
-    s.splits = few ? attn_few_splits(a) : attn_fwd_splits(a);
-    if (!few) {
+    s.splits = few ? attn_few_splits(a) : small ? 1 : attn_fwd_splits(a);
+    if (!few && !small) {
         // one spare subtile: a pair of subtiles is copied (and its second half ignored) past the end
         s.kimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
         s.vimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
@@ -499,7 +723,8 @@ int mgn_attn_launch_images(int kind, int dp, const void* args, void* stream) {
 
 extern "C" int64_t mgn_attn_fwd_workspace_bytes(const MgnAttn* a) {
     if (attn_check(a, "mgn_attn_fwd_workspace_bytes") != 0) return -1;
-    return (int64_t)fwd_space(*a, attn_is_few(*a)).total;
+    const bool few = attn_is_few(*a);
+    return (int64_t)fwd_space(*a, few, !few && attn_is_small(*a)).total;
 }
 
 extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_t out_sh, float* stats, float* out32, void* workspace,
@@ -507,8 +732,8 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
     if (const int rc = attn_check(ap, "mgn_attn_fwd")) return rc;
     const MgnAttn& a = *ap;
     if (a.n_q == 0) return 0;
-    const bool few = attn_is_few(a);
-    const FwdSpace sp = fwd_space(a, few);
+    const bool few = attn_is_few(a), small = !few && attn_is_small(a);
+    const FwdSpace sp = fwd_space(a, few, small);
     if (!out || (sp.total > 0 && (!workspace || workspace_bytes < (int64_t)sp.total))) {
         mgn_set_error("mgn_attn_fwd: null output, or a workspace of %lld bytes where %lld are needed", (long long)workspace_bytes, (long long)sp.total);
         return MGN_E_ARG;
@@ -525,6 +750,7 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
     f.heads = a.heads; f.kv_heads = a.kv_heads; f.dim = a.dim; f.c0 = a.scale * LOG2E;
     f.q_pos = a.q_pos; f.table = a.bias_table; f.lut = a.bucket_lut; f.n_bucket = a.n_bucket; f.reach = a.reach; f.axes = a.axes;
     f.out = out; f.o_st = out_st; f.o_sh = out_sh; f.stats = stats; f.out32 = a.dtype == MGN_F32 ? nullptr : out32; f.splits = sp.splits;
+    f.zero = a.zero_outside && a.q_ptr;
     if (sp.splits > 1) { f.part = (float*)(ws + sp.part); f.part_ml = (float*)(ws + sp.ml); }
     if (few) {
         mgn_attn_launch_few(kind, &f, stream);
@@ -532,7 +758,7 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
         unsigned short *kimg = (unsigned short*)(ws + sp.kimg), *vimg = (unsigned short*)(ws + sp.vimg);
         int* rec = (int*)(ws + sp.rec);
         int* kpos = (int*)(ws + sp.kpos);
-        if (a.n_k > 0) {
+        if (a.n_k > 0 && !small) {
             ImageArgs im{};
             const int units = sp.ns_k * a.kv_heads;
             im.n_job = 2; im.units = 2 * units; im.n_seg = a.n_seg; im.dim = a.dim;
@@ -544,10 +770,10 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
             mgn_attn_launch_images(kind, dp, &im, stream);
         }
         f.kimg = kimg; f.vimg = vimg; f.rec = (const i32x4*)rec; f.ns_k = sp.ns_k; f.kpos = kpos;
-        const dim3 grid((unsigned)((a.n_q / ATT_TQ + a.n_seg) * a.heads), (unsigned)sp.splits);
-        if (kind == AT_BF16) fwd_kind<AT_BF16>(f, dp, bias, grid, st);
-        else if (kind == AT_F16) fwd_kind<AT_F16>(f, dp, bias, grid, st);
-        else fwd_kind<AT_F32>(f, dp, bias, grid, st);
+        const dim3 grid((unsigned)((a.n_q / (small ? 32 : ATT_TQ) + a.n_seg) * a.heads), (unsigned)sp.splits);
+        if (kind == AT_BF16) fwd_kind<AT_BF16>(f, small, dp, bias, grid, st);
+        else if (kind == AT_F16) fwd_kind<AT_F16>(f, small, dp, bias, grid, st);
+        else fwd_kind<AT_F32>(f, small, dp, bias, grid, st);
     }
     if (sp.splits > 1) {
         if (kind == AT_BF16) join_kind<AT_BF16>(f, dp, st);

@@ -13,6 +13,7 @@ struct AttnFwd {
     const int* q_pos; const float* table; const int* lut; int n_bucket, reach, axes;
     void* out; long long o_st, o_sh; float *stats, *out32;
     int splits; float *part, *part_ml;
+    int zero;                                             // rows outside all segments become zeros
 };
 
 int mgn_attn_launch_few(int kind, const AttnFwd* f, void* stream);      // mgn_attn_few.hip
@@ -53,6 +54,12 @@ inline int attn_check(const MgnAttn* a, const char* name) {
     }
     if (bad) { mgn_set_error("%s: %s", name, bad); return MGN_E_ARG; }
     return 0;
+}
+
+// Small problems: 32 queries of a head per workgroup and no images, when tiles of 128 queries would leave most compute units
+// without work (measured: 561 x 280, 4 heads of 32, fp32: see mgn_attn_fwd.hip).
+inline bool attn_is_small(const MgnAttn& a) {
+    return (a.n_q / ATT_TQ + a.n_seg) * (int64_t)a.heads <= 256 && a.n_k / a.n_seg <= 2048;
 }
 
 // Few queries per segment: keys and values are read once where they lie, without images.

@@ -271,73 +271,87 @@ def _q8_128(kept: Q8Rows, name, rows=None):
 _ATT_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _att_rows(t, dtype, device, tail, name: str):
-    """[tokens, heads, dim] rows the attention kernels can read: same type and device as the queries, the last axis dense,
-    every row on a 16-byte border (other axes may be strided, so slices of a packed projection work)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise RuntimeError(f"{name}: expected a CUDA/HIP tensor (the HIP path has no CPU fallback)")
-    if t.dtype is not dtype or t.device != device:
-        raise RuntimeError(f"{name}: expected dtype {dtype} on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 3 or t.shape[1:] != tail:
-        raise RuntimeError(f"{name}: expected shape [tokens, {tail[0]}, {tail[1]}], got {tuple(t.shape)}")
-    per = 16 // t.element_size()
+def _att_rows(t, dtype, device, rows, heads, dim, name: str):
+    """(address, token stride, head stride) of [rows, heads, dim] rows the attention kernels can read: type and device of the
+    queries, the last axis dense, every row on a 16-byte border (other axes may be strided, so slices of a packed projection
+    work)."""
+    try:
+        ok = t.is_cuda and t.dtype is dtype and t.device == device and t.shape == (rows, heads, dim)
+    except AttributeError:
+        ok = False
+    if not ok:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(f"{name}: expected a CUDA/HIP tensor (the HIP path has no CPU fallback)")
+        raise RuntimeError(f"{name}: expected {dtype} [{rows}, {heads}, {dim}] on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     st, sh, sd = t.stride()
-    if t.numel() and (sd != 1 or st % per or sh % per or t.data_ptr() % 16):
+    p = t.data_ptr()
+    per = 3 if dtype is torch.float32 else 7
+    if (sd != 1 or (st | sh) & per or p & 15) and t.numel():
         raise RuntimeError(f"{name}: the last axis must be dense and every row start on a 16-byte border "
                            f"(strides {t.stride()}): call .contiguous()")
-    return t.data_ptr(), (st if t.shape[0] > 1 else sh * t.shape[1]), sh
+    return p, (st if rows > 1 else sh * heads), sh
 
 
 def _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale):
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
-        raise RuntimeError("cross_attention: q [queries, heads, dim] and k, v [keys, kv_heads, dim]")
-    if q.dtype not in _ATT_DTYPES:
-        raise RuntimeError(f"cross_attention: float32, bfloat16 or float16, got {q.dtype}")
-    dev, (nq, heads, dim), (nk, kv_heads) = q.device, q.shape, k.shape[:2]
+    """Checked arguments of the attention entry points (this runs once per call: the passing case is kept short)."""
+    try:
+        (nq, heads, dim), (nk, kv_heads, _) = q.shape, k.shape
+        dtype, dev = q.dtype, q.device
+        code = _ATT_DTYPES[dtype]
+    except (AttributeError, ValueError):
+        raise RuntimeError("cross_attention: q [queries, heads, dim] and k, v [keys, kv_heads, dim] tensors") from None
+    except KeyError:
+        raise RuntimeError(f"cross_attention: float32, bfloat16 or float16, got {q.dtype}") from None
     if dim % 8 or not 8 <= dim <= 128:
         raise RuntimeError(f"cross_attention: the head width must be a multiple of 8 up to 128, got {dim}")
-    if kv_heads < 1 or heads % kv_heads:
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise RuntimeError(f"cross_attention: {heads} query heads are not a multiple of {kv_heads} key heads")
-    if (q_ptr is None) != (k_ptr is None):
-        raise RuntimeError("cross_attention: segment offsets come for queries and keys, or for neither")
-    n_seg = 1 if q_ptr is None else q_ptr.shape[0] - 1
-    if n_seg < 1:
-        raise RuntimeError("cross_attention: segment offsets hold one entry more than there are segments")
-    if v.shape[0] != nk:
-        raise RuntimeError(f"cross_attention: {nk} keys but {v.shape[0]} values")
-    if key_mask is not None and key_mask.dtype is torch.bool:
-        key_mask = key_mask.view(torch.uint8)
-    reach = axes = n_bucket = 0
+    qp, qt, qh = _att_rows(q, dtype, dev, nq, heads, dim, "q")
+    kp, kt, kh = _att_rows(k, dtype, dev, nk, kv_heads, dim, "k")
+    vp, vt, vh = _att_rows(v, dtype, dev, nk, kv_heads, dim, "v")
+
+    def small(t, dt, shape, name):
+        p = _dev(t, dt, shape, name)
+        if t.device != dev:
+            raise RuntimeError(f"cross_attention: {name} is on {t.device}, the queries on {dev}")
+        return p
+    n_seg, ptrs = 1, (0, 0)
+    if q_ptr is not None or k_ptr is not None:
+        if q_ptr is None or k_ptr is None:
+            raise RuntimeError("cross_attention: segment offsets come for queries and keys, or for neither")
+        n_seg = q_ptr.shape[0] - 1 if q_ptr.dim() == 1 else 0
+        if n_seg < 1:
+            raise RuntimeError("cross_attention: segment offsets hold one entry more than there are segments")
+        ptrs = (small(q_ptr, torch.int32, (n_seg + 1,), "q_ptr"), small(k_ptr, torch.int32, (n_seg + 1,), "k_ptr"))
+    mask = 0
+    if key_mask is not None:
+        mask = small(key_mask.view(torch.uint8) if key_mask.dtype is torch.bool else key_mask, torch.uint8, (nk,), "key_mask")
+    bias, sizes = (0, 0, 0, 0), (0, 0, 0)
     if bias_table is not None:
         if bucket_lut is None or q_pos is None or k_pos is None:
             raise RuntimeError("cross_attention: the bias needs bucket_lut, q_pos and k_pos")
-        n_bucket, axes = bias_table.shape[-1], q_pos.shape[-1]
-        reach = bucket_lut.shape[0] // 2 if axes == 1 else bucket_lut.shape[0] - 1
-        if not 1 <= axes <= 3 or not 1 <= reach <= 1024 or not 1 <= n_bucket <= 64 or (axes == 1 and bucket_lut.shape[0] % 2 == 0):
+        n_bucket, axes, entries = bias_table.shape[-1], q_pos.shape[-1], bucket_lut.shape[0]
+        reach = entries // 2 if axes == 1 else entries - 1
+        if not 1 <= axes <= 3 or not 1 <= reach <= 1024 or not 1 <= n_bucket <= 64 or (axes == 1 and entries % 2 == 0):
             raise RuntimeError("cross_attention: places have one to three axes, bucket_lut 2 * reach + 1 (one axis) or reach + 1 entries "
                                "with reach <= 1024, the table at most 64 buckets")
+        bias = (small(bias_table, torch.float32, (heads, n_bucket), "bias_table"), small(bucket_lut, torch.int32, (entries,), "bucket_lut"),
+                small(q_pos, torch.int32, (nq, axes), "q_pos"), small(k_pos, torch.int32, (nk, axes), "k_pos"))
+        sizes = (n_bucket, reach, axes)
     elif bucket_lut is not None or q_pos is not None or k_pos is not None:
         raise RuntimeError("cross_attention: bucket_lut, q_pos and k_pos belong to a bias_table")
-    small = [("q_ptr", q_ptr), ("k_ptr", k_ptr), ("key_mask", key_mask), ("bias_table", bias_table), ("bucket_lut", bucket_lut),
-             ("q_pos", q_pos), ("k_pos", k_pos)]
-    for name, t in small:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"cross_attention: {name} is on {t.device}, the queries on {dev}")
-    tail = (kv_heads, dim)
-    (qp, qt, qh), (kp, kt, kh), (vp, vt, vh) = (_att_rows(q, q.dtype, dev, (heads, dim), "q"), _att_rows(k, q.dtype, dev, tail, "k"),
-                                                _att_rows(v, q.dtype, dev, tail, "v"))
-    return _lib.MgnAttn(qp, kp, vp, qt, qh, kt, kh, vt, vh,
-                        _opt(q_ptr, torch.int32, (n_seg + 1,), "q_ptr"), _opt(k_ptr, torch.int32, (n_seg + 1,), "k_ptr"),
-                        _opt(key_mask, torch.uint8, (nk,), "key_mask"), _opt(bias_table, torch.float32, (heads, n_bucket), "bias_table"),
-                        _opt(bucket_lut, torch.int32, None, "bucket_lut"), _opt(q_pos, torch.int32, (nq, axes), "q_pos"),
-                        _opt(k_pos, torch.int32, (nk, axes), "k_pos"), nq, nk, n_seg, heads, kv_heads, dim, _ATT_DTYPES[q.dtype],
-                        n_bucket, reach, axes, float(dim ** -0.5 if scale is None else scale), 0)
+    return _lib.MgnAttn(qp, kp, vp, qt, qh, kt, kh, vt, vh, *ptrs, mask, *bias, nq, nk, n_seg, heads, kv_heads, dim, code, *sizes,
+                        dim ** -0.5 if scale is None else float(scale), 0, 0)
 
 
-def _att_workspace(need: int, device) -> torch.Tensor:
+def _att_workspace(need: int, device):
+    """(address, bytes, tensor) of a workspace."""
     if need < 0:
         raise RuntimeError("cross_attention: " + _lib.lib().mgn_last_error().decode("utf-8", "replace"))
-    return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    if need == 0:
+        return 0, 0, None
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    return ws.data_ptr(), need, ws
 
 
 def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=None, bucket_lut=None, q_pos=None, k_pos=None,
@@ -352,19 +366,28 @@ def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=N
     ``stats`` float32 [2, heads, queries] receives what :func:`cross_attention_bwd` needs; ``out32`` (bfloat16 and float16,
     float32 [queries, heads, dim]) the outputs before they are rounded, for the gradient of a bias table."""
     a = _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
+    dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_ptr is None else torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    o = _att_rows(out, q.dtype, q.device, q.shape[1:], "out")
-    if out.shape[0] != q.shape[0]:
-        raise RuntimeError(f"cross_attention: {q.shape[0]} queries but {out.shape[0]} output rows")
-    st = _opt(stats, torch.float32, (2, q.shape[1], q.shape[0]), "stats")
-    o32 = _opt(out32, torch.float32, tuple(q.shape), "out32")
-    with _on_device(q.device):
-        ws = _att_workspace(_lib.lib().mgn_attn_fwd_workspace_bytes(C.byref(a)), q.device)
-        with timed("cross_attention"):
-            rc = _lib.lib().mgn_attn_fwd(C.byref(a), *o, st, o32, ws.data_ptr(), ws.numel(), _stream())
-    _lib.check(rc, "mgn_attn_fwd")
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        a.zero_outside = 1
+    nq, heads, dim = q.shape
+    o = _att_rows(out, q.dtype, dev, nq, heads, dim, "out")
+    st = 0 if stats is None else _dev(stats, torch.float32, (2, heads, nq), "stats")
+    o32 = 0 if out32 is None else _dev(out32, torch.float32, (nq, heads, dim), "out32")
+    if dev.index == torch.cuda.current_device() and _event_log is None:
+        _att_fwd(a, o, st, o32, dev)
+    else:
+        with _on_device(dev), timed("cross_attention"):
+            _att_fwd(a, o, st, o32, dev)
     return out
+
+
+def _att_fwd(a, o, st, o32, dev):
+    lib, ref = _lib.lib(), C.byref(a)
+    p, n, ws = _att_workspace(lib.mgn_attn_fwd_workspace_bytes(ref), dev)
+    rc = lib.mgn_attn_fwd(ref, *o, st, o32, p, n, _stream())
+    if rc:
+        _lib.check(rc, "mgn_attn_fwd")
 
 
 def cross_attention_bwd(g, q, k, v, out, stats, q_ptr=None, k_ptr=None, key_mask=None, bias_table=None, bucket_lut=None,
@@ -375,20 +398,19 @@ def cross_attention_bwd(g, q, k, v, out, stats, q_ptr=None, k_ptr=None, key_mask
     a = _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
     if isinstance(g, torch.Tensor) and g.dim() == 3 and (g.stride(2) != 1 or g.stride(0) % 8 or g.stride(1) % 8 or g.data_ptr() % 16):
         g = g.contiguous()                     # an expanded or transposed gradient as autograd hands it over
-    new = torch.empty_like if q_ptr is None else torch.zeros_like
-    dq, dk, dv = (new(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    a.zero_outside = 1
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     table_grad = table_grad and bias_table is not None
     dt = torch.empty_like(bias_table) if table_grad else None
-    gr, o = _att_rows(g, q.dtype, q.device, q.shape[1:], "g"), _att_rows(out, out.dtype if out.dtype is torch.float32 else q.dtype, q.device, q.shape[1:], "out")
+    nq, heads, dim = q.shape
+    gr = _att_rows(g, q.dtype, q.device, nq, heads, dim, "g")
+    o = _att_rows(out, out.dtype if out.dtype is torch.float32 else q.dtype, q.device, nq, heads, dim, "out")
     a.out_f32 = int(out.dtype is torch.float32)
-    if g.shape[0] != q.shape[0] or out.shape[0] != q.shape[0]:
-        raise RuntimeError("cross_attention_bwd: g and out have one row per query")
-    st = _dev(stats, torch.float32, (2, q.shape[1], q.shape[0]), "stats")
-    with _on_device(q.device):
-        ws = _att_workspace(_lib.lib().mgn_attn_bwd_workspace_bytes(C.byref(a), int(table_grad)), q.device)
-        with timed("cross_attention_bwd"):
-            rc = _lib.lib().mgn_attn_bwd(C.byref(a), *gr, *o, st, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                         0 if dt is None else dt.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
+    st = _dev(stats, torch.float32, (2, heads, nq), "stats")
+    with _on_device(q.device), timed("cross_attention_bwd"):
+        p, n, ws = _att_workspace(_lib.lib().mgn_attn_bwd_workspace_bytes(C.byref(a), int(table_grad)), q.device)
+        rc = _lib.lib().mgn_attn_bwd(C.byref(a), *gr, *o, st, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                     0 if dt is None else dt.data_ptr(), p, n, _stream())
     _lib.check(rc, "mgn_attn_bwd")
     return dq, dk, dv, dt
 

@@ -554,7 +554,7 @@ int mgn_train_edge_bwd_q8(const int8_t* codes, const float* scale, const float* 
  * h / (heads / kv_heads)); strides in elements, the last axis dense, every row on a 16-byte border; dim a multiple of
  * 8 up to 128; fp32, bf16 or fp16.  Sums, softmax statistics and products are fp32 (fp32 operands as two fp16 terms).
  * Segments: q_ptr / k_ptr [n_seg + 1] (device, ascending); null: one segment.  Rows outside all segments are neither
- * read nor written.  key_mask [n_k]: 0 leaves a key out; nothing is read from its rows.  A query with no key left (or
+ * read nor written (zero_outside: outputs of such rows become zeros).  key_mask [n_k]: 0 leaves a key out; nothing is read from its rows.  A query with no key left (or
  * only keys at a bias of minus infinity) gives a row of zeros and gradients of zero.
  * Bias: places [n][axes] of queries and keys as whole numbers within +-2^30; one axis: place = k - q held to
  * [-reach, reach], plus reach (table of 2 reach + 1 entries); two or three: the whole part of the distance, held to reach
@@ -572,6 +572,7 @@ typedef struct {
     int64_t n_q, n_k;
     int32_t n_seg, heads, kv_heads, dim, dtype, n_bucket, reach, axes;
     float scale;
+    int32_t zero_outside;                            /* outputs: rows outside all segments become zeros         */
     int32_t out_f32;                                 /* mgn_attn_bwd: out is fp32 whatever the operands' type       */
 } MgnAttn;
 
@@ -581,7 +582,7 @@ int mgn_attn_fwd(const MgnAttn* a, void* out, int64_t out_st, int64_t out_sh, fl
 
 /* Gradients for the output gradient g: dq [n_q][heads][dim], dk and dv [n_k][kv_heads][dim] (dense, type of the operands,
  * summed over the query heads that share a key head), dtable [heads][n_bucket] fp32 or null.  out and stats as mgn_attn_fwd
- * left them.  All sums have a fixed order.  Rows outside all segments are not written; masked keys get zeros.           */
+ * left them.  All sums have a fixed order.  Rows outside all segments as in the forward pass; masked keys get zeros.           */
 int64_t mgn_attn_bwd_workspace_bytes(const MgnAttn* a, int32_t table_grad);
 int mgn_attn_bwd(const MgnAttn* a, const void* g, int64_t g_st, int64_t g_sh, const void* out, int64_t out_st,
                  int64_t out_sh, const float* stats, void* dq, void* dk, void* dv, float* dtable, void* workspace,

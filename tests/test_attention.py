@@ -69,11 +69,11 @@ def test_the_library_refuses(bad):
 def test_null_arguments_and_small_workspaces_are_refused():
     from gnn_amd import _lib
     lib, a = _lib.lib(), args()
-    need = lib.mgn_attn_fwd_workspace_bytes(ctypes.byref(args(n_q=1000)))
+    need = lib.mgn_attn_fwd_workspace_bytes(ctypes.byref(args(n_q=100000)))
     assert need > 0
     assert lib.mgn_attn_fwd(None, 4096, 128, 32, None, None, 4096, 1 << 40, None) == -1
-    assert lib.mgn_attn_fwd(ctypes.byref(args(n_q=1000)), 4096, 128, 32, None, None, 4096, need - 1, None) == -1
-    assert lib.mgn_attn_fwd(ctypes.byref(args(n_q=1000)), 4096, 128, 32, None, None, None, need, None) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(args(n_q=100000)), 4096, 128, 32, None, None, 4096, need - 1, None) == -1
+    assert lib.mgn_attn_fwd(ctypes.byref(args(n_q=100000)), 4096, 128, 32, None, None, None, need, None) == -1
     assert lib.mgn_attn_fwd(ctypes.byref(a), None, 128, 32, None, None, 4096, 1 << 40, None) == -1
     assert lib.mgn_attn_fwd(ctypes.byref(a), 4100, 128, 32, None, None, 4096, 1 << 40, None) == -1
     need = lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(a), 0)
