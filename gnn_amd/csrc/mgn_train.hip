@@ -208,7 +208,6 @@ __global__ __launch_bounds__(NT) void train_ln_bwd_kernel(const float* __restric
 struct LinBwdArgs {
     const float* G; const float* A; const float* W; int ldw; int koff;
     const float* mask; const float* res; float* GA; float* partial; long long rows;
-    const signed char* codes; const float* scale; int mask_codes;      // A in 8 bits (mgn_train_linear_bwd_q8)
 };
 
 // Four consecutive features of a row as they were requested: fp32, or 8-bit codes and the row's scale.
@@ -330,11 +329,12 @@ constexpr int SPL = TM * H;                 // halves per plane of the image
 __device__ __forceinline__ int swz_off(int row, int ch) { return row * H + 8 * (ch ^ (((row & 3) << 2) | ((row >> 2) & 3))); }
 
 // four consecutive features k .. k+3 (k a multiple of 4) of one tile row -> the three planes
+template <int PLANE = SPL>
 __device__ __forceinline__ void splanes_store4(unsigned short* img, int row, int k, const f32x4 v) {
     u32x2 ph, pm, pl;
     split_pack4(v, ph, pm, pl);
     unsigned short* d = img + swz_off(row, k >> 3) + (k & 4);
-    *(u32x2*)(d) = ph; *(u32x2*)(d + SPL) = pm; *(u32x2*)(d + 2 * SPL) = pl;
+    *(u32x2*)(d) = ph; *(u32x2*)(d + PLANE) = pm; *(u32x2*)(d + 2 * PLANE) = pl;
 }
 
 // The transposing read needs every lane of the wave active: call from workgroup-uniform control flow only.
@@ -355,11 +355,12 @@ struct TrBase { int o[2]; };                 // hh = 0, 1
 __device__ __forceinline__ TrBase tr_base(int lane) { return TrBase{{tr_off(lane, 0, 0, 0), tr_off(lane, 0, 1, 0)}}; }
 
 // v_mfma_f32_32x32x16_bf16 operand of lane (j = lane & 31, h = lane >> 5): rows 16s + 8h + 0..7 of column 32 blk + j
+template <int PLANE = SPL>
 __device__ __forceinline__ void tr_operand3(const unsigned short* img, const TrBase& tb, int s, int blk, u32x4& xh, u32x4& xm, u32x4& xl) {
     const unsigned short* p0 = img + ((tb.o[0] ^ (32 * blk)) + 16 * H * s);
     const unsigned short* p1 = img + ((tb.o[1] ^ (32 * blk)) + 16 * H * s);
-    const u32x2 h0 = lds_tr4(p0), h1 = lds_tr4(p1), m0 = lds_tr4(p0 + SPL), m1 = lds_tr4(p1 + SPL);
-    const u32x2 l0 = lds_tr4(p0 + 2 * SPL), l1 = lds_tr4(p1 + 2 * SPL);
+    const u32x2 h0 = lds_tr4(p0), h1 = lds_tr4(p1), m0 = lds_tr4(p0 + PLANE), m1 = lds_tr4(p1 + PLANE);
+    const u32x2 l0 = lds_tr4(p0 + 2 * PLANE), l1 = lds_tr4(p1 + 2 * PLANE);
     xh = u32x4{h0[0], h0[1], h1[0], h1[1]};
     xm = u32x4{m0[0], m0[1], m1[0], m1[1]};
     xl = u32x4{l0[0], l0[1], l1[0], l1[1]};
@@ -367,17 +368,17 @@ __device__ __forceinline__ void tr_operand3(const unsigned short* img, const TrB
 
 // wave_gemm3_32 on the swizzled image.  rb = swz_off(j, h), the lane's offset for k-step 0; k-step c sits at rb ^ 16c
 // (2c + h = 2c ^ h, and the swizzle is an XOR as well), so one register carries all eight addresses.
-template <int C0, int C1>
+template <int C0, int C1, int PLANE = SPL>
 __device__ __forceinline__ f32x16 wave_gemm3_32s(const unsigned short* img, const WPlanes32& w, int rb, f32x16 acc) {
     const unsigned short* r = img + (rb ^ (16 * C0));
-    u32x4 xh = *(const u32x4*)(r), xm = *(const u32x4*)(r + SPL), xl = *(const u32x4*)(r + 2 * SPL);
+    u32x4 xh = *(const u32x4*)(r), xm = *(const u32x4*)(r + PLANE), xl = *(const u32x4*)(r + 2 * PLANE);
     __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
     for (int c = C0; c < C1; ++c) {
         u32x4 nh = xh, nm = xm, nl = xl;
         if (c + 1 < C1) {
             const unsigned short* n = img + (rb ^ (16 * (c + 1)));
-            nh = *(const u32x4*)(n); nm = *(const u32x4*)(n + SPL); nl = *(const u32x4*)(n + 2 * SPL);
+            nh = *(const u32x4*)(n); nm = *(const u32x4*)(n + PLANE); nl = *(const u32x4*)(n + 2 * PLANE);
             __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
         }
         acc = mfma32_bf16(w.p[2][c], xh, acc);   // lo * hi
@@ -441,9 +442,9 @@ __device__ __forceinline__ void load_wplanes32_t(WPlanes32& w, const float* __re
     }
 }
 
-template <bool A8> struct TileRows { f32x4 g[4]; RowPiece<A8> a[4]; f32x4 m[4], r[4]; };     // one thread's share of a tile: rows srow + 8*it, columns 4*sq ..
+struct TileRows { f32x4 g[4], a[4], m[4], r[4]; };     // one thread's share of a tile: rows srow + 8*it, columns 4*sq ..
 
-template <bool DO_GA, bool DO_DW, bool A8>
+template <bool DO_GA, bool DO_DW>
 __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned short Gs[3 * SPL];                    // G tile, three planes
     __shared__ __attribute__((aligned(16))) unsigned short As[DO_DW ? 3 * SPL : 8];        // A tile, three planes
@@ -464,23 +465,23 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
     // An absent mask / residual is read all the same, every lane at offset 0 of G (a line that stays in the cache), and
     // dropped by a select: the tile loop has no branch around a load.
     // A mask that is the layer input itself (the usual case: the ReLU output that fed this Linear) is not read twice.
-    const bool has_mask = DO_GA && (a.mask || (A8 && a.mask_codes)), has_res = DO_GA && a.res, mask_is_a = DO_GA && DO_DW && (A8 ? a.mask_codes != 0 : a.mask == a.A);
+    const bool has_mask = DO_GA && a.mask, has_res = DO_GA && a.res, mask_is_a = DO_GA && DO_DW && a.mask == a.A;
     const float* mask_p = (has_mask && !mask_is_a) ? a.mask : a.G;
     const float* res_p = has_res ? a.res : a.G;
     const size_t mmul = (has_mask && !mask_is_a) ? 1 : 0, rmul = has_res ? 1 : 0;
-    auto request = [&](TileRows<A8>& p, int tile) {
+    auto request = [&](TileRows& p, int tile) {
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-            const size_t row = (size_t)min((long long)tile * TM + srow + 8 * it, a.rows - 1), o = row * H + 4 * sq;
+            const size_t o = (size_t)min((long long)tile * TM + srow + 8 * it, a.rows - 1) * H + 4 * sq;
             p.g[it] = *(const f32x4*)(a.G + o);
-            if constexpr (DO_DW) p.a[it].request(a.A, a.codes, a.scale, row, o);
+            if constexpr (DO_DW) p.a[it] = *(const f32x4*)(a.A + o);
             if constexpr (DO_GA) { p.m[it] = *(const f32x4*)(mask_p + o * mmul); p.r[it] = *(const f32x4*)(res_p + o * rmul); }
         }
     };
     // One tile: `cur` holds its rows; the next tile's are requested into `nxt` before anything else, so they have the
     // whole pass to arrive.  The two register sets swap roles from pass to pass (the loop below is unrolled by two):
     // nothing is copied from one to the other, and no pass ends waiting for its own requests or stores.
-    auto pass = [&](TileRows<A8>& cur, TileRows<A8>& nxt, int tile) {
+    auto pass = [&](TileRows& cur, TileRows& nxt, int tile) {
         const long long base = (long long)tile * TM;
         const int nvalid = (int)min((long long)TM, a.rows - base);
         request(nxt, min(tile + 1, t1 - 1));         // the last pass requests its own rows again (never used)
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
             const f32x4 g = srow + 8 * it < nvalid ? cur.g[it] : zero4;     // rows past the end add nothing to the sums
             dbacc += g;
             splanes_store4(Gs, srow + 8 * it, 4 * sq, g);
-            if constexpr (DO_DW) splanes_store4(As, srow + 8 * it, 4 * sq, cur.a[it].get());
+            if constexpr (DO_DW) splanes_store4(As, srow + 8 * it, 4 * sq, cur.a[it]);
         }
         __syncthreads();
         if constexpr (DO_GA) {
@@ -507,17 +508,16 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 asm volatile("" : "+v"(nxt.g[it]), "+v"(nxt.m[it]), "+v"(nxt.r[it]));
-                if constexpr (DO_DW) nxt.a[it].arrived();
+                if constexpr (DO_DW) asm volatile("" : "+v"(nxt.a[it]));
             }
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 const int row = srow + 8 * it;
                 if (row < nvalid) {
                     f32x4 val = *(const f32x4*)(Ot + toff(row, sq, H / 4));
-                    const f32x4 am = DO_DW && mask_is_a ? cur.a[it].get() : cur.m[it];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const float mk = am[k];
+                        const float mk = (DO_DW && mask_is_a) ? cur.a[it][k] : cur.m[it][k];
                         val[k] = (!has_mask || mk > 0.f) ? val[k] : 0.f;
                         val[k] += has_res ? cur.r[it][k] : 0.f;
                     }
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
             }
         }
     };
-    TileRows<A8> ra, rb;
+    TileRows ra, rb;
     if (t0 < t1) request(ra, t0);
     for (int tile = t0; tile < t1; tile += 2) {
         pass(ra, rb, tile);
@@ -550,6 +550,151 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
             for (int g = 0; g < 8; ++g) sum += Ot[g * H + t];
             p[PARTIAL_W + t] = sum;
         }
+    }
+}
+
+// ------------------------------------------------------------------------ linear backward, layer input in 8 bits
+// A[r] = scale[r] * codes[r].  With scale = 2^e * m, 1 <= m < 2: the rows of G are multiplied by m before they are split, and the
+// codes times 2^e are ONE exact bf16 plane (8 significant bits), so dW = (m G)^T (2^e codes) takes three partial products
+// instead of six and a quarter of the staging; GA = (m G) W is divided by m where it leaves (two more roundings, 2^-24 each).
+//
+// Streams 4 (G) + 1 (codes) bytes in and 4 (GA) out per element.  Tiles of 64 rows, eight waves, two per SIMD: wave w takes
+// column block w & 3 of both products, of GA the rows 32 (w >> 2) .., of dW the column blocks 2 (w >> 2) and + 1 -- so each keeps
+// the weight planes of 32 columns (96 registers) and 32 accumulators.  The four-wave form on the three-plane input took
+// 678 us for 1.5M rows.
+struct LinBwdQ8Args {
+    const float* G; const signed char* codes; const float* scale; const float* W; int ldw; int koff;
+    const float* mask; const float* res; float* GA; float* partial; long long rows; int mask_codes;
+};
+
+template <bool DO_GA, bool EXTRA>
+__global__ __launch_bounds__(2 * NT, 1) void train_linear_bwd_q8_kernel(LinBwdQ8Args a) {
+    constexpr int ROWS = 2 * TM, PLANE = ROWS * H;
+    __shared__ __attribute__((aligned(16))) unsigned short Gs[3 * PLANE];                  // m G, three planes
+    __shared__ __attribute__((aligned(16))) unsigned short As[PLANE];                      // 2^e codes
+    __shared__ __attribute__((aligned(16))) float Ot[2 * tile_floats(H / 4)];              // GA tile; bias sums at the end
+
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5, cb = w & 3, half = w >> 2;
+    WPlanes32 wt;
+    if constexpr (DO_GA) load_wplanes32_t(wt, a.W, a.ldw, a.koff + 32 * cb + j, h);
+    f32x16 dw[2] = {zero16(), zero16()};
+    f32x4 dbacc = {0.f, 0.f, 0.f, 0.f};
+    const int ntiles = (int)((a.rows + ROWS - 1) / ROWS), nb = gridDim.x, rho = range_of_block(blockIdx.x, nb);
+    const int t0 = (int)((long long)rho * ntiles / nb), t1 = (int)((long long)(rho + 1) * ntiles / nb);
+    const int srow = t >> 5, sq = t & 31;                                                  // rows srow + 16 * it, columns 4 * sq ..
+    const TrBase tb = tr_base(lane);
+    struct Rows { f32x4 g[4]; int c[4]; float s[4]; } cur;
+    auto request = [&](int tile) {
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const size_t row = (size_t)min((long long)tile * ROWS + srow + 16 * it, a.rows - 1), o = row * H + 4 * sq;
+            cur.g[it] = *(const f32x4*)(a.G + o);
+            cur.c[it] = *(const int*)(a.codes + o);
+            cur.s[it] = a.scale[row];
+        }
+    };
+    if (t0 < t1) request(t0);
+    for (int tile = t0; tile < t1; ++tile) {
+        const long long base = (long long)tile * ROWS;
+        const int nvalid = (int)min((long long)ROWS, a.rows - base);
+        __syncthreads();                             // the previous tile's products and output pass are done
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const bool in = srow + 16 * it < nvalid;
+            const f32x4 g = in ? cur.g[it] : f32x4{0.f, 0.f, 0.f, 0.f};
+            dbacc += g;
+            const unsigned sb = __float_as_uint(cur.s[it]);
+            const float m = __uint_as_float((sb & 0x7fffffu) | 0x3f800000u), p2 = in ? __uint_as_float(sb & 0x7f800000u) : 0.f;
+            splanes_store4<PLANE>(Gs, srow + 16 * it, 4 * sq, g * m);
+            const int c = cur.c[it];
+            const unsigned b0 = __float_as_uint((float)(int)(signed char)c * p2), b1 = __float_as_uint((float)(int)(signed char)(c >> 8) * p2);
+            const unsigned b2 = __float_as_uint((float)(int)(signed char)(c >> 16) * p2), b3 = __float_as_uint((float)(c >> 24) * p2);
+            *(u32x2*)(As + swz_off(srow + 16 * it, sq >> 1) + 4 * (sq & 1)) = u32x2{pack_hi16(b0, b1), pack_hi16(b2, b3)};
+        }
+        // the staged rows' registers take the next tile's: it has the products and the output pass to arrive
+        int codes[4]; float by[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            codes[it] = cur.c[it];
+            by[it] = __uint_as_float((__float_as_uint(cur.s[it]) & 0x7fffffu) | 0x3f800000u);
+        }
+        request(min(tile + 1, t1 - 1));
+        __syncthreads();
+        if constexpr (DO_GA) {
+            f32x16 acc = zero16();
+            acc = wave_gemm3_32s<0, 8, PLANE>(Gs, wt, swz_off(j, h) + half * SPL, acc);
+            acc_to_tile(Ot + half * tile_floats(H / 4), acc, cb, j, h);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            u32x4 gh, gm, gl, x[2];
+            tr_operand3<PLANE>(Gs, tb, s, cb, gh, gm, gl);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int blk = 32 * (2 * half + q);
+                const u32x2 p0 = lds_tr4(As + ((tb.o[0] ^ blk) + 16 * H * s)), p1 = lds_tr4(As + ((tb.o[1] ^ blk) + 16 * H * s));
+                x[q] = u32x4{p0[0], p0[1], p1[0], p1[1]};
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) dw[q] = mfma32_bf16(gl, x[q], dw[q]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) dw[q] = mfma32_bf16(gm, x[q], dw[q]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) dw[q] = mfma32_bf16(gh, x[q], dw[q]);
+        }
+        f32x4 mk[EXTRA ? 4 : 1], rs[EXTRA ? 4 : 1];
+        if constexpr (EXTRA) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (EXTRA) {                       // requested here, behind the products: their registers are free again
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const size_t o = (size_t)min(base + srow + 16 * it, a.rows - 1) * H + 4 * sq;
+                mk[it] = *(const f32x4*)(a.mask ? a.mask + o : a.G);
+                rs[it] = *(const f32x4*)(a.res ? a.res + o : a.G);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (DO_GA) {
+            __syncthreads();
+            // the next tile's rows count as arrived before this tile's stores (one in-order counter for loads and stores)
+#pragma unroll
+            for (int it = 0; it < 4; ++it) asm volatile("" : "+v"(cur.g[it]), "+v"(cur.c[it]), "+v"(cur.s[it]));
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const int row = srow + 16 * it;
+                if (row < nvalid) {
+                    f32x4 val = *(const f32x4*)(Ot + toff(row, sq, H / 4));
+                    const float inv = __builtin_amdgcn_rcpf(by[it]);
+                    const int c = codes[it];
+                    const bool on[4] = {(signed char)c > 0, (signed char)(c >> 8) > 0, (signed char)(c >> 16) > 0, (c >> 24) > 0};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        val[k] = !a.mask_codes || on[k] ? val[k] * inv : 0.f;
+                        if constexpr (EXTRA) {
+                            val[k] = !a.mask || mk[it][k] > 0.f ? val[k] : 0.f;
+                            val[k] += a.res ? rs[it][k] : 0.f;
+                        }
+                    }
+                    *(f32x4*)(a.GA + (size_t)(base + row) * H + 4 * sq) = val;
+                }
+            }
+        }
+    }
+    float* p = a.partial + (size_t)blockIdx.x * PARTIAL;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int reg = 0; reg < 16; ++reg) {
+            const int f = 32 * cb + (reg & 3) + 8 * (reg >> 2) + 4 * h;
+            p[f * H + 32 * (2 * half + q) + j] = dw[q][reg];
+        }
+    __syncthreads();
+    *(f32x4*)(Ot + srow * H + 4 * sq) = dbacc;
+    __syncthreads();
+    if (t < H) {
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) sum += Ot[g * H + t];
+        p[PARTIAL_W + t] = sum;
     }
 }
 
@@ -1247,15 +1392,15 @@ extern "C" int mgn_train_linear_bwd(const float* G, const float* A, const float*
     MGN_REQUIRE(!dW || (A && scratch && lddw >= H), "mgn_train_linear_bwd");
     MGN_REQUIRE(!db || dW, "mgn_train_linear_bwd");
     MGN_REQUIRE(ldw % 4 == 0 || !GA, "mgn_train_linear_bwd");
-    LinBwdArgs a{G, A, W, ldw, koff, mask, res, GA, (float*)scratch, rows, nullptr, nullptr, 0};
+    LinBwdArgs a{G, A, W, ldw, koff, mask, res, GA, (float*)scratch, rows};
     const bool split = mgn_matmul_mode() >= 1;           // bf16 split products; "f32" keeps the fp32 matrix pipe
     int g = train_grid(rows, split ? 1 : 2);
     if (g > TRAIN_BLOCKS_MAX) g = TRAIN_BLOCKS_MAX - TRAIN_BLOCKS_MAX % 8;
     hipStream_t s = (hipStream_t)stream;
     if (split) {
-        if (GA && dW) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, true, false>), dim3(g), dim3(NT), 0, s, a);
-        else if (GA) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, false, false>), dim3(g), dim3(NT), 0, s, a);
-        else hipLaunchKernelGGL((train_linear_bwd3_kernel<false, true, false>), dim3(g), dim3(NT), 0, s, a);
+        if (GA && dW) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, true>), dim3(g), dim3(NT), 0, s, a);
+        else if (GA) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, false>), dim3(g), dim3(NT), 0, s, a);
+        else hipLaunchKernelGGL((train_linear_bwd3_kernel<false, true>), dim3(g), dim3(NT), 0, s, a);
     } else if (GA && dW) hipLaunchKernelGGL((train_linear_bwd_kernel<true, true>), dim3(g), dim3(NT), 0, s, a);
     else if (GA) hipLaunchKernelGGL((train_linear_bwd_kernel<true, false>), dim3(g), dim3(NT), 0, s, a);
     else hipLaunchKernelGGL((train_linear_bwd_kernel<false, true>), dim3(g), dim3(NT), 0, s, a);
@@ -1307,12 +1452,13 @@ extern "C" int mgn_train_linear_bwd_q8(const float* G, const int8_t* codes, cons
     MGN_REQUIRE(dW && scratch && lddw >= H, name);                        // codes are read for the weight gradient
     MGN_REQUIRE(!GA || (W && ldw >= H && koff >= 0 && koff + H <= ldw && ldw % 4 == 0), name);
     MGN_REQUIRE(!(mask_codes && mask) && (GA || !(mask_codes || mask || res)), name);
-    LinBwdArgs a{G, nullptr, W, ldw, koff, mask, res, GA, (float*)scratch, rows, (const signed char*)codes, scale, mask_codes};
-    int g = train_grid(rows, 1);
+    LinBwdQ8Args a{G, (const signed char*)codes, scale, W, ldw, koff, mask, res, GA, (float*)scratch, rows, mask_codes};
+    int g = train_grid((rows + 1) / 2, 1);                                  // tiles of twice TM rows
     if (g > TRAIN_BLOCKS_MAX) g = TRAIN_BLOCKS_MAX - TRAIN_BLOCKS_MAX % 8;
     const hipStream_t s = (hipStream_t)stream;
-    if (GA) hipLaunchKernelGGL((train_linear_bwd3_kernel<true, true, true>), dim3(g), dim3(NT), 0, s, a);
-    else hipLaunchKernelGGL((train_linear_bwd3_kernel<false, true, true>), dim3(g), dim3(NT), 0, s, a);
+    if (GA && (mask || res)) hipLaunchKernelGGL((train_linear_bwd_q8_kernel<true, true>), dim3(g), dim3(2 * NT), 0, s, a);
+    else if (GA) hipLaunchKernelGGL((train_linear_bwd_q8_kernel<true, false>), dim3(g), dim3(2 * NT), 0, s, a);
+    else hipLaunchKernelGGL((train_linear_bwd_q8_kernel<false, false>), dim3(g), dim3(2 * NT), 0, s, a);
     if (launch_reduce((const float*)scratch, g, PARTIAL, PARTIAL_W, lddw, dW, db ? 1 : 0, db, nullptr, nullptr, s))
         { mgn_set_error("%s: the deferred-reduction list is full", name); return MGN_E_CAP; }
     return check_launch(name);
