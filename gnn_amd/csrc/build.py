@@ -13,8 +13,10 @@ OUT = os.path.join(PKG, "libmgn_hip.so")
 # No packed fp32 instructions (v_pk_add/mul/fma_f32): some of their forms have given wrong results on this hardware.  The
 # host pass of the compiler does not know the feature and says so; that warning is harmless.
 HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# Per-file compiler flags (none at present).
-EXTRA_FLAGS = {}
+# Per-file compiler flags.  The attention kernels take maxima of matrix products only to scale by: without -fno-honor-nans every
+# operand of a maximum is first "quieted" by an instruction of its own.  NaN inputs still come out as NaN (through products, sums
+# and exponentials); no comparison in these files asks for one.
+EXTRA_FLAGS = {"mgn_attn_fwd.hip": ["-fno-honor-nans"], "mgn_attn_bwd.hip": ["-fno-honor-nans"], "mgn_attn_few.hip": ["-fno-honor-nans"]}
 
 
 def hipcc_path() -> str:

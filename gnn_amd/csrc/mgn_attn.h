@@ -30,6 +30,7 @@ enum { AT_BF16 = 0, AT_F16 = 1, AT_F32 = 2 };
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float F32_MOST = 3.402823466e38f;
 constexpr int TOP = 14;                 // operands are scaled to magnitudes below 2^TOP
+constexpr int OVER = 4;                  // the running maximum may lag behind by this much (base 2)
 constexpr int FAR_EXP = -60;            // a subtile so much smaller than the largest adds nothing in fp16; its shift stops here
 constexpr int ATT_TQ = 128;             // queries (or keys, in the key-gradient kernel) of a workgroup: 32 per wave
 constexpr int ATT_MAX_SPLITS = 256;
@@ -188,17 +189,36 @@ __device__ __forceinline__ void zero_outside(const int* ptr, int n_seg, long lon
 //   lattice (two or three axes): the whole part of the Euclidean distance, held to reach.  d2 = dx^2 + dy^2 + dz^2 is exact
 //   below 2^24 and only grows beyond, and sqrt(d2 + 1/2) lies at least 1/(4 reach) off every whole number for d2 <= reach^2:
 //   with reach <= 1024 that is 4 units in the last place, so the hardware root (1 ulp) gives the exact whole part.
-template <int BIAS>
-__device__ __forceinline__ int place(int qx, int qy, int qz, int kx, int ky, int kz, int axes, int reach, float most) {
-    if constexpr (BIAS == 1) {
+template <int AXES>
+__device__ __forceinline__ int place(int qx, int qy, int qz, int kx, int ky, int kz, int reach, float most) {
+    if constexpr (AXES == 1) {
         return min(max(kx - qx, -reach), reach) + reach;
     } else {
         const float dx = (float)(kx - qx), dy = (float)(ky - qy);
         float d2 = __builtin_fmaf(dx, dx, 0.5f);
         d2 = __builtin_fmaf(dy, dy, d2);
-        if (axes == 3) { const float dz = (float)(kz - qz); d2 = __builtin_fmaf(dz, dz, d2); }
+        if constexpr (AXES == 3) { const float dz = (float)(kz - qz); d2 = __builtin_fmaf(dz, dz, d2); }
         return (int)__builtin_amdgcn_sqrtf(fminf(d2, most));
     }
+}
+
+// Places of the four consecutive keys (queries) 8 q + 4 h .. of a subtile laid out [axis][32].
+template <int AXES>
+__device__ __forceinline__ void places4(const int* p, i32x4& x, i32x4& y, i32x4& z) {
+    x = *(const i32x4*)p;
+    y = z = x;
+    if constexpr (AXES > 1) y = *(const i32x4*)(p + 32);
+    if constexpr (AXES > 2) z = *(const i32x4*)(p + 64);
+}
+
+// Scores of masked keys to minus infinity.  Called in a branch that is taken where a subtile has masked keys; the opaque copy of
+// the bits keeps it one (the compiler would otherwise test all 16 bits in every step: a third of its vector instructions).
+__device__ __forceinline__ void mask_scores(f32x16& s, int valid, int h) {
+    unsigned bits = (unsigned)valid >> (4 * h);
+    asm volatile("" : "+v"(bits));
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if (!(bits >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -__builtin_inff();
 }
 
 __device__ __forceinline__ float bias_log2(float b) {          // finite biases stay finite in base 2
@@ -207,6 +227,49 @@ __device__ __forceinline__ float bias_log2(float b) {          // finite biases 
 }
 
 // ------------------------------------------------------------------------------------------------ copies into LDS
+// A zero the compiler knows nothing of: an address plus this is one per lane, so what is loaded from it stays in vector
+// registers until it is asked for.  (A load from a uniform address is moved into a scalar register where it is issued -- with a
+// wait for the whole memory latency.)
+__device__ __forceinline__ int lane_zero() {
+    int z;
+    asm("v_mov_b32 %0, 0" : "=v"(z));
+    return z;
+}
+
+// Exponents and valid bits of a step (key exponent, value exponent, mask), requested a step ahead and then made uniform.  Only
+// what is used is loaded: the unused part of a wider load would be overwritten early, behind a wait for the load.
+template <int KIND> struct Record {
+    int v[3];
+    __device__ __forceinline__ void request(const i32x4* at) {
+        const int* p = (const int*)at;
+        v[0] = v[1] = 0;
+        if constexpr (KIND != AT_BF16) { v[0] = p[0]; v[1] = p[1]; }
+        v[2] = p[2];
+    }
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) v[e] = __builtin_amdgcn_readfirstlane(v[e]);
+    }
+};
+
+// Linear 1 KB pieces of images on their way into LDS, by way of registers: requested at the top of a step, written at its end.
+// (Copies that go straight into LDS would save the registers, but the compiler waits for all of them before the next read
+// of ANY shared memory, which put the whole memory latency into every step: 8192 x 8192 at width 128, bf16, 301 us.)
+template <int PIECES, int NW = 4> struct Staged {
+    static constexpr int N = (PIECES + NW - 1) / NW;          // of each wave
+    u32x4 v[N];
+    template <typename F> __device__ __forceinline__ void request(int w, int lane, F source) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (PIECES % NW == 0 || NW * n + w < PIECES) v[n] = *(const u32x4*)(source(NW * n + w) + lane * 16);
+    }
+    __device__ __forceinline__ void write(void* dst, int w, int lane) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (PIECES % NW == 0 || NW * n + w < PIECES) *(u32x4*)((char*)dst + (NW * n + w) * 1024 + lane * 16) = v[n];
+    }
+};
+
 // 16 bytes per lane straight from memory into LDS (lane l's land at dst + 16 l); complete after the next workgroup barrier.
 __device__ __forceinline__ void copy16(const void* src, void* dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,

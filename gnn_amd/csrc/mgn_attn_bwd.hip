@@ -29,7 +29,7 @@ struct AttnBwd {
     int zero;                                          // rows outside all segments become zeros
 };
 
-constexpr int PSHIFT = 13;
+constexpr int PSHIFT = 15 - OVER;
 
 // ------------------------------------------------------------------------------------------------ query side
 template <int KIND, int DP, int BIAS>
@@ -93,8 +93,8 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
     if constexpr (BIAS > 0) {
         const int* p = a.qpos + ((g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1)) * (long long)a.axes * 32 + j;
         qx = p[0];
-        if (a.axes > 1) qy = p[32];
-        if (a.axes > 2) qz = p[64];
+        if (BIAS > 1) qy = p[32];
+        if (BIAS > 2) qz = p[64];
         most = (float)(a.reach * a.reach) + 0.5f;
         const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
         for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
@@ -108,8 +108,9 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
         for (int s = lane; s < n_sub; s += 64) { const i32x4 r = rec[s]; ek = max(ek, r[0]); ev = max(ev, r[1]); }
         ek = wave_max_i(ek); ev = wave_max_i(ev);
     }
-    // unit of dS in the second product: |dP - delta| < 2^(2 TOP + log2 width + 1) in units of the operands, held below 2^15
-    const int unit = KIND == AT_BF16 ? 0 : min(max(rq[1] + ev + 2 * TOP + LOG_DP - 14, -126), 126);
+    // unit of dS in the second product: |dP - delta| < 2^(2 TOP + log2 width + 1) in units of the operands, times P < 2^OVER before
+    // it is divided by its sum, held below 2^15
+    const int unit = KIND == AT_BF16 ? 0 : min(max(rq[1] + ev + 2 * TOP + LOG_DP + OVER - 14, -126), 126);
     const float down = KIND == AT_BF16 ? norm : norm * pow2i(-unit);
     float* sums = hist + w * a.n_bucket * 64 + lane;           // this lane's sums of dS by bucket
 
@@ -120,7 +121,9 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
     for (int sub = 0; sub < n_sub; ++sub) {
         const int b = sub & 1;
         if (sub + 1 < n_sub) stage(b ^ 1, sub + 1);
-        const i32x4 r = rec[sub];
+        i32x4 r = rec[sub];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) r[e] = __builtin_amdgcn_readfirstlane(r[e]);
         const u32x4 *kr = (const u32x4*)buf[b] + lane, *kt = (const u32x4*)(buf[b] + SUB) + lane, *vr = IMAGES == 3 ? (const u32x4*)(buf[b] + 2 * SUB) + lane : (const u32x4*)(a.v_r + (ksub + sub) * SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -138,23 +141,22 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
         const int sh = KIND == AT_BF16 ? 0 : max(r[0] - ek, FAR_EXP);
         const float up = KIND == AT_BF16 ? 1.f : sub & 1 ? -pow2i(r[1] + rq[1]) : pow2i(r[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
         const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
-        const unsigned valid = (unsigned)r[2];
+        if (r[2] != -1) mask_scores(s, r[2], h);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             int bk[4] = {0, 0, 0, 0};
             if constexpr (BIAS > 0) {
-                const int* p = pbuf[b] + 8 * q + 4 * h;
-                const i32x4 x = *(const i32x4*)p, y = a.axes > 1 ? *(const i32x4*)(p + 32) : x, z = a.axes > 2 ? *(const i32x4*)(p + 64) : x;
+                i32x4 x, y, z;
+                places4<BIAS>(pbuf[b] + 8 * q + 4 * h, x, y, z);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.axes, a.reach, most)];
+                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.reach, most)];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int n = 4 * q + e;
                 float x = s[n] * c;
                 if constexpr (BIAS > 0) x = __builtin_fmaf(s[n], c, tab[bk[e]]);
-                float pe = __builtin_amdgcn_exp2f(x - m);
-                if (valid != 0xffffffffu) pe = (valid >> (8 * q + 4 * h + e) & 1) ? pe : 0.f;
+                const float pe = __builtin_amdgcn_exp2f(x - m);
                 const float d = KIND == AT_BF16 ? dp[n] - delta : __builtin_fmaf(dp[n], up, -delta);
                 s[n] = pe * dn * d;
                 if constexpr (BIAS > 0)
@@ -276,8 +278,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
     if constexpr (BIAS > 0) {
         const int* p = a.kpos + kplace * a.axes * 32 + j;
         kx = p[0];
-        if (a.axes > 1) ky = p[32];
-        if (a.axes > 2) kz = p[64];
+        if (BIAS > 1) ky = p[32];
+        if (BIAS > 2) kz = p[64];
         most = (float)(a.reach * a.reach) + 0.5f;
         const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
         for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         for (int i = i0 + lane; i < i1; i += 64) { const i32x4 r = a.rec_q[qsub_of(i)]; eq = max(eq, r[0]); eg = max(eg, r[1]); }
         eq = wave_max_i(eq); eg = wave_max_i(eg);
     }
-    const int unit = KIND == AT_BF16 ? 0 : min(max(rk[1] + eg + 2 * TOP + LOG_DP - 14, -126), 126);
+    const int unit = KIND == AT_BF16 ? 0 : min(max(rk[1] + eg + 2 * TOP + LOG_DP + OVER - 14, -126), 126);
 
     f32x16 dk[NB], dv[NB];
 #pragma unroll
@@ -298,7 +300,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
     for (int item = i0; item < i1; ++item) {
         const int b = (item - i0) & 1;
         if (item + 1 < i1) stage(b ^ 1, item + 1);
-        const i32x4 r = a.rec_q[qsub_of(item)];
+        i32x4 r = a.rec_q[qsub_of(item)];
+        r[0] = __builtin_amdgcn_readfirstlane(r[0]); r[1] = __builtin_amdgcn_readfirstlane(r[1]);
         const u32x4 *qr = (const u32x4*)buf[b] + lane, *qt = (const u32x4*)(buf[b] + SUB) + lane;
         const u32x4 *gr = (const u32x4*)(buf[b] + 2 * SUB) + lane, *gt = (const u32x4*)(buf[b] + 3 * SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
@@ -325,10 +328,10 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
             const f32x4 m = *(const f32x4*)rr, norm = *(const f32x4*)(rr + 32), delta = *(const f32x4*)(rr + 64);
             int bk[4] = {0, 0, 0, 0};
             if constexpr (BIAS > 0) {
-                const int* pp = pbuf[b] + 8 * q + 4 * h;
-                const i32x4 x = *(const i32x4*)pp, y = a.axes > 1 ? *(const i32x4*)(pp + 32) : x, z = a.axes > 2 ? *(const i32x4*)(pp + 64) : x;
+                i32x4 x, y, z;
+                places4<BIAS>(pbuf[b] + 8 * q + 4 * h, x, y, z);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(x[e], y[e], z[e], kx, ky, kz, a.axes, a.reach, most)];
+                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(x[e], y[e], z[e], kx, ky, kz, a.reach, most)];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -464,7 +467,8 @@ template <int KIND, int DP>
 bool bwd_bias(const AttnBwd& b, const BwdSpace& s, int bias, hipStream_t st) {
     if (bias == 0) return bwd_launch<KIND, DP, 0>(b, s, st);
     if (bias == 1) return bwd_launch<KIND, DP, 1>(b, s, st);
-    return bwd_launch<KIND, DP, 2>(b, s, st);
+    if (bias == 2) return bwd_launch<KIND, DP, 2>(b, s, st);
+    return bwd_launch<KIND, DP, 3>(b, s, st);
 }
 template <int KIND>
 bool bwd_kind(const AttnBwd& b, const BwdSpace& s, int dp, int bias, hipStream_t st) {

@@ -106,8 +106,8 @@ __global__ __launch_bounds__(256, REP == 8 && (bias || KIND == AT_F32) ? 1 : 2) 
             p.k[u].get(kv);
             int bucket = 0;
             if constexpr (bias)
-                bucket = lutb[a.axes == 1 ? place<1>(qx, qy, qz, p.x[u], p.y[u], p.z[u], 1, a.reach, most)
-                                          : place<2>(qx, qy, qz, p.x[u], p.y[u], p.z[u], a.axes, a.reach, most)];
+                bucket = lutb[a.axes == 1 ? place<1>(qx, qy, qz, p.x[u], p.y[u], p.z[u], a.reach, most)
+                                          : place<3>(qx, qy, qz, p.x[u], p.y[u], p.z[u], a.reach, most)];   // an axis that is not there is zero on both sides
 #pragma unroll
             for (int r = 0; r < REP; ++r) {
                 float x = 0.f;

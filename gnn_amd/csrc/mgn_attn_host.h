@@ -13,6 +13,7 @@ struct AttnFwd {
     const int* q_pos; const float* table; const int* lut; int n_bucket, reach, axes;
     void* out; long long o_st, o_sh; float *stats, *out32;
     int splits; float *part, *part_ml;
+    int waves, share;                                     // of a workgroup of the tiled kernel; heads that a wave takes
     int zero;                                             // rows outside all segments become zeros
 };
 
@@ -22,7 +23,7 @@ namespace {
 
 inline int attn_kind(int dtype) { return dtype == MGN_BF16 ? AT_BF16 : dtype == MGN_F16 ? AT_F16 : AT_F32; }
 inline int attn_dp(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
-inline int attn_bias(const MgnAttn& a) { return !a.bias_table ? 0 : a.axes == 1 ? 1 : 2; }
+inline int attn_bias(const MgnAttn& a) { return a.bias_table ? a.axes : 0; }      // axes of the bias's places; 0: no bias
 inline int attn_subtiles(int64_t n, int n_seg) { return (int)(n / 32) + n_seg; }
 
 inline bool attn_bad_rows(const void* p, int64_t st, int64_t sh, int dtype) {
@@ -80,7 +81,18 @@ inline int attn_few_splits(const MgnAttn& a) {
     if (s > keys / 256) s = keys / 256;
     return (int)(s < 1 ? 1 : s > ATT_MAX_SPLITS ? ATT_MAX_SPLITS : s);
 }
-// The tiled kernel: the same, in pieces of at least 256 keys, when its query tiles leave compute units idle.
+inline int attn_fwd_waves(const MgnAttn& a) {
+    return !a.bias_table && attn_dp(a.dim) == 128 && a.dtype != MGN_F32 && (a.n_q / 256 + a.n_seg) * a.heads >= 256 ? 8 : 4;
+}
+// Two heads per wave of the tiled kernel share the places of a lattice, where the registers hold them and four workgroups per
+// compute unit are there to begin with (100 000 x 1225, 4 heads of 32, plane: fp32 380 -> 370 us, fp16 266 -> 225; of 64, fp16
+// 316 -> 305; 32 768 queries, fp32, 125 -> 112).  A place on a line is too cheap to share (295 us alone, 316 shared), and two
+// heads of 64 in fp32 spill.
+inline int attn_fwd_share(const MgnAttn& a) {
+    return a.bias_table && a.axes > 1 && attn_dp(a.dim) <= (a.dtype == MGN_F32 ? 32 : 64) && a.heads % 2 == 0 &&
+           (a.n_q / ATT_TQ + a.n_seg) * a.heads >= 1024 ? 2 : 1;
+}
+// Key ranges are split as for few queries when the query tiles leave compute units idle.
 inline int attn_fwd_splits(const MgnAttn& a) {
     const int64_t blocks = (a.n_q / ATT_TQ + a.n_seg) * a.heads, keys = a.n_k / a.n_seg;
     int64_t s = blocks > 0 ? 512 / blocks : 1;
