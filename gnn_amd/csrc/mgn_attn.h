@@ -238,17 +238,16 @@ __device__ __forceinline__ int lane_zero() {
 
 // Exponents and valid bits of a step (key exponent, value exponent, mask), requested a step ahead and then made uniform.  Only
 // what is used is loaded: the unused part of a wider load would be overwritten early, behind a wait for the load.
-template <int KIND> struct Record {
-    int v[3];
+template <int KIND, int N = 3> struct Record {
+    int v[N];
     __device__ __forceinline__ void request(const i32x4* at) {
         const int* p = (const int*)at;
-        v[0] = v[1] = 0;
-        if constexpr (KIND != AT_BF16) { v[0] = p[0]; v[1] = p[1]; }
-        v[2] = p[2];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = KIND != AT_BF16 || e == 2 ? p[e] : 0;
     }
     __device__ __forceinline__ void settle() {
 #pragma unroll
-        for (int e = 0; e < 3; ++e) v[e] = __builtin_amdgcn_readfirstlane(v[e]);
+        for (int e = 0; e < N; ++e) v[e] = __builtin_amdgcn_readfirstlane(v[e]);
     }
 };
 
@@ -269,20 +268,6 @@ template <int PIECES, int NW = 4> struct Staged {
             if (PIECES % NW == 0 || NW * n + w < PIECES) *(u32x4*)((char*)dst + (NW * n + w) * 1024 + lane * 16) = v[n];
     }
 };
-
-// 16 bytes per lane straight from memory into LDS (lane l's land at dst + 16 l); complete after the next workgroup barrier.
-__device__ __forceinline__ void copy16(const void* src, void* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-}
-__device__ __forceinline__ void copy4(const void* src, void* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
-}
-__device__ __forceinline__ void barrier_all() {               // transfers into LDS have landed, then every wave meets
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-}
 
 // ------------------------------------------------------------------------------------------------ operand images
 struct ImageJob {

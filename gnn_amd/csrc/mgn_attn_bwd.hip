@@ -31,16 +31,32 @@ struct AttnBwd {
 
 constexpr int PSHIFT = 15 - OVER;
 
+// A place's bias, base 2, and the byte offset of its bucket's sums.
+struct Entry { float bias; int offset; };
+template <int BIAS> constexpr int LUTS = BIAS == 1 ? 2 * ATT_MAX_REACH + 1 : ATT_MAX_REACH + 1;
+template <int BIAS>
+__device__ __forceinline__ void fill_entries(Entry* entry, const AttnBwd& a, int head, int stride, int t) {
+    for (int r = t; r < (BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1); r += 256) {
+        const int b = min(max(a.lut[r], 0), a.n_bucket - 1);
+        entry[r] = {bias_log2(a.table[head * a.n_bucket + b]), b * stride};
+    }
+}
+template <int BIAS>
+__device__ __forceinline__ void fill_biases(float* lutb, const AttnBwd& a, int head, int t) {
+    for (int r = t; r < (BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1); r += 256)
+        lutb[r] = bias_log2(a.table[head * a.n_bucket + min(max(a.lut[r], 0), a.n_bucket - 1)]);
+}
+constexpr int GROUP = 2;                               // sums by bucket that are read, added to and written together
+
 // ------------------------------------------------------------------------------------------------ query side
 template <int KIND, int DP, int BIAS>
-__global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void attn_dq_kernel(AttnBwd a) {
+__global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : 2) void attn_dq_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
     // fp32 at width 128 with a table: the sums by bucket take up to 64 KB, so the values are read past LDS
     constexpr int IMAGES = KIND == AT_F32 && DP == 128 && BIAS > 0 ? 2 : 3;
     __shared__ __attribute__((aligned(1024))) unsigned short buf[2][IMAGES * SUB];     // K as R, K as T, V as R
     __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 2 : 1][BIAS ? 128 : 1];
-    __shared__ unsigned char lutb[BIAS ? 2 * ATT_MAX_REACH + 1 : 1];
-    __shared__ float tab[BIAS ? ATT_MAX_BUCKETS : 1];
+    __shared__ Entry entry[BIAS ? LUTS<BIAS> : 1];                                     // by place
     extern __shared__ float hist[];                                                    // [4 waves][n_bucket][64], with a table gradient
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
@@ -61,21 +77,22 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
     const long long row = g.first + min(qi, g.len - 1);
     const long long qsub = (long long)head * a.ns_q + (g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1);
 
-    auto stage = [&](int b, int s) {
-        constexpr int BYTES = SUB * 2;
-        const char* src[3] = {(const char*)(a.k_r + (ksub + s) * SUB), (const char*)(a.k_t + (ksub + s) * SUB), (const char*)(a.v_r + (ksub + s) * SUB)};
-#pragma unroll
-        for (int n = 0; n < IMAGES * BYTES; n += 4096) {
-            const int off = n + w * 1024;
-            if (off < IMAGES * BYTES) copy16(src[off / BYTES] + off % BYTES + lane * 16, (char*)buf[b] + off);
-        }
-        if constexpr (BIAS > 0)
-            if (w == 3)
-                for (int ax = 0; ax < a.axes; ax += 2)
-                    if (ax * 32 + lane < a.axes * 32)
-                        copy4(a.kpos + (((k0 >> 5) + g.seg + s) * a.axes + ax) * 32 + lane, pbuf[b] + 32 * ax);
+    constexpr int PIECES = SUB * 2 / 1024;
+    const int last = n_sub - 1, lz = lane_zero();
+    Staged<IMAGES * PIECES> st;
+    int sp = 0;
+    auto request = [&](int s) {
+        st.request(w, lane, [&](int c) {
+            const int image = c / PIECES;
+            return (const char*)(image == 0 ? a.k_r : image == 1 ? a.k_t : a.v_r) + (ksub + s) * (SUB * 2) + (c % PIECES) * 1024;
+        });
+        if (BIAS > 0 && t < BIAS * 32) sp = a.kpos[((k0 >> 5) + g.seg + s) * (BIAS * 32) + t];
     };
-    if (n_sub > 0) stage(0, 0);
+    auto arrive = [&](int b) {
+        st.write(buf[b], w, lane);
+        if (BIAS > 0 && t < BIAS * 32) pbuf[b][t] = sp;
+    };
+    if (n_sub > 0) request(0);
 
     u32x4 qf[PL][NC], gf[PL][NC];
     {
@@ -96,9 +113,7 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
         if (BIAS > 1) qy = p[32];
         if (BIAS > 2) qz = p[64];
         most = (float)(a.reach * a.reach) + 0.5f;
-        const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
-        for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
-        if (t < a.n_bucket) tab[t] = bias_log2(a.table[head * a.n_bucket + t]);
+        fill_entries<BIAS>(entry, a, head, 256, t);
         if (a.tpart)
             for (int r = t; r < a.n_bucket * 256; r += 256) hist[r] = 0.f;
     }
@@ -112,18 +127,18 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
     // it is divided by its sum, held below 2^15
     const int unit = KIND == AT_BF16 ? 0 : min(max(rq[1] + ev + 2 * TOP + LOG_DP + OVER - 14, -126), 126);
     const float down = KIND == AT_BF16 ? norm : norm * pow2i(-unit);
-    float* sums = hist + w * a.n_bucket * 64 + lane;           // this lane's sums of dS by bucket
+    char* sums = (char*)(hist + w * a.n_bucket * 64 + lane);   // this lane's sums of dS by bucket
+    Record<KIND> r, rn;
+    if (n_sub > 0) { r.request(rec + lz); r.settle(); arrive(0); }
 
     f32x16 dq[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) dq[b] = zero16();
-    barrier_all();
+    __syncthreads();
     for (int sub = 0; sub < n_sub; ++sub) {
         const int b = sub & 1;
-        if (sub + 1 < n_sub) stage(b ^ 1, sub + 1);
-        i32x4 r = rec[sub];
-#pragma unroll
-        for (int e = 0; e < 3; ++e) r[e] = __builtin_amdgcn_readfirstlane(r[e]);
+        request(min(sub + 1, last));
+        rn.request(rec + min(sub + 1, last) + lz);
         const u32x4 *kr = (const u32x4*)buf[b] + lane, *kt = (const u32x4*)(buf[b] + SUB) + lane, *vr = IMAGES == 3 ? (const u32x4*)(buf[b] + 2 * SUB) + lane : (const u32x4*)(a.v_r + (ksub + sub) * SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -137,32 +152,46 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
             s = mma<KIND>(kr[c * 64], qf[0][c], s);
             dp = mma<KIND>(vr[c * 64], gf[0][c], dp);
         }
-        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r[0]) * pow2i(rq[0]);
-        const int sh = KIND == AT_BF16 ? 0 : max(r[0] - ek, FAR_EXP);
-        const float up = KIND == AT_BF16 ? 1.f : sub & 1 ? -pow2i(r[1] + rq[1]) : pow2i(r[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
-        const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
-        if (r[2] != -1) mask_scores(s, r[2], h);
+        int off[BIAS ? 16 : 1];                                // of the buckets' sums
+        float add[BIAS ? 16 : 1];
+        if constexpr (BIAS > 0)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            int bk[4] = {0, 0, 0, 0};
-            if constexpr (BIAS > 0) {
+            for (int q = 0; q < 4; ++q) {
                 i32x4 x, y, z;
                 places4<BIAS>(pbuf[b] + 8 * q + 4 * h, x, y, z);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.reach, most)];
+                for (int e = 0; e < 4; ++e) {
+                    const Entry en = entry[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.reach, most)];
+                    add[4 * q + e] = en.bias; off[4 * q + e] = en.offset;
+                }
             }
+        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r.v[0]) * pow2i(rq[0]);
+        const int sh = KIND == AT_BF16 ? 0 : max(r.v[0] - ek, FAR_EXP);
+        const float up = KIND == AT_BF16 ? 1.f : sub & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
+        const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
+        if (r.v[2] != -1) mask_scores(s, r.v[2], h);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = 4 * q + e;
-                float x = s[n] * c;
-                if constexpr (BIAS > 0) x = __builtin_fmaf(s[n], c, tab[bk[e]]);
-                const float pe = __builtin_amdgcn_exp2f(x - m);
-                const float d = KIND == AT_BF16 ? dp[n] - delta : __builtin_fmaf(dp[n], up, -delta);
-                s[n] = pe * dn * d;
-                if constexpr (BIAS > 0)
-                    if (a.tpart) sums[bk[e] * 64] += s[n] * whole;
-            }
+        for (int n = 0; n < 16; ++n) {
+            const float x = BIAS > 0 ? __builtin_fmaf(s[n], c, add[BIAS ? n : 0]) - m : __builtin_fmaf(s[n], c, -m);
+            const float d = KIND == AT_BF16 ? dp[n] - delta : __builtin_fmaf(dp[n], up, -delta);
+            s[n] = __builtin_amdgcn_exp2f(x) * dn * d;
         }
+        if constexpr (BIAS > 0)
+            if (a.tpart)
+#pragma unroll
+                for (int n = 0; n < 16; n += GROUP) {
+                    float v[GROUP];
+#pragma unroll
+                    for (int e = 0; e < GROUP; ++e) v[e] = *(const float*)(sums + off[n + e]);
+#pragma unroll
+                    for (int e = 0; e < GROUP; ++e) {
+#pragma unroll
+                        for (int p = 0; p < e; ++p) v[e] = off[n + e] == off[n + p] ? v[p] : v[e];
+                        v[e] = __builtin_fmaf(s[n + e], whole, v[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < GROUP; ++e) *(float*)(sums + off[n + e]) = v[e];
+                }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
             float v[8];
@@ -179,7 +208,10 @@ __global__ __launch_bounds__(256, (KIND == AT_F32 && DP == 128) ? 1 : 2) void at
                 dq[n] = mma<KIND>(kt[(kc * NB + n) * 64], hi, dq[n]);
             }
         }
-        barrier_all();
+        arrive(b ^ 1);
+        r = rn;
+        r.settle();
+        __syncthreads();
     }
     if (mine) {
 #pragma unroll
@@ -227,8 +259,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
     __shared__ __attribute__((aligned(1024))) unsigned short buf[2][4 * SUB];          // Q as R, Q as T, dO as R, dO as T
     __shared__ __attribute__((aligned(16))) float rbuf[2][128];
     __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 2 : 1][BIAS ? 128 : 1];
-    __shared__ unsigned char lutb[BIAS ? 2 * ATT_MAX_REACH + 1 : 1];
-    extern __shared__ float tab[];                                                     // [heads per key head][n_bucket], with a bias
+    __shared__ float lutb[BIAS ? LUTS<BIAS> : 1];                                      // the bias by place, of the current head
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x % a.kv_heads, rep = a.heads / a.kv_heads, split = blockIdx.y;
@@ -246,23 +277,31 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
     const long long kplace = (g.first >> 5) + g.seg + wsub, ksub = (long long)kvh * a.ns_k + kplace;
 
     auto qsub_of = [&](int item) { return (head0 + item / n_sub) * a.ns_q + qbase + item % n_sub; };
-    auto stage = [&](int b, int item) {
-        constexpr int BYTES = SUB * 2;
-        const long long s = qsub_of(item);
-        const char* src[4] = {(const char*)(a.q_r + s * SUB), (const char*)(a.q_t + s * SUB), (const char*)(a.g_r + s * SUB), (const char*)(a.g_t + s * SUB)};
-#pragma unroll
-        for (int n = 0; n < 4 * BYTES; n += 4096) {
-            const int off = n + w * 1024;
-            copy16(src[off / BYTES] + off % BYTES + lane * 16, (char*)buf[b] + off);
-        }
-        if (w < 2 && w * 64 + lane < 96) copy4(a.rows + s * 96 + w * 64 + lane, rbuf[b] + w * 64);
-        if constexpr (BIAS > 0)
-            if (w == 3)
-                for (int ax = 0; ax < a.axes; ax += 2)
-                    if (ax * 32 + lane < a.axes * 32)
-                        copy4(a.qpos + ((qbase + item % n_sub) * a.axes + ax) * 32 + lane, pbuf[b] + 32 * ax);
+    constexpr int PIECES = SUB * 2 / 1024;
+    const int lz = lane_zero();
+    int rep_at = i0 < i1 ? i0 / n_sub : 0, sub_at = i0 < i1 ? i0 % n_sub : 0;            // of the item that is requested next
+    Staged<4 * PIECES> st;
+    float sr = 0.f;
+    int sp = 0;
+    Record<KIND, 2> r, rn;
+    auto request = [&]() {
+        const long long s = (head0 + rep_at) * a.ns_q + qbase + sub_at;
+        st.request(w, lane, [&](int c) {
+            const int image = c / PIECES;
+            return (const char*)(image == 0 ? a.q_r : image == 1 ? a.q_t : image == 2 ? a.g_r : a.g_t) + s * (SUB * 2) + (c % PIECES) * 1024;
+        });
+        if (t < 96) sr = a.rows[s * 96 + t];
+        if (BIAS > 0 && t < BIAS * 32) sp = a.qpos[(qbase + sub_at) * (BIAS * 32) + t];
+        rn.request(a.rec_q + s + lz);
     };
-    if (i0 < i1) stage(0, i0);
+    auto arrive = [&](int b) {
+        st.write(buf[b], w, lane);
+        if (t < 96) rbuf[b][t] = sr;
+        if (BIAS > 0 && t < BIAS * 32) pbuf[b][t] = sp;
+        r = rn;
+        r.settle();
+    };
+    if (i0 < i1) request();
 
     u32x4 kf[PL][NC], vf[PL][NC];
     {
@@ -281,9 +320,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         if (BIAS > 1) ky = p[32];
         if (BIAS > 2) kz = p[64];
         most = (float)(a.reach * a.reach) + 0.5f;
-        const int entries = BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1;
-        for (int r = t; r < entries; r += 256) lutb[r] = (unsigned char)min(max(a.lut[r], 0), a.n_bucket - 1);
-        for (int r = t; r < rep * a.n_bucket; r += 256) tab[r] = bias_log2(a.table[head0 * a.n_bucket + r]);
+        if (i0 < i1) fill_biases<BIAS>(lutb, a, (int)head0 + rep_at, t);
     }
     int eq = 0, eg = 0;                                       // common exponents of the queries and gradients in this range
     if constexpr (KIND != AT_BF16) {
@@ -296,12 +333,15 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
     f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) { dk[b] = zero16(); dv[b] = zero16(); }
-    barrier_all();
+    if (i0 < i1) arrive(0);
+    __syncthreads();
     for (int item = i0; item < i1; ++item) {
         const int b = (item - i0) & 1;
-        if (item + 1 < i1) stage(b ^ 1, item + 1);
-        i32x4 r = a.rec_q[qsub_of(item)];
-        r[0] = __builtin_amdgcn_readfirstlane(r[0]); r[1] = __builtin_amdgcn_readfirstlane(r[1]);
+        bool next_head = false;
+        if (item + 1 < i1) {
+            if (++sub_at == n_sub) { sub_at = 0; ++rep_at; next_head = true; }
+        }
+        request();
         const u32x4 *qr = (const u32x4*)buf[b] + lane, *qt = (const u32x4*)(buf[b] + SUB) + lane;
         const u32x4 *gr = (const u32x4*)(buf[b] + 2 * SUB) + lane, *gt = (const u32x4*)(buf[b] + 3 * SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
@@ -316,29 +356,27 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
             s = mma<KIND>(qr[c * 64], kf[0][c], s);
             dp = mma<KIND>(gr[c * 64], vf[0][c], dp);
         }
-        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r[0]) * pow2i(rk[0]);
-        const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r[1] + rk[1]) : pow2i(r[1] + rk[1]);
-        const float fp = KIND == AT_BF16 ? 1.f : pow2i(PSHIFT + max(r[1] - eg, FAR_EXP));              // of P in the product with dO
-        const float fs = KIND == AT_BF16 ? 1.f : pow2i(max(r[0] - eq, FAR_EXP) - unit);               // of dS in the product with Q
-        const float* tb = tab + (item / max(n_sub, 1)) * a.n_bucket;
+        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r.v[0]) * pow2i(rk[0]);
+        const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r.v[1] + rk[1]) : pow2i(r.v[1] + rk[1]);
+        const float fp = KIND == AT_BF16 ? 1.f : pow2i(PSHIFT + max(r.v[1] - eg, FAR_EXP));            // of P in the product with dO
+        const float fs = KIND == AT_BF16 ? 1.f : pow2i(max(r.v[0] - eq, FAR_EXP) - unit);             // of dS in the product with Q
         f32x16 p;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float* rr = rbuf[b] + 8 * q + 4 * h;
             const f32x4 m = *(const f32x4*)rr, norm = *(const f32x4*)(rr + 32), delta = *(const f32x4*)(rr + 64);
-            int bk[4] = {0, 0, 0, 0};
+            float add[4] = {0.f, 0.f, 0.f, 0.f};
             if constexpr (BIAS > 0) {
                 i32x4 x, y, z;
                 places4<BIAS>(pbuf[b] + 8 * q + 4 * h, x, y, z);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) bk[e] = lutb[place<BIAS>(x[e], y[e], z[e], kx, ky, kz, a.reach, most)];
+                for (int e = 0; e < 4; ++e) add[e] = lutb[place<BIAS>(x[e], y[e], z[e], kx, ky, kz, a.reach, most)];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int n = 4 * q + e;
-                float x = s[n] * c;
-                if constexpr (BIAS > 0) x = __builtin_fmaf(s[n], c, tb[bk[e]]);
-                float pe = __builtin_amdgcn_exp2f(x - m[e]);
+                const float x = BIAS > 0 ? __builtin_fmaf(s[n], c, add[e]) - m[e] : __builtin_fmaf(s[n], c, -m[e]);
+                float pe = __builtin_amdgcn_exp2f(x);
                 if constexpr (KIND != AT_F32) pe *= norm[e];
                 const float d = KIND == AT_BF16 ? dp[n] - delta[e] : __builtin_fmaf(dp[n], up, -delta[e]);
                 s[n] = KIND == AT_BF16 ? pe * d : (pe * fs) * d;
@@ -367,7 +405,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
                 dk[n] = mma<KIND>(qt[(kc * NB + n) * 64], shi, dk[n]);
             }
         }
-        barrier_all();
+        arrive(b ^ 1);
+        __syncthreads();
+        if (BIAS > 0 && next_head) {                           // the next item is of another head
+            fill_biases<BIAS>(lutb, a, (int)head0 + rep_at, t);
+            __syncthreads();
+        }
     }
     if (ki >= g.len) return;
     const bool keep = (unsigned)rk[2] >> j & 1;                // a masked key has no gradient
@@ -457,10 +500,10 @@ bool lds_fits(K kernel, int dynamic) {
 
 template <int KIND, int DP, int BIAS>
 bool bwd_launch(const AttnBwd& b, const BwdSpace& s, hipStream_t st) {
-    const int hist = BIAS > 0 && b.tpart ? b.n_bucket * 1024 : 0, tab = BIAS > 0 ? b.heads / b.kv_heads * b.n_bucket * 4 : 0;
-    if (!lds_fits(attn_dq_kernel<KIND, DP, BIAS>, hist) || !lds_fits(attn_dkv_kernel<KIND, DP, BIAS>, tab)) return false;
+    const int hist = BIAS > 0 && b.tpart ? b.n_bucket * 1024 : 0;
+    if (!lds_fits(attn_dq_kernel<KIND, DP, BIAS>, hist)) return false;
     hipLaunchKernelGGL((attn_dq_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.q_tiles * b.heads)), dim3(256), hist, st, b);
-    if (b.n_k > 0) hipLaunchKernelGGL((attn_dkv_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.k_tiles * b.kv_heads), (unsigned)s.splits), dim3(256), tab, st, b);
+    if (b.n_k > 0) hipLaunchKernelGGL((attn_dkv_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.k_tiles * b.kv_heads), (unsigned)s.splits), dim3(256), 0, st, b);
     return true;
 }
 template <int KIND, int DP>
@@ -501,7 +544,6 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     else if (a.n_q > 0 && (attn_bad_rows(g, g_st, g_sh, a.dtype) || attn_bad_rows(out, out_st, out_sh, a.out_f32 ? MGN_F32 : a.dtype))) bad = "rows must start on 16-byte borders";
     else if (((uintptr_t)dq & 15) || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15)) bad = "gradients must start on 16-byte borders";
     else if (!workspace || workspace_bytes < (int64_t)s.total) bad = "the workspace is missing or too small";
-    else if (a.bias_table && a.heads / a.kv_heads * a.n_bucket > 4096) bad = "more than 4096 table entries per key head";
     if (bad) { mgn_set_error("mgn_attn_bwd: %s", bad); return MGN_E_ARG; }
     char* ws = (char*)workspace;
     const int kind = attn_kind(a.dtype), dp = attn_dp(a.dim), bias = attn_bias(a);
