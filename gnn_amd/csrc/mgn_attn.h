@@ -57,12 +57,14 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
 // eight consecutive values as one operand (hi), and for two planes what is left of them (lo)
 template <int KIND, bool TWO = KIND == AT_F32>
 __device__ __forceinline__ void pack8(const float* v, u32x4& hi, u32x4& lo) {
+    float minus;                                              // -1 that is not folded: v - (float)h as one mixed instruction
+    asm("v_mov_b32 %0, -1.0" : "=v"(minus));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (KIND == AT_F32 || (KIND == AT_F16 && TWO)) {
-            unsigned a, b;
-            split2_pair(v[2 * i], v[2 * i + 1], a, b);
-            hi[i] = a; lo[i] = b;
+            const f16x2 a = __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, f16x2);
+            const f32x2 b = {__builtin_fmaf((float)a[0], minus, v[2 * i]), __builtin_fmaf((float)a[1], minus, v[2 * i + 1])};
+            hi[i] = __builtin_bit_cast(unsigned, a); lo[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(b, f16x2));
         } else if constexpr (TWO) {
             const unsigned a = pack2<KIND>(v[2 * i], v[2 * i + 1]);
             hi[i] = a;

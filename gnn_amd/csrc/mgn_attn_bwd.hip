@@ -50,14 +50,14 @@ constexpr int GROUP = 2;                               // sums by bucket that ar
 
 // ------------------------------------------------------------------------------------------------ query side
 template <int KIND, int DP, int BIAS>
-__global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : 2) void attn_dq_kernel(AttnBwd a) {
+__global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
-    // fp32 at width 128 with a table: the sums by bucket take up to 64 KB, so the values are read past LDS
-    constexpr int IMAGES = KIND == AT_F32 && DP == 128 && BIAS > 0 ? 2 : 3;
-    __shared__ __attribute__((aligned(1024))) unsigned short buf[2][IMAGES * SUB];     // K as R, K as T, V as R
-    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 2 : 1][BIAS ? 128 : 1];
-    __shared__ Entry entry[BIAS ? LUTS<BIAS> : 1];                                     // by place
+    // With a bias the sums by bucket leave no room for two buffers if three workgroups are to share a compute unit
+    constexpr int BUFS = BIAS > 0 ? 1 : 2;
+    __shared__ __attribute__((aligned(1024))) unsigned short buf[BUFS][3 * SUB];  // K as R, K as T, V as R
+    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 128 : 1];
     extern __shared__ float hist[];                                                    // [4 waves][n_bucket][64], with a table gradient
+    Entry* entry = (Entry*)(hist + (a.tpart ? a.n_bucket * 256 : 0));                  // by place
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), tile = blockIdx.x / a.heads;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
 
     constexpr int PIECES = SUB * 2 / 1024;
     const int last = n_sub - 1, lz = lane_zero();
-    Staged<IMAGES * PIECES> st;
+    Staged<3 * PIECES> st;
     int sp = 0;
     auto request = [&](int s) {
         st.request(w, lane, [&](int c) {
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     };
     auto arrive = [&](int b) {
         st.write(buf[b], w, lane);
-        if (BIAS > 0 && t < BIAS * 32) pbuf[b][t] = sp;
+        if (BIAS > 0 && t < BIAS * 32) pbuf[t] = sp;
     };
     if (n_sub > 0) request(0);
 
@@ -136,10 +136,10 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     for (int b = 0; b < NB; ++b) dq[b] = zero16();
     __syncthreads();
     for (int sub = 0; sub < n_sub; ++sub) {
-        const int b = sub & 1;
+        const int b = BUFS == 2 ? sub & 1 : 0;
         request(min(sub + 1, last));
         rn.request(rec + min(sub + 1, last) + lz);
-        const u32x4 *kr = (const u32x4*)buf[b] + lane, *kt = (const u32x4*)(buf[b] + SUB) + lane, *vr = IMAGES == 3 ? (const u32x4*)(buf[b] + 2 * SUB) + lane : (const u32x4*)(a.v_r + (ksub + sub) * SUB) + lane;
+        const u32x4 *kr = (const u32x4*)buf[b] + lane, *kt = (const u32x4*)(buf[b] + SUB) + lane, *vr = (const u32x4*)(buf[b] + 2 * SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 i32x4 x, y, z;
-                places4<BIAS>(pbuf[b] + 8 * q + 4 * h, x, y, z);
+                places4<BIAS>(pbuf + 8 * q + 4 * h, x, y, z);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const Entry en = entry[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.reach, most)];
@@ -208,7 +208,8 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                 dq[n] = mma<KIND>(kt[(kc * NB + n) * 64], hi, dq[n]);
             }
         }
-        arrive(b ^ 1);
+        if (BUFS == 1) __syncthreads();
+        arrive(BUFS == 2 ? b ^ 1 : 0);
         r = rn;
         r.settle();
         __syncthreads();
@@ -500,7 +501,7 @@ bool lds_fits(K kernel, int dynamic) {
 
 template <int KIND, int DP, int BIAS>
 bool bwd_launch(const AttnBwd& b, const BwdSpace& s, hipStream_t st) {
-    const int hist = BIAS > 0 && b.tpart ? b.n_bucket * 1024 : 0;
+    const int hist = BIAS > 0 ? (b.tpart ? b.n_bucket * 1024 : 0) + (BIAS == 1 ? 2 * b.reach + 1 : b.reach + 1) * (int)sizeof(Entry) : 0;
     if (!lds_fits(attn_dq_kernel<KIND, DP, BIAS>, hist)) return false;
     hipLaunchKernelGGL((attn_dq_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.q_tiles * b.heads)), dim3(256), hist, st, b);
     if (b.n_k > 0) hipLaunchKernelGGL((attn_dkv_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.k_tiles * b.kv_heads), (unsigned)s.splits), dim3(256), 0, st, b);
