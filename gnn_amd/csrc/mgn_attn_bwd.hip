@@ -24,8 +24,9 @@ struct AttnBwd {
     const int *qpos, *kpos;                            // places [subtile][axes][32]
     const float* table; const int* lut; int n_bucket, reach, axes;
     void *dq, *dk, *dv;                                // dense [tokens][heads][dim]
-    double* tpart; float* dtable; int q_tiles;         // [q_tiles][heads][n_bucket]
-    int splits; float* part;                           // [split][2][kv_heads][ns_k][32][DP]
+    double* tpart; float* dtable; int q_tiles;         // [q_tiles][splits][heads][n_bucket]
+    int splits; float* part;                           // key side: [split][2][kv_heads][ns_k][32][DP]
+    int q_splits; float* q_part;                       // query side: [split][heads][ns_q][32][DP]
     int zero;                                          // rows outside all segments become zeros
 };
 
@@ -33,44 +34,47 @@ constexpr int PSHIFT = 15 - OVER;
 
 // A place's bias, base 2, and the byte offset of its bucket's sums.
 struct Entry { float bias; int offset; };
-template <int BIAS> constexpr int LUTS = BIAS == 1 ? 2 * ATT_MAX_REACH + 1 : ATT_MAX_REACH + 1;
+template <int BIAS> __host__ __device__ constexpr int entries(int reach) { return BIAS == 1 ? 2 * reach + 1 : reach + 1; }
+template <int BIAS> constexpr int LUTS = entries<BIAS>(ATT_MAX_REACH);
 template <int BIAS>
 __device__ __forceinline__ void fill_entries(Entry* entry, const AttnBwd& a, int head, int stride, int t) {
-    for (int r = t; r < (BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1); r += 256) {
+    for (int r = t; r < entries<BIAS>(a.reach); r += 256) {
         const int b = min(max(a.lut[r], 0), a.n_bucket - 1);
         entry[r] = {bias_log2(a.table[head * a.n_bucket + b]), b * stride};
     }
 }
 template <int BIAS>
 __device__ __forceinline__ void fill_biases(float* lutb, const AttnBwd& a, int head, int t) {
-    for (int r = t; r < (BIAS == 1 ? 2 * a.reach + 1 : a.reach + 1); r += 256)
+    for (int r = t; r < entries<BIAS>(a.reach); r += 256)
         lutb[r] = bias_log2(a.table[head * a.n_bucket + min(max(a.lut[r], 0), a.n_bucket - 1)]);
 }
 constexpr int GROUP = 2;                               // sums by bucket that are read, added to and written together
 
 // ------------------------------------------------------------------------------------------------ query side
 template <int KIND, int DP, int BIAS>
-__global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
+__global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : KIND == AT_F32 && DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
-    // With a bias the sums by bucket leave no room for two buffers if three workgroups are to share a compute unit
-    constexpr int BUFS = BIAS > 0 ? 1 : 2;
+    // fp32 with a bias: one buffer and a second barrier, since two would leave the sums by bucket no room (8192 x 4096, 8 heads of
+    // 64: 1095 -> 1028 us for the whole backward pass).  16-bit types: two (8 heads of 32, bf16: 476 us with one, 436 with two).
+    constexpr int BUFS = KIND == AT_F32 && BIAS > 0 ? 1 : 2;
     __shared__ __attribute__((aligned(1024))) unsigned short buf[BUFS][3 * SUB];  // K as R, K as T, V as R
-    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? 128 : 1];
-    extern __shared__ float hist[];                                                    // [4 waves][n_bucket][64], with a table gradient
-    Entry* entry = (Entry*)(hist + (a.tpart ? a.n_bucket * 256 : 0));                  // by place
+    __shared__ __attribute__((aligned(16))) int pbuf[BIAS ? BUFS : 1][BIAS ? 128 : 1];
+    extern __shared__ Entry entry[];                                                   // by place, ...
+    float* hist = (float*)(entry + entries<BIAS>(a.reach));                            // ... and [4 waves][n_bucket][64], with a table gradient
 
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
-    const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), tile = blockIdx.x / a.heads;
+    const int head = blockIdx.x % a.heads, kvh = head / (a.heads / a.kv_heads), tile = blockIdx.x / a.heads, split = blockIdx.y;
     if (a.zero) zero_outside<KIND>(a.q_ptr, a.n_seg, a.n_q, a.dq, (long long)a.heads * a.dim, a.dim, a.heads, a.dim);
     const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 7, tile);
     const bool live = g.local >= 0 && g.local * ATT_TQ < g.len;
     if (!live) {
-        if (BIAS > 0 && a.tpart && t < a.n_bucket) a.tpart[((long long)tile * a.heads + head) * a.n_bucket + t] = 0.0;
+        if (BIAS > 0 && a.tpart && t < a.n_bucket) a.tpart[(((long long)tile * a.q_splits + split) * a.heads + head) * a.n_bucket + t] = 0.0;
         return;
     }
     const long long k0 = seg_at(a.k_ptr, g.seg, a.n_seg, a.n_k), k1 = seg_at(a.k_ptr, g.seg + 1, a.n_seg, a.n_k);
-    const int n_sub = k1 > k0 ? (int)((k1 - k0 + 31) >> 5) : 0;
-    const long long ksub = (long long)kvh * a.ns_k + (k0 >> 5) + g.seg;
+    const int all_sub = k1 > k0 ? (int)((k1 - k0 + 31) >> 5) : 0, per = (all_sub + a.q_splits - 1) / a.q_splits;
+    const int s0 = min(split * per, all_sub), n_sub = min(s0 + per, all_sub) - s0;   // this workgroup's share of the key subtiles
+    const long long kplace = (k0 >> 5) + g.seg + s0, ksub = (long long)kvh * a.ns_k + kplace;
     const i32x4* rec = a.rec_k + ksub;
     const int qi = g.local * ATT_TQ + 32 * w + j, nsq = (g.len + 31) >> 5;
     const bool mine = qi < g.len;
@@ -86,11 +90,11 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
             const int image = c / PIECES;
             return (const char*)(image == 0 ? a.k_r : image == 1 ? a.k_t : a.v_r) + (ksub + s) * (SUB * 2) + (c % PIECES) * 1024;
         });
-        if (BIAS > 0 && t < BIAS * 32) sp = a.kpos[((k0 >> 5) + g.seg + s) * (BIAS * 32) + t];
+        if (BIAS > 0 && t < BIAS * 32) sp = a.kpos[(kplace + s) * (BIAS * 32) + t];
     };
     auto arrive = [&](int b) {
         st.write(buf[b], w, lane);
-        if (BIAS > 0 && t < BIAS * 32) pbuf[t] = sp;
+        if (BIAS > 0 && t < BIAS * 32) pbuf[b][t] = sp;
     };
     if (n_sub > 0) request(0);
 
@@ -158,7 +162,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 i32x4 x, y, z;
-                places4<BIAS>(pbuf + 8 * q + 4 * h, x, y, z);
+                places4<BIAS>(pbuf[b] + 8 * q + 4 * h, x, y, z);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const Entry en = entry[place<BIAS>(qx, qy, qz, x[e], y[e], z[e], a.reach, most)];
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
             }
         const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r.v[0]) * pow2i(rq[0]);
         const int sh = KIND == AT_BF16 ? 0 : max(r.v[0] - ek, FAR_EXP);
-        const float up = KIND == AT_BF16 ? 1.f : sub & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
+        const float up = KIND == AT_BF16 ? 1.f : (s0 + sub) & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
         const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
         if (r.v[2] != -1) mask_scores(s, r.v[2], h);
 #pragma unroll
@@ -223,7 +227,9 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? dq[n][4 * q + e] * a.scale : ldexpf(dq[n][4 * q + e] * a.scale, unit + ek);
-                if (d < a.dim) store4<KIND>(a.dq, (row * a.heads + head) * a.dim + d, v);
+                if (d >= a.dim) continue;
+                if (a.q_splits > 1) *(f32x4*)(a.q_part + (((long long)split * a.heads * a.ns_q + qsub) * 32 + j) * DP + d) = v;
+                else store4<KIND>(a.dq, (row * a.heads + head) * a.dim + d, v);
             }
     }
     if constexpr (BIAS > 0) {
@@ -235,7 +241,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                 for (int x = 0; x < 4; ++x) v += (double)hist[(x * a.n_bucket + b) * 64 + lane];
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1) v += __shfl_down(v, o);
-                if (lane == 0) a.tpart[((long long)tile * a.heads + head) * a.n_bucket + b] = v;
+                if (lane == 0) a.tpart[(((long long)tile * a.q_splits + split) * a.heads + head) * a.n_bucket + b] = v;
             }
         }
     }
@@ -440,7 +446,22 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         }
 }
 
-// dK, dV of a key = sum over the splits, in order; one thread per four values
+// dQ of a query, dK and dV of a key = sum over the splits, in order; one thread per four values.  Memory bound.
+template <int KIND>
+__global__ __launch_bounds__(256) void attn_dq_sum_kernel(AttnBwd a, int dp) {
+    const int quads = a.dim / 4;
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x, units = (long long)a.heads * a.ns_q;
+    if (item >= units * 32 * quads) return;
+    const int quad = (int)(item % quads), i = (int)(item / quads % 32);
+    const long long unit = item / quads / 32;
+    const int head = (int)(unit / a.ns_q), sub = (int)(unit % a.ns_q);
+    const Seg g = find_tile(a.q_ptr, a.n_seg, a.n_q, 5, sub);
+    if (g.local < 0 || g.local * 32 + i >= g.len) return;
+    const float* p = a.q_part + (unit * 32 + i) * dp + 4 * quad;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.q_splits; ++s) v += *(const f32x4*)(p + (long long)s * units * 32 * dp);
+    store4<KIND>(a.dq, ((g.first + g.local * 32 + i) * a.heads + head) * a.dim + 4 * quad, v);
+}
 template <int KIND>
 __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a, int dp) {
     const int quads = a.dim / 4;
@@ -463,7 +484,7 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a, int dp) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct BwdSpace { size_t q_r, q_t, g_r, g_t, k_r, k_t, v_r, rec_q, rec_k, rows, qpos, kpos, tpart, part, total; int ns_q, ns_k, q_tiles, k_tiles, splits; };
+struct BwdSpace { size_t q_r, q_t, g_r, g_t, k_r, k_t, v_r, rec_q, rec_k, rows, qpos, kpos, tpart, part, q_part, total; int ns_q, ns_k, q_tiles, k_tiles, splits, q_splits; };
 
 BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     BwdSpace s{};
@@ -477,13 +498,15 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     int64_t sp = blocks > 0 ? 1024 / blocks : 1;
     if (sp > items / 4) sp = items / 4;
     s.splits = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
+    s.q_splits = attn_round_splits(attn_tiles(a.n_q, a.n_seg, ATT_TQ) * a.heads, a.n_k / a.n_seg, 1);
     const size_t qi = (size_t)a.heads * s.ns_q * pl * 64 * dp, ki = (size_t)a.kv_heads * s.ns_k * pl * 64 * dp;
     s.q_r = take(qi); s.q_t = take(qi); s.g_r = take(qi); s.g_t = take(qi);
     s.k_r = take(ki); s.k_t = take(ki); s.v_r = take(ki);
     s.rec_q = take((size_t)a.heads * s.ns_q * 16); s.rec_k = take((size_t)a.kv_heads * s.ns_k * 16);
     s.rows = take((size_t)a.heads * s.ns_q * 96 * 4);
     if (a.bias_table) { s.qpos = take((size_t)s.ns_q * a.axes * 128); s.kpos = take((size_t)s.ns_k * a.axes * 128); }
-    if (table_grad) s.tpart = take((size_t)s.q_tiles * a.heads * a.n_bucket * 8);
+    if (table_grad) s.tpart = take((size_t)s.q_tiles * s.q_splits * a.heads * a.n_bucket * 8);
+    if (s.q_splits > 1) s.q_part = take((size_t)s.q_splits * a.heads * s.ns_q * 32 * dp * 4);
     if (s.splits > 1) s.part = take((size_t)s.splits * 2 * a.kv_heads * s.ns_k * 32 * dp * 4);
     s.total = at;
     return s;
@@ -501,9 +524,9 @@ bool lds_fits(K kernel, int dynamic) {
 
 template <int KIND, int DP, int BIAS>
 bool bwd_launch(const AttnBwd& b, const BwdSpace& s, hipStream_t st) {
-    const int hist = BIAS > 0 ? (b.tpart ? b.n_bucket * 1024 : 0) + (BIAS == 1 ? 2 * b.reach + 1 : b.reach + 1) * (int)sizeof(Entry) : 0;
+    const int hist = BIAS > 0 ? (b.tpart ? b.n_bucket * 1024 : 0) + entries<BIAS>(b.reach) * (int)sizeof(Entry) : 0;
     if (!lds_fits(attn_dq_kernel<KIND, DP, BIAS>, hist)) return false;
-    hipLaunchKernelGGL((attn_dq_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.q_tiles * b.heads)), dim3(256), hist, st, b);
+    hipLaunchKernelGGL((attn_dq_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.q_tiles * b.heads), (unsigned)s.q_splits), dim3(256), hist, st, b);
     if (b.n_k > 0) hipLaunchKernelGGL((attn_dkv_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.k_tiles * b.kv_heads), (unsigned)s.splits), dim3(256), 0, st, b);
     return true;
 }
@@ -518,6 +541,10 @@ template <int KIND>
 bool bwd_kind(const AttnBwd& b, const BwdSpace& s, int dp, int bias, hipStream_t st) {
     const bool fits = dp == 32 ? bwd_bias<KIND, 32>(b, s, bias, st) : dp == 64 ? bwd_bias<KIND, 64>(b, s, bias, st) : bwd_bias<KIND, 128>(b, s, bias, st);
     if (!fits) return false;
+    if (s.q_splits > 1) {
+        const long long items = (long long)b.heads * s.ns_q * 32 * (b.dim / 4);
+        hipLaunchKernelGGL((attn_dq_sum_kernel<KIND>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, b, dp);
+    }
     if (s.splits > 1) {
         const long long items = (long long)b.kv_heads * s.ns_k * 32 * (b.dim / 4);
         hipLaunchKernelGGL((attn_dkv_sum_kernel<KIND>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, b, dp);
@@ -585,9 +612,10 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     b.table = a.bias_table; b.lut = a.bucket_lut; b.n_bucket = a.n_bucket; b.reach = a.reach; b.axes = a.axes;
     b.dq = dq; b.dk = dk; b.dv = dv; b.dtable = dtable; b.tpart = dtable ? (double*)(ws + s.tpart) : nullptr; b.q_tiles = s.q_tiles;
     b.zero = a.zero_outside && a.q_ptr; b.splits = s.splits; b.part = (float*)(ws + s.part);
+    b.q_splits = s.q_splits; b.q_part = (float*)(ws + s.q_part);
     const bool fits = kind == AT_BF16 ? bwd_kind<AT_BF16>(b, s, dp, bias, st) : kind == AT_F16 ? bwd_kind<AT_F16>(b, s, dp, bias, st)
                                                                                            : bwd_kind<AT_F32>(b, s, dp, bias, st);
     if (!fits) { mgn_set_error("mgn_attn_bwd: %d buckets at width %d do not fit the compute unit's local memory", a.n_bucket, a.dim); return MGN_E_ARG; }
-    if (dtable) hipLaunchKernelGGL(attn_table_kernel, dim3((unsigned)(a.heads * a.n_bucket)), dim3(64), 0, st, b.tpart, dtable, s.q_tiles, a.heads * a.n_bucket);
+    if (dtable) hipLaunchKernelGGL(attn_table_kernel, dim3((unsigned)(a.heads * a.n_bucket)), dim3(64), 0, st, b.tpart, dtable, s.q_tiles * s.q_splits, a.heads * a.n_bucket);
     return check_launch("mgn_attn_bwd");
 }

@@ -887,10 +887,41 @@ __global__ __launch_bounds__(64 * NW) void attn_join_kernel(AttnFwd a) {
     }
 }
 
+// The same for up to eight pieces: four outputs per thread, which reads all factors itself.  Memory bound.
+template <int KIND, int DP>
+__global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnFwd a) {
+    constexpr int QUADS = DP / 4;
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x, stride = a.heads * a.n_q;
+    const int quad = (int)(item % QUADS), head = (int)(item / QUADS % a.heads);
+    const long long row = item / QUADS / a.heads, at = head * a.n_q + row;
+    if (row < seg_at(a.q_ptr, 0, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, a.n_seg, a.n_seg, a.n_q)) return;
+    float m = -__builtin_inff(), l = 0.f;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * stride + at)]);
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const f32x2 ml = *(const f32x2*)(a.part_ml + 2 * (s * stride + at));
+        const float f = __builtin_amdgcn_exp2f(ml[0] - base);
+        l = __builtin_fmaf(f, ml[1], l);
+        o += f * *(const f32x4*)(a.part + (s * stride + at) * DP + 4 * quad);
+    }
+    if (4 * quad < a.dim) {
+        o *= l > 0.f ? 1.0f / l : 0.f;
+        store4<KIND>(a.out, row * a.o_st + head * a.o_sh + 4 * quad, o);
+        if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + 4 * quad) = o;
+    }
+    if (quad == 0 && a.stats) {
+        a.stats[(long long)head * a.n_q + row] = m;
+        a.stats[(long long)(a.heads + head) * a.n_q + row] = l;
+    }
+}
+
 template <int KIND, int DP>
 void join_dp(const AttnFwd& f, hipStream_t st) {
     const dim3 grid((unsigned)(f.n_q * f.heads));
-    if (f.splits > 32) hipLaunchKernelGGL((attn_join_kernel<KIND, DP, 4>), grid, dim3(256), 0, st, f);
+    if (f.splits <= 8) hipLaunchKernelGGL((attn_join_rows_kernel<KIND, DP>), dim3((unsigned)((f.n_q * f.heads * (DP / 4) + 255) / 256)), dim3(256), 0, st, f);
+    else if (f.splits > 32) hipLaunchKernelGGL((attn_join_kernel<KIND, DP, 4>), grid, dim3(256), 0, st, f);
     else hipLaunchKernelGGL((attn_join_kernel<KIND, DP, 1>), grid, dim3(64), 0, st, f);
 }
 template <int KIND>
