@@ -347,3 +347,44 @@ def test_only_the_wanted_gradients():
     o.backward(g)
     assert_close(leaf.grad, reference(q, k, v, g, **kw), "dk")
     assert not attention.cross_attention(q, k, v, **kw).requires_grad
+
+
+# The kernels chosen for many workgroups, reached by many heads and segments instead of long inputs.
+@pytest.mark.parametrize("dtype,dim", [(F32, 32), (F32, 24), (F16, 64), (BF16, 40)])
+@pytest.mark.parametrize("axes", [2, 3])
+def test_two_heads_that_share_places(axes, dtype, dim):
+    nq, nk = [9, 0, 33, 1, 5, 130, 2, 7, 40, 3, 8, 6, 64, 4, 11, 31], [70, 33, 0, 5, 64, 90, 31, 1, 65, 40, 2, 8, 100, 7, 32, 20]
+    q, k, v, g = make(sum(nq) + 5, sum(nk) + 6, heads=64, kv_heads=16, dim=dim, dtype=dtype)
+    gen = torch.Generator().manual_seed(8)
+    mask = (torch.rand(k.shape[0], generator=gen) > 0.2).to(DEV)
+    mask[70:103] = False
+    check(q, k, v, g, q_ptr=ptr(nq, 2), k_ptr=ptr(nk, 3), key_mask=mask, **bias_args(q.shape[0], k.shape[0], 64, axes, 40))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_wide_heads_in_workgroups_of_eight_waves(dtype):
+    nq, nk = [300, 1, 0, 256, 40], [129, 0, 64, 300, 31]
+    q, k, v, g = make(sum(nq) + 3, sum(nk) + 2, heads=64, kv_heads=8, dim=128, dtype=dtype)
+    check(q, k, v, g, q_ptr=ptr(nq, 1), k_ptr=ptr(nk, 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("axes", [0, 1, 2])
+def test_key_ranges_split_to_fill_rounds(axes, dtype):
+    """Key ranges split for the forward pass and for the query gradient: pieces of uneven length, one without keys."""
+    nq, nk = [11, 20, 0, 13, 9, 31, 8, 7, 1], [2100, 4000, 500, 0, 1, 3000, 33, 5000, 4001]
+    q, k, v, g = make(sum(nq) + 4, sum(nk) + 9, heads=64, kv_heads=32, dim=16, dtype=dtype)
+    gen = torch.Generator().manual_seed(8)
+    mask = (torch.rand(k.shape[0], generator=gen) > 0.3).to(DEV)
+    mask[5 + 2100:5 + 2100 + 1990] = False
+    kw = bias_args(q.shape[0], k.shape[0], 64, axes, 200) if axes else {}
+    check(q, k, v, g, q_ptr=ptr(nq, 2), k_ptr=ptr(nk, 5), key_mask=mask, **kw)
+
+
+def test_rows_outside_a_split_forward_are_left_as_they_were():
+    from gnn_amd import ops
+    q, k, v, _ = make(3 * 40 + 20, 9 * 2048 + 5, heads=8)
+    out = torch.full_like(q, 7.0)
+    args = dict(q_ptr=ptr([40, 40, 40], 6), k_ptr=ptr([6000, 6000, 6000], 5))
+    ops.cross_attention(q, k, v, out=out, **args)
+    assert_close(out, reference(q, k, v, **args), "o", outside_kept=7.0)
