@@ -16,7 +16,7 @@ HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Per-file compiler flags.  The attention kernels take maxima of matrix products only to scale by: without -fno-honor-nans every
 # operand of a maximum is first "quieted" by an instruction of its own.  NaN inputs still come out as NaN (through products, sums
 # and exponentials); no comparison in these files asks for one.
-EXTRA_FLAGS = {"mgn_attn_fwd.hip": ["-fno-honor-nans"], "mgn_attn_bwd.hip": ["-fno-honor-nans"], "mgn_attn_few.hip": ["-fno-honor-nans"]}
+EXTRA_FLAGS = {"mgn_attn_fwd.hip": ["-fno-honor-nans"], "mgn_attn_bwd.hip": ["-fno-honor-nans"]}
 
 
 def hipcc_path() -> str:
@@ -29,7 +29,7 @@ def hipcc_path() -> str:
 def needs_build() -> bool:
     if not os.path.exists(OUT):
         return True
-    newest = max(os.path.getmtime(os.path.join(HERE, f)) for f in os.listdir(HERE) if f.endswith((".hip", ".cpp", ".h")))
+    newest = max(os.path.getmtime(os.path.join(HERE, f)) for f in os.listdir(HERE) if f.endswith((".hip", ".cpp", ".h", ".py")))
     newest = max(newest, os.path.getmtime(os.path.join(PKG, "..", "include", "mgn_hip.h")))
     return newest > os.path.getmtime(OUT)
 
@@ -46,7 +46,7 @@ def _compile(src: str, obj: str, verbose: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """One object per translation unit under ``_obj/`` (recompiled when the source or any header is newer), the
+    """One object per translation unit under ``_obj/`` (recompiled when the source, any header or this file is newer), the
     units compiled side by side, then one link."""
     if not force and not needs_build():
         return OUT
@@ -54,7 +54,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     objdir = os.path.join(HERE, "_obj")
     os.makedirs(objdir, exist_ok=True)
     headers = [os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith(".h")]
-    headers.append(os.path.join(PKG, "..", "include", "mgn_hip.h"))
+    headers += [os.path.join(PKG, "..", "include", "mgn_hip.h"), os.path.join(HERE, "build.py")]       # the flags are in this file
     newest_header = max(os.path.getmtime(h) for h in headers)
     jobs, objs = [], []
     for s in SOURCES:

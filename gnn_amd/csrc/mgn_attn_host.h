@@ -57,13 +57,19 @@ inline int attn_check(const MgnAttn* a, const char* name) {
     return 0;
 }
 
-// Small problems: 32 queries of a head per workgroup and no images, when tiles of 128 queries would leave most compute units
-// without work (measured: 561 x 280, 4 heads of 32, fp32: see mgn_attn_fwd.hip).
+// Small problems: 32 queries of a head per workgroup and no images, one launch instead of two.  It converts a subtile anew in
+// every workgroup, so it pays while a workgroup's chain of subtiles is short and there is little work in all (us, images against
+// small): fp32, 4 heads of 32: 561 x 280 18.7 / 14.0, 4000 x 1000 28.5 / 24.7, 500 x 2000 23.4 / 31.4, 7900 x 2000 51 / 77;
+// 8 heads of 64: 500 x 500 25.6 / 16.2, 4000 x 500 28.3 / 56.1; bf16, 4 heads of 32: 500 x 500 18.8 / 14.7, 500 x 1000 21.5 /
+// 25.2; 4 heads of 128: 500 x 250 18.9 / 21.1.
 inline bool attn_is_small(const MgnAttn& a) {
-    return (a.n_q / ATT_TQ + a.n_seg) * (int64_t)a.heads <= 256 && a.n_k / a.n_seg <= 2048;
+    const int64_t chain = a.n_k / a.n_seg * attn_dp(a.dim);
+    return chain <= (a.dtype == MGN_F32 ? 32768 : 16384) && (a.n_q / 32 + a.n_seg) * (int64_t)a.heads * chain <= 1 << 24;
 }
 
-// Few queries per segment: keys and values are read once where they lie, without images.
+// Few queries per segment: keys and values are read where they lie, once for each query, without images.  64 segments of 8192
+// keys, 8 heads of 128, bf16 (us, images against few): 1 query each 1347 / 376, 4 each 1349 / 652, 8 each 1369 / 1088; 50 000
+// keys, 8 heads over 2 key heads of 128: 4 queries 60 / 53, 8 queries 60 / 73.
 inline bool attn_is_few(const MgnAttn& a) { return a.n_q <= 4 * (int64_t)a.n_seg; }
 
 inline int attn_few_chunk(const MgnAttn& a) {                           // query heads that share a pass over a key head
@@ -74,13 +80,16 @@ inline int attn_few_blocks(const MgnAttn& a) {
     const int rep = a.heads / a.kv_heads, c = attn_few_chunk(a);
     return (int)(a.n_q * a.kv_heads * ((rep + c - 1) / c));
 }
-// Split key ranges until there are about four workgroups per compute unit, in pieces of at least 256 keys.
+// Split key ranges until there are about four workgroups per compute unit, in pieces of at least 256 keys (within 3 % of two or
+// eight workgroups, and of 128 keys; pieces of 512 keys take 30 instead of 26.5 us for one query over 100 000 keys in fp32).
 inline int attn_few_splits(const MgnAttn& a) {
     const int64_t blocks = attn_few_blocks(a), keys = a.n_k / a.n_seg;
     int64_t s = blocks > 0 ? 1024 / blocks : 1;
     if (s > keys / 256) s = keys / 256;
     return (int)(s < 1 ? 1 : s > ATT_MAX_SPLITS ? ATT_MAX_SPLITS : s);
 }
+// Eight waves share the images of a tile of keys where 256 queries per workgroup still reach every compute unit.  Width 128,
+// 16 bits (us, four waves against eight): 8192 x 8192 318 / 290, 4096 x 8192 181 / 169, 32 768 x 1024 173 / 179.
 inline int attn_fwd_waves(const MgnAttn& a) {
     return !a.bias_table && attn_dp(a.dim) == 128 && a.dtype != MGN_F32 && (a.n_q / 256 + a.n_seg) * a.heads >= 256 ? 8 : 4;
 }

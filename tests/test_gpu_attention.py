@@ -388,3 +388,30 @@ def test_rows_outside_a_split_forward_are_left_as_they_were():
     args = dict(q_ptr=ptr([40, 40, 40], 6), k_ptr=ptr([6000, 6000, 6000], 5))
     ops.cross_attention(q, k, v, out=out, **args)
     assert_close(out, reference(q, k, v, **args), "o", outside_kept=7.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("nq,nk,heads,dim", [(2, 300, 4, 32), (60, 90, 4, 32), (700, 1500, 8, 64), (1000, 700, 64, 32)])
+@pytest.mark.parametrize("axes", [0, 2])
+def test_nan_comes_out_where_it_went_in(nq, nk, heads, dim, dtype, axes):
+    """A NaN in a query is its row's alone; in a key it reaches every query of the key's segment, in a value one column."""
+    from gnn_amd import ops
+    kw = bias_args(nq, 2 * nk, heads, axes, 30) if axes else {}
+    kw.update(q_ptr=ptr([nq // 2, nq - nq // 2]), k_ptr=ptr([nk, nk]))
+    q, k, v, _ = make(nq, 2 * nk, heads, heads, dim, dtype)
+    want = ops.cross_attention(q, k, v, **kw)
+    assert torch.isfinite(want).all()
+    for which, at in ((0, (0, 1, 3)), (1, (nk + 5, 2, 7)), (2, (3, 1, 4))):
+        ops_in = [q, k, v]
+        ops_in[which] = ops_in[which].clone()
+        ops_in[which][at] = math.nan
+        o = ops.cross_attention(*ops_in, **kw)
+        hit = torch.zeros_like(o, dtype=torch.bool)
+        if which == 0:
+            hit[0, 1] = True
+        elif which == 1:
+            hit[nq // 2:, 2] = True
+        else:
+            hit[:nq // 2, 1, 4] = True
+        assert torch.isnan(o[hit]).all()
+        assert torch.isfinite(o[~hit]).all()
