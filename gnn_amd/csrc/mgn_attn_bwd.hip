@@ -51,6 +51,14 @@ __device__ __forceinline__ void fill_biases(float* lutb, const AttnBwd& a, int h
 constexpr int GROUP = 2;                               // sums by bucket that are read, added to and written together
 
 // ------------------------------------------------------------------------------------------------ query side
+// A workgroup: 128 queries of one head, 32 per wave, against the key subtiles of its split; three images a step, requested a step
+// ahead into registers.  A lane owns a query: its statistics are registers, and its sums of dS by bucket a column of LDS that no
+// other lane touches, two entries read, added to and written at a time (adding the second to the first where both are one bucket;
+// readout of 20 000 x 2501 in us for 1 / 2 / 4 / 8 at a time: 753 / 741 / 744 / 771, without the sums 684).
+//
+// Bound by the vector unit with a bias (about 390 vector instructions a step of 32 x 32 beside 18 products): 20 000 x 2501, 4 heads
+// of 32, fp32, plane, table trained, 302 us and 7 for the sum of its two pieces.  Without one by the latency of a step's chain:
+// 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 83 us = 0.57 PFLOP/s.
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : KIND == AT_F32 && DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
@@ -260,6 +268,8 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict
 // ------------------------------------------------------------------------------------------------ key side
 // A workgroup: 128 keys of one key head, 32 per wave, against its share of the (query head, query subtile) pairs that read
 // them.  Here the lane owns a key: rows of the products are queries, whose statistics come through LDS.
+// Bound like the query side.  Measured at its two problems: 284 us (fp32, plane: 380 vector instructions a step beside 24
+// products) and 117 us = 0.54 PFLOP/s (bf16, four query heads to a key head).
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
@@ -493,9 +503,11 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     auto take = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) & ~(size_t)255; return p; };
     s.ns_q = attn_subtiles(a.n_q, a.n_seg); s.ns_k = attn_subtiles(a.n_k, a.n_seg);
     s.q_tiles = (int)(a.n_q / ATT_TQ) + a.n_seg; s.k_tiles = (int)(a.n_k / ATT_TQ) + a.n_seg;
-    // workgroups of the key side: about four per compute unit, in shares of at least four query subtiles
-    const int64_t blocks = (int64_t)s.k_tiles * a.kv_heads, items = (a.n_q / 32 / a.n_seg + 1) * (a.heads / a.kv_heads);
-    int64_t sp = blocks > 0 ? 1024 / blocks : 1;
+    // workgroups of the key side: two per compute unit, as many as fit at once, in shares of at least four query subtiles (backward
+    // pass in us for 256 / 512 / 1024 / 2048 workgroups: 20 000 x 2501, 4 heads of 32, fp32, plane 539 / 470 / 473 / 469; four
+    // segments of 1800 x 1800, 8 heads of 64, fp16, line 225 / 223 / 242 / 258)
+    const int64_t blocks = attn_tiles(a.n_k, a.n_seg, ATT_TQ) * a.kv_heads, items = (a.n_q / 32 / a.n_seg + 1) * (a.heads / a.kv_heads);
+    int64_t sp = blocks > 0 ? 512 / blocks : 1;
     if (sp > items / 4) sp = items / 4;
     s.splits = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
     s.q_splits = attn_round_splits(attn_tiles(a.n_q, a.n_seg, ATT_TQ) * a.heads, a.n_k / a.n_seg, 1);

@@ -2,9 +2,12 @@
 // lie, in whole rows, and all arithmetic is fp32.
 //
 // Memory bound: bytes = keys x (key + value row).  A workgroup takes one query token, up to eight query heads that share a
-// key head, and one piece of the keys; LPR lanes share a row (8 elements each), so a load of a wave
-// covers 64 / LPR rows; four loads (two for fp32) of keys and of values are worked on while as many are on their way.  Every row group keeps its own running maximum and sum, joined
-// over the wave by exchanges and over the waves through LDS; pieces are joined by attn_join_kernel in a fixed order.
+// key head, and one piece of the keys; LPR lanes share a row (8 elements each), so a load of a wave covers 64 / LPR rows; four
+// loads (two for fp32) of keys and of values are worked on while as many are on their way.  Every row group keeps its own
+// running maximum and sum, joined over the wave by exchanges and over the waves through LDS; pieces are joined in a fixed order.
+// Measured: one query in each of 64 streams over 358 608 ragged keys, 16 heads over 4 key heads of 128, bf16, 177 us, 4.2 TB/s
+// (a copy reaches 4.8, a plain read 4.0); one query over 100 000 keys, 4 heads of 32, fp32, with bias, 30 us, 3.4 TB/s, of which
+// the launches of its two kernels are 8.
 #include "mgn_attn_host.h"
 
 #include <type_traits>

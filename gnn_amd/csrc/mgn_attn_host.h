@@ -58,13 +58,14 @@ inline int attn_check(const MgnAttn* a, const char* name) {
 }
 
 // Small problems: 32 queries of a head per workgroup and no images, one launch instead of two.  It converts a subtile anew in
-// every workgroup, so it pays while a workgroup's chain of subtiles is short and there is little work in all (us, images against
-// small): fp32, 4 heads of 32: 561 x 280 18.7 / 14.0, 4000 x 1000 28.5 / 24.7, 500 x 2000 23.4 / 31.4, 7900 x 2000 51 / 77;
-// 8 heads of 64: 500 x 500 25.6 / 16.2, 4000 x 500 28.3 / 56.1; bf16, 4 heads of 32: 500 x 500 18.8 / 14.7, 500 x 1000 21.5 /
-// 25.2; 4 heads of 128: 500 x 250 18.9 / 21.1.
+// every workgroup, so it pays while all workgroups are resident at once, a workgroup's chain of subtiles is short and there is
+// little work in all (us, images against small): fp32, 4 heads of 32: 561 x 280 18.7 / 14.0, 4000 x 1000 28.5 / 24.7, 6000 x 300
+// 17.6 / 17.1, 12 000 x 150 17.8 / 21.3, 100 000 x 20 36 / 102, 500 x 2000 23.4 / 31.4, 7900 x 2000 51 / 77; 8 heads of 64: 500 x
+// 500 25.6 / 16.2, 4000 x 500 28.3 / 56.1; bf16, 4 heads of 32: 500 x 500 18.8 / 14.7, 500 x 1000 21.5 / 25.2; 4 heads of 128:
+// 500 x 250 18.9 / 21.1.
 inline bool attn_is_small(const MgnAttn& a) {
-    const int64_t chain = a.n_k / a.n_seg * attn_dp(a.dim);
-    return chain <= (a.dtype == MGN_F32 ? 32768 : 16384) && (a.n_q / 32 + a.n_seg) * (int64_t)a.heads * chain <= 1 << 24;
+    const int64_t chain = a.n_k / a.n_seg * attn_dp(a.dim), blocks = (a.n_q / 32 + a.n_seg) * (int64_t)a.heads;
+    return blocks <= 512 && chain <= (a.dtype == MGN_F32 ? 32768 : 16384) && blocks * chain <= 1 << 24;
 }
 
 // Few queries per segment: keys and values are read where they lie, once for each query, without images.  64 segments of 8192
