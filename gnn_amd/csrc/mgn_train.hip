@@ -1038,6 +1038,13 @@ __global__ __launch_bounds__(64) void reduce_many_kernel(ReduceManyArgs a) {
     else r.vec[(i - r.mcount) / H][(i - r.mcount) % H] = sum;
 }
 
+// Rows of zeros, 16 bytes per lane and step: a kernel and not a memset, so that a captured launch sequence holds kernels only (memset
+// nodes of a replayed graph have given wrong results).
+__global__ __launch_bounds__(NT) void zero_rows_kernel(float* __restrict__ x, long long quads) {
+    for (long long i = (long long)blockIdx.x * NT + threadIdx.x; i < quads; i += (long long)gridDim.x * NT)
+        *(f32x4*)(x + 4 * i) = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 // ------------------------------------------------------------------------ segmented row sums
 __global__ __launch_bounds__(NT) void segment_sum_kernel(const float* __restrict__ src, const int* __restrict__ rowptr,
                                                          const int* __restrict__ order, float* __restrict__ out,
@@ -1415,7 +1422,7 @@ static int edge_bwd(const char* name, EdgeBwdArgs a, float* dW1, float* db1, flo
     MGN_REQUIRE((a.el || (a.codes && a.scale)) && a.gaggr && a.ps && a.pr && a.sender && a.recv && a.rowptr && a.w0 && a.w1 && a.b1 && a.ln_w, name);
     MGN_REQUIRE(a.g1 && a.dpr && dW1 && db1 && dgamma && dbeta && a.partial, name);
     // receivers without in-edges are never visited by the scan
-    if (hipMemsetAsync(a.dpr, 0, (size_t)n_nodes * H * sizeof(float), s) != hipSuccess) return check_launch(name);
+    hipLaunchKernelGGL(zero_rows_kernel, dim3(stream_grid(n_nodes, 32)), dim3(NT), 0, s, a.dpr, (long long)n_nodes * (H / 4));
     a.n_nodes = (int)n_nodes; a.n_edges = (int)n_edges;
     const int g = train_grid(n_edges, 1);
     if (a.codes) hipLaunchKernelGGL(train_edge_bwd_kernel<true>, dim3(g), dim3(NT), 0, s, a);
