@@ -415,3 +415,21 @@ def test_nan_comes_out_where_it_went_in(nq, nk, heads, dim, dtype, axes):
             hit[:nq // 2, 1, 4] = True
         assert torch.isnan(o[hit]).all()
         assert torch.isfinite(o[~hit]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("axes,dim", [(2, 32), (3, 64), (2, 128)])
+def test_buckets_listed_for_the_backward_pass(axes, dim, dtype):
+    """Ragged segments, all 64 buckets, masked keys; the lists are read by both backward kernels."""
+    nq, nk = [700, 0, 33, 640, 200], [900, 64, 0, 300, 500]
+    q, k, v, g = make(sum(nq) + 7, sum(nk) + 3, heads=4, kv_heads=2, dim=dim, dtype=dtype)
+    gen = torch.Generator().manual_seed(8)
+    mask = (torch.rand(k.shape[0], generator=gen) > 0.2).to(DEV)
+    check(q, k, v, g, q_ptr=ptr(nq, 4), k_ptr=ptr(nk, 1), key_mask=mask, **bias_args(q.shape[0], k.shape[0], 4, axes, 300, 64))
+
+
+@pytest.mark.parametrize("heads,nq,nk", [(1, [1300, 200], [1200, 300]), (2, [1, 2, 3, 0] * 256, [3, 2, 1, 1] * 256)])
+def test_lattice_backward_without_lists(heads, nq, nk):
+    """One head has nobody to share a list with; very many segments would take too large a one."""
+    q, k, v, g = make(sum(nq), sum(nk), heads=heads, kv_heads=1)
+    check(q, k, v, g, q_ptr=ptr(nq), k_ptr=ptr(nk), **bias_args(sum(nq), sum(nk), heads, 2, 50))
