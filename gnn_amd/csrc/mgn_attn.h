@@ -238,6 +238,19 @@ __device__ __forceinline__ int lane_zero() {
     return z;
 }
 
+// Operand T (contraction over the tokens) of an image R in LDS: lane (i, h) gets x[token t(kc, h, e)][32 b + i], see above.  Two
+// transposing reads, each of four tokens' 16-element chunks; tr_lane() is the lane's share of the address, in halves.
+__device__ __forceinline__ int tr_lane(int lane) {
+    const int r = lane >> 2 & 3, s = lane & 3;
+    return (lane >> 4 & 1) * 512 + (s >> 1) * 256 + (4 * (lane >> 5) + r) * 8 + (s & 1) * 4;
+}
+template <int DP>
+__device__ __forceinline__ u32x4 tr_read(const unsigned short* image, int at, int plane, int kc, int b) {
+    const unsigned short* p = image + at + (plane * 32 * DP + b * 1024 + kc * 128);
+    const u32x2 lo = lds_tr4(p), hi = lds_tr4(p + 64);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
 // Exponents and valid bits of a step (key exponent, value exponent, mask), requested a step ahead and then made uniform.  Only
 // what is used is loaded: the unused part of a wider load would be overwritten early, behind a wait for the load.
 template <int KIND, int N = 3> struct Record {
@@ -276,7 +289,7 @@ struct ImageJob {
     const void* x; long long st, sh;             // rows: element strides of tokens and heads
     const int* ptr; const uint8_t* mask;
     long long T; int heads, n_sub, first_unit;   // n_sub: subtiles of a head; units of this job start at first_unit
-    unsigned short* R; unsigned short* Tt;       // images (either may be null)
+    unsigned short* R; unsigned short* Tt;       // images (either may be null; Tt only where ImageArgs::transposed)
     int* ex; int* valid;                         // exponent of (head, subtile), 4 ints apart; valid bits of the tokens
     const int* pos; int* pos_out; int axes;      // places [T][axes] -> [subtile][axes][32]
     const void* o; long long o_st, o_sh;         // gradient job: the outputs (fp32 or the type of the rows), ...
@@ -284,7 +297,7 @@ struct ImageJob {
     int alternate;                               // negate odd subtiles (see mgn_attn_bwd.hip)
     const float* stats; float* rows;             // rows: [head][subtile][3][32] = maximum, 1/sum (fp32: 1), <do, o> (fp32: / sum)
 };
-struct ImageArgs { ImageJob job[4]; int n_job, units, n_seg, dim; };
+struct ImageArgs { ImageJob job[4]; int n_job, units, n_seg, dim, transposed; };
 
 }  // namespace
 

@@ -16,8 +16,8 @@ namespace {
 
 struct AttnBwd {
     const int *q_ptr, *k_ptr; long long n_q, n_k; int n_seg, heads, kv_heads, dim; float c0, scale;
-    const unsigned short *q_r, *q_t, *g_r, *g_t;       // images of queries and output gradients, [heads][ns_q]
-    const unsigned short *k_r, *k_t, *v_r;             // images of keys and values, [kv_heads][ns_k]
+    const unsigned short *q_r, *g_r;                   // images R of queries and output gradients, [heads][ns_q]
+    const unsigned short *k_r, *v_r;                   // of keys and values, [kv_heads][ns_k]
     const i32x4 *rec_q, *rec_k;                        // exponents {q, g} and {k, v, valid keys}
     const float* rows;                                 // [heads][ns_q][3][32]
     int ns_q, ns_k;
@@ -103,8 +103,8 @@ __global__ __launch_bounds__(256) void attn_buckets_kernel(AttnBwd a) {
 constexpr int GROUP = 2;                               // sums by bucket that are read, added to and written together
 
 // ------------------------------------------------------------------------------------------------ query side
-// A workgroup: 128 queries of one head, 32 per wave, against the key subtiles of its split; three images a step, requested a step
-// ahead into registers.  A lane owns a query: its statistics are registers, and its sums of dS by bucket a column of LDS that no
+// A workgroup: 128 queries of one head, 32 per wave, against the key subtiles of its split; two images a step, requested a step ahead
+// into registers and read both as they are and transposed.  A lane owns a query: its statistics are registers, and its sums of dS by bucket a column of LDS that no
 // other lane touches, two entries read, added to and written at a time (adding the second to the first where both are one bucket;
 // readout of 20 000 x 2501 in us for 1 / 2 / 4 / 8 at a time: 753 / 741 / 744 / 771, without the sums 684, before buckets were listed).
 //
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     // 64: 1095 -> 1028 us for the whole backward pass).  16-bit types: two (8 heads of 32, bf16: 476 us with one, 436 with two).
     constexpr int AXES = BIAS == LISTED ? 0 : BIAS;
     constexpr int BUFS = KIND == AT_F32 && BIAS > 0 ? 1 : 2;
-    __shared__ __attribute__((aligned(1024))) unsigned short buf[BUFS][3 * SUB];  // K as R, K as T, V as R
+    __shared__ __attribute__((aligned(1024))) unsigned short buf[BUFS][2 * SUB];  // K, V
     __shared__ __attribute__((aligned(16))) int pbuf[AXES ? BUFS : 1][AXES ? 128 : 1];
     extern __shared__ Entry entry[];                                                   // by place, ...
     float* hist = (float*)(entry + entries<BIAS>(a.reach));                            // ... and [4 waves][n_bucket][64], with a table gradient
@@ -143,8 +143,8 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     const long long qsub = (long long)head * a.ns_q + (g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1);
 
     constexpr int PIECES = SUB * 2 / 1024;
-    const int last = n_sub - 1, lz = lane_zero();
-    Staged<3 * PIECES> st;
+    const int last = n_sub - 1, lz = lane_zero(), tl = tr_lane(lane);
+    Staged<2 * PIECES> st;
     int sp = 0;
     u32x4 listed{}, listed_next{};
     const long long qplace = (g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1);
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     auto request = [&](int s) {
         st.request(w, lane, [&](int c) {
             const int image = c / PIECES;
-            return (const char*)(image == 0 ? a.k_r : image == 1 ? a.k_t : a.v_r) + (ksub + s) * (SUB * 2) + (c % PIECES) * 1024;
+            return (const char*)(image == 0 ? a.k_r : a.v_r) + (ksub + s) * (SUB * 2) + (c % PIECES) * 1024;
         });
         if (AXES > 0 && t < AXES * 32) sp = a.kpos[(kplace + s) * (AXES * 32) + t];
         if constexpr (BIAS == LISTED) listed_next = lists[(long long)s * 64];
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
         const int b = BUFS == 2 ? sub & 1 : 0;
         request(min(sub + 1, last));
         rn.request(rec + min(sub + 1, last) + lz);
-        const u32x4 *kr = (const u32x4*)buf[b] + lane, *kt = (const u32x4*)(buf[b] + SUB) + lane, *vr = (const u32x4*)(buf[b] + 2 * SUB) + lane;
+        const u32x4 *kr = (const u32x4*)buf[b] + lane, *vr = (const u32x4*)(buf[b] + SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -276,11 +276,12 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
             pack8<KIND>(v, hi, lo);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
+                const u32x4 k1 = tr_read<DP>(buf[b], tl, 0, kc, n);
                 if constexpr (PL == 2) {
-                    dq[n] = mma<KIND>(kt[((2 + kc) * NB + n) * 64], hi, dq[n]);
-                    dq[n] = mma<KIND>(kt[(kc * NB + n) * 64], lo, dq[n]);
+                    dq[n] = mma<KIND>(tr_read<DP>(buf[b], tl, 1, kc, n), hi, dq[n]);
+                    dq[n] = mma<KIND>(k1, lo, dq[n]);
                 }
-                dq[n] = mma<KIND>(kt[(kc * NB + n) * 64], hi, dq[n]);
+                dq[n] = mma<KIND>(k1, hi, dq[n]);
             }
         }
         if (BUFS == 1) __syncthreads();
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
-    __shared__ __attribute__((aligned(1024))) unsigned short buf[2][4 * SUB];          // Q as R, Q as T, dO as R, dO as T
+    __shared__ __attribute__((aligned(1024))) unsigned short buf[2][2 * SUB];          // Q, dO
     __shared__ __attribute__((aligned(16))) float rbuf[2][128];
     constexpr int AXES = BIAS == LISTED ? 0 : BIAS;
     __shared__ __attribute__((aligned(16))) int pbuf[AXES ? 2 : 1][AXES ? 128 : 1];
@@ -359,9 +360,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
 
     auto qsub_of = [&](int item) { return (head0 + item / n_sub) * a.ns_q + qbase + item % n_sub; };
     constexpr int PIECES = SUB * 2 / 1024;
-    const int lz = lane_zero();
+    const int lz = lane_zero(), tl = tr_lane(lane);
     int rep_at = i0 < i1 ? i0 / n_sub : 0, sub_at = i0 < i1 ? i0 % n_sub : 0;            // of the item that is requested next
-    Staged<4 * PIECES> st;
+    Staged<2 * PIECES> st;
     float sr = 0.f;
     int sp = 0;
     u32x4 listed{}, listed_next{};
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         const long long s = (head0 + rep_at) * a.ns_q + qbase + sub_at;
         st.request(w, lane, [&](int c) {
             const int image = c / PIECES;
-            return (const char*)(image == 0 ? a.q_r : image == 1 ? a.q_t : image == 2 ? a.g_r : a.g_t) + s * (SUB * 2) + (c % PIECES) * 1024;
+            return (const char*)(image == 0 ? a.q_r : a.g_r) + s * (SUB * 2) + (c % PIECES) * 1024;
         });
         if (t < 96) sr = a.rows[s * 96 + t];
         if (AXES > 0 && t < AXES * 32) sp = a.qpos[(qbase + sub_at) * (AXES * 32) + t];
@@ -428,8 +429,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
             if (++sub_at == n_sub) { sub_at = 0; ++rep_at; next_head = true; }
         }
         request();
-        const u32x4 *qr = (const u32x4*)buf[b] + lane, *qt = (const u32x4*)(buf[b] + SUB) + lane;
-        const u32x4 *gr = (const u32x4*)(buf[b] + 2 * SUB) + lane, *gt = (const u32x4*)(buf[b] + 3 * SUB) + lane;
+        const u32x4 *qr = (const u32x4*)buf[b] + lane, *gr = (const u32x4*)(buf[b] + SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -486,14 +486,15 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
             pack8<KIND>(v, shi, slo);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
+                const u32x4 g1 = tr_read<DP>(buf[b] + SUB, tl, 0, kc, n), q1 = tr_read<DP>(buf[b], tl, 0, kc, n);
                 if constexpr (PL == 2) {
-                    dv[n] = mma<KIND>(gt[((2 + kc) * NB + n) * 64], phi, dv[n]);
-                    dk[n] = mma<KIND>(qt[((2 + kc) * NB + n) * 64], shi, dk[n]);
-                    dv[n] = mma<KIND>(gt[(kc * NB + n) * 64], plo, dv[n]);
-                    dk[n] = mma<KIND>(qt[(kc * NB + n) * 64], slo, dk[n]);
+                    dv[n] = mma<KIND>(tr_read<DP>(buf[b] + SUB, tl, 1, kc, n), phi, dv[n]);
+                    dk[n] = mma<KIND>(tr_read<DP>(buf[b], tl, 1, kc, n), shi, dk[n]);
+                    dv[n] = mma<KIND>(g1, plo, dv[n]);
+                    dk[n] = mma<KIND>(q1, slo, dk[n]);
                 }
-                dv[n] = mma<KIND>(gt[(kc * NB + n) * 64], phi, dv[n]);
-                dk[n] = mma<KIND>(qt[(kc * NB + n) * 64], shi, dk[n]);
+                dv[n] = mma<KIND>(g1, phi, dv[n]);
+                dk[n] = mma<KIND>(q1, shi, dk[n]);
             }
         }
         arrive(b ^ 1);
@@ -568,7 +569,7 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a, int dp) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct BwdSpace { size_t q_r, q_t, g_r, g_t, k_r, k_t, v_r, rec_q, rec_k, rows, qpos, kpos, tpart, part, q_part, by_query, by_key, total; int ns_q, ns_k, q_tiles, k_tiles, splits, q_splits; bool listed; };
+struct BwdSpace { size_t q_r, g_r, k_r, v_r, rec_q, rec_k, rows, qpos, kpos, tpart, part, q_part, by_query, by_key, total; int ns_q, ns_k, q_tiles, k_tiles, splits, q_splits; bool listed; };
 
 BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     BwdSpace s{};
@@ -586,8 +587,7 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     s.splits = (int)(sp < 1 ? 1 : sp > 64 ? 64 : sp);
     s.q_splits = attn_round_splits(attn_tiles(a.n_q, a.n_seg, ATT_TQ) * a.heads, a.n_k / a.n_seg, 1);
     const size_t qi = (size_t)a.heads * s.ns_q * pl * 64 * dp, ki = (size_t)a.kv_heads * s.ns_k * pl * 64 * dp;
-    s.q_r = take(qi); s.q_t = take(qi); s.g_r = take(qi); s.g_t = take(qi);
-    s.k_r = take(ki); s.k_t = take(ki); s.v_r = take(ki);
+    s.q_r = take(qi); s.g_r = take(qi); s.k_r = take(ki); s.v_r = take(ki);
     s.rec_q = take((size_t)a.heads * s.ns_q * 16); s.rec_k = take((size_t)a.kv_heads * s.ns_k * 16);
     s.rows = take((size_t)a.heads * s.ns_q * 96 * 4);
     // Buckets listed once where a place is dear (a lattice), at least two heads share it and there are subtiles enough to pay for the
@@ -684,13 +684,13 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     };
     if (a.n_q > 0) {
         ImageJob& q = add(a.q, a.q_st, a.q_sh, true);
-        q.R = half(s.q_r); q.Tt = half(s.q_t); q.ex = rec_q; q.pos = bias ? a.q_pos : nullptr; q.pos_out = (int*)(ws + s.qpos);
+        q.R = half(s.q_r); q.ex = rec_q; q.pos = bias ? a.q_pos : nullptr; q.pos_out = (int*)(ws + s.qpos);
         ImageJob& o = add(g, g_st, g_sh, true);
-        o.R = half(s.g_r); o.Tt = half(s.g_t); o.ex = rec_q + 1; o.o = out; o.o_f32 = a.out_f32 || a.dtype == MGN_F32; o.o_st = out_st; o.o_sh = out_sh; o.stats = stats; o.rows = (float*)(ws + s.rows);
+        o.R = half(s.g_r); o.ex = rec_q + 1; o.o = out; o.o_f32 = a.out_f32 || a.dtype == MGN_F32; o.o_st = out_st; o.o_sh = out_sh; o.stats = stats; o.rows = (float*)(ws + s.rows);
     }
     if (a.n_k > 0) {
         ImageJob& k = add(a.k, a.k_st, a.k_sh, false);
-        k.R = half(s.k_r); k.Tt = half(s.k_t); k.ex = rec_k; k.valid = rec_k + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = (int*)(ws + s.kpos);
+        k.R = half(s.k_r); k.ex = rec_k; k.valid = rec_k + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = (int*)(ws + s.kpos);
         ImageJob& v = add(a.v, a.v_st, a.v_sh, false);
         v.R = half(s.v_r); v.ex = rec_k + 1; v.alternate = kind != AT_BF16;
     }
@@ -699,7 +699,7 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     AttnBwd b{};
     b.q_ptr = a.q_ptr; b.k_ptr = a.k_ptr; b.n_q = a.n_q; b.n_k = a.n_k; b.n_seg = a.n_seg; b.heads = a.heads; b.kv_heads = a.kv_heads; b.dim = a.dim;
     b.c0 = a.scale * LOG2E; b.scale = a.scale;
-    b.q_r = half(s.q_r); b.q_t = half(s.q_t); b.g_r = half(s.g_r); b.g_t = half(s.g_t); b.k_r = half(s.k_r); b.k_t = half(s.k_t); b.v_r = half(s.v_r);
+    b.q_r = half(s.q_r); b.g_r = half(s.g_r); b.k_r = half(s.k_r); b.v_r = half(s.v_r);
     b.rec_q = (const i32x4*)rec_q; b.rec_k = (const i32x4*)rec_k; b.rows = (const float*)(ws + s.rows); b.ns_q = s.ns_q; b.ns_k = s.ns_k;
     b.qpos = (const int*)(ws + s.qpos); b.kpos = (const int*)(ws + s.kpos);
     b.table = a.bias_table; b.lut = a.bucket_lut; b.n_bucket = a.n_bucket; b.reach = a.reach; b.axes = a.axes;

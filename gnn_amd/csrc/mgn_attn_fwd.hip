@@ -103,6 +103,7 @@ __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
             if constexpr (PL == 2) dst[(NC + c) * 64] = lo[c];
         }
     }
+    if (!a.transposed) return;
     // every wave of the workgroup takes both rounds, whatever its job asks for: the barriers are met by all
 #pragma unroll
     for (int p = 0; p < PL; ++p) {
@@ -1060,7 +1061,7 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
         if (a.n_k > 0 && !small) {
             ImageArgs im{};
             const int units = sp.ns_k * a.kv_heads;
-            im.n_job = 2; im.units = 2 * units; im.n_seg = a.n_seg; im.dim = a.dim;
+            im.n_job = 2; im.transposed = 1; im.units = 2 * units; im.n_seg = a.n_seg; im.dim = a.dim;
             ImageJob& k = im.job[0];
             k.x = a.k; k.st = a.k_st; k.sh = a.k_sh; k.ptr = a.k_ptr; k.mask = a.key_mask; k.T = a.n_k; k.heads = a.kv_heads; k.n_sub = sp.ns_k;
             k.R = kimg; k.ex = rec; k.valid = rec + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = kpos; k.axes = a.axes;

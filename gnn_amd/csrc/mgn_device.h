@@ -203,6 +203,13 @@ __device__ __forceinline__ void split2_pair(float a, float b, unsigned& p1, unsi
     p2 = __builtin_bit_cast(unsigned, l);
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Four columns' worth of a 4 x 16 block per 16 lanes: lane 4q + p of the 16 gives the address of row q, columns 4p .. 4p + 3, and gets
+// column 4q + p of the four rows.  The transposing read needs every lane of the wave active: call from workgroup-uniform control flow only.
+__device__ __forceinline__ u32x2 lds_tr4(const unsigned short* p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
 // four consecutive fp32 -> per plane two dwords (4 fp16)
 __device__ __forceinline__ void split2_pack4(const f32x4 v, u32x2& p1, u32x2& p2) {
     unsigned a1, a2, b1, b2;

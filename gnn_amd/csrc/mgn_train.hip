@@ -322,7 +322,6 @@ __global__ __launch_bounds__(NT, 2) void train_linear_bwd_kernel(LinBwdArgs a) {
 // free of bank conflicts (scripts/micro/tr_read.hip checks the lane map and the swizzle on the device).
 // One workgroup per CU (weight planes and gradient accumulators take 160 registers per lane); the next tile's rows
 // are requested as soon as the current tile's have been staged.
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int SPL = TM * H;                 // halves per plane of the image
 
@@ -335,11 +334,6 @@ __device__ __forceinline__ void splanes_store4(unsigned short* img, int row, int
     split_pack4(v, ph, pm, pl);
     unsigned short* d = img + swz_off(row, k >> 3) + (k & 4);
     *(u32x2*)(d) = ph; *(u32x2*)(d + PLANE) = pm; *(u32x2*)(d + 2 * PLANE) = pl;
-}
-
-// The transposing read needs every lane of the wave active: call from workgroup-uniform control flow only.
-__device__ __forceinline__ u32x2 lds_tr4(const unsigned short* p) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
 // halves offset of this lane's address for the block of rows 16s + 8h + 4hh + 0..3, columns 32 blk + 16 gg + 0..15
