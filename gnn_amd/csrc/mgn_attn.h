@@ -10,6 +10,7 @@
 // back linearly (no bank conflicts, no address arithmetic, no padding or masking left to do):
 //   image R (contraction over the head's width):  [plane][width / 16][lane][8],  element = x[token i][16 c + 8 h + e]
 //   image T (contraction over the 32 tokens):     [plane][2][width / 32][lane][8], element = x[token t(kc, h, e)][32 b + i]
+//   (values in the forward pass; the backward pass, which needs most operands both ways, reads image R transposed: tr_read)
 // with t = 16 kc + 4 h + e (e < 4), 16 kc + 8 + 4 h + e - 4 (e >= 4): the order in which a lane already holds the scores of
 // one column after a product (rows 8 g + 4 h + t), so probabilities go from one product into the next without a shuffle.
 // A segment's first subtile in an image is floor(first token / 32) + segment: no two segments share a subtile, and no table

@@ -8,7 +8,7 @@
 // The table's gradient sums dS over very many pairs, and every row of dS sums to zero: an error that all entries share grows
 // with their number where the sum itself cancels.  Two such errors are kept out.  The fp16 matrix instruction rounds its sums
 // downwards, so dP comes out low everywhere (a 1e-5 error of the table at 20 000 queries): the values' images of odd subtiles
-// are negated, dP of those comes out high, and what is left has either sign (3e-7).  And <dO_i, o_i> has to be made of outputs
+// are negated, dP of those comes out high, and what is left has either sign (6e-7).  And <dO_i, o_i> has to be made of outputs
 // that were not rounded to 16 bits: the forward pass keeps them in fp32 where a table is trained (out32).
 #include "mgn_attn_host.h"
 
@@ -109,7 +109,7 @@ constexpr int GROUP = 2;                               // sums by bucket that ar
 // readout of 20 000 x 2501 in us for 1 / 2 / 4 / 8 at a time: 753 / 741 / 744 / 771, without the sums 684, before buckets were listed).
 //
 // Bound by the vector unit with a bias (18 products a step beside about 260 vector instructions with listed buckets, 390
-// without): 20 000 x 2501, 4 heads of 32, fp32, plane, table trained, 225 us and 7 for the sum of its two pieces.  Without one by
+// without): 20 000 x 2501, 4 heads of 32, fp32, plane, table trained, 211 us and 7 for the sum of its two pieces.  Without one by
 // the latency of a step's chain: 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 83 us = 0.57 PFLOP/s.
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : KIND == AT_F32 && DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict
 // ------------------------------------------------------------------------------------------------ key side
 // A workgroup: 128 keys of one key head, 32 per wave, against its share of the (query head, query subtile) pairs that read
 // them.  Here the lane owns a key: rows of the products are queries, whose statistics come through LDS.
-// Bound like the query side.  Measured at its two problems: 260 us (fp32, plane, listed buckets, 24 products a step)
+// Bound like the query side.  Measured at its two problems: 249 us (fp32, plane, listed buckets, 24 products a step)
 // and 117 us = 0.54 PFLOP/s (bf16, four query heads to a key head).
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
@@ -578,9 +578,9 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     auto take = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) & ~(size_t)255; return p; };
     s.ns_q = attn_subtiles(a.n_q, a.n_seg); s.ns_k = attn_subtiles(a.n_k, a.n_seg);
     s.q_tiles = (int)(a.n_q / ATT_TQ) + a.n_seg; s.k_tiles = (int)(a.n_k / ATT_TQ) + a.n_seg;
-    // workgroups of the key side: two per compute unit, as many as fit at once, in shares of at least four query subtiles (backward
-    // pass in us for 256 / 512 / 1024 / 2048 workgroups: 20 000 x 2501, 4 heads of 32, fp32, plane 539 / 470 / 473 / 469; four
-    // segments of 1800 x 1800, 8 heads of 64, fp16, line 225 / 223 / 242 / 258)
+    // workgroups of the key side: two per compute unit, in shares of at least four query subtiles (backward pass in us for 512 / 768 /
+    // 1024 workgroups: 20 000 x 2501, 4 heads of 32, fp32, plane 455 / 446 / 464; 16 segments of 1123 x 804, 8 heads over 2 of 64,
+    // bf16 198 / 227 / 211; four of 1339 x 1339, 8 heads of 64, fp16, line 165 / 175 / 174; with 256 the first took 15 % longer)
     const int64_t blocks = attn_tiles(a.n_k, a.n_seg, ATT_TQ) * a.kv_heads, items = (a.n_q / 32 / a.n_seg + 1) * (a.heads / a.kv_heads);
     int64_t sp = blocks > 0 ? 512 / blocks : 1;
     if (sp > items / 4) sp = items / 4;

@@ -7,8 +7,8 @@ namespace {
 // ---------------------------------------------------------------------------------------------- operand images
 // One wave per (head, subtile): lane (i, h) reads the elements 16 c + 8 h .. + 7 of token i, which are its share of image R;
 // image T is read back from a row-major copy in LDS.  Memory bound: 4 bytes read and 4 (R) or 8 (R and T) written per element.
-// Measured: the seven images of a backward pass over 17 973 queries, 8 heads of 64, and 12 870 keys, 2 heads, bf16: 29 us for
-// 146 MB, 5.0 TB/s.
+// Measured: the four images of a backward pass over 17 973 queries, 8 heads of 64, and 12 870 keys, 2 heads, bf16: 25 us for
+// 105 MB, 4.3 TB/s.
 template <int KIND, int DP>
 __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, LD = DP + 2;
