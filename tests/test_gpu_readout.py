@@ -146,3 +146,38 @@ def test_refusals():
             CrossScaleReadout(128, heads)
     with pytest.raises(NotImplementedError):
         CrossScaleReadout(64)
+
+
+@pytest.mark.parametrize("cells", [(20, 14), (60, 48)])
+def test_readout_bias_and_8_bit_activations_together(cells):
+    """Training steps of a model that reads its coarse graph by attention and keeps its activations in 8 bits: the same numbers
+    eagerly and from a captured step, whose replays alternate with rollouts of the model on the same mesh."""
+    from gnn_amd.meshgraphnet import EncodeProcessDecodeMultiScale
+    from gnn_amd.optim import FusedAdam
+    from gnn_amd.training import CapturedTrainStep
+    g = graph_to(O.synthetic_graph(*cells, seed=3, with_target=True), DEV)
+    runs = []
+    for captured in (False, True):
+        torch.manual_seed(11)
+        model = EncodeProcessDecodeMultiScale(10, 7, hidden_size=128, process_steps=2, coarse_process_steps=1, node_out_dim=3, attention=False,
+                                              with_mat_params=False, time_dim=1, device=DEV, sample_ratio=0.5, coarse_readout="attention").to(DEV).train()
+        model.coarse_start = 0
+        model.activation_bits = 8
+        opt = FusedAdam(model.parameters(), lr=1e-3, capturable=captured)
+        step = CapturedTrainStep(model, opt) if captured else None
+        seen = []
+        for _ in range(5):
+            if captured:
+                total = step(g)[0]
+            else:
+                opt.zero_grad()
+                total = model.loss(g)[0]
+                total.backward()
+                opt.step()
+            seen.append(float(total.detach()))
+            with torch.no_grad():
+                seen.append(float(model.forward(g).double().norm()))
+        seen.append(float(model.readout.bias_table.detach().double().norm()))
+        runs.append(seen)
+    assert runs[0] == runs[1] and all(v == v and abs(v) != float("inf") for v in runs[0])
+    assert runs[0][-1] > 0                                                # the table, zeros at first, has moved
