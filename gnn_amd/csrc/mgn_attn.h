@@ -239,16 +239,27 @@ __device__ __forceinline__ int lane_zero() {
     return z;
 }
 
-// Operand T (contraction over the tokens) of an image R in LDS: lane (i, h) gets x[token t(kc, h, e)][32 b + i], see above.  Two
-// transposing reads, each of four tokens' 16-element chunks; tr_lane() is the lane's share of the address, in halves.
-__device__ __forceinline__ int tr_lane(int lane) {
-    const int r = lane >> 2 & 3, s = lane & 3;
-    return (lane >> 4 & 1) * 512 + (s >> 1) * 256 + (4 * (lane >> 5) + r) * 8 + (s & 1) * 4;
+// Image R in LDS, read both ways.  Operand T (contraction over the tokens): lane (i, h) gets x[token t(kc, h, e)][32 b + i], see
+// above, by two transposing reads, each of four tokens' 16-element chunks.  Four of the chunks that 32 lanes read lie whole multiples
+// of 512 bytes apart, in the same banks; so token groups of four are stored rotated, group n of (chunk c, half h) at n ^ (h + 2 (c & 1)),
+// which spreads them over all 64 banks and costs no instruction in a step (both offsets below are a lane's own).
+// Byte offset of lane (i, h)'s 16 bytes within a chunk of 1 KB:
+__device__ __forceinline__ int rot_lane(int lane, int odd) {
+    const int h = lane >> 5;
+    return h * 512 + (((lane & 31) * 16) ^ (64 * (h + 2 * odd)));
+}
+template <int NC>
+__device__ __forceinline__ u32x4 rot_read(const unsigned short* image, int even, int odd, int plane, int c) {
+    return *(const u32x4*)((const char*)image + ((c & 1 ? odd : even) + (plane * NC + c) * 1024));
+}
+__device__ __forceinline__ int tr_lane(int lane) {             // bytes, tokens 0 .. 3 (+ 8 at this ^ 128)
+    const int r = lane >> 2 & 3, s = lane & 3, g = lane >> 4 & 1;
+    return g * 1024 + (s >> 1) * 512 + ((64 * (lane >> 5) + 16 * r) ^ (64 * ((s >> 1) + 2 * g))) + (s & 1) * 8;
 }
 template <int DP>
 __device__ __forceinline__ u32x4 tr_read(const unsigned short* image, int at, int plane, int kc, int b) {
-    const unsigned short* p = image + at + (plane * 32 * DP + b * 1024 + kc * 128);
-    const u32x2 lo = lds_tr4(p), hi = lds_tr4(p + 64);
+    const char* p = (const char*)image + (plane * 64 * DP + b * 2048 + kc * 256);
+    const u32x2 lo = lds_tr4((const unsigned short*)(p + at)), hi = lds_tr4((const unsigned short*)(p + (at ^ 128)));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
@@ -278,10 +289,15 @@ template <int PIECES, int NW = 4> struct Staged {
         for (int n = 0; n < N; ++n)
             if (PIECES % NW == 0 || NW * n + w < PIECES) v[n] = *(const u32x4*)(source(NW * n + w) + lane * 16);
     }
-    __device__ __forceinline__ void write(void* dst, int w, int lane) const {
+    __device__ __forceinline__ void write(void* dst, int w, int lane) const { write_at(dst, w, lane * 16); }
+    __device__ __forceinline__ void write_rotated(void* dst, int w, int lane) const {
+        static_assert(NW % 2 == 0, "a wave's pieces are all even or all odd chunks");
+        write_at(dst, w, rot_lane(lane, w & 1));
+    }
+    __device__ __forceinline__ void write_at(void* dst, int w, int off) const {
 #pragma unroll
         for (int n = 0; n < N; ++n)
-            if (PIECES % NW == 0 || NW * n + w < PIECES) *(u32x4*)((char*)dst + (NW * n + w) * 1024 + lane * 16) = v[n];
+            if (PIECES % NW == 0 || NW * n + w < PIECES) *(u32x4*)((char*)dst + (NW * n + w) * 1024 + off) = v[n];
     }
 };
 

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     const long long qsub = (long long)head * a.ns_q + (g.first >> 5) + g.seg + min(g.local * 4 + w, nsq - 1);
 
     constexpr int PIECES = SUB * 2 / 1024;
-    const int last = n_sub - 1, lz = lane_zero(), tl = tr_lane(lane);
+    const int last = n_sub - 1, lz = lane_zero(), tl = tr_lane(lane), even = rot_lane(lane, 0), odd = rot_lane(lane, 1);
     Staged<2 * PIECES> st;
     int sp = 0;
     u32x4 listed{}, listed_next{};
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
         if constexpr (BIAS == LISTED) listed_next = lists[(long long)s * 64];
     };
     auto arrive = [&](int b) {
-        st.write(buf[b], w, lane);
+        st.write_rotated(buf[b], w, lane);
         if (AXES > 0 && t < AXES * 32) pbuf[b][t] = sp;
         listed = listed_next;
     };
@@ -211,18 +211,18 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
         const int b = BUFS == 2 ? sub & 1 : 0;
         request(min(sub + 1, last));
         rn.request(rec + min(sub + 1, last) + lz);
-        const u32x4 *kr = (const u32x4*)buf[b] + lane, *vr = (const u32x4*)(buf[b] + SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
+            const u32x4 k1 = rot_read<NC>(buf[b], even, odd, 0, c), v1 = rot_read<NC>(buf[b] + SUB, even, odd, 0, c);
             if constexpr (PL == 2) {
-                s = mma<KIND>(kr[(NC + c) * 64], qf[0][c], s);
-                dp = mma<KIND>(vr[(NC + c) * 64], gf[0][c], dp);
-                s = mma<KIND>(kr[c * 64], qf[PL - 1][c], s);
-                dp = mma<KIND>(vr[c * 64], gf[PL - 1][c], dp);
+                s = mma<KIND>(rot_read<NC>(buf[b], even, odd, 1, c), qf[0][c], s);
+                dp = mma<KIND>(rot_read<NC>(buf[b] + SUB, even, odd, 1, c), gf[0][c], dp);
+                s = mma<KIND>(k1, qf[PL - 1][c], s);
+                dp = mma<KIND>(v1, gf[PL - 1][c], dp);
             }
-            s = mma<KIND>(kr[c * 64], qf[0][c], s);
-            dp = mma<KIND>(vr[c * 64], gf[0][c], dp);
+            s = mma<KIND>(k1, qf[0][c], s);
+            dp = mma<KIND>(v1, gf[0][c], dp);
         }
         int off[BIAS ? 16 : 1];                                // of the buckets' sums
         float add[BIAS ? 16 : 1];
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
 
     auto qsub_of = [&](int item) { return (head0 + item / n_sub) * a.ns_q + qbase + item % n_sub; };
     constexpr int PIECES = SUB * 2 / 1024;
-    const int lz = lane_zero(), tl = tr_lane(lane);
+    const int lz = lane_zero(), tl = tr_lane(lane), even = rot_lane(lane, 0), odd = rot_lane(lane, 1);
     int rep_at = i0 < i1 ? i0 / n_sub : 0, sub_at = i0 < i1 ? i0 % n_sub : 0;            // of the item that is requested next
     Staged<2 * PIECES> st;
     float sr = 0.f;
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         rn.request(a.rec_q + s + lz);
     };
     auto arrive = [&](int b) {
-        st.write(buf[b], w, lane);
+        st.write_rotated(buf[b], w, lane);
         if (t < 96) rbuf[b][t] = sr;
         if (AXES > 0 && t < AXES * 32) pbuf[b][t] = sp;
         listed = listed_next;
@@ -429,18 +429,18 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
             if (++sub_at == n_sub) { sub_at = 0; ++rep_at; next_head = true; }
         }
         request();
-        const u32x4 *qr = (const u32x4*)buf[b] + lane, *gr = (const u32x4*)(buf[b] + SUB) + lane;
         f32x16 s = zero16(), dp = zero16();
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
+            const u32x4 q1 = rot_read<NC>(buf[b], even, odd, 0, c), g1 = rot_read<NC>(buf[b] + SUB, even, odd, 0, c);
             if constexpr (PL == 2) {
-                s = mma<KIND>(qr[(NC + c) * 64], kf[0][c], s);
-                dp = mma<KIND>(gr[(NC + c) * 64], vf[0][c], dp);
-                s = mma<KIND>(qr[c * 64], kf[PL - 1][c], s);
-                dp = mma<KIND>(gr[c * 64], vf[PL - 1][c], dp);
+                s = mma<KIND>(rot_read<NC>(buf[b], even, odd, 1, c), kf[0][c], s);
+                dp = mma<KIND>(rot_read<NC>(buf[b] + SUB, even, odd, 1, c), vf[0][c], dp);
+                s = mma<KIND>(q1, kf[PL - 1][c], s);
+                dp = mma<KIND>(g1, vf[PL - 1][c], dp);
             }
-            s = mma<KIND>(qr[c * 64], kf[0][c], s);
-            dp = mma<KIND>(gr[c * 64], vf[0][c], dp);
+            s = mma<KIND>(q1, kf[0][c], s);
+            dp = mma<KIND>(g1, vf[0][c], dp);
         }
         const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r.v[0]) * pow2i(rk[0]);
         const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r.v[1] + rk[1]) : pow2i(r.v[1] + rk[1]);
