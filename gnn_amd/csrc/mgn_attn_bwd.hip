@@ -109,8 +109,8 @@ constexpr int GROUP = 2;                               // sums by bucket that ar
 // readout of 20 000 x 2501 in us for 1 / 2 / 4 / 8 at a time: 753 / 741 / 744 / 771, without the sums 684, before buckets were listed).
 //
 // Bound by the vector unit with a bias (18 products a step beside about 260 vector instructions with listed buckets, 390
-// without): 20 000 x 2501, 4 heads of 32, fp32, plane, table trained, 211 us and 7 for the sum of its two pieces.  Without one by
-// the latency of a step's chain: 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 83 us = 0.57 PFLOP/s.
+// without): 20 000 x 2501, 4 heads of 32, fp32, plane, table trained, 214 us and 7 for the sum of its two pieces.  Without one by
+// the latency of a step's chain: 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 80 us = 0.59 PFLOP/s.
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : KIND == AT_F32 && DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
@@ -332,8 +332,8 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict
 // ------------------------------------------------------------------------------------------------ key side
 // A workgroup: 128 keys of one key head, 32 per wave, against its share of the (query head, query subtile) pairs that read
 // them.  Here the lane owns a key: rows of the products are queries, whose statistics come through LDS.
-// Bound like the query side.  Measured at its two problems: 249 us (fp32, plane, listed buckets, 24 products a step)
-// and 117 us = 0.54 PFLOP/s (bf16, four query heads to a key head).
+// Bound like the query side.  Measured at its two problems: 260 us (fp32, plane, listed buckets, 24 products a step)
+// and 106 us = 0.59 PFLOP/s (bf16, four query heads to a key head).
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
