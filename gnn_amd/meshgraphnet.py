@@ -377,6 +377,27 @@ class EncodeProcessDecodeMultiScale(nn.Module):
             plan = cg.__dict__["readout_plan"] = self.readout.plan(mesh_pos, cg.first, sizes, cg.block_sizes)
         return plan
 
+    def captured_parts(self, graph, training: bool = False) -> list:
+        """What launches recorded for ``graph`` go on reading: its topology, coarse graph, readout plan and the workspaces.  The
+        model keeps these in caches that a call on another mesh replaces, so whoever records launches calls this first (nothing
+        is then built while recording) and keeps the list for as long as it replays them."""
+        def looked_up(topo):
+            topo.min_in_degree()
+            if training:
+                topo.sender_view()
+            return topo
+        parts = [looked_up(self.topology(graph))]
+        if self.sample_ratio > 0:
+            cg = self._coarse_graph(graph)
+            parts += [cg, looked_up(cg.topology)]
+            if self.coarse_readout == "attention":
+                parts.append(self._readout_plan(cg, graph["mesh_pos"], None, graph))
+        parts += [self.__dict__.get(k) for k in ("_ws", "_cws", "_pk", "_cpk")]
+        for nrm in (self.node_features_normalizer, self.edge_features_normalizer, self.output_normalizer) + \
+                ((self.coarse_edge_features_normalizer,) if self.sample_ratio > 0 else ()):
+            parts += nrm.captured_buffers()
+        return parts
+
     def _coarse_workspace(self, device, cg, n_own):
         nc, ec = cg.num_nodes, cg.topology.num_edges
         cw = self.__dict__.get("_cws")

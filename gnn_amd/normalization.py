@@ -66,13 +66,33 @@ class Normalizer(nn.Module):
         """Keeps a copy of ``_acc_count`` in device memory and lets the update kernel advance it, so
         that a captured (HIP graph) launch sequence stays valid from step to step.  ``_acc_count``
         itself is still advanced on the host by every call that goes through :meth:`stats_for`; a
-        caller that replays captured launches advances it with :meth:`count_replayed`."""
+        caller that replays captured launches advances it with :meth:`count_replayed`.
+
+        Several captured sequences may use one normaliser (a training step and a rollout between its replays): they share the
+        one copy, and every call with ``on`` is paired with one without it."""
         w = self._work()
-        if on:
-            w["count_dev"] = torch.tensor([self._acc_count], dtype=torch.int64, device=self._acc_sum.device)
+        users = w.get("count_users", 0) + (1 if on else -1)
+        if users > 0:
+            w["count_users"] = users
+            if on:
+                self.sync_device_count()
         else:
+            w.pop("count_users", None)
             w.pop("count_dev", None)
         return self
+
+    def sync_device_count(self):
+        """Writes the host's ``_acc_count`` into the device copy of :meth:`use_device_count`, in place."""
+        w = self._work()
+        if "count_dev" in w:
+            w["count_dev"].fill_(self._acc_count)
+        else:
+            w["count_dev"] = torch.tensor([self._acc_count], dtype=torch.int64, device=self._acc_sum.device)
+
+    def captured_buffers(self):
+        """The buffers that launches recorded now go on reading and writing; whoever replays them keeps these alive (a larger
+        mesh gets a larger scratch buffer in place of this one)."""
+        return [t for t in self._work().values() if isinstance(t, torch.Tensor)]
 
     def count_replayed(self, rows: int):
         """Host bookkeeping for one replay of a captured accumulating call (core/normalization.py:36-37)."""

@@ -51,6 +51,13 @@ class _StepGraph:
         self.norms = feature_norms + (model.output_normalizer,)
         for nr in self.norms:
             nr.use_device_count(True)
+        try:
+            self._record(feature_norms)
+        except BaseException:
+            self.close()
+            raise
+
+    def _record(self, feature_norms):
         self.accumulating = [nr._num_accumulations < nr._max_accumulations for nr in feature_norms]
         state = self._snapshot()
         side = torch.cuda.Stream()
@@ -60,6 +67,7 @@ class _StepGraph:
         torch.cuda.current_stream().wait_stream(side)
         self._restore(state)
         counts = [(nr._acc_count, nr._num_accumulations) for nr in self.norms]
+        self.held = self.model.captured_parts(self.cur)    # read by every replay, whatever the model's caches hold by then
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.pred = self._body()
@@ -85,7 +93,7 @@ class _StepGraph:
         for nr, (s1, s2, cnt, num) in zip(self.norms, norms):
             nr._acc_sum.copy_(s1); nr._acc_sum_squared.copy_(s2)
             nr._acc_count, nr._num_accumulations = cnt, num
-            nr.use_device_count(True)               # device copy of the count back in step
+            nr.sync_device_count()
         self.cur["world_pos"].copy_(world); self.cur["phi"].copy_(phi)
 
     def valid(self) -> bool:

@@ -511,7 +511,7 @@ class CapturedTrainStep:
         self.norms = (model.node_features_normalizer, model.edge_features_normalizer, model.output_normalizer)
         if model.sample_ratio > 0:
             self.norms += (model.coarse_edge_features_normalizer,)
-        self.graph = self.static = self.out = None
+        self.graph = self.static = self.out = self.held = None
         self.done = None
 
     def _eager(self, frame):
@@ -558,6 +558,9 @@ class CapturedTrainStep:
 
     def _capture(self):
         dev = torch.device(self.model.device)
+        # built anew here, outside the capture, if a call on another mesh has replaced them since the eager step; the graph
+        # reads them in every replay, whatever the model's caches hold by then
+        self.held = self.model.captured_parts(self.static, training=True)
         for nr in self.norms:
             nr.use_device_count(True)
         self.flags = self._accumulating()
@@ -570,6 +573,7 @@ class CapturedTrainStep:
             total.backward()
             self.opt.step()
             self.out = (total.detach(), ux.detach(), uy.detach(), phi.detach())
+        self.held += [buf for nr in self.norms for buf in nr.captured_buffers()]      # as the capture used them
         # the capture ran the host bookkeeping of one step (optimiser step counts, normaliser counts) without
         # executing anything: that bookkeeping belongs to the first replay
         self.rows_added = [nr._acc_count - c for nr, c in zip(self.norms, counts)]
@@ -581,10 +585,11 @@ class CapturedTrainStep:
         return tuple(t.clone() for t in self.out)
 
     def close(self):
-        for nr in self.norms:
-            nr.use_device_count(False)
         had_graph = self.graph is not None
-        self.graph = self.static = self.out = None
+        if had_graph:
+            for nr in self.norms:
+                nr.use_device_count(False)
+        self.graph = self.static = self.out = self.held = None
         if had_graph:
             ops.raise_if_out_of_range("CapturedTrainStep")
 

@@ -181,3 +181,54 @@ def test_readout_bias_and_8_bit_activations_together(cells):
         runs.append(seen)
     assert runs[0] == runs[1] and all(v == v and abs(v) != float("inf") for v in runs[0])
     assert runs[0][-1] > 0                                                # the table, zeros at first, has moved
+
+
+@pytest.mark.parametrize("readout", ["copy", "attention"])
+def test_captured_step_owns_what_it_reads(readout):
+    """Between the calls of a captured training step the model predicts and rolls out on other meshes and on another copy of the
+    same coordinates, which replaces its coarse graph, workspaces and scratch, and freed memory is overwritten: the same losses
+    as the eager sequence, bit for bit."""
+    import gnn_amd
+    from gnn_amd.meshgraphnet import EncodeProcessDecodeMultiScale
+    from gnn_amd.optim import FusedAdam
+    from gnn_amd.rollout import rollout
+    from gnn_amd.training import CapturedTrainStep
+    g = graph_to(O.synthetic_graph(16, 10, seed=3, with_target=True), DEV)
+    others = [graph_to(O.synthetic_graph(nx, ny, seed=4), DEV) for nx, ny in ((9, 7), (40, 30))]
+    clone = graph_to(O.synthetic_graph(16, 10, seed=3), DEV)
+    traj = gnn_amd.synthetic_frames(12, 8, n_frames=4, seed=2)
+
+    def disturb(model):
+        with torch.no_grad():
+            for other in others + [clone]:
+                model.predict(other)
+        seen = float(rollout(model, traj, use_graph=True)["pred"].double().norm())
+        junk = [torch.full((n,), float("nan"), device=DEV) for n in (100, 1000, 5000, 20000, 100000) for _ in range(8)]
+        torch.cuda.synchronize()
+        del junk
+        return seen
+    runs = []
+    for captured in (False, True):
+        torch.manual_seed(11)
+        model = EncodeProcessDecodeMultiScale(10, 7, hidden_size=128, process_steps=2, coarse_process_steps=1, node_out_dim=3, attention=False,
+                                              with_mat_params=False, time_dim=1, device=DEV, sample_ratio=0.5, coarse_readout=readout).to(DEV).train()
+        model.coarse_start = 0
+        opt = FusedAdam(model.parameters(), lr=1e-3, capturable=captured)
+        step = CapturedTrainStep(model, opt) if captured else None
+        seen = []
+        for _ in range(5):
+            if captured:
+                seen.append(float(step(g)[0]))
+            else:
+                opt.zero_grad()
+                total = model.loss(g)[0]
+                total.backward()
+                opt.step()
+                seen.append(float(total.detach()))
+            seen.append(disturb(model))
+        if captured:
+            assert step.graph is not None and step.held
+            step.close()
+            assert step.held is None
+        runs.append(seen)
+    assert runs[0] == runs[1] and all(v == v for v in runs[0])
