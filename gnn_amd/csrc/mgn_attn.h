@@ -224,6 +224,10 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int valid, int h) {
         if (!(bits >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -__builtin_inff();
 }
 
+// What the products of two scaled operands are multiplied with.  Held to normal numbers: with two blocks of zeros it would be zero,
+// and minus infinity, the score of a masked key, times zero is no number.
+__device__ __forceinline__ float score_factor(float c) { return fminf(fmaxf(c, 0x1p-126f), F32_MOST); }
+
 __device__ __forceinline__ float bias_log2(float b) {          // finite biases stay finite in base 2
     const float v = b * LOG2E;
     return __builtin_isinf(b) ? v : fminf(fmaxf(v, -F32_MOST), F32_MOST);

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                     add[4 * q + e] = en.bias; off[4 * q + e] = en.offset;
                 }
             }
-        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r.v[0]) * pow2i(rq[0]);
+        const float c = KIND == AT_BF16 ? a.c0 : score_factor(a.c0 * pow2i(r.v[0]) * pow2i(rq[0]));
         const int sh = KIND == AT_BF16 ? 0 : max(r.v[0] - ek, FAR_EXP);
         const float up = KIND == AT_BF16 ? 1.f : (s0 + sub) & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
         const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
             s = mma<KIND>(q1, kf[0][c], s);
             dp = mma<KIND>(g1, vf[0][c], dp);
         }
-        const float c = KIND == AT_BF16 ? a.c0 : a.c0 * pow2i(r.v[0]) * pow2i(rk[0]);
+        const float c = KIND == AT_BF16 ? a.c0 : score_factor(a.c0 * pow2i(r.v[0]) * pow2i(rk[0]));
         const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r.v[1] + rk[1]) : pow2i(r.v[1] + rk[1]);
         const float fp = KIND == AT_BF16 ? 1.f : pow2i(PSHIFT + max(r.v[1] - eg, FAR_EXP));            // of P in the product with dO
         const float fs = KIND == AT_BF16 ? 1.f : pow2i(max(r.v[0] - eq, FAR_EXP) - unit);             // of dS in the product with Q

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
     };
     // scores of a step: scaled (with a bias; without one when the exponentials are taken), masked; returns the largest
     auto finish = [&](f32x16& x, int b, int ex, int valid) {
-        c = KIND == AT_BF16 ? cq : cq * pow2i(ex);
+        c = KIND == AT_BF16 ? cq : score_factor(cq * pow2i(ex));
         if constexpr (BIAS > 0) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
         }
 #pragma unroll
         for (int i = 0; i < HEADS; ++i) {
-            const float c = KIND == AT_BF16 ? cq[i] : cq[i] * pow2i(r[i].v[0]);
+            const float c = KIND == AT_BF16 ? cq[i] : score_factor(cq[i] * pow2i(r[i].v[0]));
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], c, *(const float*)((const char*)(lutb + i * LUTS) + idx[e]));
             if (r[i].v[2] != -1) mask_scores(s, r[i].v[2], h);
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
             }
             s = mma<KIND>(kh[c], qh[c], s);
         }
-        const float c = KIND == AT_BF16 ? cq : cq * pow2i(ek);
+        const float c = KIND == AT_BF16 ? cq : score_factor(cq * pow2i(ek));
         float top = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {

@@ -1,0 +1,34 @@
+"""Attention on operands of very different sizes: blocks that are zero, tiny or masked beside ordinary ones, rows far larger or
+smaller than their neighbours, NaN and infinities.  Values and gradients against tests/attention_reference.py, whose bounds are
+relative to the sums of magnitudes of each result's own row."""
+import math
+
+import pytest
+import torch
+
+from attention_reference import assert_close, reference
+from test_gpu_attention import BF16, DEV, F16, F32, bias_args, check, make, ptr
+
+pytestmark = pytest.mark.gpu
+
+# small problems, the tiled kernel, the tiled kernel with two heads per wave (with a lattice bias), split key ranges
+SHAPES = [(60, 200, 4, 32), (300, 1500, 8, 64), (1100, 300, 64, 32), (700, 2500, 4, 24), (130, 2200, 2, 128)]
+
+
+def bias(nq, nk, heads, axes):
+    return bias_args(nq, nk, heads, axes, 30) if axes else {}
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("axes", [0, 1, 2])
+@pytest.mark.parametrize("nq,nk,heads,dim", SHAPES)
+def test_zero_and_tiny_queries_beside_masked_keys(nq, nk, heads, dim, axes, dtype):
+    """A padded batch: queries of zero and of 1e-3 beside whole blocks of masked keys and a masked end."""
+    q, k, v, g = make(nq, nk, heads, heads, dim, dtype)
+    q[:40] = 0
+    q[40:50] *= 1e-3
+    mask = torch.ones(nk, dtype=torch.bool, device=DEV)
+    mask[32:100] = False
+    mask[nk - 45:] = False
+    check(q, k, v, g, key_mask=mask, **bias(nq, nk, heads, axes))
+    check(torch.zeros_like(q), k * 1e-3, v, g, key_mask=mask, **bias(nq, nk, heads, axes))
