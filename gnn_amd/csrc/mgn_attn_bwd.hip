@@ -34,6 +34,22 @@ constexpr int LISTED = 4;                              // a bias whose buckets a
 
 constexpr int PSHIFT = 15 - OVER;
 
+// Sums in units of 2^unit that follow what is added to them (fp16 formats).  An addend x of a block with exponent ex enters as
+// x 2^(ex - unit); one that would pass UNIT_OVER raises the unit to where the largest lies below 2^UNIT_TOP, so that a few that
+// grow slowly do not raise it every time and the smallest numbers of fp16 stay 2^-36 of it away.
+constexpr int UNIT_LEAST = -126, UNIT_TOP = 12;
+constexpr float UNIT_OVER = 0x1p15f;
+__device__ __forceinline__ float unit_factor(int e) { return __builtin_amdgcn_ldexpf(1.f, min(e, 127)); }
+__device__ __forceinline__ int raised_unit(int unit, float most, int ex) {
+    return max(unit, (int)((__float_as_uint(most) >> 23) & 0xff) - 126 + ex - UNIT_TOP);
+}
+__device__ __forceinline__ float largest16(const f32x16& s) {
+    float m = fmaxf(fabsf(s[0]), fabsf(s[1]));
+#pragma unroll
+    for (int e = 2; e < 16; e += 2) m = fmaxf(m, fmaxf(fabsf(s[e]), fabsf(s[e + 1])));
+    return m;
+}
+
 // A place's bias, base 2, and the byte offset of its bucket's sums.
 struct Entry { float bias; int offset; };
 // Entries by bucket reach over all values a list can hold.
@@ -113,7 +129,7 @@ constexpr int GROUP = 2;                               // sums by bucket that ar
 // the latency of a step's chain: 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 80 us = 0.59 PFLOP/s.
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : KIND == AT_F32 && DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
-    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
+    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP;
     // fp32 with a bias: one buffer and a second barrier, since two would leave the sums by bucket no room (8192 x 4096, 8 heads of
     // 64: 1095 -> 1028 us for the whole backward pass).  16-bit types: two (8 heads of 32, bf16: 476 us with one, 436 with two).
     constexpr int AXES = BIAS == LISTED ? 0 : BIAS;
@@ -174,7 +190,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
     }
     const i32x4 rq = a.rec_q[qsub];
     const float* rp = a.rows + qsub * 96;
-    const float m = mine ? rp[j] : __builtin_inff(), norm = rp[32 + j], delta = mine ? rp[64 + j] : 0.f;
+    const float m = mine ? rp[j] : __builtin_inff(), norm = KIND == AT_F32 ? 1.f : rp[32 + j], delta = mine ? rp[64 + j] : 0.f;
     int qx = 0, qy = 0, qz = 0;
     float most = 0.f;
     if constexpr (BIAS > 0) {
@@ -189,16 +205,10 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
         if (a.tpart)
             for (int r = t; r < a.n_bucket * 256; r += 256) hist[r] = 0.f;
     }
-    int ek = 0, ev = 0;                                       // common exponents of this segment's keys and values
-    if constexpr (KIND != AT_BF16) {
-        ek = ev = -126;
-        for (int s = lane; s < n_sub; s += 64) { const i32x4 r = rec[s]; ek = max(ek, r[0]); ev = max(ev, r[1]); }
-        ek = wave_max_i(ek); ev = wave_max_i(ev);
-    }
-    // unit of dS in the second product: |dP - delta| < 2^(2 TOP + log2 width + 1) in units of the operands, times P < 2^OVER before
-    // it is divided by its sum, held below 2^15
-    const int unit = KIND == AT_BF16 ? 0 : min(max(rq[1] + ev + 2 * TOP + LOG_DP + OVER - 14, -126), 126);
-    const float down = KIND == AT_BF16 ? norm : norm * pow2i(-unit);
+    // Exponent of this query's sums in the second product: dS enters scaled by it and is held below 2^UNIT_MOST.  It follows the dS
+    // that actually come (their sizes differ by many orders between queries, and with the keys' weights), as the maximum of a
+    // softmax does: when one does not fit, it rises and the sums so far are scaled down.
+    int unit = UNIT_LEAST;
     char* sums = (char*)(hist + w * a.n_bucket * 64 + lane);   // this lane's sums of dS by bucket
     Record<KIND> r, rn;
     if (n_sub > 0) { r.request(rec + lz); r.settle(); arrive(0); }
@@ -241,15 +251,13 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                 }
             }
         const float c = KIND == AT_BF16 ? a.c0 : score_factor(a.c0 * pow2i(r.v[0]) * pow2i(rq[0]));
-        const int sh = KIND == AT_BF16 ? 0 : max(r.v[0] - ek, FAR_EXP);
-        const float up = KIND == AT_BF16 ? 1.f : (s0 + sub) & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]), dn = KIND == AT_BF16 ? down : down * pow2i(sh);
-        const float whole = KIND == AT_BF16 ? 1.f : pow2i(unit - sh);
+        const float up = KIND == AT_BF16 ? 1.f : (s0 + sub) & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]);
         if (r.v[2] != -1) mask_scores(s, r.v[2], h);
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
             const float x = BIAS > 0 ? __builtin_fmaf(s[n], c, add[BIAS ? n : 0]) - m : __builtin_fmaf(s[n], c, -m);
             const float d = KIND == AT_BF16 ? dp[n] - delta : __builtin_fmaf(dp[n], up, -delta);
-            s[n] = __builtin_amdgcn_exp2f(x) * dn * d;
+            s[n] = __builtin_amdgcn_exp2f(x) * d;                  // dS times this query's sum of exponentials
         }
         if constexpr (BIAS > 0)
             if (a.tpart)
@@ -262,11 +270,27 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                     for (int e = 0; e < GROUP; ++e) {
 #pragma unroll
                         for (int p = 0; p < e; ++p) v[e] = off[n + e] == off[n + p] ? v[p] : v[e];
-                        v[e] = __builtin_fmaf(s[n + e], whole, v[e]);
+                        v[e] = __builtin_fmaf(s[n + e], norm, v[e]);
                     }
 #pragma unroll
                     for (int e = 0; e < GROUP; ++e) *(float*)(sums + off[n + e]) = v[e];
                 }
+        if constexpr (KIND != AT_BF16) {
+            float most = largest16(s);
+            float f = unit_factor(r.v[0] - unit);
+            if (__any(most * f > UNIT_OVER)) {                     // the two halves of a query's keys only meet here
+                const int to = raised_unit(unit, fmaxf(most, __shfl_xor(most, 32)), r.v[0]);
+                const float by = unit_factor(unit - to);
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) dq[n][e] *= by;
+                unit = to;
+                f = unit_factor(r.v[0] - unit);
+            }
+#pragma unroll
+            for (int n = 0; n < 16; ++n) s[n] *= f;
+        }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
             float v[8];
@@ -298,7 +322,10 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                 const int d = 32 * n + 8 * q + 4 * h;
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? dq[n][4 * q + e] * a.scale : ldexpf(dq[n][4 * q + e] * a.scale, unit + ek);
+                for (int e = 0; e < 4; ++e) {
+                    const float x = dq[n][4 * q + e] * (a.scale * norm);
+                    v[e] = KIND == AT_BF16 ? x : ldexpf(x, unit);
+                }
                 if (d >= a.dim) continue;
                 if (a.q_splits > 1) *(f32x4*)(a.q_part + (((long long)split * a.heads * a.ns_q + qsub) * 32 + j) * DP + d) = v;
                 else store4<KIND>(a.dq, (row * a.heads + head) * a.dim + d, v);

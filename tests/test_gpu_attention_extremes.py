@@ -32,3 +32,25 @@ def test_zero_and_tiny_queries_beside_masked_keys(nq, nk, heads, dim, axes, dtyp
     mask[nk - 45:] = False
     check(q, k, v, g, key_mask=mask, **bias(nq, nk, heads, axes))
     check(torch.zeros_like(q), k * 1e-3, v, g, key_mask=mask, **bias(nq, nk, heads, axes))
+
+
+@pytest.mark.parametrize("axes", [0, 2])
+@pytest.mark.parametrize("nq,nk,heads,dim", SHAPES)
+def test_fp32_gradient_rows_beside_larger_ones(nq, nk, heads, dim, axes):
+    for size in (1e4, 1e6):
+        q, k, v, g = make(nq, nk, heads, heads, dim, F32)
+        g[5::32] *= size
+        check(q, k, v, g, **bias(nq, nk, heads, axes))
+
+
+@pytest.mark.parametrize("dim", [32, 64])
+@pytest.mark.parametrize("apart", [10, 14])
+def test_fp16_query_gradients_beside_larger_ones(apart, dim):
+    """Rows 2^apart smaller than a neighbour at thousands of keys: no gradient sinks into the smallest numbers of fp16."""
+    from gnn_amd import attention
+    q, k, v, g = make(96, 5000, 2, 2, dim, F16)
+    g *= 2.0 ** (10 - apart)
+    g[5::32] *= 2.0 ** apart
+    leaf = q.detach().requires_grad_()
+    dq, = torch.autograd.grad(attention.cross_attention(leaf, k, v), leaf, g)
+    assert_close(dq, reference(q, k, v, g), "dq")
