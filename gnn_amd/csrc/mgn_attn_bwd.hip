@@ -32,8 +32,6 @@ struct AttnBwd {
 };
 constexpr int LISTED = 4;                              // a bias whose buckets are read from there; 1 .. 3: places of so many axes
 
-constexpr int PSHIFT = 15 - OVER;
-
 // Sums in units of 2^unit that follow what is added to them (fp16 formats).  An addend x of a block with exponent ex enters as
 // x 2^(ex - unit); one that would pass UNIT_OVER raises the unit to where the largest lies below 2^UNIT_TOP, so that a few that
 // grow slowly do not raise it every time and the smallest numbers of fp16 stay 2^-36 of it away.
@@ -42,6 +40,23 @@ constexpr float UNIT_OVER = 0x1p15f;
 __device__ __forceinline__ float unit_factor(int e) { return __builtin_amdgcn_ldexpf(1.f, min(e, 127)); }
 __device__ __forceinline__ int raised_unit(int unit, float most, int ex) {
     return max(unit, (int)((__float_as_uint(most) >> 23) & 0xff) - 126 + ex - UNIT_TOP);
+}
+// ACC: the sums stay in accumulation registers, where the products keep them.  (The compiler gives plain multiplications in this
+// rare branch a second copy of all of them and then spills: dK and dV of 8192 x 4096, 8 heads of 128, fp32, whole backward pass
+// 1683 instead of 1452 us.)  What a product wrote may be read 19 cycles after it was issued, and read by a product 2 after it was
+// written: the waits are in the statement.
+template <bool ACC> __device__ __forceinline__ void scale16(f32x16& s, float by) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        if constexpr (ACC) {
+            float x = s[e], t;
+            if (e == 0) asm volatile("s_nop 15\n\ts_nop 7\n\tv_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1\n\ts_nop 3" : "+a"(x), "=&v"(t) : "v"(by));
+            else asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1\n\ts_nop 3" : "+a"(x), "=&v"(t) : "v"(by));
+            s[e] = x;
+        } else {
+            s[e] *= by;
+        }
+    }
 }
 __device__ __forceinline__ float largest16(const f32x16& s) {
     float m = fmaxf(fabsf(s[0]), fabsf(s[1]));
@@ -282,9 +297,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                 const int to = raised_unit(unit, fmaxf(most, __shfl_xor(most, 32)), r.v[0]);
                 const float by = unit_factor(unit - to);
 #pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) dq[n][e] *= by;
+                for (int n = 0; n < NB; ++n) scale16<DP == 128>(dq[n], by);
                 unit = to;
                 f = unit_factor(r.v[0] - unit);
             }
@@ -363,7 +376,7 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict
 // and 106 us = 0.59 PFLOP/s (bf16, four query heads to a key head).
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
-    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP, LOG_DP = DP == 32 ? 5 : DP == 64 ? 6 : 7;
+    constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP;
     __shared__ __attribute__((aligned(1024))) unsigned short buf[2][2 * SUB];          // Q, dO
     __shared__ __attribute__((aligned(16))) float rbuf[2][128];
     constexpr int AXES = BIAS == LISTED ? 0 : BIAS;
@@ -385,8 +398,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
     const int ki = g.local * ATT_TQ + 32 * w + j, nsk = (g.len + 31) >> 5, wsub = min(g.local * 4 + w, nsk - 1);
     const long long kplace = (g.first >> 5) + g.seg + wsub, ksub = (long long)kvh * a.ns_k + kplace;
 
-    auto qsub_of = [&](int item) { return (head0 + item / n_sub) * a.ns_q + qbase + item % n_sub; };
-    constexpr int PIECES = SUB * 2 / 1024;
+constexpr int PIECES = SUB * 2 / 1024;
     const int lz = lane_zero(), tl = tr_lane(lane), even = rot_lane(lane, 0), odd = rot_lane(lane, 1);
     int rep_at = i0 < i1 ? i0 / n_sub : 0, sub_at = i0 < i1 ? i0 % n_sub : 0;            // of the item that is requested next
     Staged<2 * PIECES> st;
@@ -436,13 +448,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         most = (float)(a.reach * a.reach) + 0.5f;
         if (i0 < i1) fill_biases<BIAS>(lutb, a, (int)head0 + rep_at, t);
     }
-    int eq = 0, eg = 0;                                       // common exponents of the queries and gradients in this range
-    if constexpr (KIND != AT_BF16) {
-        eq = eg = -126;
-        for (int i = i0 + lane; i < i1; i += 64) { const i32x4 r = a.rec_q[qsub_of(i)]; eq = max(eq, r[0]); eg = max(eg, r[1]); }
-        eq = wave_max_i(eq); eg = wave_max_i(eg);
-    }
-    const int unit = KIND == AT_BF16 ? 0 : min(max(rk[1] + eg + 2 * TOP + LOG_DP + OVER - 14, -126), 126);
+    // Exponents of this key's sums, dV of P and dK of dS: as for a query's (attn_dq_kernel).  P is small for every query where a key
+    // has little weight, and dS holds <g, o>, the values of all the other keys: neither is bounded by this key's own block.
+    int unit_p = UNIT_LEAST, unit_s = UNIT_LEAST;
 
     f32x16 dk[NB], dv[NB];
 #pragma unroll
@@ -471,8 +479,6 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
         }
         const float c = KIND == AT_BF16 ? a.c0 : score_factor(a.c0 * pow2i(r.v[0]) * pow2i(rk[0]));
         const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r.v[1] + rk[1]) : pow2i(r.v[1] + rk[1]);
-        const float fp = KIND == AT_BF16 ? 1.f : pow2i(PSHIFT + max(r.v[1] - eg, FAR_EXP));            // of P in the product with dO
-        const float fs = KIND == AT_BF16 ? 1.f : pow2i(max(r.v[0] - eq, FAR_EXP) - unit);             // of dS in the product with Q
         f32x16 p;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -497,9 +503,27 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
                 float pe = __builtin_amdgcn_exp2f(x);
                 if constexpr (KIND != AT_F32) pe *= norm[e];
                 const float d = KIND == AT_BF16 ? dp[n] - delta[e] : __builtin_fmaf(dp[n], up, -delta[e]);
-                s[n] = KIND == AT_BF16 ? pe * d : (pe * fs) * d;
-                p[n] = KIND == AT_BF16 ? pe : pe * fp;
+                s[n] = pe * d;
+                p[n] = pe;
             }
+        }
+        if constexpr (KIND != AT_BF16) {
+            const float most_p = largest16(p), most_s = largest16(s);
+            float fp = unit_factor(r.v[1] - unit_p), fs = unit_factor(r.v[0] - unit_s);
+            if (__any(fmaxf(most_p * fp, most_s * fs) > UNIT_OVER)) {      // the two halves of a key's queries only meet here
+                const int to_p = raised_unit(unit_p, fmaxf(most_p, __shfl_xor(most_p, 32)), r.v[1]);
+                const int to_s = raised_unit(unit_s, fmaxf(most_s, __shfl_xor(most_s, 32)), r.v[0]);
+                const float by_p = unit_factor(unit_p - to_p), by_s = unit_factor(unit_s - to_s);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    scale16<DP == 128>(dv[n], by_p);
+                    scale16<DP == 128>(dk[n], by_s);
+                }
+                unit_p = to_p; unit_s = to_s;
+                fp = unit_factor(r.v[1] - unit_p); fs = unit_factor(r.v[0] - unit_s);
+            }
+#pragma unroll
+            for (int n = 0; n < 16; ++n) { p[n] *= fp; s[n] *= fs; }
         }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
@@ -546,8 +570,8 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBw
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x = dk[n][4 * q + e] * a.scale, y = dv[n][4 * q + e];
-                vk[e] = !keep ? 0.f : KIND == AT_BF16 ? x : ldexpf(x, unit + eq);
-                vv[e] = !keep ? 0.f : KIND == AT_BF16 ? y : ldexpf(y, eg - PSHIFT);
+                vk[e] = !keep ? 0.f : KIND == AT_BF16 ? x : ldexpf(x, unit_s);
+                vv[e] = !keep ? 0.f : KIND == AT_BF16 ? y : ldexpf(y, unit_p);
             }
             if (a.splits > 1) {
                 *(f32x4*)(part + d) = vk; *(f32x4*)(part + vpart + d) = vv;
