@@ -224,6 +224,32 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int valid, int h) {
         if (!(bits >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -__builtin_inff();
 }
 
+// Sums of probabilities times values in fp16 formats: kept in units of 2^unit (relative to 2^m, m the running maximum), where unit
+// follows the largest (probability x size of its values) so far, as m follows the scores.  (One large value that weighs nothing
+// must not push all other probabilities into the smallest numbers of fp16.)  A block's probabilities enter times 2^(ev - unit), ev its
+// values' exponent.  `unit` is any real number: what rounds in it is made up for in the factor that the sums so far are scaled with.
+constexpr float SUM_UNIT_LEAST = -200.f;
+// Raises the maximum to the scores' `top` and the unit to what a block with this top and exponent ev needs; *l: the sum of exponentials.
+// Returns the factor for the sums of values.
+__device__ __forceinline__ float raise_sums(float& m, float& unit, float& l, float top, float ev, bool scaled) {
+    const float mn = fmaxf(m, top), zero = mn == -__builtin_inff() ? 0.f : mn, lowered = m - zero;
+    const float al = __builtin_amdgcn_exp2f(lowered);
+    float by = al;
+    if (scaled) {
+        const float to = fmaxf(fmaxf(unit + lowered, top - zero + ev), SUM_UNIT_LEAST);
+        by = __builtin_amdgcn_exp2f(lowered + (unit - to));
+        unit = to;
+    }
+    l *= al;
+    m = mn;
+    return by;
+}
+// x 2^e for a real e
+__device__ __forceinline__ float scale_real(float x, float e) {
+    const float whole = rintf(e);
+    return ldexpf(x * __builtin_amdgcn_exp2f(e - whole), (int)whole);
+}
+
 // What the products of two scaled operands are multiplied with.  Held to normal numbers: with two blocks of zeros it would be zero,
 // and minus infinity, the score of a masked key, times zero is no number.
 __device__ __forceinline__ float score_factor(float c) { return fminf(fmaxf(c, 0x1p-126f), F32_MOST); }

@@ -227,17 +227,10 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
         for (int r = t; r < entries; r += 64 * NW)
             lutb[r] = bias_log2(a.table[head * a.n_bucket + min(max(a.lut[r], 0), a.n_bucket - 1)]);
     }
-    int ev = 0;                                                 // common exponent of the values in this range
-    if constexpr (KIND != AT_BF16) {
-        ev = -126;
-        for (int s = lane; s < n_it; s += 64) ev = max(ev, rec[s][1]);
-        ev = __builtin_amdgcn_readfirstlane(wave_max_i(ev));
-    }
-
     f32x16 o[NB], s;
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = zero16();
-    float m = -__builtin_inff(), l = 0.f, c = 0.f;
+    float m = -__builtin_inff(), l = 0.f, c = 0.f, unit = SUM_UNIT_LEAST;
     u32x4 kf[PL][NC], vf[PL][2][NB];
     auto key_operands = [&](int b) {
         const u32x4* kp = (const u32x4*)kbuf[b] + lane;
@@ -308,15 +301,13 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
             for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) vf[p][kc][n] = vp[((p * 2 + kc) * NB + n) * 64];
-        if (__any(top > m + (float)OVER)) {                     // the two halves of a query's keys only meet here
-            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-            const float al = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.f : mn));
-            l *= al;
-#pragma unroll
+        const float ev = (float)r.v[1];                         // the values' exponent
+        if (__any((KIND == AT_BF16 ? top - m : top - m + fmaxf(ev - unit, 0.f)) > (float)OVER)) {
+            const float by = raise_sums(m, unit, l, fmaxf(top, __shfl_xor(top, 32)), ev, KIND != AT_BF16);
+#pragma unroll                                                  // (the two halves of a query's keys only meet here)
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[n][e] *= al;
-            m = mn;
+                for (int e = 0; e < 16; ++e) o[n][e] *= by;
         }
         float base = m == -__builtin_inff() ? 0.f : m;
         if (BIAS > 0 && __any(fabsf(base) > 0x1p20f)) {         // biases near the ends of their type: a shift added to the
@@ -326,7 +317,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
         }
         __builtin_amdgcn_sched_barrier(0);
         // ---- scores of the next step on the matrix unit, exponentials of this one on the vector unit
-        const float sh = KIND == AT_BF16 ? 0.f : (float)(SHIFT + max(r.v[1] - ev, FAR_EXP)), back = sh - base, cs = c;
+        const float sh = KIND == AT_BF16 ? 0.f : (float)SHIFT + fmaxf(ev - unit, (float)FAR_EXP), back = sh - base, cs = c;
         f32x16 sn = scores();
         float sum = 0.f;
         u32x4 ph[2], plo[2];
@@ -370,7 +361,6 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
     l += __shfl_xor(l, 32);
     if (qi >= g.len) return;
     const float inv = a.splits > 1 ? 1.f : l > 0.f ? 1.0f / l : 0.f;
-    const int back = KIND == AT_BF16 ? 0 : ev - SHIFT;
     const long long prow = ((long long)split * a.heads + head) * a.n_q + row;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -379,7 +369,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
             const int d = 32 * n + 8 * q + 4 * h;
             f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[n][4 * q + e] * inv : ldexpf(o[n][4 * q + e] * inv, back);
+            for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[n][4 * q + e] * inv : scale_real(o[n][4 * q + e] * inv, unit - SHIFT);
             if (a.splits > 1) *(f32x4*)(a.part + prow * DP + d) = v;
             else if (d < a.dim) {
                 store4<KIND>(a.out, row * a.o_st + head * a.o_sh + d, v);
@@ -478,24 +468,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
         for (int i = 0; i < HEADS; ++i) lutb[i * LUTS + r] = bias_log2(a.table[(head0 + i) * a.n_bucket + b]);
     }
     const i32x4* rec[HEADS];
-    int ev[HEADS];                                                 // common exponents of the values in this range
     const int lz = lane_zero();
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
         rec[i] = a.rec + (long long)((head0 + i) / rep) * a.ns_k + sub0;
-        ev[i] = 0;
-        if constexpr (KIND != AT_BF16) {
-            ev[i] = -126;
-            for (int s = lane; s < n_it; s += 64) ev[i] = max(ev[i], rec[i][s][1]);
-            ev[i] = __builtin_amdgcn_readfirstlane(wave_max_i(ev[i]));
-        }
     }
     f32x16 o[HEADS][NB];
-    float m[HEADS], l[HEADS];
+    float m[HEADS], l[HEADS], unit[HEADS];
     Record<KIND> r[HEADS], rn[HEADS];
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
-        m[i] = -__builtin_inff(); l[i] = 0.f;
+        m[i] = -__builtin_inff(); l[i] = 0.f; unit[i] = SUM_UNIT_LEAST;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[i][b] = zero16();
         if (n_it > 0) { r[i].request(rec[i] + lz); r[i].settle(); }
@@ -538,15 +521,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
             float top = fmaxf(s[0], s[1]);
 #pragma unroll
             for (int e = 2; e < 16; e += 2) top = fmaxf(top, fmaxf(s[e], s[e + 1]));
-            if (__any(top > m[i] + (float)OVER)) {              // the two halves of a query's keys only meet here
-                const float mn = fmaxf(m[i], fmaxf(top, __shfl_xor(top, 32)));
-                const float al = __builtin_amdgcn_exp2f(m[i] - (mn == -__builtin_inff() ? 0.f : mn));
-                l[i] *= al;
-#pragma unroll
+            const float ev = (float)r[i].v[1];                  // the values' exponent
+            if (__any((KIND == AT_BF16 ? top - m[i] : top - m[i] + fmaxf(ev - unit[i], 0.f)) > (float)OVER)) {
+                const float by = raise_sums(m[i], unit[i], l[i], fmaxf(top, __shfl_xor(top, 32)), ev, KIND != AT_BF16);
+#pragma unroll                                                  // (the two halves of a query's keys only meet here)
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][n][e] *= al;
-                m[i] = mn;
+                    for (int e = 0; e < 16; ++e) o[i][n][e] *= by;
             }
             float base = m[i] == -__builtin_inff() ? 0.f : m[i];
             if (__any(fabsf(base) > 0x1p20f)) {                 // biases near the ends of their type (see attn_fwd_kernel)
@@ -556,7 +537,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
             }
             f32x16 next;
             if (i + 1 < HEADS) next = scores(i + 1);
-            const float sh = KIND == AT_BF16 ? 0.f : (float)(SHIFT + max(r[i].v[1] - ev[i], FAR_EXP)), back = sh - base;
+            const float sh = KIND == AT_BF16 ? 0.f : (float)SHIFT + fmaxf(ev - unit[i], (float)FAR_EXP), back = sh - base;
             const u32x4* vp = (const u32x4*)(buf[b] + (i * 2 + 1) * SUB) + lane;
             float sum = 0.f;
 #pragma unroll
@@ -590,7 +571,6 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
         const int head = head0 + i;
         if (qi >= g.len) continue;
         const float inv = a.splits > 1 ? 1.f : l[i] > 0.f ? 1.0f / l[i] : 0.f;
-        const int back = KIND == AT_BF16 ? 0 : ev[i] - SHIFT;
         const long long prow = ((long long)split * a.heads + head) * a.n_q + row;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -599,7 +579,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
                 const int d = 32 * n + 8 * q + 4 * h;
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[i][n][4 * q + e] * inv : ldexpf(o[i][n][4 * q + e] * inv, back);
+                for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[i][n][4 * q + e] * inv : scale_real(o[i][n][4 * q + e] * inv, unit[i] - SHIFT);
                 if (a.splits > 1) *(f32x4*)(a.part + prow * DP + d) = v;
                 else if (d < a.dim) {
                     store4<KIND>(a.out, row * a.o_st + head * a.o_sh + d, v);
@@ -683,8 +663,7 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
     f32x16 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = zero16();
-    float m = -__builtin_inff(), l = 0.f;
-    int ev = -126;                                              // exponent of the values' sums so far
+    float m = -__builtin_inff(), l = 0.f, unit = SUM_UNIT_LEAST;
     for (int sub = w; sub < n_sub; sub += 4) {
         const int key = 32 * sub + j;
         const bool use = key < klen && (!a.mask || a.mask[k0 + key]);
@@ -767,15 +746,12 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
             top = fmaxf(top, s[e]);
         }
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
-        const int en = max(ev, e1);
-        const float al = __builtin_amdgcn_exp2f(m - base), ao = al * pow2i(ev - en), sh = pow2i(SHIFT + max(e1 - en, FAR_EXP));
-        l *= al;
+        const float by = raise_sums(m, unit, l, top, (float)e1, KIND != AT_BF16), base = m == -__builtin_inff() ? 0.f : m;
+        const float sh = __builtin_amdgcn_exp2f((float)SHIFT + fminf(fmaxf((float)e1 - unit, (float)FAR_EXP), 110.f));   // finite: no key yet
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[b][e] *= ao;
-        m = mn; ev = en;
+            for (int e = 0; e < 16; ++e) o[b][e] *= by;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             s[e] = __builtin_amdgcn_exp2f(s[e] - base);
@@ -798,14 +774,13 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
         }
     }
     l += __shfl_xor(l, 32);
-    const int back = KIND == AT_BF16 ? 0 : ev - SHIFT;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[n][4 * q + e] : ldexpf(o[n][4 * q + e], back);
+            for (int e = 0; e < 4; ++e) v[e] = KIND == AT_BF16 ? o[n][4 * q + e] : scale_real(o[n][4 * q + e], unit - SHIFT);
             *(f32x4*)&sums[w][j][32 * n + 8 * q + 4 * h] = v;
         }
     if (h == 0) { mls[w][0][j] = m; mls[w][1][j] = l; }

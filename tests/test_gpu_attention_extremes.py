@@ -6,10 +6,62 @@ import math
 import pytest
 import torch
 
-from attention_reference import assert_close, reference
+from attention_reference import assert_close, buckets, reference
 from test_gpu_attention import BF16, DEV, F16, F32, bias_args, check, make, ptr
 
 pytestmark = pytest.mark.gpu
+
+def run(q, k, v, g, **kw):
+    """Outputs and gradients of the public entry point."""
+    from gnn_amd import attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    if kw.get("bias_table") is not None:
+        leaves.append(kw["bias_table"].detach().requires_grad_())
+        kw = dict(kw, bias_table=leaves[3])
+    o = attention.cross_attention(*leaves[:3], **kw)
+    return dict(zip(("o", "dq", "dk", "dv", "dtable"), (o.detach(),) + torch.autograd.grad(o, leaves, g)))
+
+
+def sized_rows(x):
+    """Size a row is scaled by: its own largest magnitude, or that of its 32 neighbours where it is within 2^14 of it (or zero)."""
+    out = x.abs().amax(-1)
+    for at in range(0, x.shape[0], 32):
+        rows = out[at:at + 32]
+        most = rows.amax(0, keepdim=True)
+        out[at:at + 32] = torch.where((rows == 0) | (rows * 2.0 ** 14 >= most), most.expand_as(rows), rows)
+    return out.clamp_min(2.0 ** -126)
+
+
+def smallest_digits(ref, q, k, v, g, bias_table=None, bucket_lut=None, q_pos=None, k_pos=None):
+    """Adds to the bounds what the smallest number of fp16 takes from a sum of addends of very different sizes.
+
+    An addend w x of a sum enters as (w 2^(ex - unit)) (x 2^-ex) with 2^ex the size of x's row and the sum's unit such that the
+    largest w 2^ex so far was at least 2^11 in it (raised to 2^11 .. 2^12, forwards to 2^11).  The two terms of the first factor
+    leave at most half the smallest number of fp16, 2^-25: 2^-36 of the largest w 2^ex.  So the sum is off by at most 2^-36 of
+    max(|w| X) sum(|x| / X), X the rows' sizes, 1 or 2 times 2^ex each (2^-34)."""
+    q, k, v, g = (t.detach().cpu().double() for t in (q, k, v, g))
+    rep, scale = q.shape[1] // k.shape[1], q.shape[2] ** -0.5
+    xq, xk, xv, xg = (sized_rows(t) for t in (q, k, v, g))
+    bk = None if bias_table is None else buckets(q_pos.cpu(), k_pos.cpu(), bucket_lut.cpu())
+    for h in range(q.shape[1]):
+        c = h // rep
+        s = q[:, h] @ k[:, c].T * scale
+        if bk is not None:
+            s = s + bias_table.detach().cpu().double()[h][bk]
+        p = torch.softmax(s, 1)
+        o = p @ v[:, c]
+        ds = p * (g[:, h] @ v[:, c].T - (g[:, h] * o).sum(1, keepdim=True))
+        for name, w, x, size, col, by in (("o", p, v[:, c], xv[:, c], h, 1.0), ("dq", ds, k[:, c], xk[:, c], h, scale),
+                                          ("dk", ds.T, q[:, h], xq[:, h], c, scale), ("dv", p.T, g[:, h], xg[:, h], c, 1.0)):
+            ref[name + "_tol"][:, col] += 2.0 ** -34 * by * (w.abs() * size).amax(1, keepdim=True) * (x.abs() / size[:, None]).sum(0)
+
+
+def check_sizes(q, k, v, g, **kw):
+    got, ref = run(q, k, v, g, **kw), reference(q, k, v, g, **kw)
+    smallest_digits(ref, q, k, v, g, **kw)
+    for name, t in got.items():
+        assert_close(t, ref, name)
+
 
 # small problems, the tiled kernel, the tiled kernel with two heads per wave (with a lattice bias), split key ranges
 SHAPES = [(60, 200, 4, 32), (300, 1500, 8, 64), (1100, 300, 64, 32), (700, 2500, 4, 24), (130, 2200, 2, 128)]
@@ -53,7 +105,7 @@ def test_fp32_gradient_rows_beside_larger_ones(nq, nk, heads, dim, axes):
     for size in (1e4, 1e6):
         q, k, v, g = make(nq, nk, heads, heads, dim, F32)
         g[5::32] *= size
-        check(q, k, v, g, **bias(nq, nk, heads, axes))
+        check_sizes(q, k, v, g, **bias(nq, nk, heads, axes))
 
 
 @pytest.mark.parametrize("dim", [32, 64])
@@ -64,6 +116,20 @@ def test_fp16_gradient_rows_beside_larger_ones(apart, dim):
     g *= 2.0 ** (10 - apart)
     g[5::32] *= 2.0 ** apart
     check(q, k, v, g)
+
+
+@pytest.mark.parametrize("axes", [0, 1, 2])
+@pytest.mark.parametrize("nq,nk,heads,dim", SHAPES + [(2, 3000, 4, 32)])
+def test_large_values_that_weigh_nothing(nq, nk, heads, dim, axes):
+    """A value 1e3 .. 1e10 times the others at a weight near e^-60, in a block of its own, first or later."""
+    for size in (1e3, 1e6, 1e10):
+        for where in (slice(0, 32), slice(64, 96)):
+            q, k, v, g = make(nq, nk, heads, heads, dim, F32)
+            q[..., 0] = 4.0
+            k[..., 0] = 0.0
+            k[where, :, 0] = -15.0 * dim ** 0.5
+            v[where] *= size
+            check_sizes(q, k, v, g, **bias(nq, nk, heads, axes))
 
 
 @pytest.mark.parametrize("nq,nk,heads,dim", SHAPES)
