@@ -17,8 +17,8 @@
 // of tile offsets is needed.  Rows past a segment's end and masked keys are zeros.
 //
 // Number formats.  bf16: operands as they are.  fp16: one plane, scaled per subtile by a power of two.  fp32: two fp16 planes
-// x = 2^e (h1 + h2) with the subtile's own e (residual 2^-22 of the value, 2^-39 of the subtile's largest magnitude), three
-// partial products per product.  The exponents go into constants that each product is multiplied with anyway.
+// x = 2^e (h1 + h2) with the subtile's own e, or the row's where the subtile's rows are far apart in size (residual 2^-22 of the
+// value, 2^-25 of the row's largest magnitude), three partial products per product.  The exponents go into constants that each product is multiplied with anyway.
 #pragma once
 #include "mgn_device.h"
 
@@ -134,6 +134,49 @@ __device__ __forceinline__ int scale_exp(float top) {
     return top == 0.f ? -126 : min(max(e + 1 - TOP, -126), 114);
 }
 
+// Exponent of a block of 32 rows as the images' records hold it, and whether some of its rows have one of their own (rows whose
+// largest element is less than 2^-APART of the block's): such a row's elements are scaled by it, and what they are multiplied
+// into is corrected by the difference, in branches that other blocks do not take.  So an element loses nothing to a large neighbour
+// row: its two fp16 terms leave 2^-22 of it, or 2^-25 of its own row's largest element.
+constexpr int APART = 14;
+__device__ __forceinline__ int block_word(int ex, bool apart) { return (ex & 0xffff) | (apart ? 0x10000 : 0); }
+__device__ __forceinline__ int block_exp(int word) { return (int)(short)word; }
+__device__ __forceinline__ bool block_apart(int word) { return (word & 0x10000) != 0; }
+// differences of the rows 8 q + 4 h .. + 3, q < 4, which a lane's scores belong to
+struct RowFix { i32x4 f[4]; };
+__device__ __forceinline__ RowFix row_fix(const int* of_block, int h) {
+    RowFix r;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) r.f[q] = *(const i32x4*)(of_block + 8 * q + 4 * h);
+    return r;
+}
+__device__ __forceinline__ void apply_fix(f32x16& s, const RowFix& r) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_ldexpf(s[e], r.f[e >> 2][e & 3]);
+}
+// 2^e, zero below the smallest number, the largest power of two where it would be infinite
+__device__ __forceinline__ float unit_factor(int e) { return __builtin_amdgcn_ldexpf(1.f, min(e, 127)); }
+
+// largest magnitude of N values, infinities left out: they stay what they are under any scaling and set none for their neighbours
+template <int N> __device__ __forceinline__ float finite_top(const float (*v)[8]) {
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, (__float_as_uint(v[c][e]) & 0x7fffffffu) < 0x7f800000u ? fabsf(v[c][e]) : 0.f);
+    return top;
+}
+// The same for a row that lanes l and l + 32 hold half of each; the second pass is taken where there is an infinity.
+template <int N> __device__ __forceinline__ float row_top(const float (*v)[8]) {
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
+    if (__any(__float_as_uint(top) >= 0x7f800000u)) top = finite_top<N>(v);
+    return fmaxf(top, __shfl_xor(top, 32));
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
@@ -229,20 +272,36 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int valid, int h) {
 // must not push all other probabilities into the smallest numbers of fp16.)  A block's probabilities enter times 2^(ev - unit), ev its
 // values' exponent.  `unit` is any real number: what rounds in it is made up for in the factor that the sums so far are scaled with.
 constexpr float SUM_UNIT_LEAST = -200.f;
-// Raises the maximum to the scores' `top` and the unit to what a block with this top and exponent ev needs; *l: the sum of exponentials.
-// Returns the factor for the sums of values.
-__device__ __forceinline__ float raise_sums(float& m, float& unit, float& l, float top, float ev, bool scaled) {
-    const float mn = fmaxf(m, top), zero = mn == -__builtin_inff() ? 0.f : mn, lowered = m - zero;
-    const float al = __builtin_amdgcn_exp2f(lowered);
-    float by = al;
-    if (scaled) {
-        const float to = fmaxf(fmaxf(unit + lowered, top - zero + ev), SUM_UNIT_LEAST);
-        by = __builtin_amdgcn_exp2f(lowered + (unit - to));
-        unit = to;
-    }
-    l *= al;
+// Raises the maximum to the scores' `top` and scales *l, the sum of exponentials; returns how far the old maximum lies below (<= 0).
+__device__ __forceinline__ float raise_max(float& m, float& l, float top) {
+    const float mn = fmaxf(m, top), lowered = m - (mn == -__builtin_inff() ? 0.f : mn);
+    l *= __builtin_amdgcn_exp2f(lowered);
     m = mn;
+    return lowered;
+}
+// Raises the unit to `need`, the largest (probability x size of its values) of a block, log 2 and relative to 2^m; returns the factor
+// for the sums so far.
+__device__ __forceinline__ float raise_unit(float& unit, float lowered, float need) {
+    const float to = fmaxf(fmaxf(unit + lowered, need), SUM_UNIT_LEAST), by = __builtin_amdgcn_exp2f(lowered + (unit - to));
+    unit = to;
     return by;
+}
+// ACC: the sums stay in accumulation registers, where the products keep them.  (The compiler gives plain multiplications in this
+// rare branch a second copy of all of them and then spills: dK and dV of 8192 x 4096, 8 heads of 128, fp32, whole backward pass
+// 1683 instead of 1452 us.)  What a product wrote may be read 19 cycles after it was issued, and read by a product 2 after it was
+// written: the waits are in the statement.
+template <bool ACC> __device__ __forceinline__ void scale16(f32x16& s, float by) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        if constexpr (ACC) {
+            float x = s[e], t;
+            if (e == 0) asm volatile("s_nop 15\n\ts_nop 7\n\tv_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1\n\ts_nop 3" : "+a"(x), "=&v"(t) : "v"(by));
+            else asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1\n\ts_nop 3" : "+a"(x), "=&v"(t) : "v"(by));
+            s[e] = x;
+        } else {
+            s[e] *= by;
+        }
+    }
 }
 // x 2^e for a real e
 __device__ __forceinline__ float scale_real(float x, float e) {
@@ -337,7 +396,8 @@ struct ImageJob {
     const int* ptr; const uint8_t* mask;
     long long T; int heads, n_sub, first_unit;   // n_sub: subtiles of a head; units of this job start at first_unit
     unsigned short* R; unsigned short* Tt;       // images (either may be null; Tt only where ImageArgs::transposed)
-    int* ex; int* valid;                         // exponent of (head, subtile), 4 ints apart; valid bits of the tokens
+    int* ex; int* valid;                         // block word of (head, subtile), 4 ints apart; valid bits of the tokens
+    int* fix;                                    // [head][subtile][32]: a row's exponent less the block's (fp16 formats)
     const int* pos; int* pos_out; int axes;      // places [T][axes] -> [subtile][axes][32]
     const void* o; long long o_st, o_sh;         // gradient job: the outputs (fp32 or the type of the rows), ...
     int o_f32;

@@ -19,6 +19,7 @@ struct AttnBwd {
     const unsigned short *q_r, *g_r;                   // images R of queries and output gradients, [heads][ns_q]
     const unsigned short *k_r, *v_r;                   // of keys and values, [kv_heads][ns_k]
     const i32x4 *rec_q, *rec_k;                        // exponents {q, g} and {k, v, valid keys}
+    const int *fix_q, *fix_g, *fix_k, *fix_v;          // rows' own exponents, [heads][subtile][32]
     const float* rows;                                 // [heads][ns_q][3][32]
     int ns_q, ns_k;
     const int *qpos, *kpos;                            // places [subtile][axes][32]
@@ -37,26 +38,8 @@ constexpr int LISTED = 4;                              // a bias whose buckets a
 // grow slowly do not raise it every time and the smallest numbers of fp16 stay 2^-36 of it away.
 constexpr int UNIT_LEAST = -126, UNIT_TOP = 12;
 constexpr float UNIT_OVER = 0x1p15f;
-__device__ __forceinline__ float unit_factor(int e) { return __builtin_amdgcn_ldexpf(1.f, min(e, 127)); }
 __device__ __forceinline__ int raised_unit(int unit, float most, int ex) {
     return max(unit, (int)((__float_as_uint(most) >> 23) & 0xff) - 126 + ex - UNIT_TOP);
-}
-// ACC: the sums stay in accumulation registers, where the products keep them.  (The compiler gives plain multiplications in this
-// rare branch a second copy of all of them and then spills: dK and dV of 8192 x 4096, 8 heads of 128, fp32, whole backward pass
-// 1683 instead of 1452 us.)  What a product wrote may be read 19 cycles after it was issued, and read by a product 2 after it was
-// written: the waits are in the statement.
-template <bool ACC> __device__ __forceinline__ void scale16(f32x16& s, float by) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        if constexpr (ACC) {
-            float x = s[e], t;
-            if (e == 0) asm volatile("s_nop 15\n\ts_nop 7\n\tv_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1\n\ts_nop 3" : "+a"(x), "=&v"(t) : "v"(by));
-            else asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %2, %1\n\tv_accvgpr_write_b32 %0, %1\n\ts_nop 3" : "+a"(x), "=&v"(t) : "v"(by));
-            s[e] = x;
-        } else {
-            s[e] *= by;
-        }
-    }
 }
 __device__ __forceinline__ float largest16(const f32x16& s) {
     float m = fmaxf(fabsf(s[0]), fabsf(s[1]));
@@ -204,6 +187,8 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
             for (int c = 0; c < NC; ++c) { qf[p][c] = qp[(p * NC + c) * 64]; gf[p][c] = gp[(p * NC + c) * 64]; }
     }
     const i32x4 rq = a.rec_q[qsub];
+    int eq = 0, eg = 0;                                       // exponents of this query and its gradient
+    if constexpr (KIND != AT_BF16) { eq = block_exp(rq[0]) + a.fix_q[qsub * 32 + j]; eg = block_exp(rq[1]) + a.fix_g[qsub * 32 + j]; }
     const float* rp = a.rows + qsub * 96;
     const float m = mine ? rp[j] : __builtin_inff(), norm = KIND == AT_F32 ? 1.f : rp[32 + j], delta = mine ? rp[64 + j] : 0.f;
     int qx = 0, qy = 0, qz = 0;
@@ -265,9 +250,16 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                     add[4 * q + e] = en.bias; off[4 * q + e] = en.offset;
                 }
             }
-        const float c = KIND == AT_BF16 ? a.c0 : score_factor(a.c0 * pow2i(r.v[0]) * pow2i(rq[0]));
-        const float up = KIND == AT_BF16 ? 1.f : (s0 + sub) & 1 ? -pow2i(r.v[1] + rq[1]) : pow2i(r.v[1] + rq[1]);
-        if (r.v[2] != -1) mask_scores(s, r.v[2], h);
+        const float c = KIND == AT_BF16 ? a.c0 : score_factor(ldexpf(a.c0, block_exp(r.v[0]) + eq));
+        const float up = KIND == AT_BF16 ? 1.f : (s0 + sub) & 1 ? -unit_factor(block_exp(r.v[1]) + eg) : unit_factor(block_exp(r.v[1]) + eg);
+        const bool apart = KIND != AT_BF16 && block_apart(r.v[0] | r.v[1]);
+        if (r.v[2] != -1 || apart) {
+            if (apart) {                                       // rows with exponents of their own
+                apply_fix(s, row_fix(a.fix_k + (ksub + sub) * 32, h));
+                apply_fix(dp, row_fix(a.fix_v + (ksub + sub) * 32, h));
+            }
+            mask_scores(s, r.v[2], h);
+        }
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
             const float x = BIAS > 0 ? __builtin_fmaf(s[n], c, add[BIAS ? n : 0]) - m : __builtin_fmaf(s[n], c, -m);
@@ -291,15 +283,17 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
                     for (int e = 0; e < GROUP; ++e) *(float*)(sums + off[n + e]) = v[e];
                 }
         if constexpr (KIND != AT_BF16) {
-            float most = largest16(s);
-            float f = unit_factor(r.v[0] - unit);
+            if (block_apart(r.v[0])) apply_fix(s, row_fix(a.fix_k + (ksub + sub) * 32, h));
+            const float most = largest16(s);
+            const int ek = block_exp(r.v[0]);
+            float f = unit_factor(ek - unit);
             if (__any(most * f > UNIT_OVER)) {                     // the two halves of a query's keys only meet here
-                const int to = raised_unit(unit, fmaxf(most, __shfl_xor(most, 32)), r.v[0]);
+                const int to = raised_unit(unit, fmaxf(most, __shfl_xor(most, 32)), ek);
                 const float by = unit_factor(unit - to);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) scale16<DP == 128>(dq[n], by);
                 unit = to;
-                f = unit_factor(r.v[0] - unit);
+                f = unit_factor(ek - unit);
             }
 #pragma unroll
             for (int n = 0; n < 16; ++n) s[n] *= f;
@@ -436,6 +430,8 @@ constexpr int PIECES = SUB * 2 / 1024;
             for (int c = 0; c < NC; ++c) { kf[p][c] = kp[(p * NC + c) * 64]; vf[p][c] = vp[(p * NC + c) * 64]; }
     }
     const i32x4 rk = a.rec_k[ksub];
+    int ek = 0, ev = 0;                                       // exponents of this key and its value
+    if constexpr (KIND != AT_BF16) { ek = block_exp(rk[0]) + a.fix_k[ksub * 32 + j]; ev = block_exp(rk[1]) + a.fix_v[ksub * 32 + j]; }
     int kx = 0, ky = 0, kz = 0;
     float most = 0.f;
     if constexpr (BIAS > 0) {
@@ -460,6 +456,7 @@ constexpr int PIECES = SUB * 2 / 1024;
     for (int item = i0; item < i1; ++item) {
         const int b = (item - i0) & 1;
         bool next_head = false;
+        const long long qsub_at = (head0 + rep_at) * a.ns_q + qbase + sub_at;      // of this item
         if (item + 1 < i1) {
             if (++sub_at == n_sub) { sub_at = 0; ++rep_at; next_head = true; }
         }
@@ -477,8 +474,12 @@ constexpr int PIECES = SUB * 2 / 1024;
             s = mma<KIND>(q1, kf[0][c], s);
             dp = mma<KIND>(g1, vf[0][c], dp);
         }
-        const float c = KIND == AT_BF16 ? a.c0 : score_factor(a.c0 * pow2i(r.v[0]) * pow2i(rk[0]));
-        const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -pow2i(r.v[1] + rk[1]) : pow2i(r.v[1] + rk[1]);
+        const float c = KIND == AT_BF16 ? a.c0 : score_factor(ldexpf(a.c0, block_exp(r.v[0]) + ek));
+        const float up = KIND == AT_BF16 ? 1.f : wsub & 1 ? -unit_factor(block_exp(r.v[1]) + ev) : unit_factor(block_exp(r.v[1]) + ev);
+        if (KIND != AT_BF16 && block_apart(r.v[0] | r.v[1])) {
+            apply_fix(s, row_fix(a.fix_q + qsub_at * 32, h));
+            apply_fix(dp, row_fix(a.fix_g + qsub_at * 32, h));
+        }
         f32x16 p;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -508,11 +509,16 @@ constexpr int PIECES = SUB * 2 / 1024;
             }
         }
         if constexpr (KIND != AT_BF16) {
+            if (block_apart(r.v[0] | r.v[1])) {
+                apply_fix(s, row_fix(a.fix_q + qsub_at * 32, h));
+                apply_fix(p, row_fix(a.fix_g + qsub_at * 32, h));
+            }
             const float most_p = largest16(p), most_s = largest16(s);
-            float fp = unit_factor(r.v[1] - unit_p), fs = unit_factor(r.v[0] - unit_s);
+            const int eq = block_exp(r.v[0]), eg = block_exp(r.v[1]);
+            float fp = unit_factor(eg - unit_p), fs = unit_factor(eq - unit_s);
             if (__any(fmaxf(most_p * fp, most_s * fs) > UNIT_OVER)) {      // the two halves of a key's queries only meet here
-                const int to_p = raised_unit(unit_p, fmaxf(most_p, __shfl_xor(most_p, 32)), r.v[1]);
-                const int to_s = raised_unit(unit_s, fmaxf(most_s, __shfl_xor(most_s, 32)), r.v[0]);
+                const int to_p = raised_unit(unit_p, fmaxf(most_p, __shfl_xor(most_p, 32)), eg);
+                const int to_s = raised_unit(unit_s, fmaxf(most_s, __shfl_xor(most_s, 32)), eq);
                 const float by_p = unit_factor(unit_p - to_p), by_s = unit_factor(unit_s - to_s);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
@@ -520,7 +526,7 @@ constexpr int PIECES = SUB * 2 / 1024;
                     scale16<DP == 128>(dk[n], by_s);
                 }
                 unit_p = to_p; unit_s = to_s;
-                fp = unit_factor(r.v[1] - unit_p); fs = unit_factor(r.v[0] - unit_s);
+                fp = unit_factor(eg - unit_p); fs = unit_factor(eq - unit_s);
             }
 #pragma unroll
             for (int n = 0; n < 16; ++n) { p[n] *= fp; s[n] *= fs; }
@@ -620,7 +626,7 @@ __global__ __launch_bounds__(256) void attn_dkv_sum_kernel(AttnBwd a, int dp) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct BwdSpace { size_t q_r, g_r, k_r, v_r, rec_q, rec_k, rows, qpos, kpos, tpart, part, q_part, by_query, by_key, total; int ns_q, ns_k, q_tiles, k_tiles, splits, q_splits; bool listed; };
+struct BwdSpace { size_t q_r, g_r, k_r, v_r, rec_q, rec_k, fix_q, fix_g, fix_k, fix_v, rows, qpos, kpos, tpart, part, q_part, by_query, by_key, total; int ns_q, ns_k, q_tiles, k_tiles, splits, q_splits; bool listed; };
 
 BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     BwdSpace s{};
@@ -640,6 +646,8 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     const size_t qi = (size_t)a.heads * s.ns_q * pl * 64 * dp, ki = (size_t)a.kv_heads * s.ns_k * pl * 64 * dp;
     s.q_r = take(qi); s.g_r = take(qi); s.k_r = take(ki); s.v_r = take(ki);
     s.rec_q = take((size_t)a.heads * s.ns_q * 16); s.rec_k = take((size_t)a.kv_heads * s.ns_k * 16);
+    const size_t qf = (size_t)a.heads * s.ns_q * 128, kf = (size_t)a.kv_heads * s.ns_k * 128;
+    s.fix_q = take(qf); s.fix_g = take(qf); s.fix_k = take(kf); s.fix_v = take(kf);
     s.rows = take((size_t)a.heads * s.ns_q * 96 * 4);
     // Buckets listed once where a place is dear (a lattice), at least two heads share it and there are subtiles enough to pay for the
     // launch, up to 1 GB in all.  Backward pass in us without and with: 20 000 x 2501, 4 heads of 32, fp32, plane 599 / 510, in space
@@ -721,6 +729,7 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     const int kind = attn_kind(a.dtype), dp = attn_dp(a.dim), bias = attn_bias(a);
     const hipStream_t st = (hipStream_t)stream;
     auto half = [&](size_t at) { return (unsigned short*)(ws + at); };
+    auto ints = [&](size_t at) { return (int*)(ws + at); };
     int *rec_q = (int*)(ws + s.rec_q), *rec_k = (int*)(ws + s.rec_k);
     ImageArgs im{};
     im.n_seg = a.n_seg; im.dim = a.dim;
@@ -735,21 +744,22 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     };
     if (a.n_q > 0) {
         ImageJob& q = add(a.q, a.q_st, a.q_sh, true);
-        q.R = half(s.q_r); q.ex = rec_q; q.pos = bias ? a.q_pos : nullptr; q.pos_out = (int*)(ws + s.qpos);
+        q.R = half(s.q_r); q.ex = rec_q; q.fix = ints(s.fix_q); q.pos = bias ? a.q_pos : nullptr; q.pos_out = (int*)(ws + s.qpos);
         ImageJob& o = add(g, g_st, g_sh, true);
-        o.R = half(s.g_r); o.ex = rec_q + 1; o.o = out; o.o_f32 = a.out_f32 || a.dtype == MGN_F32; o.o_st = out_st; o.o_sh = out_sh; o.stats = stats; o.rows = (float*)(ws + s.rows);
+        o.R = half(s.g_r); o.ex = rec_q + 1; o.fix = ints(s.fix_g); o.o = out; o.o_f32 = a.out_f32 || a.dtype == MGN_F32; o.o_st = out_st; o.o_sh = out_sh; o.stats = stats; o.rows = (float*)(ws + s.rows);
     }
     if (a.n_k > 0) {
         ImageJob& k = add(a.k, a.k_st, a.k_sh, false);
-        k.R = half(s.k_r); k.ex = rec_k; k.valid = rec_k + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = (int*)(ws + s.kpos);
+        k.R = half(s.k_r); k.ex = rec_k; k.fix = ints(s.fix_k); k.valid = rec_k + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = (int*)(ws + s.kpos);
         ImageJob& v = add(a.v, a.v_st, a.v_sh, false);
-        v.R = half(s.v_r); v.ex = rec_k + 1; v.alternate = kind != AT_BF16;
+        v.R = half(s.v_r); v.ex = rec_k + 1; v.fix = ints(s.fix_v); v.alternate = kind != AT_BF16;
     }
     im.units = units;
     if (units > 0) mgn_attn_launch_images(kind, dp, &im, stream);
     AttnBwd b{};
     b.q_ptr = a.q_ptr; b.k_ptr = a.k_ptr; b.n_q = a.n_q; b.n_k = a.n_k; b.n_seg = a.n_seg; b.heads = a.heads; b.kv_heads = a.kv_heads; b.dim = a.dim;
     b.c0 = a.scale * LOG2E; b.scale = a.scale;
+    b.fix_q = ints(s.fix_q); b.fix_g = ints(s.fix_g); b.fix_k = ints(s.fix_k); b.fix_v = ints(s.fix_v);
     b.q_r = half(s.q_r); b.g_r = half(s.g_r); b.k_r = half(s.k_r); b.v_r = half(s.v_r);
     b.rec_q = (const i32x4*)rec_q; b.rec_k = (const i32x4*)rec_k; b.rows = (const float*)(ws + s.rows); b.ns_q = s.ns_q; b.ns_k = s.ns_k;
     b.qpos = (const int*)(ws + s.qpos); b.kpos = (const int*)(ws + s.kpos);

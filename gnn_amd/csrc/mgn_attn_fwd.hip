@@ -71,25 +71,24 @@ __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
     if (job.pos && head == 0 && h == 0)
         for (int ax = 0; ax < job.axes; ++ax) job.pos_out[((long long)sub * job.axes + ax) * 32 + i] = inside ? job.pos[row * job.axes + ax] : 0;
 
-    float top = 0.f;
+    int ex = 0;
+    bool apart = false;
     if constexpr (KIND != AT_BF16) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
-        top = wave_max(top);
-    }
-    const int ex = scale_exp<KIND>(top);
-    if (KIND != AT_BF16) {
-        const float by = job.alternate && (g.local & 1) ? -pow2i(-ex) : pow2i(-ex);
+        const float top = row_top<NC>(v), most = wave_max(top);
+        ex = scale_exp<KIND>(most);
+        int er = ex;
+        apart = __any(top > 0.f && top < most * (1.f / (1 << APART)));
+        if (apart && top > 0.f && top < most * (1.f / (1 << APART))) er = scale_exp<KIND>(top);
+        const float by = job.alternate && (g.local & 1) ? -pow2i(-er) : pow2i(-er);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[c][e] *= by;
+        if (h == 0) job.fix[at * 32 + i] = er - ex;
     }
     const unsigned long long bits = __ballot(use);
     if (lane == 0) {
-        job.ex[at * 4] = ex;
+        job.ex[at * 4] = block_word(ex, apart);
         if (job.valid) job.valid[at * 4] = (int)(unsigned)bits;
     }
     u32x4 hi[NC], lo[NC];
@@ -172,6 +171,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
     const char* kimg = (const char*)(a.kimg + ((long long)kvh * a.ns_k + sub0) * SUB);
     const char* vimg = (const char*)(a.vimg + ((long long)kvh * a.ns_k + sub0) * SUB);
     const i32x4* rec = a.rec + (long long)kvh * a.ns_k + sub0;
+    const int *kfix = a.kfix + ((long long)kvh * a.ns_k + sub0) * 32, *vfix = a.vfix + ((long long)kvh * a.ns_k + sub0) * 32;
 
     Staged<PIECES, NW> sk, sv;
     int sp = 0;
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
     const int qi = (g.local << TILE_LOG) + 32 * w + j;
     const long long row = g.first + min(qi, g.len - 1);
     u32x4 qh[NC], ql[NC];                                       // the queries' operand, scaled per row
-    float cq = a.c0;
+    int eq = 0;                                                 // by 2^-eq
     {
         float v[NC][8], top = 0.f;
 #pragma unroll
@@ -204,9 +204,8 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
         }
         if constexpr (KIND != AT_BF16) {
-            const int ex = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
-            cq *= pow2i(ex);
-            const float by = pow2i(-ex);
+            eq = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
+            const float by = pow2i(-eq);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -251,20 +250,29 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
         }
         return x;
     };
-    // scores of a step: scaled (with a bias; without one when the exponentials are taken), masked; returns the largest
-    auto finish = [&](f32x16& x, int b, int ex, int valid) {
-        c = KIND == AT_BF16 ? cq : score_factor(cq * pow2i(ex));
-        if constexpr (BIAS > 0) {
+    auto biased = [&](f32x16& x, int b) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                i32x4 px, py, pz;
-                places4<BIAS>(pbuf[b] + 8 * q + 4 * h, px, py, pz);
+        for (int q = 0; q < 4; ++q) {
+            i32x4 px, py, pz;
+            places4<BIAS>(pbuf[b] + 8 * q + 4 * h, px, py, pz);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[4 * q + e] = __builtin_fmaf(x[4 * q + e], c, lutb[place<BIAS>(qx, qy, qz, px[e], py[e], pz[e], a.reach, most)]);
-            }
+            for (int e = 0; e < 4; ++e)
+                x[4 * q + e] = __builtin_fmaf(x[4 * q + e], c, lutb[place<BIAS>(qx, qy, qz, px[e], py[e], pz[e], a.reach, most)]);
         }
-        if (valid != -1) mask_scores(x, valid, h);
+    };
+    // scores of a step: scaled (with a bias; without one when the exponentials are taken), masked; returns the largest
+    auto finish = [&](f32x16& x, int b, int word, int valid, int it) {
+        const bool apart = KIND != AT_BF16 && block_apart(word);
+        c = KIND == AT_BF16 ? a.c0 : score_factor(ldexpf(a.c0, eq + block_exp(word)));
+        if constexpr (BIAS > 0) biased(x, b);
+        if (valid != -1 || apart) {
+            if (apart) {                                        // key rows with exponents of their own
+                if constexpr (BIAS > 0) x = scores();           // the keys' operand is still there: once more, without the bias
+                apply_fix(x, row_fix(kfix + (long long)it * 32, h));
+                if constexpr (BIAS > 0) biased(x, b);
+            }
+            mask_scores(x, valid, h);
+        }
         float top = fmaxf(x[0], x[1]);
 #pragma unroll
         for (int e = 2; e < 16; e += 2) top = fmaxf(top, fmaxf(x[e], x[e + 1]));
@@ -284,7 +292,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
         __syncthreads();
         key_operands(0);
         s = scores();
-        top = finish(s, 0, r.v[0], r.v[2]);
+        top = finish(s, 0, r.v[0], r.v[2], 0);
         arrive_k(1);
         __syncthreads();
     }
@@ -301,15 +309,30 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
             for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
                 for (int n = 0; n < NB; ++n) vf[p][kc][n] = vp[((p * 2 + kc) * NB + n) * 64];
-        const float ev = (float)r.v[1];                         // the values' exponent
-        if (__any((KIND == AT_BF16 ? top - m : top - m + fmaxf(ev - unit, 0.f)) > (float)OVER)) {
-            const float by = raise_sums(m, unit, l, fmaxf(top, __shfl_xor(top, 32)), ev, KIND != AT_BF16);
-#pragma unroll                                                  // (the two halves of a query's keys only meet here)
-            for (int n = 0; n < NB; ++n)
+        const float ev = (float)block_exp(r.v[1]);              // the values' exponent
+        const bool apart = KIND != AT_BF16 && block_apart(r.v[1]);
+        if (__any((KIND == AT_BF16 ? top - m : top - m + fmaxf(ev - unit, 0.f)) > (float)OVER) || apart) {
+            const float most = fmaxf(top, __shfl_xor(top, 32)), lowered = raise_max(m, l, most);       // the two halves of a
+            const float zero = m == -__builtin_inff() ? 0.f : m;                                       // query's keys only meet here
+            float need = most - zero, by;
+            if (apart) {                                        // every value row has its own exponent: its probability takes it
+                const RowFix f = row_fix(vfix + (long long)it * 32, h);
+                need = -__builtin_inff();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[n][e] *= by;
+                for (int e = 0; e < 16; ++e) {
+                    s[e] = (BIAS > 0 ? s[e] : s[e] * c) - zero;
+                    l += __builtin_amdgcn_exp2f(s[e]);
+                    s[e] += (float)f.f[e >> 2][e & 3];
+                    need = fmaxf(need, s[e]);
+                }
+                need = fmaxf(need, __shfl_xor(need, 32));
+            }
+            if constexpr (KIND == AT_BF16) by = __builtin_amdgcn_exp2f(lowered);
+            else by = raise_unit(unit, lowered, need + ev);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) scale16<KIND == AT_F32 && DP == 128>(o[n], by);
         }
-        float base = m == -__builtin_inff() ? 0.f : m;
+        float base = m == -__builtin_inff() || apart ? 0.f : m;
         if (BIAS > 0 && __any(fabsf(base) > 0x1p20f)) {         // biases near the ends of their type: a shift added to the
 #pragma unroll                                                  // maximum would be rounded away
             for (int e = 0; e < 16; ++e) s[e] -= base;
@@ -317,7 +340,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
         }
         __builtin_amdgcn_sched_barrier(0);
         // ---- scores of the next step on the matrix unit, exponentials of this one on the vector unit
-        const float sh = KIND == AT_BF16 ? 0.f : (float)SHIFT + fmaxf(ev - unit, (float)FAR_EXP), back = sh - base, cs = c;
+        const float sh = KIND == AT_BF16 ? 0.f : (float)SHIFT + fmaxf(ev - unit, (float)FAR_EXP), back = sh - base, cs = apart ? 1.f : c;
         f32x16 sn = scores();
         float sum = 0.f;
         u32x4 ph[2], plo[2];
@@ -339,7 +362,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
         }
         __builtin_amdgcn_sched_barrier(0);
         // ---- sums of this step on the matrix unit, bias and maximum of the next one on the vector unit
-        l += KIND == AT_BF16 ? sum : sum * __builtin_amdgcn_exp2f(-sh);
+        l += KIND == AT_BF16 ? sum : sum * (apart ? 0.f : __builtin_amdgcn_exp2f(-sh));
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
@@ -350,7 +373,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
             }
         s = sn;
         r = rn;
-        top = finish(s, b ^ 1, r.v[0], r.v[2]);
+        top = finish(s, b ^ 1, r.v[0], r.v[2], min(it + 1, last));
         sv.write(vbuf[b ^ 1], w, lane);
         arrive_k(b);
         rn = rnn;
@@ -431,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
     const int qi = g.local * ATT_TQ + 32 * w + j;
     const long long row = g.first + min(qi, g.len - 1);
     u32x4 qh[HEADS][NC], ql[PL == 2 ? HEADS : 1][NC];
-    float cq[HEADS];
+    int eq[HEADS];
 #pragma unroll
     for (int i = 0; i < HEADS; ++i) {
         float v[NC][8], top = 0.f;
@@ -446,11 +469,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
         }
-        cq[i] = a.c0;
+        eq[i] = 0;
         if constexpr (KIND != AT_BF16) {
-            const int ex = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
-            cq[i] *= pow2i(ex);
-            const float by = pow2i(-ex);
+            eq[i] = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
+            const float by = pow2i(-eq[i]);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -514,22 +536,51 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
         }
 #pragma unroll
         for (int i = 0; i < HEADS; ++i) {
-            const float c = KIND == AT_BF16 ? cq[i] : score_factor(cq[i] * pow2i(r[i].v[0]));
+            const float c = KIND == AT_BF16 ? a.c0 : score_factor(ldexpf(a.c0, eq[i] + block_exp(r[i].v[0])));
+            const long long block = ((long long)((head0 + i) / rep) * a.ns_k + sub0 + it) * 32;
+            auto biased = [&] {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], c, *(const float*)((const char*)(lutb + i * LUTS) + idx[e]));
-            if (r[i].v[2] != -1) mask_scores(s, r[i].v[2], h);
+                for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(s[e], c, *(const float*)((const char*)(lutb + i * LUTS) + idx[e]));
+            };
+            biased();
+            const bool apart_k = KIND != AT_BF16 && block_apart(r[i].v[0]);
+            if (r[i].v[2] != -1 || apart_k) {
+                if (apart_k) {                                  // key rows with exponents of their own: once more, without the bias
+                    s = scores(i);
+                    apply_fix(s, row_fix(a.kfix + block, h));
+                    biased();
+                }
+                mask_scores(s, r[i].v[2], h);
+            }
             float top = fmaxf(s[0], s[1]);
 #pragma unroll
             for (int e = 2; e < 16; e += 2) top = fmaxf(top, fmaxf(s[e], s[e + 1]));
-            const float ev = (float)r[i].v[1];                  // the values' exponent
-            if (__any((KIND == AT_BF16 ? top - m[i] : top - m[i] + fmaxf(ev - unit[i], 0.f)) > (float)OVER)) {
-                const float by = raise_sums(m[i], unit[i], l[i], fmaxf(top, __shfl_xor(top, 32)), ev, KIND != AT_BF16);
-#pragma unroll                                                  // (the two halves of a query's keys only meet here)
+            const float ev = (float)block_exp(r[i].v[1]);       // the values' exponent
+            const bool apart = KIND != AT_BF16 && block_apart(r[i].v[1]);
+            if (__any((KIND == AT_BF16 ? top - m[i] : top - m[i] + fmaxf(ev - unit[i], 0.f)) > (float)OVER) || apart) {   // as in attn_fwd_kernel
+                const float most = fmaxf(top, __shfl_xor(top, 32)), lowered = raise_max(m[i], l[i], most);
+                const float zero = m[i] == -__builtin_inff() ? 0.f : m[i];
+                float need = most - zero, by;
+                if (apart) {
+                    const RowFix f = row_fix(a.vfix + block, h);
+                    need = -__builtin_inff();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        s[e] -= zero;
+                        l[i] += __builtin_amdgcn_exp2f(s[e]);
+                        s[e] += (float)f.f[e >> 2][e & 3];
+                        need = fmaxf(need, s[e]);
+                    }
+                    need = fmaxf(need, __shfl_xor(need, 32));
+                }
+                if constexpr (KIND == AT_BF16) by = __builtin_amdgcn_exp2f(lowered);
+                else by = raise_unit(unit[i], lowered, need + ev);
+#pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[i][n][e] *= by;
             }
-            float base = m[i] == -__builtin_inff() ? 0.f : m[i];
+            float base = m[i] == -__builtin_inff() || apart ? 0.f : m[i];
             if (__any(fabsf(base) > 0x1p20f)) {                 // biases near the ends of their type (see attn_fwd_kernel)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] -= base;
@@ -557,7 +608,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
                     o[i][n] = mma<KIND>(vp[(kc * NB + n) * 64], ph, o[i][n]);
                 }
             }
-            l[i] += KIND == AT_BF16 ? sum : sum * __builtin_amdgcn_exp2f(-sh);
+            l[i] += KIND == AT_BF16 ? sum : sum * (apart ? 0.f : __builtin_amdgcn_exp2f(-sh));
             s = next;
         }
         arrive(b ^ 1);
@@ -621,7 +672,7 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
     const long long row = g.first + min(qi, g.len - 1);
 
     u32x4 qh[NC], ql[NC];
-    float cq = a.c0;
+    int eq = 0;
     {
         float v[NC][8], top = 0.f;
 #pragma unroll
@@ -635,9 +686,8 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
             for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
         }
         if constexpr (KIND != AT_BF16) {
-            const int ex = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
-            cq *= pow2i(ex);
-            const float by = pow2i(-ex);
+            eq = scale_exp<KIND>(fmaxf(top, __shfl_xor(top, 32)));
+            const float by = pow2i(-eq);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -669,18 +719,11 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
         const bool use = key < klen && (!a.mask || a.mask[k0 + key]);
         const unsigned valid = (unsigned)__ballot(use);         // both halves of the wave hold the same keys
         u32x4 kh[NC], kl[NC], vh[2][NB], vl[2][NB];
-        int ek = 0, e1 = 0;
+        int ek = 0, e1 = 0, fk = 0;                             // exponents of the keys and values; what row j's own differs by
+        bool apart_k = false, apart_v = false;
+        float fv[16];                                           // what the values' rows of this lane's scores have of their own
         {
-            float v[NC][8], top = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = 16 * c + 8 * h;
-                if (use && d < a.dim) load8<KIND>(a.k, (k0 + key) * a.k_st + kvh * a.k_sh + d, v[c]);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
-            }
-            float x[2][NB][8], topv = 0.f;                      // values: column 32 b + j of keys 16 kc + 4 h + (0 .. 3, 8 .. 11)
+            float x[2][NB][8];                                  // values: column 32 b + j of keys 16 kc + 4 h + (0 .. 3, 8 .. 11)
 #pragma unroll
             for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
@@ -691,30 +734,68 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
                         x[kc][b][e] = (valid >> n & 1) && d < a.dim ? load1<KIND>(a.v, (k0 + 32 * sub + n) * a.v_st + kvh * a.v_sh + d) : 0.f;
                     }
             if constexpr (KIND != AT_BF16) {
+                // a lane has a column of the rows: their sizes meet in ballots, one per row of either half of the wave
+                float most[16], top = 0.f;
+                auto sizes = [&](bool finite) {
+                    top = 0.f;
 #pragma unroll
-                for (int c = 0; c < NC; ++c)
+                    for (int n = 0; n < 16; ++n) {
+                        most[n] = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[c][e]));
+                        for (int b = 0; b < NB; ++b) {
+                            const float y = fabsf(x[n >> 3][b][n & 7]);
+                            most[n] = fmaxf(most[n], finite && __float_as_uint(y) >= 0x7f800000u ? 0.f : y);
+                        }
+                        top = fmaxf(top, most[n]);
+                    }
+                };
+                sizes(false);
+                if (__any(__float_as_uint(top) >= 0x7f800000u)) sizes(true);
+                top = wave_max(top);
+                e1 = scale_exp<KIND>(top);
+                const float least = top * (1.f / (1 << APART)), bv = pow2i(-e1);
 #pragma unroll
-                for (int kc = 0; kc < 2; ++kc)
+                for (int n = 0; n < 16; ++n) {
+                    const unsigned long long near = __ballot(most[n] >= least), some = __ballot(most[n] > 0.f);
+                    apart_v |= ((unsigned)near == 0 && (unsigned)some != 0) || (near >> 32 == 0 && some >> 32 != 0);
+                }
+                if (apart_v) {
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+                    for (int n = 0; n < 16; ++n) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) topv = fmaxf(topv, fabsf(x[kc][b][e]));
+                        for (int o2 = 16; o2 > 0; o2 >>= 1) most[n] = fmaxf(most[n], __shfl_xor(most[n], o2));
+                        const int own = most[n] > 0.f && most[n] < least ? scale_exp<KIND>(most[n]) : e1;
+                        fv[n] = (float)(own - e1);
 #pragma unroll
-                for (int o2 = 32; o2 > 0; o2 >>= 1) { top = fmaxf(top, __shfl_xor(top, o2)); topv = fmaxf(topv, __shfl_xor(topv, o2)); }
-                ek = scale_exp<KIND>(top); e1 = scale_exp<KIND>(topv);
-                const float bk = pow2i(-ek), bv = pow2i(-e1);
+                        for (int b = 0; b < NB; ++b) x[n >> 3][b][n & 7] *= pow2i(-own);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 16; ++n)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) x[n >> 3][b][n & 7] *= bv;
+                }
+            }
+            float v[NC][8];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 16 * c + 8 * h;
+                if (use && d < a.dim) load8<KIND>(a.k, (k0 + key) * a.k_st + kvh * a.k_sh + d, v[c]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+            }
+            if constexpr (KIND != AT_BF16) {
+                const float top = row_top<NC>(v), most = wave_max(top);
+                ek = scale_exp<KIND>(most);
+                const bool far = top > 0.f && top < most * (1.f / (1 << APART));
+                apart_k = __any(far);
+                if (far) fk = scale_exp<KIND>(top) - ek;
+                const float bk = pow2i(-ek - fk);
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[c][e] *= bk;
-#pragma unroll
-                for (int kc = 0; kc < 2; ++kc)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[kc][b][e] *= bv;
             }
 #pragma unroll
             for (int c = 0; c < NC; ++c) pack8<KIND>(v[c], kh[c], kl[c]);
@@ -732,7 +813,10 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
             }
             s = mma<KIND>(kh[c], qh[c], s);
         }
-        const float c = KIND == AT_BF16 ? cq : score_factor(cq * pow2i(ek));
+        const float c = KIND == AT_BF16 ? a.c0 : score_factor(ldexpf(a.c0, eq + ek));
+        if (apart_k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = ldexpf(s[e], __shfl(fk, 8 * (e >> 2) + 4 * h + (e & 3)));
         float top = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -746,8 +830,21 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
             top = fmaxf(top, s[e]);
         }
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float by = raise_sums(m, unit, l, top, (float)e1, KIND != AT_BF16), base = m == -__builtin_inff() ? 0.f : m;
-        const float sh = __builtin_amdgcn_exp2f((float)SHIFT + fminf(fmaxf((float)e1 - unit, (float)FAR_EXP), 110.f));   // finite: no key yet
+        const float lowered = raise_max(m, l, top), base = m == -__builtin_inff() ? 0.f : m;
+        float by, need = top - base;
+        if constexpr (KIND == AT_BF16) {
+            by = __builtin_amdgcn_exp2f(lowered);
+        } else {
+            if (apart_v) {
+                need = -__builtin_inff();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) need = fmaxf(need, s[e] - base + fv[e]);
+                need = fmaxf(need, __shfl_xor(need, 32));
+            }
+            by = raise_unit(unit, lowered, need + (float)e1);
+        }
+        auto shift = [&](float x) { return __builtin_amdgcn_exp2f((float)SHIFT + fminf(fmaxf(x - unit, (float)FAR_EXP), 110.f)); };  // finite: no key yet
+        const float sh = KIND == AT_BF16 ? 1.f : shift((float)e1);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -756,7 +853,7 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
         for (int e = 0; e < 16; ++e) {
             s[e] = __builtin_amdgcn_exp2f(s[e] - base);
             l += s[e];
-            if constexpr (KIND != AT_BF16) s[e] *= sh;
+            if constexpr (KIND != AT_BF16) s[e] *= apart_v ? shift((float)e1 + fv[e]) : sh;
         }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
@@ -962,7 +1059,7 @@ void image_kind(const ImageArgs& a, int dp, hipStream_t st) {
 }
 
 // workspace of the forward pass, in this order (256-byte aligned pieces)
-struct FwdSpace { size_t kimg, vimg, rec, kpos, part, ml, total; int ns_k, splits; };
+struct FwdSpace { size_t kimg, vimg, rec, kfix, vfix, kpos, part, ml, total; int ns_k, splits; };
 
 FwdSpace fwd_space(const MgnAttn& a, bool few, bool small) {
     FwdSpace s{};
@@ -975,6 +1072,7 @@ FwdSpace fwd_space(const MgnAttn& a, bool few, bool small) {
         s.kimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
         s.vimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
         s.rec = take((size_t)a.kv_heads * s.ns_k * 16);
+        s.kfix = take((size_t)a.kv_heads * s.ns_k * 128); s.vfix = take((size_t)a.kv_heads * s.ns_k * 128);
         s.kpos = take(a.bias_table ? (size_t)(s.ns_k + 1) * a.axes * 128 : 0);
     }
     if (s.splits > 1) {
@@ -1039,12 +1137,13 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
             im.n_job = 2; im.transposed = 1; im.units = 2 * units; im.n_seg = a.n_seg; im.dim = a.dim;
             ImageJob& k = im.job[0];
             k.x = a.k; k.st = a.k_st; k.sh = a.k_sh; k.ptr = a.k_ptr; k.mask = a.key_mask; k.T = a.n_k; k.heads = a.kv_heads; k.n_sub = sp.ns_k;
-            k.R = kimg; k.ex = rec; k.valid = rec + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = kpos; k.axes = a.axes;
+            k.R = kimg; k.ex = rec; k.fix = (int*)(ws + sp.kfix); k.valid = rec + 2; k.pos = bias ? a.k_pos : nullptr; k.pos_out = kpos; k.axes = a.axes;
             ImageJob& v = im.job[1];
-            v = k; v.x = a.v; v.st = a.v_st; v.sh = a.v_sh; v.first_unit = units; v.R = nullptr; v.Tt = vimg; v.ex = rec + 1; v.valid = nullptr; v.pos = nullptr;
+            v = k; v.x = a.v; v.st = a.v_st; v.sh = a.v_sh; v.first_unit = units; v.R = nullptr; v.Tt = vimg; v.ex = rec + 1; v.fix = (int*)(ws + sp.vfix); v.valid = nullptr; v.pos = nullptr;
             mgn_attn_launch_images(kind, dp, &im, stream);
         }
         f.kimg = kimg; f.vimg = vimg; f.rec = (const i32x4*)rec; f.ns_k = sp.ns_k; f.kpos = kpos;
+        f.kfix = (const int*)(ws + sp.kfix); f.vfix = (const int*)(ws + sp.vfix);
         f.waves = small ? 4 : attn_fwd_waves(a);
         f.share = small ? 1 : attn_fwd_share(a);
         const dim3 grid((unsigned)((a.n_q / (small ? 32 : 32 * f.waves) + a.n_seg) * (a.heads / f.share)), (unsigned)sp.splits);

@@ -9,7 +9,7 @@ struct AttnFwd {
     const void *q, *k, *v; long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
     const uint8_t* mask; const int* k_pos;
     const int *q_ptr, *k_ptr; long long n_q, n_k; int n_seg, heads, kv_heads, dim; float c0;
-    const unsigned short *kimg, *vimg; const i32x4* rec; int ns_k; const int* kpos;
+    const unsigned short *kimg, *vimg; const i32x4* rec; int ns_k; const int *kfix, *vfix, *kpos;
     const int* q_pos; const float* table; const int* lut; int n_bucket, reach, axes;
     void* out; long long o_st, o_sh; float *stats, *out32;
     int splits; float *part, *part_ml;

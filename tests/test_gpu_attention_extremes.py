@@ -102,7 +102,7 @@ def test_blocks_of_zero_or_tiny_values(nq, nk, heads, dim, axes, dtype):
 @pytest.mark.parametrize("axes", [0, 2])
 @pytest.mark.parametrize("nq,nk,heads,dim", SHAPES)
 def test_fp32_gradient_rows_beside_larger_ones(nq, nk, heads, dim, axes):
-    for size in (1e4, 1e6):
+    for size in (1e4, 1e6, 1e10):
         q, k, v, g = make(nq, nk, heads, heads, dim, F32)
         g[5::32] *= size
         check_sizes(q, k, v, g, **bias(nq, nk, heads, axes))
@@ -121,9 +121,9 @@ def test_fp16_gradient_rows_beside_larger_ones(apart, dim):
 @pytest.mark.parametrize("axes", [0, 1, 2])
 @pytest.mark.parametrize("nq,nk,heads,dim", SHAPES + [(2, 3000, 4, 32)])
 def test_large_values_that_weigh_nothing(nq, nk, heads, dim, axes):
-    """A value 1e3 .. 1e10 times the others at a weight near e^-60, in a block of its own, first or later."""
+    """A value 1e3 .. 1e10 times the others at a weight near e^-60, in a block of its own and among ordinary rows, first or last."""
     for size in (1e3, 1e6, 1e10):
-        for where in (slice(0, 32), slice(64, 96)):
+        for where in (slice(0, 32), slice(64, 65), slice(nk - 3, nk)):
             q, k, v, g = make(nq, nk, heads, heads, dim, F32)
             q[..., 0] = 4.0
             k[..., 0] = 0.0
@@ -143,6 +143,16 @@ def test_fp16_large_values_that_weigh_nothing(nq, nk, heads, dim):
     check(q, k, v, g)
 
 
+@pytest.mark.parametrize("nq,nk,heads,dim", SHAPES)
+def test_rows_of_every_size_side_by_side(nq, nk, heads, dim):
+    """Neighbouring values and gradients sixteen orders of magnitude apart; keys and queries six."""
+    gen = torch.Generator().manual_seed(4)
+    spread = lambda n, by: (10.0 ** (by * (2 * torch.rand(n, generator=gen) - 1)))[:, None, None].to(DEV)  # noqa: E731
+    q, k, v, g = make(nq, nk, heads, heads, dim, F32)
+    check_sizes(q, k, v * spread(nk, 8), g * spread(nq, 8))
+    check_sizes(q * spread(nq, 3) * 1e-3, k * spread(nk, 3) * 1e-3, v, g)
+
+
 def test_keys_of_little_weight_keep_their_gradients():
     """Keys that a bias of -20 holds down for every query: their own gradients keep their digits."""
     q, k, v, g = make(200, 300)
@@ -150,3 +160,19 @@ def test_keys_of_little_weight_keep_their_gradients():
     kw["q_pos"], kw["k_pos"] = torch.zeros(200, 1, dtype=torch.int32, device=DEV), (torch.arange(300, device=DEV)[:, None] // 60 % 2).int()
     kw["bias_table"] = torch.where(torch.arange(16, device=DEV) == kw["bucket_lut"][2], -20.0, 0.0).expand(4, 16).contiguous()
     check(q, k, v, g, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("axes", [0, 2])
+@pytest.mark.parametrize("nq,nk,heads,dim", SHAPES + [(2, 3000, 4, 32)])
+def test_an_infinite_value_spoils_its_column_only(nq, nk, heads, dim, axes, dtype):
+    from gnn_amd import ops
+    q, k, v, _ = make(nq, nk, heads, heads, dim, dtype)
+    kw = bias(nq, nk, heads, axes)
+    v[37, 1, 3] = 0
+    ref = reference(q, k, v, **kw)
+    v[37, 1, 3] = math.inf
+    o = ops.cross_attention(q, k, v, **kw)
+    assert not torch.isfinite(o[:, 1, 3]).any()
+    o[:, 1, 3] = ref["o"][:, 1, 3].to(o)
+    assert_close(o, ref, "o")
