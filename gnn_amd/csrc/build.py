@@ -14,8 +14,8 @@ OUT = os.path.join(PKG, "libmgn_hip.so")
 # host pass of the compiler does not know the feature and says so; that warning is harmless.
 HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Per-file compiler flags.  The attention kernels take maxima of matrix products only to scale by: without -fno-honor-nans every
-# operand of a maximum is first "quieted" by an instruction of its own.  NaN inputs still come out as NaN (through products, sums
-# and exponentials); no comparison in these files asks for one.
+# operand of a maximum is first "quieted" by an instruction of its own.  The flag leaves a maximum or comparison of a NaN undefined,
+# so nothing in these files decides by one: where a NaN input must come out as NaN (softmax sums, biases) its bits are tested.
 EXTRA_FLAGS = {"mgn_attn_fwd.hip": ["-fno-honor-nans"], "mgn_attn_bwd.hip": ["-fno-honor-nans"]}
 
 

@@ -267,6 +267,18 @@ __device__ __forceinline__ void mask_scores(f32x16& s, int valid, int h) {
         if (!(bits >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -__builtin_inff();
 }
 
+// Where a NaN decides something it is looked for in its bits, which the compiler must not take for a float's: some of these files
+// are compiled without regard for NaN in maxima and comparisons (see build.py), and it turns tests of bits into such comparisons.
+__device__ __forceinline__ unsigned magnitude_bits(float x) {
+    unsigned b = __float_as_uint(x) & 0x7fffffffu;
+    asm("" : "+v"(b));
+    return b;
+}
+__device__ __forceinline__ bool finite_bits(float x) { return magnitude_bits(x) < 0x7f800000u; }
+__device__ __forceinline__ bool zero_bits(float x) { return magnitude_bits(x) == 0; }
+// 1 / l of a softmax's sum; 0 for a row without keys; NaN where a score was NaN or overflowed
+__device__ __forceinline__ float inverse_sum(float l) { return zero_bits(l) ? 0.f : 1.0f / l; }
+
 // Sums of probabilities times values in fp16 formats: kept in units of 2^unit (relative to 2^m, m the running maximum), where unit
 // follows the largest (probability x size of its values) so far, as m follows the scores.  (One large value that weighs nothing
 // must not push all other probabilities into the smallest numbers of fp16.)  A block's probabilities enter times 2^(ev - unit), ev its
@@ -276,6 +288,7 @@ constexpr float SUM_UNIT_LEAST = -200.f;
 __device__ __forceinline__ float raise_max(float& m, float& l, float top) {
     const float mn = fmaxf(m, top), lowered = m - (mn == -__builtin_inff() ? 0.f : mn);
     l *= __builtin_amdgcn_exp2f(lowered);
+    if (mn > 0.f && !finite_bits(mn)) asm("v_mov_b32 %0, 0x7fc00000" : "=v"(l));      // a score overflowed: no softmax
     m = mn;
     return lowered;
 }
@@ -315,7 +328,7 @@ __device__ __forceinline__ float score_factor(float c) { return fminf(fmaxf(c, 0
 
 __device__ __forceinline__ float bias_log2(float b) {          // finite biases stay finite in base 2
     const float v = b * LOG2E;
-    return __builtin_isinf(b) ? v : fminf(fmaxf(v, -F32_MOST), F32_MOST);
+    return finite_bits(b) ? fminf(fmaxf(v, -F32_MOST), F32_MOST) : v;
 }
 
 // ------------------------------------------------------------------------------------------------ copies into LDS

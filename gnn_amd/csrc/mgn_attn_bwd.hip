@@ -758,7 +758,7 @@ extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int6
     if (units > 0) mgn_attn_launch_images(kind, dp, &im, stream);
     AttnBwd b{};
     b.q_ptr = a.q_ptr; b.k_ptr = a.k_ptr; b.n_q = a.n_q; b.n_k = a.n_k; b.n_seg = a.n_seg; b.heads = a.heads; b.kv_heads = a.kv_heads; b.dim = a.dim;
-    b.c0 = a.scale * LOG2E; b.scale = a.scale;
+    b.c0 = std::min(a.scale * LOG2E, F32_MOST); b.scale = a.scale;
     b.fix_q = ints(s.fix_q); b.fix_g = ints(s.fix_g); b.fix_k = ints(s.fix_k); b.fix_v = ints(s.fix_v);
     b.q_r = half(s.q_r); b.g_r = half(s.g_r); b.k_r = half(s.k_r); b.v_r = half(s.v_r);
     b.rec_q = (const i32x4*)rec_q; b.rec_k = (const i32x4*)rec_k; b.rows = (const float*)(ws + s.rows); b.ns_q = s.ns_q; b.ns_k = s.ns_k;

@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, REP == 8 && (bias || KIND == AT_F32) ? 1 : 2) 
             *(f32x4*)(a.part + at * dp + c) = v;
             if (c == 0) { a.part_ml[2 * at] = top; a.part_ml[2 * at + 1] = sum; }
         } else {
-            v *= sum > 0.f ? 1.0f / sum : 0.f;
+            v *= inverse_sum(sum);
             store4<KIND>(a.out, row * a.o_st + head * a.o_sh + c, v);
             if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + c) = v;
             if (c == 0 && a.stats) {

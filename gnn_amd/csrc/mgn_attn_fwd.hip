@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
             }
         }
         dot += __shfl_xor(dot, 32);
-        const float il = l > 0.f ? 1.0f / l : 0.f;
+        const float il = inverse_sum(l);
         if constexpr (KIND == AT_F32) {
             dot *= il;
 #pragma unroll
@@ -63,9 +63,9 @@ __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
         }
         if (h == 0) {
             float* r = job.rows + at * 96;
-            r[i] = l > 0.f ? m : __builtin_inff();            // an empty row, or none: every exp2(score - m) is zero
+            r[i] = zero_bits(l) ? __builtin_inff() : m;       // an empty row, or none: every exp2(score - m) is zero
             r[32 + i] = KIND == AT_F32 ? 1.f : il;
-            r[64 + i] = l > 0.f ? dot : 0.f;
+            r[64 + i] = zero_bits(l) ? 0.f : dot;
         }
     }
     if (job.pos && head == 0 && h == 0)
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
 
     l += __shfl_xor(l, 32);
     if (qi >= g.len) return;
-    const float inv = a.splits > 1 ? 1.f : l > 0.f ? 1.0f / l : 0.f;
+    const float inv = a.splits > 1 ? 1.f : inverse_sum(l);
     const long long prow = ((long long)split * a.heads + head) * a.n_q + row;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
         l[i] += __shfl_xor(l[i], 32);
         const int head = head0 + i;
         if (qi >= g.len) continue;
-        const float inv = a.splits > 1 ? 1.f : l[i] > 0.f ? 1.0f / l[i] : 0.f;
+        const float inv = a.splits > 1 ? 1.f : inverse_sum(l[i]);
         const long long prow = ((long long)split * a.heads + head) * a.n_q + row;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -896,7 +896,7 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
             total = __builtin_fmaf(f, mls[n][1][r], total);
             v += f * *(const f32x4*)&sums[n][r][d];
         }
-        v *= total > 0.f ? 1.0f / total : 0.f;
+        v *= inverse_sum(total);
         const long long out = g.first + g.local * 32 + r;
         store4<KIND>(a.out, out * a.o_st + head * a.o_sh + d, v);
         if (P2) *(f32x4*)(a.out32 + (out * a.heads + head) * a.dim + d) = v;
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(64 * NW) void attn_join_kernel(AttnFwd a) {
     }
     if (row < seg_at(a.q_ptr, 0, a.n_seg, a.n_q) || row >= seg_at(a.q_ptr, a.n_seg, a.n_seg, a.n_q)) return;
     if (t < QUADS && 4 * quad < a.dim) {
-        o *= l > 0.f ? 1.0f / l : 0.f;
+        o *= inverse_sum(l);
         store4<KIND>(a.out, row * a.o_st + head * a.o_sh + 4 * quad, o);
         if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + 4 * quad) = o;
     }
@@ -987,7 +987,7 @@ __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnFwd a) {
         o += f * *(const f32x4*)(a.part + (s * stride + at) * DP + 4 * quad);
     }
     if (4 * quad < a.dim) {
-        o *= l > 0.f ? 1.0f / l : 0.f;
+        o *= inverse_sum(l);
         store4<KIND>(a.out, row * a.o_st + head * a.o_sh + 4 * quad, o);
         if (KIND != AT_F32 && a.out32) *(f32x4*)(a.out32 + (row * a.heads + head) * a.dim + 4 * quad) = o;
     }
@@ -1120,7 +1120,7 @@ extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_
     f.q = a.q; f.q_st = a.q_st; f.q_sh = a.q_sh;
     f.k = a.k; f.k_st = a.k_st; f.k_sh = a.k_sh; f.v = a.v; f.v_st = a.v_st; f.v_sh = a.v_sh; f.mask = a.key_mask; f.k_pos = a.k_pos;
     f.q_ptr = a.q_ptr; f.k_ptr = a.k_ptr; f.n_seg = a.n_seg; f.n_q = a.n_q; f.n_k = a.n_k;
-    f.heads = a.heads; f.kv_heads = a.kv_heads; f.dim = a.dim; f.c0 = a.scale * LOG2E;
+    f.heads = a.heads; f.kv_heads = a.kv_heads; f.dim = a.dim; f.c0 = std::min(a.scale * LOG2E, F32_MOST);
     f.q_pos = a.q_pos; f.table = a.bias_table; f.lut = a.bucket_lut; f.n_bucket = a.n_bucket; f.reach = a.reach; f.axes = a.axes;
     f.out = out; f.o_st = out_st; f.o_sh = out_sh; f.stats = stats; f.out32 = a.dtype == MGN_F32 ? nullptr : out32; f.splits = sp.splits;
     f.zero = a.zero_outside && a.q_ptr;

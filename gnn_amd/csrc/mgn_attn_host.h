@@ -2,6 +2,7 @@
 #pragma once
 #include "mgn_attn.h"
 
+#include <algorithm>
 #include <cmath>
 
 // Arguments of the forward kernels (tiled, few queries, join).

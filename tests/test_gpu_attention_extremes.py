@@ -176,3 +176,50 @@ def test_an_infinite_value_spoils_its_column_only(nq, nk, heads, dim, axes, dtyp
     assert not torch.isfinite(o[:, 1, 3]).any()
     o[:, 1, 3] = ref["o"][:, 1, 3].to(o)
     assert_close(o, ref, "o")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("nq,nk,heads,dim", [(60, 90, 4, 32), (700, 1500, 8, 64), (500, 300, 2, 128)])
+@pytest.mark.parametrize("axes", [0, 1, 2])
+def test_nan_reaches_the_gradients_it_belongs_to(nq, nk, heads, dim, dtype, axes):
+    """A NaN in a query, key, value or bias, and a score that overflows: every gradient that plain arithmetic makes NaN is NaN, the
+    other segment's and the other heads' are finite.  None hides as the zero of a row without keys."""
+    kw = bias(nq, 2 * nk, heads, axes)
+    kw.update(q_ptr=ptr([nq // 2, nq - nq // 2]), k_ptr=ptr([nk, nk]))
+    first, head = slice(0, nq // 2), 1
+    cases = ["query", "key", "value", "overflow"] + ["bias"] * (axes > 0)
+    for case in cases:
+        q, k, v, g = make(nq, 2 * nk, heads, heads, dim, dtype)
+        args = dict(kw)
+        if case == "query":
+            q[3, head, 5] = math.nan
+        elif case == "key":
+            k[40, head, 5] = math.nan
+        elif case == "value":
+            v[40, head, 5] = math.nan
+        elif case == "overflow":
+            args["scale"] = 3e38
+            q[:, [h for h in range(heads) if h != head]] = 0
+        else:
+            args["bias_table"] = kw["bias_table"].clone()
+            args["bias_table"][head] = math.nan
+        got = run(q, k, v, g, **args)
+        seg = (slice(0, nk),) if case in ("query", "key", "value") else (slice(0, 2 * nk),)
+        rows = {"query": slice(3, 4), "key": first, "value": first}.get(case, slice(0, nq))
+        hit = {n: torch.zeros_like(got[n], dtype=torch.bool) for n in got}
+        hit["o"][rows, head] = case != "value"
+        if case == "value":
+            hit["o"][rows, head, 5] = True
+        hit["dq"][rows, head] = True
+        hit["dk"][seg[0], head] = True
+        hit["dv"][seg[0], head] = case != "value"
+        if axes:
+            hit["dtable"][head] = True
+        for name, t in got.items():
+            if name == "dtable":                                    # buckets without a pair of that row stay finite
+                assert torch.isnan(t[head]).any() and torch.isfinite(t[hit[name].logical_not()]).all(), (case, name)
+                continue
+            assert torch.isnan(t[hit[name]]).all(), (case, name)
+            if case == "overflow" and name == "dq":
+                continue                    # the other heads' dq, scale dS K at a scale of 3e38, overflows itself
+            assert torch.isfinite(t[~hit[name]]).all(), (case, name)
