@@ -17,6 +17,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import ops
 from ._lib import H
@@ -104,6 +105,8 @@ def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=N
                     scale: Optional[float] = None):
     """:func:`gnn_amd.ops.cross_attention` with gradients of ``q``, ``k``, ``v`` and ``bias_table`` where they are wanted."""
     grads = (q, k, v, bias_table)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in grads):
+        raise RuntimeError("cross_attention: no forward-mode derivative; an operand carries a tangent, which would be dropped")
     if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or v.requires_grad or (bias_table is not None and bias_table.requires_grad)):
         return ops.cross_attention(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_pos, scale)
     live = _guard_capture(grads)

@@ -82,3 +82,23 @@ def test_null_arguments_and_small_workspaces_are_refused():
         bad = list(ok)
         bad[i] = v
         assert lib.mgn_attn_bwd(ctypes.byref(a), *bad) == -1, i
+
+
+def test_forward_mode_tangents_are_refused():
+    """They would be dropped without a word where no operand requires a gradient."""
+    from torch.autograd import forward_ad
+    from gnn_amd import attention
+    x = torch.zeros(4, 2, 32)
+    with forward_ad.dual_level():
+        for at in range(3):
+            ops = [x, x, x]
+            ops[at] = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="tangent"):
+                attention.cross_attention(*ops)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                attention.cross_attention(*ops)
+        table = forward_ad.make_dual(torch.zeros(2, 4), torch.ones(2, 4))
+        with pytest.raises(RuntimeError, match="tangent"):
+            attention.cross_attention(x, x, x, bias_table=table)
+        with pytest.raises(RuntimeError, match="CUDA/HIP"):                  # no tangent: the ordinary checks
+            attention.cross_attention(x, x, x)
