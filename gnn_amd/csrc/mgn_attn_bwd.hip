@@ -12,6 +12,8 @@
 // that were not rounded to 16 bits: the forward pass keeps them in fp32 where a table is trained (out32).
 #include "mgn_attn_host.h"
 
+#include <atomic>
+
 namespace {
 
 struct AttnBwd {
@@ -664,19 +666,29 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
 }
 
 // Whether the kernel fits the 160 KB of LDS with this much dynamic memory, which beyond 64 KB has to be asked for.  A launch
-// that does not fit is never made: it would end the process's queue, not return an error.
-template <typename K>
-bool lds_fits(K kernel, int dynamic) {
+// that does not fit is never made: it would end the process's queue, not return an error.  The function's limit is set once for each
+// device, to all that is left beside its static memory: it belongs to the function, not to a call, and two threads may be launching.
+template <auto kernel>
+bool lds_fits(int dynamic) {
+    static std::atomic<int> room[64];                          // by device: bytes left, plus one
     if (dynamic == 0) return true;
-    hipFuncAttributes at;
-    if (hipFuncGetAttributes(&at, (const void*)kernel) != hipSuccess || at.sharedSizeBytes + (size_t)dynamic > 160 * 1024) return false;
-    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, dynamic) == hipSuccess;
+    int dev;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+    int left = room[dev].load(std::memory_order_acquire) - 1;
+    if (left < 0) {
+        hipFuncAttributes at;
+        if (hipFuncGetAttributes(&at, (const void*)kernel) != hipSuccess || at.sharedSizeBytes > 160 * 1024) return false;
+        left = 160 * 1024 - (int)at.sharedSizeBytes;
+        if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, left) != hipSuccess) return false;
+        room[dev].store(left + 1, std::memory_order_release);
+    }
+    return dynamic <= left;
 }
 
 template <int KIND, int DP, int BIAS>
 bool bwd_launch(const AttnBwd& b, const BwdSpace& s, hipStream_t st) {
     const int hist = BIAS > 0 ? (b.tpart ? b.n_bucket * 1024 : 0) + entries<BIAS>(b.reach) * (int)sizeof(Entry) : 0;
-    if (!lds_fits(attn_dq_kernel<KIND, DP, BIAS>, hist)) return false;
+    if (!lds_fits<attn_dq_kernel<KIND, DP, BIAS>>(hist)) return false;
     hipLaunchKernelGGL((attn_dq_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.q_tiles * b.heads), (unsigned)s.q_splits), dim3(256), hist, st, b);
     if (b.n_k > 0) hipLaunchKernelGGL((attn_dkv_kernel<KIND, DP, BIAS>), dim3((unsigned)(s.k_tiles * b.kv_heads), (unsigned)s.splits), dim3(256), 0, st, b);
     return true;

@@ -433,3 +433,33 @@ def test_lattice_backward_without_lists(heads, nq, nk):
     """One head has nobody to share a list with; very many segments would take too large a one."""
     q, k, v, g = make(sum(nq), sum(nk), heads=heads, kv_heads=1)
     check(q, k, v, g, q_ptr=ptr(nq), k_ptr=ptr(nk), **bias_args(sum(nq), sum(nk), heads, 2, 50))
+
+
+def test_two_threads_with_different_bucket_counts():
+    """The backward pass asks for LDS by the number of buckets; threads that launch side by side do not set it under each other."""
+    import threading
+    from gnn_amd import ops
+    jobs = []
+    for n_buckets in (4, 64):
+        q, k, v, g = make(140, 100, heads=2, kv_heads=2, dim=64)
+        kw = bias_args(140, 100, 2, 1, 90, n_buckets)
+        st = torch.empty(2, 2, 140, device=DEV)
+        o = ops.cross_attention(q, k, v, stats=st, **kw)
+        jobs.append(lambda q=q, k=k, v=v, g=g, o=o, st=st, kw=kw: ops.cross_attention_bwd(g, q, k, v, o, st, **kw))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def loop(at):
+        try:
+            for _ in range(50):
+                if not all(torch.equal(a, b) for a, b in zip(jobs[at](), want[at])):
+                    bad.append(at)
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+    threads = [threading.Thread(target=loop, args=(at,)) for at in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
