@@ -235,15 +235,16 @@ __device__ __forceinline__ void zero_outside(const int* ptr, int n_seg, long lon
 //   lattice (two or three axes): the whole part of the Euclidean distance, held to reach.  d2 = dx^2 + dy^2 + dz^2 is exact
 //   below 2^24 and only grows beyond, and sqrt(d2 + 1/2) lies at least 1/(4 reach) off every whole number for d2 <= reach^2:
 //   with reach <= 1024 that is 4 units in the last place, so the hardware root (1 ulp) gives the exact whole part.
+//   Differences saturate, so any places on either side are right: one instruction either way.
 template <int AXES>
 __device__ __forceinline__ int place(int qx, int qy, int qz, int kx, int ky, int kz, int reach, float most) {
     if constexpr (AXES == 1) {
-        return min(max(kx - qx, -reach), reach) + reach;
+        return min(max(__builtin_elementwise_sub_sat(kx, qx), -reach), reach) + reach;
     } else {
-        const float dx = (float)(kx - qx), dy = (float)(ky - qy);
+        const float dx = (float)__builtin_elementwise_sub_sat(kx, qx), dy = (float)__builtin_elementwise_sub_sat(ky, qy);
         float d2 = __builtin_fmaf(dx, dx, 0.5f);
         d2 = __builtin_fmaf(dy, dy, d2);
-        if constexpr (AXES == 3) { const float dz = (float)(kz - qz); d2 = __builtin_fmaf(dz, dz, d2); }
+        if constexpr (AXES == 3) { const float dz = (float)__builtin_elementwise_sub_sat(kz, qz); d2 = __builtin_fmaf(dz, dz, d2); }
         return (int)__builtin_amdgcn_sqrtf(fminf(d2, most));
     }
 }

@@ -463,3 +463,26 @@ def test_two_threads_with_different_bucket_counts():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("nq,nk,heads", [(1, 300, 4), (40, 300, 4), (1200, 300, 64), (700, 2000, 4)])
+@pytest.mark.parametrize("axes", [1, 2, 3])
+def test_places_over_the_whole_range_of_int32(nq, nk, heads, axes, monkeypatch):
+    """Differences of places that do not fit 32 bits are far, not near or on the other side."""
+    import attention_reference
+
+    def held(q_pos, k_pos, lut):
+        # squares of such differences do not fit 64 bits: everything beyond +-4096 is beyond the reach of 50 on any axis
+        reach = lut.shape[0] // 2 if axes == 1 else lut.shape[0] - 1
+        d = (k_pos.long()[None] - q_pos.long()[:, None]).clamp(-4096, 4096)
+        if axes == 1:
+            return lut.long()[d[..., 0].clamp(-reach, reach) + reach]
+        return lut.long()[(d * d).sum(-1).double().sqrt().long().clamp(max=reach)]
+    monkeypatch.setattr(attention_reference, "buckets", held)
+    kw = bias_args(nq, nk, heads, axes, 50)
+    gen = torch.Generator().manual_seed(6)
+    ends = torch.tensor([-2 ** 31, -2 ** 31 + 3, -2 ** 30 - 1, -7, 0, 5, 2 ** 30 + 1, 2 ** 31 - 40, 2 ** 31 - 1], dtype=torch.int32)
+    for name, n in (("q_pos", nq), ("k_pos", nk)):
+        kw[name] = ends[torch.randint(0, 9, (n, axes), generator=gen)].to(DEV)
+    q, k, v, g = make(nq, nk, heads, heads)
+    check(q, k, v, g, **kw)
