@@ -719,14 +719,14 @@ bool bwd_kind(const AttnBwd& b, const BwdSpace& s, int dp, int bias, hipStream_t
 }  // namespace
 
 extern "C" int64_t mgn_attn_bwd_workspace_bytes(const MgnAttn* a, int32_t table_grad) {
-    if (attn_check(a, "mgn_attn_bwd_workspace_bytes") != 0) return -1;
+    if (attn_check(a, "mgn_attn_bwd_workspace_bytes", true) != 0) return -1;
     return (int64_t)bwd_space(*a, table_grad && a->bias_table).total;
 }
 
 extern "C" int mgn_attn_bwd(const MgnAttn* ap, const void* g, int64_t g_st, int64_t g_sh, const void* out, int64_t out_st,
                             int64_t out_sh, const float* stats, void* dq, void* dk, void* dv, float* dtable, void* workspace,
                             int64_t workspace_bytes, void* stream) {
-    if (const int rc = attn_check(ap, "mgn_attn_bwd")) return rc;
+    if (const int rc = attn_check(ap, "mgn_attn_bwd", true)) return rc;
     const MgnAttn& a = *ap;
     const char* bad = nullptr;
     const BwdSpace s = bwd_space(a, dtable != nullptr);

@@ -1097,14 +1097,14 @@ int mgn_attn_launch_images(int kind, int dp, const void* args, void* stream) {
 }
 
 extern "C" int64_t mgn_attn_fwd_workspace_bytes(const MgnAttn* a) {
-    if (attn_check(a, "mgn_attn_fwd_workspace_bytes") != 0) return -1;
+    if (attn_check(a, "mgn_attn_fwd_workspace_bytes", false) != 0) return -1;
     const bool few = attn_is_few(*a);
     return (int64_t)fwd_space(*a, few, !few && attn_is_small(*a)).total;
 }
 
 extern "C" int mgn_attn_fwd(const MgnAttn* ap, void* out, int64_t out_st, int64_t out_sh, float* stats, float* out32, void* workspace,
                             int64_t workspace_bytes, void* stream) {
-    if (const int rc = attn_check(ap, "mgn_attn_fwd")) return rc;
+    if (const int rc = attn_check(ap, "mgn_attn_fwd", false)) return rc;
     const MgnAttn& a = *ap;
     if (a.n_q == 0) return 0;
     const bool few = attn_is_few(a), small = !few && attn_is_small(a);

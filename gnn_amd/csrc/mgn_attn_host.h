@@ -32,7 +32,31 @@ inline bool attn_bad_rows(const void* p, int64_t st, int64_t sh, int dtype) {
     return ((uintptr_t)p & 15) || st % per || sh % per || st < 0 || sh < 0;
 }
 
-inline int attn_check(const MgnAttn* a, const char* name) {
+// Few queries per segment: keys and values are read where they lie, once for each query, without images.  64 segments of 8192
+// keys, 8 heads of 128, bf16 (us, images against few): 1 query each 1347 / 376, 4 each 1349 / 652, 8 each 1369 / 1088; 50 000
+// keys, 8 heads over 2 key heads of 128: 4 queries 60 / 53, 8 queries 60 / 73.
+inline bool attn_is_few(const MgnAttn& a) { return a.n_q <= 4 * (int64_t)a.n_seg; }
+
+inline int attn_few_chunk(const MgnAttn& a) {                           // query heads that share a pass over a key head
+    const int rep = a.heads / a.kv_heads;
+    return rep >= 8 ? 8 : rep > 2 ? 4 : rep;
+}
+inline int64_t attn_few_blocks(const MgnAttn& a) {
+    const int rep = a.heads / a.kv_heads, c = attn_few_chunk(a);
+    return a.n_q * a.kv_heads * ((rep + c - 1) / c);
+}
+
+// A launch has fewer than 2^32 threads: 2^24 - 1 workgroups of 256.  What the entry point would launch for these counts, at most (a
+// grid of tiles has one more per segment; images take four (head, subtile) pairs to a workgroup).
+inline bool attn_launches(const MgnAttn& a, bool backward) {
+    const int64_t most = (1 << 24) - 1, q_images = (a.n_q / 32 + a.n_seg) * (int64_t)a.heads, k_images = (a.n_k / 32 + a.n_seg) * (int64_t)a.kv_heads;
+    const int64_t q_tiles = (a.n_q / 128 + a.n_seg) * (int64_t)a.heads, k_tiles = (a.n_k / 128 + a.n_seg) * (int64_t)a.kv_heads;
+    if (backward) return q_images + k_images <= 2 * most && q_tiles <= most && k_tiles <= most;
+    if (attn_is_few(a)) return attn_few_blocks(a) <= most;
+    return k_images <= 2 * most && q_tiles <= most;
+}
+
+inline int attn_check(const MgnAttn* a, const char* name, bool backward) {
     const char* bad = nullptr;
     if (!a) bad = "null arguments";
     else if (a->dtype != MGN_F32 && a->dtype != MGN_BF16 && a->dtype != MGN_F16) bad = "unknown type";
@@ -48,6 +72,7 @@ inline int attn_check(const MgnAttn* a, const char* name) {
         bad = "rows must start on 16-byte borders";
     else if ((a->n_q / 32 + a->n_seg) * (int64_t)a->heads > 0x3fffffffLL || (a->n_k / 32 + a->n_seg) * (int64_t)a->kv_heads > 0x3fffffffLL)
         bad = "too many tokens x heads";
+    else if (!attn_launches(*a, backward)) bad = "too many (segments + tokens / 128) x heads for one launch";
     else if (a->bias_table) {
         if (!a->bucket_lut || (a->n_q > 0 && !a->q_pos) || (a->n_k > 0 && !a->k_pos)) bad = "the bias needs a bucket table and places";
         else if (a->axes < 1 || a->axes > 3) bad = "places have one to three axes";
@@ -69,19 +94,6 @@ inline bool attn_is_small(const MgnAttn& a) {
     return blocks <= 512 && chain <= (a.dtype == MGN_F32 ? 32768 : 16384) && blocks * chain <= 1 << 24;
 }
 
-// Few queries per segment: keys and values are read where they lie, once for each query, without images.  64 segments of 8192
-// keys, 8 heads of 128, bf16 (us, images against few): 1 query each 1347 / 376, 4 each 1349 / 652, 8 each 1369 / 1088; 50 000
-// keys, 8 heads over 2 key heads of 128: 4 queries 60 / 53, 8 queries 60 / 73.
-inline bool attn_is_few(const MgnAttn& a) { return a.n_q <= 4 * (int64_t)a.n_seg; }
-
-inline int attn_few_chunk(const MgnAttn& a) {                           // query heads that share a pass over a key head
-    const int rep = a.heads / a.kv_heads;
-    return rep >= 8 ? 8 : rep > 2 ? 4 : rep;
-}
-inline int attn_few_blocks(const MgnAttn& a) {
-    const int rep = a.heads / a.kv_heads, c = attn_few_chunk(a);
-    return (int)(a.n_q * a.kv_heads * ((rep + c - 1) / c));
-}
 // Split key ranges until there are about four workgroups per compute unit, in pieces of at least 256 keys (within 3 % of two or
 // eight workgroups, and of 128 keys; pieces of 512 keys take 30 instead of 26.5 us for one query over 100 000 keys in fp32).
 inline int attn_few_splits(const MgnAttn& a) {

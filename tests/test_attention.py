@@ -102,3 +102,25 @@ def test_forward_mode_tangents_are_refused():
             attention.cross_attention(x, x, x, bias_table=table)
         with pytest.raises(RuntimeError, match="CUDA/HIP"):                  # no tangent: the ordinary checks
             attention.cross_attention(x, x, x)
+
+
+@pytest.mark.parametrize("fits,kw", [
+    (True, dict(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 20, n_k=1 << 20, heads=15, kv_heads=15)),
+    (False, dict(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 22, n_k=1 << 20, heads=16, kv_heads=16)),
+    (False, dict(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 22, n_k=1 << 20, heads=1024, kv_heads=1024)),
+    (True, dict(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 23, n_k=1 << 20, heads=8, kv_heads=8)),
+    (False, dict(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 23, n_k=1 << 20, heads=16, kv_heads=16)),
+    (False, dict(n_q=1000, n_k=1 << 30, heads=4, kv_heads=4, n_seg=1)),
+    (True, dict(n_q=4, n_k=1 << 30, heads=4, kv_heads=4, n_seg=1)),
+    (True, dict(n_q=1 << 28, n_k=1000, heads=4, kv_heads=4, n_seg=1))])
+def test_counts_that_no_launch_takes_are_refused(fits, kw):
+    """A grid has fewer than 2^32 threads; what does not fit is an error of the host's checks, not of the launch."""
+    from gnn_amd import _lib
+    lib, a = _lib.lib(), args(**kw)
+    assert (lib.mgn_attn_fwd_workspace_bytes(ctypes.byref(a)) >= 0) is fits
+    if not fits:
+        assert b"launch" in lib.mgn_last_error() or b"tokens x heads" in lib.mgn_last_error()
+        assert lib.mgn_attn_fwd(ctypes.byref(a), 4096, 128, 32, None, None, 4096, 1 << 50, None) == -1
+    many = args(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 20, n_k=1 << 20, heads=17, kv_heads=17)
+    assert lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(many), 0) == -1
+    assert lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(args(n_q=1 << 20, n_k=1 << 20, heads=8, kv_heads=8)), 0) > 0
