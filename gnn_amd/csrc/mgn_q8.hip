@@ -110,11 +110,18 @@ __global__ __launch_bounds__(256) void q8_restore_kernel(const signed char* __re
     }
 }
 
+constexpr long long LAUNCH_ROWS = 1 << 26;      // a launch has fewer than 2^32 threads, 32 (or 8) of them for a row
+
 template <int DT, int NCH, int U>
 void rows_vec(bool vec, const void* x, signed char* codes, float* scale, long long rows, int width, int keep, hipStream_t st) {
-    const dim3 grid((unsigned)((rows + 8 * U - 1) / (8 * U)));
-    if (vec) hipLaunchKernelGGL((q8_rows_kernel<DT, NCH, U, true>), grid, dim3(256), 0, st, x, codes, scale, rows, width, keep);
-    else hipLaunchKernelGGL((q8_rows_kernel<DT, NCH, U, false>), grid, dim3(256), 0, st, x, codes, scale, rows, width, keep);
+    for (long long at = 0; at < rows; at += LAUNCH_ROWS) {
+        const long long n = rows - at < LAUNCH_ROWS ? rows - at : LAUNCH_ROWS;
+        const void* xs = (const typename Elem<DT>::T*)x + at * width;
+        signed char* cs = codes + at * width;
+        const dim3 grid((unsigned)((n + 8 * U - 1) / (8 * U)));
+        if (vec) hipLaunchKernelGGL((q8_rows_kernel<DT, NCH, U, true>), grid, dim3(256), 0, st, xs, cs, scale + at, n, width, keep);
+        else hipLaunchKernelGGL((q8_rows_kernel<DT, NCH, U, false>), grid, dim3(256), 0, st, xs, cs, scale + at, n, width, keep);
+    }
 }
 template <int DT>
 void rows_dt(bool vec, const void* x, signed char* codes, float* scale, long long rows, int width, int keep, hipStream_t st) {

@@ -231,3 +231,17 @@ def test_combinations_that_are_refused():
             model.loss(g)
     finally:
         ops.set_matmul_mode(prev)
+
+
+def test_more_rows_than_one_launch_takes():
+    """Rows beyond 2^26 go into a second launch; widths that are not a multiple of four as well."""
+    from gnn_amd import ops
+    rows = (1 << 26) + 1000
+    x = torch.arange(rows, dtype=torch.int32, device="cuda").remainder_(251).to(torch.float16).add_(1).unsqueeze(1)
+    kept = ops.q8_rows(x)
+    assert bool((kept.codes == 127).all())
+    one = (torch.arange(1, 252, dtype=torch.float64, device="cuda") / 127).float()       # rounded once, from 64 bits
+    scales = bool((kept.scale == one[x[:, 0].long() - 1]).all())
+    assert scales
+    back = bool((ops.q8_restore(kept, torch.float16) == x).all())            # 127 fl(m / 127) is within 2^-23 of m, a fp16 number
+    assert back
