@@ -51,10 +51,12 @@ class RelativeBuckets:
 
     def lut(self, device) -> torch.Tensor:
         """Bucket of every place, int32 [2 * reach + 1] on a line, else [reach + 1]."""
-        key = str(device)
-        if key not in self._by_dev:
-            self._by_dev[key] = self.table.to(device)
-        return self._by_dev[key]
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:           # the current one, which may be another at the next call
+            device = torch.device("cuda", torch.cuda.current_device())
+        if device not in self._by_dev:
+            self._by_dev[device] = self.table.to(device)
+        return self._by_dev[device]
 
 
 class _Live:

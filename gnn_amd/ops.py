@@ -124,6 +124,14 @@ def _opt(t: Optional[torch.Tensor], dtype, shape, name: str) -> int:
     return 0 if t is None else _dev(t, dtype, shape, name)
 
 
+def _dev_on(t, dtype, shape, device, name: str) -> int:
+    """:func:`_dev` of a tensor on ``device``: entry points that make the first operand's device current for their launches."""
+    p = _dev(t, dtype, shape, name)
+    if t.device != device:
+        raise RuntimeError(f"{name}: on {t.device}, the other operands on {device}")
+    return p
+
+
 class MlpWeights:
     """Device pointers of one two-Linear MLP; keeps the tensors alive."""
 
@@ -244,7 +252,7 @@ def q8_rows(x, keep_nonzero: bool = False, out: Optional[Q8Rows] = None) -> Q8Ro
         out = Q8Rows(torch.empty(rows, width, dtype=torch.int8, device=x.device), torch.empty(rows, dtype=torch.float32, device=x.device))
     with _on_device(x.device):
         rc = _lib.lib().mgn_q8_rows(_dev(x, x.dtype, None, "x"), _ATT_DTYPES[x.dtype], rows, width, int(bool(keep_nonzero)),
-                                    _dev(out.codes, torch.int8, (rows, width), "codes"), _dev(out.scale, torch.float32, (rows,), "scale"), _stream())
+                                    _dev_on(out.codes, torch.int8, (rows, width), x.device, "codes"), _dev_on(out.scale, torch.float32, (rows,), x.device, "scale"), _stream())
     _lib.check(rc, "mgn_q8_rows")
     return out
 
@@ -257,8 +265,9 @@ def q8_restore(kept: Q8Rows, dtype=torch.float32, out=None) -> torch.Tensor:
     if out is None:
         out = torch.empty(rows, width, dtype=dtype, device=kept.codes.device)
     with _on_device(kept.codes.device):
-        rc = _lib.lib().mgn_q8_restore(_dev(kept.codes, torch.int8, (rows, width), "codes"), _dev(kept.scale, torch.float32, (rows,), "scale"),
-                                       rows, width, _ATT_DTYPES[dtype], _dev(out, dtype, (rows, width), "out"), _stream())
+        dev = kept.codes.device
+        rc = _lib.lib().mgn_q8_restore(_dev(kept.codes, torch.int8, (rows, width), "codes"), _dev_on(kept.scale, torch.float32, (rows,), dev, "scale"),
+                                       rows, width, _ATT_DTYPES[dtype], _dev_on(out, dtype, (rows, width), dev, "out"), _stream())
     _lib.check(rc, "mgn_q8_restore")
     return out
 
@@ -311,10 +320,7 @@ def _att_args(q, k, v, q_ptr, k_ptr, key_mask, bias_table, bucket_lut, q_pos, k_
     vp, vt, vh = _att_rows(v, dtype, dev, nk, kv_heads, dim, "v")
 
     def small(t, dt, shape, name):
-        p = _dev(t, dt, shape, name)
-        if t.device != dev:
-            raise RuntimeError(f"cross_attention: {name} is on {t.device}, the queries on {dev}")
-        return p
+        return _dev_on(t, dt, shape, dev, "cross_attention: " + name)
     n_seg, ptrs = 1, (0, 0)
     if q_ptr is not None or k_ptr is not None:
         if q_ptr is None or k_ptr is None:
@@ -372,8 +378,8 @@ def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=N
         a.zero_outside = 1
     nq, heads, dim = q.shape
     o = _att_rows(out, q.dtype, dev, nq, heads, dim, "out")
-    st = 0 if stats is None else _dev(stats, torch.float32, (2, heads, nq), "stats")
-    o32 = 0 if out32 is None else _dev(out32, torch.float32, (nq, heads, dim), "out32")
+    st = 0 if stats is None else _dev_on(stats, torch.float32, (2, heads, nq), dev, "stats")
+    o32 = 0 if out32 is None else _dev_on(out32, torch.float32, (nq, heads, dim), dev, "out32")
     if dev.index == torch.cuda.current_device() and _event_log is None:
         _att_fwd(a, o, st, o32, dev)
     else:
@@ -406,7 +412,7 @@ def cross_attention_bwd(g, q, k, v, out, stats, q_ptr=None, k_ptr=None, key_mask
     gr = _att_rows(g, q.dtype, q.device, nq, heads, dim, "g")
     o = _att_rows(out, out.dtype if out.dtype is torch.float32 else q.dtype, q.device, nq, heads, dim, "out")
     a.out_f32 = int(out.dtype is torch.float32)
-    st = _dev(stats, torch.float32, (2, heads, nq), "stats")
+    st = _dev_on(stats, torch.float32, (2, heads, nq), q.device, "stats")
     with _on_device(q.device), timed("cross_attention_bwd"):
         p, n, ws = _att_workspace(_lib.lib().mgn_attn_bwd_workspace_bytes(C.byref(a), int(table_grad)), q.device)
         rc = _lib.lib().mgn_attn_bwd(C.byref(a), *gr, *o, st, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),

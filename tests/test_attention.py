@@ -124,3 +124,32 @@ def test_counts_that_no_launch_takes_are_refused(fits, kw):
     many = args(n_seg=1 << 20, q_ptr=64, k_ptr=64, n_q=1 << 20, n_k=1 << 20, heads=17, kv_heads=17)
     assert lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(many), 0) == -1
     assert lib.mgn_attn_bwd_workspace_bytes(ctypes.byref(args(n_q=1 << 20, n_k=1 << 20, heads=8, kv_heads=8)), 0) > 0
+
+
+def test_operands_on_another_device_are_refused(monkeypatch):
+    """Checked by the tensors' attributes alone: stand-ins for tensors of two cards."""
+    from gnn_amd import ops
+    from gnn_amd.attention import RelativeBuckets
+
+    class Stub:
+        is_cuda, dtype, shape = True, torch.float32, (2, 3)
+
+        def __init__(self, at):
+            self.device = torch.device("cuda", at)
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 4096
+    assert ops._dev_on(Stub(0), torch.float32, (2, 3), torch.device("cuda", 0), "stats") == 4096
+    with pytest.raises(RuntimeError, match="stats: on cuda:1"):
+        ops._dev_on(Stub(1), torch.float32, (2, 3), torch.device("cuda", 0), "stats")
+    # "cuda" is the current card of each call
+    seen = []
+    b = RelativeBuckets(4, 3, 2)
+    b.table = type("T", (), {"to": lambda self, d: seen.append(d) or d})()
+    for at in (0, 1, 0):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda at=at: at)
+        assert b.lut("cuda") == torch.device("cuda", at)
+    assert seen == [torch.device("cuda", 0), torch.device("cuda", 1)]
