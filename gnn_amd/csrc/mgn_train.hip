@@ -550,7 +550,8 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
 // ------------------------------------------------------------------------ linear backward, layer input in 8 bits
 // A[r] = scale[r] * codes[r].  With scale = 2^e * m, 1 <= m < 2: the rows of G are multiplied by m before they are split, and the
 // codes times 2^e are ONE exact bf16 plane (8 significant bits), so dW = (m G)^T (2^e codes) takes three partial products
-// instead of six and a quarter of the staging; GA = (m G) W is divided by m where it leaves (two more roundings, 2^-24 each).
+// instead of six and a quarter of the staging; GA = (m G) W is multiplied with 1 / m where it leaves (three more roundings of
+// 2^-24 each: m G, 1 / m and this product).
 //
 // Streams 4 (G) + 1 (codes) bytes in and 4 (GA) out per element.  Tiles of 64 rows, eight waves, two per SIMD: wave w takes
 // column block w & 3 of both products, of GA the rows 32 (w >> 2) .., of dW the column blocks 2 (w >> 2) and + 1 -- so each keeps
@@ -658,7 +659,8 @@ __global__ __launch_bounds__(2 * NT, 1) void train_linear_bwd_q8_kernel(LinBwdQ8
                 const int row = srow + 16 * it;
                 if (row < nvalid) {
                     f32x4 val = *(const f32x4*)(Ot + toff(row, sq, H / 4));
-                    const float inv = __builtin_amdgcn_rcpf(by[it]);
+                    const float near = __builtin_amdgcn_rcpf(by[it]);        // off by up to 2^-23; one step of Newton's iteration: 2^-24
+                    const float inv = __builtin_fmaf(__builtin_fmaf(-by[it], near, 1.f), near, near);
                     const int c = codes[it];
                     const bool on[4] = {(signed char)c > 0, (signed char)(c >> 8) > 0, (signed char)(c >> 16) > 0, (c >> 24) > 0};
 #pragma unroll

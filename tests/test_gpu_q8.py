@@ -245,3 +245,21 @@ def test_more_rows_than_one_launch_takes():
     assert scales
     back = bool((ops.q8_restore(kept, torch.float16) == x).all())            # 127 fl(m / 127) is within 2^-23 of m, a fp16 number
     assert back
+
+
+@pytest.mark.parametrize("rows", [64, 777])
+def test_input_gradient_keeps_its_digits_under_the_row_scales(rows):
+    """GA does not depend on the layer input, but is formed with the rows' scales and freed of them again.  Bound: 8 steps of 16
+    products, 6 partial products each, so 48 sums in fp32 that may each drop up to 2^-23 of what they hold; the terms left out of
+    the three-term splits, less than 2^-23; m G, 1 / m and their product, 3 roundings of 2^-24; all of the sum of magnitudes."""
+    from gnn_amd import ops
+    gen = torch.Generator().manual_seed(rows)
+    a = torch.randn(rows, 128, generator=gen) * torch.exp(4 * torch.randn(rows, 1, generator=gen))
+    a[:, 0] = a.abs().amax(1) * (1 + torch.rand(rows, generator=gen))             # scales all over [1, 2) 2^e
+    g, w = torch.randn(rows, 128, generator=gen).to(DEV), torch.randn(128, 128, generator=gen).to(DEV)
+    scratch = torch.empty(ops.train_scratch_bytes(), dtype=torch.uint8, device=DEV)
+    ga, dw = torch.empty_like(g), torch.empty_like(w)
+    ops.train_linear_bwd(g, scratch, a=ops.q8_rows(a.to(DEV)), w=w, ga=ga, dw=dw)
+    g64, w64 = g.double().cpu(), w.double().cpu()
+    tol = (48 + 1 + 1.5) * 2.0 ** -23 * (g64.abs() @ w64.abs())
+    assert ((ga.double().cpu() - g64 @ w64).abs() <= tol).all()
