@@ -60,22 +60,40 @@ class RelativeBuckets:
 
 
 class _Live:
-    """Stands for an eager autograd graph of this module that is still alive, with the leaves it accumulates into."""
+    """Stands for an eager autograd graph of this module that is still alive, with the roots that lead to the leaves it
+    accumulates into: leaves themselves, or the nodes that made an operand (the graph holds them anyway)."""
     alive: "weakref.WeakSet" = weakref.WeakSet()
 
-    def __init__(self, leaves):
-        self.leaves = leaves
+    def __init__(self, roots):
+        self.roots = roots
         _Live.alive.add(self)
+
+
+def _leaves(roots) -> set:
+    """Identities of the leaves that gradients reach from ``roots``."""
+    found, seen, todo = set(), set(), list(roots)
+    while todo:
+        at = todo.pop()
+        if isinstance(at, torch.Tensor):
+            found.add(id(at))
+        elif at not in seen:
+            seen.add(at)
+            leaf = getattr(at, "variable", None)              # the node that accumulates into a leaf
+            if leaf is not None:
+                found.add(id(leaf))
+            todo += [n for n, _ in at.next_functions if n is not None]
+    return found
 
 
 def _guard_capture(tensors):
     """Leaves of a graph that is recorded into a HIP graph must not be held by an eager graph: their gradients would be
     accumulated on the eager graph's stream, which is not being captured, and the process would end."""
-    leaves = tuple(id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf)
+    roots = tuple(t if t.grad_fn is None else t.grad_fn for t in tensors if t is not None and t.requires_grad)
     if not torch.cuda.is_current_stream_capturing():
-        return _Live(leaves)
+        return _Live(roots)
+    mine = _leaves(roots)
     for other in list(_Live.alive):
-        if set(other.leaves) & set(leaves):
+        if _leaves(other.roots) & mine:
             raise RuntimeError("cross_attention: an eager result of the same leaves is still alive while a HIP graph is being captured; "
                                "delete it first (its gradients would be accumulated outside the capture)")
     return None

@@ -153,3 +153,21 @@ def test_operands_on_another_device_are_refused(monkeypatch):
         monkeypatch.setattr(torch.cuda, "current_device", lambda at=at: at)
         assert b.lut("cuda") == torch.device("cuda", at)
     assert seen == [torch.device("cuda", 0), torch.device("cuda", 1)]
+
+
+def test_capture_guard_looks_behind_operands_to_their_leaves(monkeypatch):
+    """An operand is seldom a leaf: a projection's weights are, and an eager graph that holds them is found through it."""
+    from gnn_amd import attention
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    w, other = torch.randn(8, 8, requires_grad=True), torch.randn(8, 8, requires_grad=True)
+    x = torch.randn(4, 8)
+    live = attention._guard_capture((x @ w, (x @ w).relu(), None, x))
+    assert live is not None
+    capturing[0] = True
+    for t in (w, x @ w, (x @ w).view(2, 2, 8), (x @ other) * (x @ w)):
+        with pytest.raises(RuntimeError, match="still alive"):
+            attention._guard_capture((t,))
+    assert attention._guard_capture((x @ other, x)) is None
+    del live
+    assert attention._guard_capture((x @ w,)) is None
