@@ -124,6 +124,8 @@ class _CrossAttention(torch.autograd.Function):
 def cross_attention(q, k, v, q_ptr=None, k_ptr=None, key_mask=None, bias_table=None, bucket_lut=None, q_pos=None, k_pos=None,
                     scale: Optional[float] = None):
     """:func:`gnn_amd.ops.cross_attention` with gradients of ``q``, ``k``, ``v`` and ``bias_table`` where they are wanted."""
+    if not all(isinstance(t, torch.Tensor) and t.dim() == 3 for t in (q, k, v)):
+        raise RuntimeError("cross_attention: q [queries, heads, dim] and k, v [keys, kv_heads, dim] tensors")
     grads = (q, k, v, bias_table)
     if getattr(forward_ad, "_current_level", 0) >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in grads):
         raise RuntimeError("cross_attention: no forward-mode derivative; an operand carries a tangent, which would be dropped")

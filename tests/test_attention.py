@@ -171,3 +171,15 @@ def test_capture_guard_looks_behind_operands_to_their_leaves(monkeypatch):
     assert attention._guard_capture((x @ other, x)) is None
     del live
     assert attention._guard_capture((x @ w,)) is None
+
+
+def test_operands_that_are_no_rows_of_heads_are_refused():
+    """Also where a gradient is wanted, in front of anything that looks at their shape."""
+    from gnn_amd import attention
+    x = torch.zeros(4, 2, 32)
+    for bad in (None, 3.0, torch.zeros(4, 64), torch.zeros(4, 64, requires_grad=True), torch.zeros(1, 4, 2, 32, requires_grad=True)):
+        for at in range(3):
+            ops = [x, x, x]
+            ops[at] = bad
+            with pytest.raises(RuntimeError, match="cross_attention: q"):
+                attention.cross_attention(*ops)
