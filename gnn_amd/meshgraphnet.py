@@ -371,11 +371,12 @@ class EncodeProcessDecodeMultiScale(nn.Module):
         """Places and segments of the attention readout; kept with the coarse graph they belong to."""
         if halo is not None:
             raise NotImplementedError('coarse_readout="attention": not on a partitioned mesh')
-        plan = cg.__dict__.get("readout_plan")
-        if plan is None:
+        of = (self.readout.reach, self.readout.num_buckets)         # what the plan depends on beside the mesh
+        kept = cg.__dict__.get("readout_plan")
+        if kept is None or kept[0] != of:
             sizes = tuple(int(b) for b in graph["batch_sizes"]) if "batch_sizes" in graph else None
-            plan = cg.__dict__["readout_plan"] = self.readout.plan(mesh_pos, cg.first, sizes, cg.block_sizes)
-        return plan
+            kept = cg.__dict__["readout_plan"] = (of, self.readout.plan(mesh_pos, cg.first, sizes, cg.block_sizes))
+        return kept[1]
 
     def captured_parts(self, graph, training: bool = False) -> list:
         """What launches recorded for ``graph`` go on reading: its topology, coarse graph, readout plan and the workspaces.  The

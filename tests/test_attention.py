@@ -183,3 +183,18 @@ def test_operands_that_are_no_rows_of_heads_are_refused():
             ops[at] = bad
             with pytest.raises(RuntimeError, match="cross_attention: q"):
                 attention.cross_attention(*ops)
+
+
+def test_readout_plan_follows_the_readouts_reach():
+    """Kept with the coarse graph, but a readout of another reach or with other buckets gets its own."""
+    from gnn_amd.meshgraphnet import EncodeProcessDecodeMultiScale
+    model = EncodeProcessDecodeMultiScale(10, 7, node_out_dim=3, sample_ratio=0.5, coarse_readout="attention")
+    pos = torch.rand(20, 2, generator=torch.Generator().manual_seed(1))
+    cg = type("Coarse", (), {})()
+    cg.first, cg.block_sizes = torch.arange(0, 20, 2), None
+    first = model._readout_plan(cg, pos, None, {})
+    assert model._readout_plan(cg, pos, None, {}) is first and int(first["q_pos"].max()) == 128
+    from gnn_amd.attention import CrossScaleReadout
+    model.readout = CrossScaleReadout(reach=16, num_buckets=8)
+    second = model._readout_plan(cg, pos, None, {})
+    assert int(second["q_pos"].max()) == 16 and second["bucket_lut"].shape[0] == 17
