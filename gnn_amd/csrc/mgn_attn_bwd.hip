@@ -37,11 +37,12 @@ constexpr int LISTED = 4;                              // a bias whose buckets a
 
 // Sums in units of 2^unit that follow what is added to them (fp16 formats).  An addend x of a block with exponent ex enters as
 // x 2^(ex - unit); one that would pass UNIT_OVER raises the unit to where the largest lies below 2^UNIT_TOP, so that a few that
-// grow slowly do not raise it every time and the smallest numbers of fp16 stay 2^-36 of it away.
-constexpr int UNIT_LEAST = -126, UNIT_TOP = 12;
+// grow slowly do not raise it every time and the smallest numbers of fp16 stay 2^-36 of it away.  The factor is one power of two, so
+// a block of large exponent raises the unit as well; the first one does.
+constexpr int UNIT_LEAST = -1000, UNIT_TOP = 12, FACTOR_MOST = 126;
 constexpr float UNIT_OVER = 0x1p15f;
 __device__ __forceinline__ int raised_unit(int unit, float most, int ex) {
-    return max(unit, (int)((__float_as_uint(most) >> 23) & 0xff) - 126 + ex - UNIT_TOP);
+    return max(max(unit, ex - FACTOR_MOST), (int)((__float_as_uint(most) >> 23) & 0xff) - 126 + ex - UNIT_TOP);
 }
 __device__ __forceinline__ float largest16(const f32x16& s) {
     float m = fmaxf(fabsf(s[0]), fabsf(s[1]));
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
         if (a.tpart)
             for (int r = t; r < a.n_bucket * 256; r += 256) hist[r] = 0.f;
     }
-    // Exponent of this query's sums in the second product: dS enters scaled by it and is held below 2^UNIT_MOST.  It follows the dS
+    // Exponent of this query's sums in the second product: dS enters scaled by it and is held below UNIT_OVER.  It follows the dS
     // that actually come (their sizes differ by many orders between queries, and with the keys' weights), as the maximum of a
     // softmax does: when one does not fit, it rises and the sums so far are scaled down.
     int unit = UNIT_LEAST;
@@ -288,14 +289,14 @@ __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 
             if (block_apart(r.v[0])) apply_fix(s, row_fix(a.fix_k + (ksub + sub) * 32, h));
             const float most = largest16(s);
             const int ek = block_exp(r.v[0]);
-            float f = unit_factor(ek - unit);
-            if (__any(most * f > UNIT_OVER)) {                     // the two halves of a query's keys only meet here
+            float f = ldexpf(1.f, ek - unit);
+            if (__any(ek - unit > FACTOR_MOST || most * f > UNIT_OVER)) {                     // the two halves of a query's keys only meet here
                 const int to = raised_unit(unit, fmaxf(most, __shfl_xor(most, 32)), ek);
                 const float by = unit_factor(unit - to);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) scale16<DP == 128>(dq[n], by);
                 unit = to;
-                f = unit_factor(ek - unit);
+                f = ldexpf(1.f, ek - unit);
             }
 #pragma unroll
             for (int n = 0; n < 16; ++n) s[n] *= f;
@@ -517,8 +518,8 @@ constexpr int PIECES = SUB * 2 / 1024;
             }
             const float most_p = largest16(p), most_s = largest16(s);
             const int eq = block_exp(r.v[0]), eg = block_exp(r.v[1]);
-            float fp = unit_factor(eg - unit_p), fs = unit_factor(eq - unit_s);
-            if (__any(fmaxf(most_p * fp, most_s * fs) > UNIT_OVER)) {      // the two halves of a key's queries only meet here
+            float fp = ldexpf(1.f, eg - unit_p), fs = ldexpf(1.f, eq - unit_s);
+            if (__any(max(eg - unit_p, eq - unit_s) > FACTOR_MOST || fmaxf(most_p * fp, most_s * fs) > UNIT_OVER)) {      // the two halves of a key's queries only meet here
                 const int to_p = raised_unit(unit_p, fmaxf(most_p, __shfl_xor(most_p, 32)), eg);
                 const int to_s = raised_unit(unit_s, fmaxf(most_s, __shfl_xor(most_s, 32)), eq);
                 const float by_p = unit_factor(unit_p - to_p), by_s = unit_factor(unit_s - to_s);
@@ -528,7 +529,7 @@ constexpr int PIECES = SUB * 2 / 1024;
                     scale16<DP == 128>(dk[n], by_s);
                 }
                 unit_p = to_p; unit_s = to_s;
-                fp = unit_factor(eg - unit_p); fs = unit_factor(eq - unit_s);
+                fp = ldexpf(1.f, eg - unit_p); fs = ldexpf(1.f, eq - unit_s);
             }
 #pragma unroll
             for (int n = 0; n < 16; ++n) { p[n] *= fp; s[n] *= fs; }
@@ -648,7 +649,7 @@ BwdSpace bwd_space(const MgnAttn& a, bool table_grad) {
     const size_t qi = (size_t)a.heads * s.ns_q * pl * 64 * dp, ki = (size_t)a.kv_heads * s.ns_k * pl * 64 * dp;
     s.q_r = take(qi); s.g_r = take(qi); s.k_r = take(ki); s.v_r = take(ki);
     s.rec_q = take((size_t)a.heads * s.ns_q * 16); s.rec_k = take((size_t)a.kv_heads * s.ns_k * 16);
-    const size_t qf = (size_t)a.heads * s.ns_q * 128, kf = (size_t)a.kv_heads * s.ns_k * 128;
+    const size_t row = a.dtype == MGN_BF16 ? 0 : 128, qf = (size_t)a.heads * s.ns_q * row, kf = (size_t)a.kv_heads * s.ns_k * row;
     s.fix_q = take(qf); s.fix_g = take(qf); s.fix_k = take(kf); s.fix_v = take(kf);
     s.rows = take((size_t)a.heads * s.ns_q * 96 * 4);
     // Buckets listed once where a place is dear (a lattice), at least two heads share it and there are subtiles enough to pay for the

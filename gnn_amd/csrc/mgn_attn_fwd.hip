@@ -1074,7 +1074,8 @@ FwdSpace fwd_space(const MgnAttn& a, bool few, bool small) {
         s.kimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
         s.vimg = take((size_t)a.kv_heads * s.ns_k * pl * 64 * dp);
         s.rec = take((size_t)a.kv_heads * s.ns_k * 16);
-        s.kfix = take((size_t)a.kv_heads * s.ns_k * 128); s.vfix = take((size_t)a.kv_heads * s.ns_k * 128);
+        const size_t fix = a.dtype == MGN_BF16 ? 0 : (size_t)a.kv_heads * s.ns_k * 128;
+        s.kfix = take(fix); s.vfix = take(fix);
         s.kpos = take(a.bias_table ? (size_t)(s.ns_k + 1) * a.axes * 128 : 0);
     }
     if (s.splits > 1) {

@@ -223,3 +223,25 @@ def test_nan_reaches_the_gradients_it_belongs_to(nq, nk, heads, dim, dtype, axes
             if case == "overflow" and name == "dq":
                 continue                    # the other heads' dq, scale dS K at a scale of 3e38, overflows itself
             assert torch.isfinite(t[~hit[name]]).all(), (case, name)
+
+
+def test_tiny_gradients_and_weights_beside_large_operands():
+    """Factors that do not fit one power of two: gradients of 1e-34 that meet keys (queries) of 1e9, and keys at a weight of e^-80 whose
+    queries have gradients of 1e30."""
+    q, k, v, g = make(200, 300)
+    check(q * 1e-9, k * 1e9, v, g * 1e-34)
+    check(q * 1e9, k * 1e-9, v, g * 1e-34)
+    check(q, k, v, g * 1e-36)
+    kw = bias_args(200, 300, 4, 1, 1)
+    kw["q_pos"], kw["k_pos"] = torch.zeros(200, 1, dtype=torch.int32, device=DEV), (torch.arange(300, device=DEV)[:, None] // 60 % 2).int()
+    kw["bias_table"] = torch.where(torch.arange(16, device=DEV) == kw["bucket_lut"][2], -80.0, 0.0).expand(4, 16).contiguous()
+    for q, k, v, g in ((q, k, v, g * 1e30), (q * 1e9, k * 1e-9, v * 1e-15, g * 1e30)):
+        got, ref = run(q, k, v, g, **kw), reference(q, k, v, g, **kw)
+        # e^-80 is 2^-115.4, and a weight below 2^-126 is zero: the exponential gives no smaller number.  Each pair may lose that much.
+        for h in range(4):
+            qh, vh, gh = (t[:, h].double().cpu().abs() for t in (q, v, g))
+            ref["dv_tol"][:, h] += 2.0 ** -126 * gh.sum(0)
+            d_p = gh @ vh.T + (gh * ref["o"][:, h].abs()).sum(1, keepdim=True)
+            ref["dk_tol"][:, h] += 2.0 ** -126 * 32 ** -0.5 * (d_p.T @ qh)
+        for name, t in got.items():
+            assert_close(t, ref, name)
