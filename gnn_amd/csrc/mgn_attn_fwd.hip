@@ -723,8 +723,27 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
         u32x4 kh[NC], kl[NC], vh[2][NB], vl[2][NB];
         int ek = 0, e1 = 0, fk = 0;                             // exponents of the keys and values; what row j's own differs by
         bool apart_k = false, apart_v = false;
+        int kx[BIAS ? 16 : 1], ky[BIAS > 1 ? 16 : 1], kz[BIAS > 2 ? 16 : 1];
+        auto places = [&] {                                     // of this lane's keys
+            if constexpr (BIAS > 0)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int* p = a.k_pos + (k0 + min(32 * sub + 8 * (e >> 2) + 4 * h + (e & 3), klen - 1)) * a.axes;
+                    kx[e] = p[0]; ky[BIAS > 1 ? e : 0] = BIAS > 1 ? p[1] : 0; kz[BIAS > 2 ? e : 0] = BIAS > 2 ? p[2] : 0;
+                }
+        };
         float fv[16];                                           // what the values' rows of this lane's scores have of their own
         {
+            if constexpr (DP == 32) places();                   // requested with the rows; wider heads have no registers for them
+            float v[NC][8];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 16 * c + 8 * h;
+                if (use && d < a.dim) load8<KIND>(a.k, (k0 + key) * a.k_st + kvh * a.k_sh + d, v[c]);
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+            }
             float x[2][NB][8];                                  // values: column 32 b + j of keys 16 kc + 4 h + (0 .. 3, 8 .. 11)
 #pragma unroll
             for (int kc = 0; kc < 2; ++kc)
@@ -736,68 +755,76 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
                         x[kc][b][e] = (valid >> n & 1) && d < a.dim ? load1<KIND>(a.v, (k0 + 32 * sub + n) * a.v_st + kvh * a.v_sh + d) : 0.f;
                     }
             if constexpr (KIND != AT_BF16) {
-                // a lane has a column of the rows: their sizes meet in ballots, one per row of either half of the wave
-                float most[16], top = 0.f;
+                // Sizes of the key rows (a lane has half a row) and of the value rows (a lane has a column: 16 elements of each half's rows)
+                float most[16], topk = 0.f, topv = 0.f, low = F32_MOST;
                 auto sizes = [&](bool finite) {
-                    top = 0.f;
+                    topk = finite ? finite_top<NC>(v) : topk;
+                    topv = 0.f;
 #pragma unroll
                     for (int n = 0; n < 16; ++n) {
                         most[n] = 0.f;
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
                             const float y = fabsf(x[n >> 3][b][n & 7]);
-                            most[n] = fmaxf(most[n], finite && __float_as_uint(y) >= 0x7f800000u ? 0.f : y);
+                            most[n] = fmaxf(most[n], finite && !finite_bits(y) ? 0.f : y);
                         }
-                        top = fmaxf(top, most[n]);
+                        topv = fmaxf(topv, most[n]);
                     }
                 };
-                sizes(false);
-                if (__any(__float_as_uint(top) >= 0x7f800000u)) sizes(true);
-                top = wave_max(top);
-                e1 = scale_exp<KIND>(top);
-                const float least = top * (1.f / (1 << APART)), bv = pow2i(-e1);
+                float mk, mv;                                   // of the block
+                auto meet = [&] {
+                    topk = fmaxf(topk, __shfl_xor(topk, 32));
+                    mk = topk; mv = fmaxf(topv, __shfl_xor(topv, 32));
 #pragma unroll
-                for (int n = 0; n < 16; ++n) {
-                    const unsigned long long near = __ballot(most[n] >= least), some = __ballot(most[n] > 0.f);
-                    apart_v |= ((unsigned)near == 0 && (unsigned)some != 0) || (near >> 32 == 0 && some >> 32 != 0);
-                }
-                if (apart_v) {
+                    for (int o2 = 16; o2 > 0; o2 >>= 1) { mk = fmaxf(mk, __shfl_xor(mk, o2)); mv = fmaxf(mv, __shfl_xor(mv, o2)); }
+                    ek = scale_exp<KIND>(mk); e1 = scale_exp<KIND>(mv);
+                };
+                constexpr float FAR = 1.f / (1 << APART);
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) topk = fmaxf(topk, fabsf(v[c][e]));
+                sizes(false);
+                meet();
+                // None of the value rows is far below the others if in either half of the wave one lane has no small element (masked
+                // rows aside).  Where that does not clear them, or there is an infinity, the rows are looked at one by one.
+                if (valid == 0xffffffffu)
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) low = fminf(low, most[n]);
+                else
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) low = valid >> (4 * h) >> (8 * (n >> 2) + (n & 3)) & 1 ? fminf(low, most[n]) : low;
+                const unsigned long long clear = __ballot(low >= mv * FAR);
+                if ((unsigned)clear == 0 || clear >> 32 == 0 || __any((topk > 0.f && topk < mk * FAR) || !finite_bits(fmaxf(mk, mv)))) {
+                    sizes(true);
+                    meet();
+                    const bool far = topk > 0.f && topk < mk * FAR;
+                    apart_k = __any(far);
+                    if (far) fk = scale_exp<KIND>(topk) - ek;
 #pragma unroll
                     for (int n = 0; n < 16; ++n) {
 #pragma unroll
                         for (int o2 = 16; o2 > 0; o2 >>= 1) most[n] = fmaxf(most[n], __shfl_xor(most[n], o2));
-                        const int own = most[n] > 0.f && most[n] < least ? scale_exp<KIND>(most[n]) : e1;
+                        const int own = most[n] > 0.f && most[n] < mv * FAR ? scale_exp<KIND>(most[n]) : e1;
                         fv[n] = (float)(own - e1);
+                        apart_v |= __any(own != e1);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) x[n >> 3][b][n & 7] *= pow2i(-own);
+                        for (int b = 0; b < NB; ++b) x[n >> 3][b][n & 7] = ldexpf(x[n >> 3][b][n & 7], e1 - own);
                     }
-                } else {
 #pragma unroll
-                    for (int n = 0; n < 16; ++n)
+                    for (int c = 0; c < NC; ++c)
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) x[n >> 3][b][n & 7] *= bv;
+                        for (int e = 0; e < 8; ++e) v[c][e] = ldexpf(v[c][e], -fk);
                 }
-            }
-            float v[NC][8];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = 16 * c + 8 * h;
-                if (use && d < a.dim) load8<KIND>(a.k, (k0 + key) * a.k_st + kvh * a.k_sh + d, v[c]);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
-            }
-            if constexpr (KIND != AT_BF16) {
-                const float top = row_top<NC>(v), most = wave_max(top);
-                ek = scale_exp<KIND>(most);
-                const bool far = top > 0.f && top < most * (1.f / (1 << APART));
-                apart_k = __any(far);
-                if (far) fk = scale_exp<KIND>(top) - ek;
-                const float bk = pow2i(-ek - fk);
+                const float bk = pow2i(-ek), bv = pow2i(-e1);
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[c][e] *= bk;
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) x[n >> 3][b][n & 7] *= bv;
             }
 #pragma unroll
             for (int c = 0; c < NC; ++c) pack8<KIND>(v[c], kh[c], kl[c]);
@@ -819,15 +846,14 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
         if (apart_k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = ldexpf(s[e], __shfl(fk, 8 * (e >> 2) + 4 * h + (e & 3)));
+        if constexpr (DP != 32) places();
         float top = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int n = 8 * (e >> 2) + 4 * h + (e & 3);
             float x = s[e] * c;
-            if constexpr (BIAS > 0) {
-                const int* p = a.k_pos + (k0 + min(32 * sub + n, klen - 1)) * a.axes;
-                x = __builtin_fmaf(s[e], c, lutb[place<BIAS>(qx, qy, qz, p[0], BIAS > 1 ? p[1] : 0, BIAS > 2 ? p[2] : 0, a.reach, most)]);
-            }
+            if constexpr (BIAS > 0)
+                x = __builtin_fmaf(s[e], c, lutb[place<BIAS>(qx, qy, qz, kx[e], ky[BIAS > 1 ? e : 0], kz[BIAS > 2 ? e : 0], a.reach, most)]);
             s[e] = valid >> n & 1 ? x : -__builtin_inff();
             top = fmaxf(top, s[e]);
         }
@@ -855,7 +881,14 @@ __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 
         for (int e = 0; e < 16; ++e) {
             s[e] = __builtin_amdgcn_exp2f(s[e] - base);
             l += s[e];
-            if constexpr (KIND != AT_BF16) s[e] *= apart_v ? shift((float)e1 + fv[e]) : sh;
+        }
+        if constexpr (KIND != AT_BF16) {
+            if (apart_v)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] *= shift((float)e1 + fv[e]);
+            else
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] *= sh;
         }
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
