@@ -418,7 +418,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
 // plane, 370 us in fp32 and 225 us in fp16 (a head at a time 380 and 266).
 constexpr int HEADS = 2;
 template <int KIND, int DP, int BIAS, bool P2>
-__global__ __launch_bounds__(256, 2) void attn_fwd_heads_kernel(AttnFwd a) {
+__global__ __launch_bounds__(256, DP == 32 && KIND != AT_F32 ? 3 : 2) void attn_fwd_heads_kernel(AttnFwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP;
     constexpr int SHIFT = KIND == AT_BF16 ? 0 : 15 - OVER, PIECES = SUB * 2 / 1024;
     constexpr int LUTS = ATT_MAX_REACH + 4;
