@@ -16,9 +16,14 @@
 // A segment's first subtile in an image is floor(first token / 32) + segment: no two segments share a subtile, and no table
 // of tile offsets is needed.  Rows past a segment's end and masked keys are zeros.
 //
-// Number formats.  bf16: operands as they are.  fp16: one plane, scaled per subtile by a power of two.  fp32: two fp16 planes
+// Number formats.  bf16: operands as they are.  fp16: one plane, scaled by a power of two as the next.  fp32: two fp16 planes
 // x = 2^e (h1 + h2) with the subtile's own e, or the row's where the subtile's rows are far apart in size (residual 2^-22 of the
-// value, 2^-25 of the row's largest magnitude), three partial products per product.  The exponents go into constants that each product is multiplied with anyway.
+// value, 2^-25 of the row's largest magnitude), three partial products per product.  The exponents go into constants that each
+// product is multiplied with anyway.  Probabilities and dS enter the second products in units that follow their own size: in two
+// planes (fp32: what is left is 2^-36 of the largest addend of a sum) or, in the 16-bit types, in one, rounded to half a step of the
+// type as the results are (errors of 2.4e-3 where results rounded once have 1.7e-3 in bf16, 2.9e-4 and 2.1e-4 in fp16).  A second plane
+// would add half as many products again; it is taken for the probabilities where a bias table is trained (P2, out32), since the
+// table's gradient is a sum that cancels.  A weight below 2^-126 of its row's largest is zero.
 #pragma once
 #include "mgn_device.h"
 

@@ -73,7 +73,7 @@ __device__ __forceinline__ void fill_biases(float* lutb, const AttnBwd& a, int h
 // Buckets of all pairs of a segment, once for all heads and both kernels, as lists of 16 bytes per lane in the order in which each
 // kernel's lanes hold a subtile's scores: a lane of the query side 16 keys of its query, of the key side 16 queries of its key.  A
 // wave takes one subtile of queries and every gridDim.y-th subtile of keys.  Bound by the vector unit and the two writes: 20 000 x
-// 2501, 27 us, 102 MB, 3.8 TB/s; it spares dQ and the table 75 us and dK, dV 25 us of 300 and 285 with four heads.
+// 2501, 23 us, 102 MB, 4.4 TB/s; it spares dQ and the table 75 us and dK, dV 25 us of 300 and 285 with four heads.
 template <int BIAS>
 __global__ __launch_bounds__(256) void attn_buckets_kernel(AttnBwd a) {
     __shared__ unsigned char lutb[LUTS<BIAS>];
@@ -126,8 +126,8 @@ constexpr int GROUP = 2;                               // sums by bucket that ar
 // readout of 20 000 x 2501 in us for 1 / 2 / 4 / 8 at a time: 753 / 741 / 744 / 771, without the sums 684, before buckets were listed).
 //
 // Bound by the vector unit with a bias (18 products a step beside about 260 vector instructions with listed buckets, 390
-// without): 20 000 x 2501, 4 heads of 32, fp32, plane, table trained, 214 us and 7 for the sum of its two pieces.  Without one by
-// the latency of a step's chain: 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 80 us = 0.59 PFLOP/s.
+// without): 20 000 x 2501, 4 heads of 32, fp32, plane, table trained, 179 us and 7 for the sum of its two pieces.  Without one by
+// the latency of a step's chain: 17 973 x 12 870 in 16 segments, 8 heads of 64, bf16, 75 us = 0.63 PFLOP/s.
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 && (KIND == AT_F32 || BIAS > 0) ? 1 : KIND == AT_F32 && DP == 32 && BIAS > 0 ? 3 : 2) void attn_dq_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP;
@@ -369,8 +369,8 @@ __global__ __launch_bounds__(64) void attn_table_kernel(const double* __restrict
 // ------------------------------------------------------------------------------------------------ key side
 // A workgroup: 128 keys of one key head, 32 per wave, against its share of the (query head, query subtile) pairs that read
 // them.  Here the lane owns a key: rows of the products are queries, whose statistics come through LDS.
-// Bound like the query side.  Measured at its two problems: 260 us (fp32, plane, listed buckets, 24 products a step)
-// and 106 us = 0.59 PFLOP/s (bf16, four query heads to a key head).
+// Bound like the query side.  Measured at its two problems: 204 us (fp32, plane, listed buckets, 24 products a step)
+// and 100 us = 0.63 PFLOP/s (bf16, four query heads to a key head).
 template <int KIND, int DP, int BIAS>
 __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnBwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP;

@@ -7,8 +7,8 @@ namespace {
 // ---------------------------------------------------------------------------------------------- operand images
 // One wave per (head, subtile): lane (i, h) reads the elements 16 c + 8 h .. + 7 of token i, which are its share of image R;
 // image T is read back from a row-major copy in LDS.  Memory bound: 4 bytes read and 4 (R) or 8 (R and T) written per element.
-// Measured: the four images of a backward pass over 17 973 queries, 8 heads of 64, and 12 870 keys, 2 heads, bf16: 25 us for
-// 105 MB, 4.3 TB/s.
+// Measured: the four images of a backward pass over 17 973 queries, 8 heads of 64, and 12 870 keys, 2 heads, bf16: 24 us for
+// 105 MB, 4.4 TB/s.
 template <int KIND, int DP>
 __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, LD = DP + 2;
@@ -144,9 +144,9 @@ __global__ __launch_bounds__(256) void attn_image_kernel(ImageArgs a) {
 // ahead than values.  The maximum is only raised when a score exceeds it by more than OVER (base 2): until then probabilities up
 // to 2^OVER are as good as ones up to 1, and rescaling the sums, due in most steps of a wave otherwise, becomes rare.
 //
-// Measured, images included: 8192 x 8192, 8 heads of 128, bf16, 286 us, 0.96 PFLOP/s, three quarters of a large library product:
+// Measured, images included: 8192 x 8192, 8 heads of 128, bf16, 277 us, 0.99 PFLOP/s, 78 % of a large library product:
 // bound by the matrix unit and by what exponentials do not hide under it.  20 000 x 2501, 4 heads of 32, fp32, places on a plane:
-// 188 us with the join of two pieces; bound by the vector unit (330 vector instructions a step beside 12 products).
+// 172 us with the join of two pieces; bound by the vector unit (340 vector instructions a step beside 12 products).
 template <int KIND, int DP, int BIAS, bool P2, int NW>
 __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ? 1 : 2) void attn_fwd_kernel(AttnFwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, SUB = PL * 32 * DP;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(64 * NW, (KIND == AT_F32 && DP == 128) || NW == 8 ?
 // The tiled kernel with a bias by distance on a lattice where a wave takes two heads of the same 32 queries: the place of a
 // (query, key) pair, a dozen vector instructions, is found once for both, and the products of the second head are issued before
 // the exponentials of the first.  Bound by the vector unit.  Measured: 100 000 queries x 1225 keys, 4 heads of 32, places on a
-// plane, 370 us in fp32 and 225 us in fp16 (a head at a time 380 and 266).
+// plane, 364 us in fp32 and 243 us in fp16 (a head at a time 382 and 298).
 constexpr int HEADS = 2;
 template <int KIND, int DP, int BIAS, bool P2>
 __global__ __launch_bounds__(256, DP == 32 && KIND != AT_F32 ? 3 : 2) void attn_fwd_heads_kernel(AttnFwd a) {
@@ -654,7 +654,7 @@ __global__ __launch_bounds__(256, DP == 32 && KIND != AT_F32 ? 3 : 2) void attn_
 // One launch and no images: a workgroup takes 32 queries of a head, its four waves every fourth subtile of the keys, which they
 // read where they lie (keys row by row, values column by column, both straight into operand registers) and scale themselves;
 // the waves' sums meet in LDS.  Latency bound: what counts is the length of the chain, not the conversions done again in
-// every workgroup.  Measured: 561 x 280, 4 heads of 32, fp32: 9.8 us, 14.0 us as a call from Python.
+// every workgroup.  Measured: 561 x 280, 4 heads of 32, fp32: 10.9 us, 14 to 15 us as a call from Python.
 template <int KIND, int DP, int BIAS, bool P2>
 __global__ __launch_bounds__(256, DP == 128 || (KIND == AT_F32 && DP == 64) ? 1 : 2) void attn_small_kernel(AttnFwd a) {
     constexpr int PL = planes<KIND>(), NC = DP / 16, NB = DP / 32, LD = DP + 4;
@@ -1002,7 +1002,7 @@ __global__ __launch_bounds__(64 * NW) void attn_join_kernel(AttnFwd a) {
 }
 
 // The same for up to eight pieces: four outputs per thread, which reads all factors itself.  Memory bound.  Measured: 20 000
-// queries, 4 heads of 32, two pieces, 8.7 us, 3.5 TB/s (a wave per query and head 34 us).
+// queries, 4 heads of 32, two pieces, 9.0 us, 3.5 TB/s (a wave per query and head 34 us).
 template <int KIND, int DP>
 __global__ __launch_bounds__(256) void attn_join_rows_kernel(AttnFwd a) {
     constexpr int QUADS = DP / 4;

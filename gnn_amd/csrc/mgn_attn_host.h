@@ -85,10 +85,10 @@ inline int attn_check(const MgnAttn* a, const char* name, bool backward) {
 
 // Small problems: 32 queries of a head per workgroup and no images, one launch instead of two.  It converts a subtile anew in
 // every workgroup, so it pays while all workgroups are resident at once, a workgroup's chain of subtiles is short and there is
-// little work in all (us, images against small): fp32, 4 heads of 32: 561 x 280 18.7 / 14.0, 4000 x 1000 28.5 / 24.7, 6000 x 300
-// 17.6 / 17.1, 12 000 x 150 17.8 / 21.3, 100 000 x 20 36 / 102, 500 x 2000 23.4 / 31.4, 7900 x 2000 51 / 77; 8 heads of 64: 500 x
-// 500 25.6 / 16.2, 4000 x 500 28.3 / 56.1; bf16, 4 heads of 32: 500 x 500 18.8 / 14.7, 500 x 1000 21.5 / 25.2; 4 heads of 128:
-// 500 x 250 18.9 / 21.1.
+// little work in all (us, images against small): fp32, 4 heads of 32: 561 x 280 16.1 / 12.1, 4000 x 1000 26.3 / 26.1, 6000 x 300
+// 16.2 / 18.7, 12 000 x 150 16.5 / 23.4, 100 000 x 20 31 / 114, 500 x 2000 21.7 / 37.3, 7900 x 2000 49 / 88; 8 heads of 64: 500 x
+// 500 24.9 / 17.6, 4000 x 500 27.1 / 65.7, fp16, 500 x 250 16.6 / 15.5; bf16, 4 heads of 32: 500 x 500 16.1 / 13.7, 500 x 1000 18.9 /
+// 24.1; 4 heads of 128: 500 x 250 17.5 / 20.5.
 inline bool attn_is_small(const MgnAttn& a) {
     const int64_t chain = a.n_k / a.n_seg * attn_dp(a.dim), blocks = (a.n_q / 32 + a.n_seg) * (int64_t)a.heads;
     return blocks <= 512 && chain <= (a.dtype == MGN_F32 ? 32768 : 16384) && blocks * chain <= 1 << 24;
@@ -108,8 +108,8 @@ inline int attn_fwd_waves(const MgnAttn& a) {
     return !a.bias_table && attn_dp(a.dim) == 128 && a.dtype != MGN_F32 && (a.n_q / 256 + a.n_seg) * a.heads >= 256 ? 8 : 4;
 }
 // Two heads per wave of the tiled kernel share the places of a lattice, where the registers hold them and four workgroups per
-// compute unit are there to begin with (100 000 x 1225, 4 heads of 32, plane: fp32 380 -> 370 us, fp16 266 -> 225; of 64, fp16
-// 316 -> 305; 32 768 queries, fp32, 125 -> 112).  A place on a line is too cheap to share (295 us alone, 316 shared), and two
+// compute unit are there to begin with (100 000 x 1225, 4 heads of 32, plane: fp32 382 -> 364 us, fp16 298 -> 243; of 64, fp16
+// 380 -> 321; 32 768 queries, fp32, 132 -> 115).  A place on a line is too cheap to share (295 us alone, 316 shared), and two
 // heads of 64 in fp32 spill.
 inline int attn_fwd_share(const MgnAttn& a) {
     return a.bias_table && a.axes > 1 && attn_dp(a.dim) <= (a.dtype == MGN_F32 ? 32 : 64) && a.heads % 2 == 0 &&

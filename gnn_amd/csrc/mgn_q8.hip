@@ -4,7 +4,7 @@
 //
 // Memory bound: 4 (2) bytes read and 1 written per element and 4 per row.  32 lanes share a row, each with 16-byte pieces,
 // so a row of 128 fp32 values is one load per lane; several rows per lane are requested before the first is reduced.
-// Measured at 1 498 001 x 128 fp32: kept in 202 us, restored in 160 us, 0.97 GB each: 4.8 and 6.0 TB/s (a large copy 4.8).
+// Measured at 1 498 001 x 128 fp32: kept in 202 us, restored in 159 us, 0.97 GB each: 4.8 and 6.1 TB/s (a large copy 4.8).
 #include "mgn_device.h"
 
 namespace {

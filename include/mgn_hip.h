@@ -552,10 +552,13 @@ int mgn_train_edge_bwd_q8(const int8_t* codes, const float* scale, const float* 
  *
  * Rows: q [n_q][heads][dim], k and v [n_k][kv_heads][dim], heads a multiple of kv_heads (query head h reads key head
  * h / (heads / kv_heads)); strides in elements, the last axis dense, every row on a 16-byte border; dim a multiple of
- * 8 up to 128; fp32, bf16 or fp16.  Sums, softmax statistics and products are fp32 (fp32 operands as two fp16 terms).
+ * 8 up to 128; fp32, bf16 or fp16.  Sums, softmax statistics and products are fp32 (fp32 operands as two fp16 terms
+ * scaled by block or row, 2^-22 of a value; in the 16-bit types probabilities and dS are rounded to the type where they are multiplied
+ * with values, keys, queries and gradients, to two terms of it for out32).  This holds in every matrix mode (MGN_MATMUL).
  * Segments: q_ptr / k_ptr [n_seg + 1] (device, ascending); null: one segment.  Rows outside all segments are neither
  * read nor written (zero_outside: outputs of such rows become zeros).  key_mask [n_k]: 0 leaves a key out; nothing is read from its rows.  A query with no key left (or
- * only keys at a bias of minus infinity) gives a row of zeros and gradients of zero.
+ * only keys at a bias of minus infinity) gives a row of zeros and gradients of zero.  A NaN in an operand, or a
+ * score that overflows, makes every result that it enters NaN; an infinity makes the scores of its key, or its value's column, so.
  * Bias: places [n][axes] of queries and keys, any int32; one axis: place = k - q held to
  * [-reach, reach], plus reach (table of 2 reach + 1 entries); two or three: the whole part of the distance, held to reach
  * (reach + 1 entries).  bucket_lut values are held to [0, n_bucket).  reach <= 1024, n_bucket <= 64.
