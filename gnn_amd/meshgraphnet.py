@@ -379,7 +379,7 @@ class EncodeProcessDecodeMultiScale(nn.Module):
         return kept[1]
 
     def captured_parts(self, graph, training: bool = False) -> list:
-        """What launches recorded for ``graph`` go on reading: its topology, coarse graph, readout plan and the workspaces.  The
+        """What launches recorded for ``graph`` go on reading: its topology, coarse graph, readout plan, workspaces and the normalisers' scratch.  The
         model keeps these in caches that a call on another mesh replaces, so whoever records launches calls this first (nothing
         is then built while recording) and keeps the list for as long as it replays them."""
         def looked_up(topo):
@@ -393,7 +393,8 @@ class EncodeProcessDecodeMultiScale(nn.Module):
             parts += [cg, looked_up(cg.topology)]
             if self.coarse_readout == "attention":
                 parts.append(self._readout_plan(cg, graph["mesh_pos"], None, graph))
-        parts += [self.__dict__.get(k) for k in ("_ws", "_cws", "_pk", "_cpk")]
+        if not training:                          # a training step makes its buffers itself
+            parts += [self.__dict__.get(k) for k in ("_ws", "_cws", "_pk", "_cpk")]
         for nrm in (self.node_features_normalizer, self.edge_features_normalizer, self.output_normalizer) + \
                 ((self.coarse_edge_features_normalizer,) if self.sample_ratio > 0 else ()):
             parts += nrm.captured_buffers()

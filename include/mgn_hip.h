@@ -558,7 +558,7 @@ int mgn_train_edge_bwd_q8(const int8_t* codes, const float* scale, const float* 
  * Segments: q_ptr / k_ptr [n_seg + 1] (device, ascending); null: one segment.  Rows outside all segments are neither
  * read nor written (zero_outside: outputs of such rows become zeros).  key_mask [n_k]: 0 leaves a key out; nothing is read from its rows.  A query with no key left (or
  * only keys at a bias of minus infinity) gives a row of zeros and gradients of zero.  A NaN in an operand, or a
- * score that overflows, makes every result that it enters NaN; an infinity makes the scores of its key, or its value's column, so.
+ * score that overflows upwards, makes every result that it enters NaN; an infinity makes the scores of its key, or its value's column, so.
  * Bias: places [n][axes] of queries and keys, any int32; one axis: place = k - q held to
  * [-reach, reach], plus reach (table of 2 reach + 1 entries); two or three: the whole part of the distance, held to reach
  * (reach + 1 entries).  bucket_lut values are held to [0, n_bucket).  reach <= 1024, n_bucket <= 64.
