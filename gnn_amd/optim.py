@@ -45,6 +45,10 @@ class FusedAdam(torch.optim.Optimizer):
         _lib.check(rc, "mgn_adam_hyper")
         return rec
 
+    def captured_buffers(self) -> list:
+        """What the step that was just captured goes on reading; whoever replays it keeps these alive."""
+        return list(self.__dict__.get("_tables", {}).values()) + list(self.__dict__.get("_hyper", {}).values())
+
     def advance_host(self):
         """The host part of a step whose device part is replayed from a captured graph: step counts, and the update's
         scalars (from the current ``lr`` of every group) into the pinned records the graph copies from.  The caller
@@ -118,9 +122,18 @@ class FusedAdam(torch.optim.Optimizer):
                     # asynchronous upload from a pinned buffer that is kept (allocating pinned memory is not legal under
                     # stream capture, an asynchronous copy from it is); the previous copy may not have run yet: wait
                     rec = self._write_hyper(gi, group, step)            # creates the record, waits for its event
-                    pin = self.__dict__.setdefault("_pinned_rows", {}).get(gi)
-                    if pin is None or pin.shape != host_rows.shape:
-                        pin = self._pinned_rows[gi] = torch.empty(host_rows.shape, dtype=torch.int64).pin_memory()
+                    # a captured copy reads its rows in every replay, so it gets a buffer of its own, made by an earlier
+                    # eager step: one that later eager steps rewrote would point the replays at their gradients
+                    rows_of, spare = self.__dict__.setdefault("_pinned_rows", {}), self.__dict__.setdefault("_pinned_spare", {})
+                    if torch.cuda.is_current_stream_capturing():
+                        pin = spare.pop(gi, None)
+                        if pin is None or pin.shape != host_rows.shape:
+                            raise RuntimeError("FusedAdam: run one eager step with these parameters before a step is captured")
+                    else:
+                        for kept in (rows_of, spare):
+                            if gi not in kept or kept[gi].shape != host_rows.shape:
+                                kept[gi] = torch.empty(host_rows.shape, dtype=torch.int64).pin_memory()
+                        pin = rows_of[gi]
                     pin.copy_(host_rows)
                     host_rows = pin
                     table = torch.empty(host_rows.shape, dtype=torch.int64, device=dev)

@@ -573,7 +573,7 @@ class CapturedTrainStep:
             total.backward()
             self.opt.step()
             self.out = (total.detach(), ux.detach(), uy.detach(), phi.detach())
-        self.held += [buf for nr in self.norms for buf in nr.captured_buffers()]      # as the capture used them
+        self.held += [buf for nr in self.norms for buf in nr.captured_buffers()] + self.opt.captured_buffers()     # as the capture used them
         # the capture ran the host bookkeeping of one step (optimiser step counts, normaliser counts) without
         # executing anything: that bookkeeping belongs to the first replay
         self.rows_added = [nr._acc_count - c for nr, c in zip(self.norms, counts)]

@@ -671,3 +671,36 @@ def test_training_step_is_additive_over_disconnected_meshes():
         worst = max(worst, float((gu[k].double() - ga[k].double() - gb[k].double()).norm()) / scale)
     print("union vs sum of the parts, worst gradient deviation relative to the larger part: %.2e" % worst)
     assert worst < 1e-4
+
+
+def test_eager_steps_on_another_mesh_between_replays():
+    """The optimiser's pointer table of a captured step is its own: eager steps of the same model and optimiser on another mesh, with
+    gradients elsewhere in memory, do not redirect the replays.  Same losses as the eager sequence, bit for bit."""
+    from gnn_amd.meshgraphnet import EncodeProcessDecodeMultiScale
+    from gnn_amd.optim import FusedAdam
+    from gnn_amd.training import CapturedTrainStep
+    frames = [graph_to(O.synthetic_graph(nx, ny, seed=s, with_target=True), DEV) for nx, ny, s in ((16, 10, 3), (25, 14, 4))]
+    runs = []
+    for captured in (False, True):
+        torch.manual_seed(11)
+        model = EncodeProcessDecodeMultiScale(10, 7, hidden_size=128, process_steps=2, coarse_process_steps=0, node_out_dim=3, attention=False,
+                                              with_mat_params=False, time_dim=1, device=DEV, sample_ratio=0.0).to(DEV).train()
+        opt = FusedAdam(model.parameters(), lr=1e-3, capturable=captured)
+        step = CapturedTrainStep(model, opt) if captured else None
+
+        def eager(frame):
+            opt.zero_grad()
+            total = model.loss(frame)[0]
+            total.backward()
+            opt.step()
+            return float(total.detach())
+        seen = []
+        for i in range(6):
+            seen.append(float(step(frames[0])[0]) if captured else eager(frames[0]))
+            if i:
+                keep = [torch.full((n,), float("nan"), device=DEV) for n in (128, 16384, 49152) for _ in range(4)]
+                seen.append(eager(frames[1]))
+                del keep
+        seen += [float(p.detach().double().norm()) for p in model.parameters()]
+        runs.append(seen)
+    assert runs[0] == runs[1] and all(v == v for v in runs[0])
