@@ -564,19 +564,27 @@ class CapturedTrainStep:
         for nr in self.norms:
             nr.use_device_count(True)
         self.flags = self._accumulating()
-        counts = [nr._acc_count for nr in self.norms]
+        before = [(nr._acc_count, nr._num_accumulations) for nr in self.norms]
         torch.cuda.synchronize(dev)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.opt.zero_grad()
-            total, ux, uy, phi = self.model.loss(self.static, check_range=False)
-            total.backward()
-            self.opt.step()
-            self.out = (total.detach(), ux.detach(), uy.detach(), phi.detach())
+        graph = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(graph):
+                self.opt.zero_grad()
+                total, ux, uy, phi = self.model.loss(self.static, check_range=False)
+                total.backward()
+                self.opt.step()
+                self.out = (total.detach(), ux.detach(), uy.detach(), phi.detach())
+        except BaseException:                       # nothing was recorded that could be replayed
+            for nr, (count, times) in zip(self.norms, before):
+                nr._acc_count, nr._num_accumulations = count, times
+                nr.use_device_count(False)
+            self.held = self.out = None
+            raise
+        self.graph = graph
         self.held += [buf for nr in self.norms for buf in nr.captured_buffers()] + self.opt.captured_buffers()     # as the capture used them
         # the capture ran the host bookkeeping of one step (optimiser step counts, normaliser counts) without
         # executing anything: that bookkeeping belongs to the first replay
-        self.rows_added = [nr._acc_count - c for nr, c in zip(self.norms, counts)]
+        self.rows_added = [nr._acc_count - c for nr, (c, _) in zip(self.norms, before)]
         self.done = torch.cuda.Event()
 
     def _replay(self):

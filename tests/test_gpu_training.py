@@ -704,3 +704,32 @@ def test_eager_steps_on_another_mesh_between_replays():
         seen += [float(p.detach().double().norm()) for p in model.parameters()]
         runs.append(seen)
     assert runs[0] == runs[1] and all(v == v for v in runs[0])
+
+
+def test_a_capture_that_fails_leaves_the_step_as_it_was():
+    """An error while the step is being recorded: no empty graph is replayed afterwards, the normalisers' counts are what they
+    were, and the next call records anew."""
+    from gnn_amd.meshgraphnet import EncodeProcessDecodeMultiScale
+    from gnn_amd.optim import FusedAdam
+    from gnn_amd.training import CapturedTrainStep
+    g = graph_to(O.synthetic_graph(16, 10, seed=3, with_target=True), DEV)
+    runs = []
+    for fails in (False, True):
+        torch.manual_seed(11)
+        model = EncodeProcessDecodeMultiScale(10, 7, hidden_size=128, process_steps=2, coarse_process_steps=0, node_out_dim=3, attention=False,
+                                              with_mat_params=False, time_dim=1, device=DEV, sample_ratio=0.0).to(DEV).train()
+        step = CapturedTrainStep(model, FusedAdam(model.parameters(), lr=1e-3, capturable=True))
+        seen = [float(step(g)[0])]
+        if fails:
+            def broken(*a, **k):
+                raise RuntimeError("in the middle of it")
+            model.loss = broken
+            with pytest.raises(RuntimeError, match="in the middle"):
+                step(g)
+            del model.loss
+            assert step.graph is None and step.held is None
+            assert all(nr._work().get("count_dev") is None for nr in step.norms)
+        seen += [float(step(g)[0]) for _ in range(4)]
+        assert step.graph is not None
+        runs.append(seen + [nr._acc_count for nr in step.norms])
+    assert runs[0] == runs[1]
