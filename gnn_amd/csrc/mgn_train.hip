@@ -555,7 +555,7 @@ __global__ __launch_bounds__(NT, 1) void train_linear_bwd3_kernel(LinBwdArgs a) 
 //
 // Streams 4 (G) + 1 (codes) bytes in and 4 (GA) out per element.  Tiles of 64 rows, eight waves, two per SIMD: wave w takes
 // column block w & 3 of both products, of GA the rows 32 (w >> 2) .., of dW the column blocks 2 (w >> 2) and + 1 -- so each keeps
-// the weight planes of 32 columns (96 registers) and 32 accumulators.  Measured: 1 498 001 rows 468 us = 3.7 TB/s, 473 to 516 us as a call from box to box (a copy of as many
+// the weight planes of 32 columns (96 registers) and 32 accumulators.  Measured: 1 498 001 rows 468 us = 3.7 TB/s, 473 to 516 us as a call from card to card (a copy of as many
 // bytes 362 us, its nine partial products at a large product's rate 346 us: both at once; the four-wave form on the three-plane
 // input took 678 us); 561 rows 12.6 us, the latency of one tile and of the reduction of the partial sums.
 struct LinBwdQ8Args {
